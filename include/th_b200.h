@@ -388,6 +388,76 @@ int th_cast(int n_tensors, const void *const *src_dev, void *const *dst_dev, con
  * (laid out [w_in | w_hid | w_out | b_in | b_hid | b_out]) into a normalised 16-bit gradient buffer. */
 int th_scale_cast(const float *src_dev, void *dst_dev, int64_t n_elems, float scale, int dtype, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Layers wider than the fused MLP.  NO COUNTERPART IN THE REFERENCE, whose fused network ends at 64
+ * columns: a root-mean-square norm, linear layers on 8-bit integers, and the products and 8-bit rows of
+ * a linear layer that keeps its input in 8 bits for the backward pass.
+ *
+ * Matrices are rows of `d` elements with unit stride inside a row; strides count elements.
+ * 8-bit rows:  a = max(max_k |x_k|, 2^-100);  q_k = rint(x_k * (127 / a));  scale = a / 127, in float32.
+ * They start on 16 bytes (pointer and stride); bytes between d and the stride are never read.  A row
+ * that holds an infinity or a NaN gets zeros and the scale NaN.
+ * ------------------------------------------------------------------------------------------ */
+
+/* y = s * rstd * gain with s = x, or s = x + residual rounded to `dtype` and written to sum_dev
+ * (contiguous; given exactly when the residual is), rstd = 1 / sqrt(mean_k s_k^2 + eps).  y is contiguous;
+ * rstd_dev (fp32 per row, for the backward pass) may be null.  The gain is float32 or of the rows' type. */
+int th_rms_norm_fwd(const void *x_dev, int64_t x_stride, const void *residual_dev, int64_t residual_stride,
+                    const void *gain_dev, int gain_dtype, void *sum_dev, void *y_dev, float *rstd_dev,
+                    int64_t rows, int d, float eps, int dtype, void *stream);
+
+/* The same with y as 8-bit rows. */
+int th_rms_norm_int8(const void *x_dev, int64_t x_stride, const void *residual_dev, int64_t residual_stride,
+                     const void *gain_dev, int gain_dtype, void *sum_dev, void *q_dev, int64_t q_stride,
+                     float *scale_dev, int64_t rows, int d, float eps, int dtype, void *stream);
+
+int64_t th_rms_norm_bwd_workspace_bytes(int64_t rows, int d, int dtype);
+
+/* Backward from s and rstd.  grad_sum_dev (may be null) is the gradient of s as an output; grad_x_dev, contiguous,
+ * is the gradient of x and of the residual alike.  grad_gain_dev (of the gain's type) may be null, then no scratch
+ * is needed.  Sums run in a fixed order: results repeat bit for bit. */
+int th_rms_norm_bwd(const void *sum_dev, int64_t sum_stride, const void *gain_dev, int gain_dtype,
+                    const float *rstd_dev, const void *grad_y_dev, int64_t gy_stride, const void *grad_sum_dev,
+                    int64_t gs_stride, void *grad_x_dev, void *grad_gain_dev, void *workspace_dev,
+                    int64_t workspace_bytes, int64_t rows, int d, int dtype, void *stream);
+
+/* Rows to 8 bits, and back (q * scale rounded to `dtype`). */
+int th_quantize_rows(const void *x_dev, int64_t x_stride, void *q_dev, int64_t q_stride, float *scale_dev,
+                     int64_t rows, int d, int dtype, void *stream);
+int th_dequantize_rows(const void *q_dev, int64_t q_stride, const float *scale_dev, void *out_dev,
+                       int64_t out_stride, int64_t rows, int d, int dtype, void *stream);
+
+/* out[c] = sum over rows of g[r, c], float32 sums in a fixed order, rounded to `dtype`. */
+int64_t th_column_sum_workspace_bytes(int64_t rows, int d);
+int th_column_sum(const void *g_dev, int64_t g_stride, void *out_dev, void *workspace_dev,
+                  int64_t workspace_bytes, int64_t rows, int d, int dtype, void *stream);
+
+/* y[r, n] = scale[r] * weight_scale[n] * sum_k q[r, k] weight[n, k] + bias[n]: 8-bit rows on both sides, exact
+ * 32-bit integer sums (d_in up to 131071), y and bias in `dtype`; the bias may be null. */
+int64_t th_int8_linear_workspace_bytes(int64_t rows, int d_in, int d_out);
+int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev,
+                   int64_t weight_stride, const float *weight_scale_dev, const void *bias_dev, void *y_dev,
+                   int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
+                   int d_out, int dtype, void *stream);
+
+/* The products of a linear layer in 16 bits with float32 sums: y = x w^T + b, grad_x = grad_y w and
+ * grad_w = grad_y^T x (contiguous).  Operand rows start on 16 bytes (pointer and stride); outputs may lie anywhere.
+ * One size of scratch covers the three.  Results repeat bit for bit. */
+int64_t th_linear_workspace_bytes(int64_t rows, int d_in, int d_out);
+int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *weight_dev, int64_t weight_stride,
+                  const void *bias_dev, void *y_dev, int64_t y_stride, void *workspace_dev,
+                  int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *weight_dev,
+                        int64_t weight_stride, void *grad_x_dev, int64_t gx_stride, void *workspace_dev,
+                        int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
+                         void *grad_weight_dev, void *workspace_dev, int64_t workspace_bytes, int64_t rows,
+                         int d_in, int d_out, int dtype, void *stream);
+
+/* Device-side status word of these products (0 = fine, 1 = a bounded wait ran out and results are invalid).
+ * Synchronises the device. */
+int th_linear_tc_status(void);
+
 #ifdef __cplusplus
 }
 #endif

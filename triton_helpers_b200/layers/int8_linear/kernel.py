@@ -1,0 +1,176 @@
+r"""Linear layers on 8-bit integers, and the 8-bit rows they take, on hand-written sm_100a kernels.
+
+There is no such operator in triton_helpers; this module follows the conventions of its fused MLP
+(``triton_helpers/layers/fully_fused_mlp/kernel.py:640-686``): a functional entry point, assertions on shapes,
+``TypeError`` for types, weights as ``(out, in)``.
+
+8-bit rows hold a matrix as signed integers with one float32 scale per row::
+
+    a = max(max_k |x_k|, 2^-100)      q_k = rint(x_k * (127 / a))      scale = a / 127        (float32)
+
+A row that holds an infinity or a NaN has zeros and the scale NaN, so it reads back as NaN throughout.  With one scale per
+token and one per output channel a linear layer is an integer product and a factor per output::
+
+    y[t, n] = scale[t] * weight.scale[n] * sum_k q[t, k] * weight.q[n, k] + bias[n]
+
+The sums are exact in 32 bits (up to 131071 inputs) and rounded once, to the type of the result.
+"""
+from typing import NamedTuple, Optional, Union
+
+import torch
+from torch import Tensor
+
+from ... import _lib
+
+MAX_INPUTS = 131071  # 128 * 128 * 131071 < 2^31
+
+
+class Int8Rows(NamedTuple):
+    r"""``q``: int8 ``(..., K)``, laid out by ``quantize_rows`` with rows that start on 16 bytes; ``scale``: float32 ``(...)``."""
+
+    q: Tensor
+    scale: Tensor
+
+
+def float_dtype(t: Tensor, what: str) -> torch.dtype:
+    if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"{what} must be float16, bfloat16 or float32, got {t.dtype}")
+    return t.dtype
+
+
+def refuse_gradients(what: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def rows2d(t: Tensor, width: int) -> Tensor:
+    r"""``t`` as rows of ``width`` elements with unit stride inside a row; a copy only where the strides ask for it."""
+    t = t.reshape(-1, width)
+    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
+
+
+def row_stride(t: Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def empty_int8_rows(lead, width: int, device: torch.device) -> Int8Rows:
+    pitch = -(-width // 16) * 16
+    rows = 1
+    for n in lead:
+        rows *= n
+    q = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+    return Int8Rows(q[:, :width].view(*lead, width), torch.empty(lead, dtype=torch.float32, device=device))
+
+
+def int8_rows2d(rows: Int8Rows, what: str) -> Int8Rows:
+    r"""Checks 8-bit rows and returns them as a matrix whose rows start on 16 bytes (copied where they do not)."""
+    q, scale = rows
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"{what}: 8-bit rows are int8 with float32 scales, got {q.dtype} and {scale.dtype}")
+    assert q.dim() >= 1 and q.shape[-1] >= 1, f"{what}: 8-bit rows need at least one column"
+    assert scale.shape == q.shape[:-1], f"{what}: one scale per row: {tuple(scale.shape)} for rows {tuple(q.shape)}"
+    width = q.shape[-1]
+    q, scale = q.reshape(-1, width), scale.reshape(-1).contiguous()
+    if q.numel() and ((width > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (q.shape[0] > 1 and (q.stride(0) % 16 or q.stride(0) < width))):
+        q = empty_int8_rows((q.shape[0],), width, q.device).q.copy_(q)
+    return Int8Rows(q, scale)
+
+
+def int8_stride(q: Tensor) -> int:
+    return q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
+
+
+@torch.no_grad()
+def quantize_rows(x: Tensor) -> Int8Rows:
+    r"""8-bit rows of ``x`` (..., K), float16, bfloat16 or float32; no gradient."""
+    assert x.dim() >= 1 and x.shape[-1] >= 1, "8-bit rows need at least one column"
+    float_dtype(x, "x")
+    device = _lib.require_cuda(x)
+    width = x.shape[-1]
+    x2d = rows2d(x, width)
+    out = empty_int8_rows(x.shape[:-1], width, device)
+    with torch.cuda.device(device):
+        _lib.check(
+            _lib.lib().th_quantize_rows(
+                x2d.data_ptr(), row_stride(x2d), out.q.data_ptr(), -(-width // 16) * 16, out.scale.data_ptr(), x2d.shape[0], width,
+                _lib.dtype_code(x), _lib.stream_ptr(device),
+            ),
+            "th_quantize_rows",
+        )  # fmt: skip
+    return out
+
+
+@torch.no_grad()
+def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> Tensor:
+    r"""``q * scale`` of 8-bit rows, rounded once to ``dtype`` (float16, bfloat16 or float32); contiguous."""
+    lead, width = rows.q.shape[:-1], rows.q.shape[-1]
+    q, scale = int8_rows2d(rows, "dequantize_rows")
+    device = _lib.require_cuda(q, scale)
+    out = torch.empty((*lead, width), dtype=dtype, device=device)
+    float_dtype(out, "dtype")
+    with torch.cuda.device(device):
+        _lib.check(
+            _lib.lib().th_dequantize_rows(
+                q.data_ptr(), int8_stride(q), scale.data_ptr(), out.data_ptr(), width, q.shape[0], width, _lib.dtype_code(out),
+                _lib.stream_ptr(device),
+            ),
+            "th_dequantize_rows",
+        )  # fmt: skip
+    return out
+
+
+def int8_linear(
+    x: Union[Tensor, Int8Rows], weight: Int8Rows, bias: Optional[Tensor] = None, dtype: Optional[torch.dtype] = None
+) -> Tensor:
+    r"""Linear layer with 8-bit weights; a float ``x`` is turned into 8-bit rows on the way.  No gradient.
+
+    Args:
+        x: float16, bfloat16 or float32 tensor, or 8-bit rows (of ``quantize_rows`` or ``rms_norm_int8``)
+        weight: 8-bit rows of the ``(out, in)`` weight matrix
+        bias: of the result's type, or ``None``
+        dtype: type of the result; that of ``x`` by default, and required where ``x`` is 8-bit rows
+
+    Shapes:
+        - x: :math:`(..., D_{in})`, output: :math:`(..., D_{out})`, bias: :math:`(D_{out},)`
+    """
+    if isinstance(x, Int8Rows):
+        if dtype is None:
+            raise TypeError("8-bit rows do not say the type of the result: pass dtype")
+        refuse_gradients("int8_linear", bias)
+        rows = x
+    else:
+        refuse_gradients("int8_linear", x, bias)
+        dtype = float_dtype(x, "x") if dtype is None else dtype
+        rows = None
+    if dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"the result must be float16, bfloat16 or float32, got {dtype}")
+    with torch.no_grad():
+        if rows is None:
+            rows = quantize_rows(x)
+        lead = rows.q.shape[:-1]
+        q, scale = int8_rows2d(rows, "x")
+        assert weight.q.dim() == 2, "the weight is a matrix of 8-bit rows"
+        w, w_scale = int8_rows2d(weight, "weight")
+        d_out, d_in = w.shape
+        assert q.shape[1] == d_in, f"Input dimension mismatch: {q.shape[1]} and {d_in}"
+        assert d_out >= 1, "the weight needs at least one row"
+        assert d_in <= MAX_INPUTS, f"Input dimension {d_in} too large for 32-bit sums"
+        assert bias is None or bias.shape == (d_out,), "Bias shape mismatch"
+        if bias is not None and bias.dtype != dtype:
+            raise TypeError(f"the bias must be of the result's type {dtype}, got {bias.dtype}")
+        device = _lib.require_cuda(q, scale, w, w_scale, bias)
+        bias = None if bias is None else bias.contiguous()
+        y = torch.empty((*lead, d_out), dtype=dtype, device=device)
+        lib = _lib.lib()
+        with torch.cuda.device(device):
+            ws_bytes = lib.th_int8_linear_workspace_bytes(q.shape[0], d_in, d_out)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+            _lib.check(
+                lib.th_int8_linear(
+                    q.data_ptr(), int8_stride(q), scale.data_ptr(), w.data_ptr(), int8_stride(w), w_scale.data_ptr(), _lib.ptr(bias),
+                    y.data_ptr(), d_out, _lib.ptr(workspace), ws_bytes, q.shape[0], d_in, d_out, _lib.DTYPE_CODE[dtype],
+                    _lib.stream_ptr(device),
+                ),
+                "th_int8_linear",
+            )  # fmt: skip
+    return y
