@@ -18,6 +18,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
@@ -25,6 +26,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <strings.h>
@@ -1249,6 +1251,377 @@ PyObject *py_train_gradients(PyObject *, PyObject *const *args, Py_ssize_t n_arg
     END_HANDLE_TH_ERRORS
 }
 
+// ---- layers for wide networks: norm, 8-bit rows, 8-bit and checkpointed linear layers -------------------------
+//
+// Measured on a B200, host time of one pass, calls back to back: NORMTOKEN.
+
+int64_t pitch16(int64_t width) { return (width + 15) / 16 * 16; }
+
+// 8-bit rows in the layout the kernels take: `lead` x width, rows on 16 bytes
+Tensor empty_int8(c10::IntArrayRef lead, int64_t rows, int64_t width, c10::Device device) {
+    const int64_t pitch = pitch16(width);
+    Tensor q = empty_like_shape({rows * pitch}, at::kChar, device);
+    c10::SmallVector<int64_t, 6> sizes(lead.begin(), lead.end()), strides(lead.size() + 1, 1);
+    sizes.push_back(width);
+    int64_t step = pitch;
+    for (size_t k = lead.size(); k-- > 0;) {
+        strides[k] = step;
+        step *= lead[k];
+    }
+    q.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+    return q;
+}
+
+bool float_code(const Tensor &t, int &code) {
+    code = dtype_code(t.scalar_type());
+    return code >= 0;
+}
+
+// x (..., d) and what goes with it in a norm
+struct NormCall {
+    Tensor x, gain, residual;
+    Rows xr, rr;
+    int64_t d = 0;
+    int code = TH_F32, gain_code = TH_F32;
+    float eps = 0.f;
+};
+
+bool norm_call(NormCall &c, PyObject *const *args, Py_ssize_t n_args) {
+    double eps;
+    if (n_args != 4 || !usual_mode() || !take(args[0], c.x) || !take(args[1], c.gain) || !take(args[2], c.residual) || !take(args[3], eps)) return false;
+    if (!plain(c.x) || c.x.dim() < 1 || c.x.numel() == 0 || !float_code(c.x, c.code)) return false;
+    c.d = c.x.size(-1);
+    c.eps = static_cast<float>(eps);
+    if (!plain(c.gain) || c.gain.dim() != 1 || c.gain.size(0) != c.d || !c.gain.is_contiguous() || c.gain.device() != c.x.device()) return false;
+    if (!float_code(c.gain, c.gain_code) || (c.gain_code != c.code && c.gain_code != TH_F32)) return false;
+    if (c.d > (1 << 24) || !rows_of(c.x, c.d, c.xr)) return false;
+    if (!c.residual.defined()) return true;
+    return plain(c.residual) && c.residual.scalar_type() == c.x.scalar_type() && c.residual.device() == c.x.device() && c.residual.sizes() == c.x.sizes() &&
+           rows_of(c.residual, c.d, c.rr);
+}
+
+struct RmsNormNode : public Node {
+    SavedVariable s, gain, rstd;
+    int64_t rows = 0, d = 0;
+    c10::SmallVector<int64_t, 6> shape;
+    at::ScalarType type = at::kFloat, gain_type = at::kFloat;
+
+    std::string name() const override { return "RMSNormBackward"; }
+    void release_variables() override {
+        s.reset_data();
+        gain.reset_data();
+        rstd.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(3);
+        const Tensor added = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined()) {  // only the sum was used
+            if (task_should_compute_output(0)) out[0] = added;
+            if (task_should_compute_output(2)) out[2] = added;
+            return out;
+        }
+        Tensor ss = s.unpack(shared_from_this()), g = gain.unpack(), r = rstd.unpack();
+        at::NoGradGuard no_grad;
+        ss = same(ss, type, rows * d);
+        g = restored(g, gain_type, d);
+        r = restored(r, at::kFloat, rows);
+        c10::cuda::CUDAGuard guard(ss.device());
+        const auto as_rows = [&](const Tensor &t) { return rows_or_copy(t.scalar_type() == type ? t : t.to(type), d); };
+        const Rows sr = rows_or_copy(ss, d), gy = as_rows(grads[0]), gs = added.defined() ? as_rows(added) : Rows();
+        const bool wants_gain = task_should_compute_output(1);
+        const int code = dtype_code(type);
+        const Tensor dx = empty_like_shape(shape, type, ss.device()), dg = wants_gain ? empty_same(g) : Tensor();
+        const int64_t bytes = wants_gain ? th_rms_norm_bwd_workspace_bytes(rows, static_cast<int>(d), code) : 0;
+        const Tensor workspace = bytes ? empty_like_shape({bytes}, at::kByte, ss.device()) : Tensor();
+        check(th_rms_norm_bwd(ptr(sr.keep), sr.stride, ptr(g), dtype_code(gain_type), r.data_ptr<float>(), ptr(gy.keep), gy.stride, ptr(gs.keep), gs.stride,
+                              ptr(dx), ptr(dg), ptr(workspace), bytes, rows, static_cast<int>(d), code, current_stream()),
+              "th_rms_norm_bwd");
+        if (task_should_compute_output(0)) out[0] = dx;
+        if (task_should_compute_output(2)) out[2] = dx;
+        out[1] = dg;
+        return out;
+    }
+};
+
+PyObject *pair_of(PyObject *a, PyObject *b, PyObject *c = nullptr) {
+    PyObject *t = a && b ? PyTuple_New(c ? 3 : 2) : nullptr;
+    if (!t) {
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        Py_XDECREF(c);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(t, 0, a);
+    PyTuple_SET_ITEM(t, 1, b);
+    if (c) PyTuple_SET_ITEM(t, 2, c);
+    return t;
+}
+
+// rms_norm(x, weight, residual, eps)
+PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    NormCall c;
+    if (!norm_call(c, args, n_args)) TH_NOT_MINE;
+    const bool added = c.residual.defined();
+    Tensor y, s;
+    {
+        NoGil release;
+        const bool grad = torch::autograd::compute_requires_grad(c.x, c.gain, c.residual);
+        std::shared_ptr<RmsNormNode> node;
+        if (grad) {
+            node = make_node<RmsNormNode>(torch::autograd::collect_next_edges(c.x, c.gain, c.residual));
+            node->rows = c.xr.n;
+            node->d = c.d;
+            node->shape.assign(c.x.sizes().begin(), c.x.sizes().end());
+            node->type = c.x.scalar_type();
+            node->gain_type = c.gain.scalar_type();
+            node->gain = SavedVariable(c.gain, false);
+        }
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            c10::cuda::CUDAGuard guard(c.x.device());
+            y = empty_like_shape(c.x.sizes(), c.x.scalar_type(), c.x.device());
+            if (added) s = empty_same(y);
+            const Tensor rstd = grad ? empty_like_shape({c.xr.n}, at::kFloat, c.x.device()) : Tensor();
+            check(th_rms_norm_fwd(ptr(c.x), c.xr.stride, ptr(c.residual), c.rr.stride, ptr(c.gain), c.gain_code, ptr(s), ptr(y),
+                                  static_cast<float *>(ptr(rstd)), c.xr.n, static_cast<int>(c.d), c.eps, c.code, current_stream()),
+                  "th_rms_norm_fwd");
+            if (grad) node->rstd = SavedVariable(rstd, false);
+        }
+        if (grad) {
+            torch::autograd::set_history(y, node);
+            if (added) torch::autograd::set_history(s, node);
+            node->s = added ? SavedVariable(s, true) : SavedVariable(c.x, false);
+        }
+    }
+    PyObject *out = THPVariable_Wrap(std::move(y));
+    return added ? pair_of(out, THPVariable_Wrap(std::move(s))) : out;
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_int8(x, weight, residual, eps) -> (q, scale) or (q, scale, x + residual)
+PyObject *py_rms_norm_int8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    NormCall c;
+    if (!norm_call(c, args, n_args) || torch::autograd::compute_requires_grad(c.x, c.gain, c.residual)) TH_NOT_MINE;
+    const auto lead = c.x.sizes().slice(0, c.x.dim() - 1);
+    Tensor q, scale, s;
+    {
+        NoGil release;
+        at::AutoDispatchBelowADInplaceOrView below;
+        c10::cuda::CUDAGuard guard(c.x.device());
+        q = empty_int8(lead, c.xr.n, c.d, c.x.device());
+        scale = empty_like_shape(lead, at::kFloat, c.x.device());
+        if (c.residual.defined()) s = empty_like_shape(c.x.sizes(), c.x.scalar_type(), c.x.device());
+        check(th_rms_norm_int8(ptr(c.x), c.xr.stride, ptr(c.residual), c.rr.stride, ptr(c.gain), c.gain_code, ptr(s), ptr(q), pitch16(c.d),
+                               static_cast<float *>(ptr(scale)), c.xr.n, static_cast<int>(c.d), c.eps, c.code, current_stream()),
+              "th_rms_norm_int8");
+    }
+    const bool added = s.defined();
+    PyObject *a = THPVariable_Wrap(std::move(q)), *b = THPVariable_Wrap(std::move(scale));
+    return pair_of(a, b, added ? THPVariable_Wrap(std::move(s)) : nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
+// A matrix of 8-bit rows as the products take them
+bool int8_rows(const Tensor &q, const Tensor &scale, Rows &r) {
+    if (!plain(q) || !plain(scale) || q.scalar_type() != at::kChar || scale.scalar_type() != at::kFloat || q.dim() < 1 || q.numel() == 0) return false;
+    if (!scale.is_contiguous() || scale.device() != q.device() || scale.sizes() != q.sizes().slice(0, q.dim() - 1)) return false;
+    const int64_t width = q.size(-1);
+    r.keep = q;
+    r.n = q.numel() / width;
+    r.stride = pitch16(width);
+    if (reinterpret_cast<uintptr_t>(ptr(q)) % 16 || (width > 1 && q.stride(-1) != 1)) return false;
+    if (r.n > 1) {  // evenly spaced rows
+        int64_t step = 0;
+        for (int64_t k = q.dim() - 2; k >= 0; --k) {
+            if (q.size(k) == 1) continue;
+            if (step == 0) r.stride = q.stride(k);
+            else if (q.stride(k) != step) return false;
+            step = q.stride(k) * q.size(k);
+        }
+    }
+    return r.stride % 16 == 0 && r.stride >= width;
+}
+
+// int8_linear(x, q, scale, weight q, weight scale, bias, dtype): x a float tensor or None, otherwise q and scale are None
+PyObject *py_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Tensor x, q, scale, wq, w_scale, bias;
+    if (n_args != 7 || !usual_mode() || !take(args[0], x) || !take(args[1], q) || !take(args[2], scale) || !take(args[3], wq) || !take(args[4], w_scale) ||
+        !take(args[5], bias) || !(args[6] == Py_None || THPDtype_Check(args[6])))
+        TH_NOT_MINE;
+    Rows w, rows;
+    if (!wq.defined() || wq.dim() != 2 || !int8_rows(wq, w_scale, w)) TH_NOT_MINE;
+    const int64_t d_out = wq.size(0), d_in = wq.size(1);
+    if (d_in > 131071) TH_NOT_MINE;
+    int x_code = TH_F32;
+    if (x.defined()) {
+        if (q.defined() || !plain(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) != d_in || !float_code(x, x_code) || x.device() != wq.device() ||
+            !rows_of(x, d_in, rows))
+            TH_NOT_MINE;
+    } else if (args[6] == Py_None || !q.defined() || q.size(-1) != d_in || q.device() != wq.device() || !int8_rows(q, scale, rows)) {
+        TH_NOT_MINE;
+    }
+    const at::ScalarType type = args[6] == Py_None ? x.scalar_type() : reinterpret_cast<THPDtype *>(args[6])->scalar_type;
+    const int code = dtype_code(type);
+    if (code < 0 || (bias.defined() && (!plain(bias) || bias.dim() != 1 || bias.size(0) != d_out || !bias.is_contiguous() || bias.scalar_type() != type ||
+                                        bias.device() != wq.device())))
+        TH_NOT_MINE;
+    if (torch::autograd::compute_requires_grad(x, bias)) TH_NOT_MINE;
+    Tensor y;
+    {
+        NoGil release;
+        at::AutoDispatchBelowADInplaceOrView below;
+        c10::cuda::CUDAGuard guard(wq.device());
+        c10::SmallVector<int64_t, 6> shape((x.defined() ? x : q).sizes().begin(), (x.defined() ? x : q).sizes().end());
+        shape.back() = d_out;
+        y = empty_like_shape(shape, type, wq.device());
+        const int di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+        // one buffer: the rows in 8 bits, their scales, and the product's scratch
+        const int64_t pitch = pitch16(d_in), scratch = th_int8_linear_workspace_bytes(rows.n, di, dn);
+        const int64_t held = x.defined() ? rows.n * pitch : 0, scales = x.defined() ? pitch16(4 * rows.n) : 0;
+        const Tensor buffer = held + scratch ? empty_like_shape({held + scales + scratch}, at::kByte, wq.device()) : Tensor();
+        char *base = static_cast<char *>(ptr(buffer));
+        const void *qp = x.defined() ? base : ptr(q);
+        float *sp = x.defined() ? reinterpret_cast<float *>(base + held) : static_cast<float *>(ptr(scale));
+        if (x.defined())
+            check(th_quantize_rows(ptr(x), rows.stride, base, pitch, sp, rows.n, di, x_code, current_stream()), "th_quantize_rows");
+        check(th_int8_linear(qp, x.defined() ? pitch : rows.stride, sp, ptr(wq), w.stride, static_cast<const float *>(ptr(w_scale)), ptr(bias), ptr(y), d_out,
+                             scratch ? base + held + scales : nullptr, scratch, rows.n, di, dn, code, current_stream()),
+              "th_int8_linear");
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// Rows of a 16-bit product's operand: they start on 16 bytes; a padded copy where they do not
+Rows operand_rows(const Tensor &t, int64_t width) {
+    Rows r;
+    if (rows_of(t, width, r)) {
+        if (r.n <= 1) r.stride = (width + 7) / 8 * 8;
+        if (r.stride % 8 == 0 && reinterpret_cast<uintptr_t>(ptr(t)) % 16 == 0) return r;
+    }
+    r.n = t.numel() / width;
+    r.stride = (width + 7) / 8 * 8;
+    r.keep = empty_like_shape({r.n, r.stride}, t.scalar_type(), t.device());
+    r.keep.narrow(1, 0, width).copy_(t.reshape({r.n, width}));
+    return r;
+}
+
+struct CheckpointedLinearNode : public Node {
+    SavedVariable weight, q, scale;
+    int64_t rows = 0, d_in = 0, d_out = 0;
+    c10::SmallVector<int64_t, 6> shape;
+    at::ScalarType type = at::kHalf;
+    bool keeps_weight = false, keeps_rows = false;
+
+    std::string name() const override { return "CheckpointedLinearBackward"; }
+    void release_variables() override {
+        weight.reset_data();
+        q.reset_data();
+        scale.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        Tensor w, q8, s;
+        if (keeps_weight) w = weight.unpack();
+        if (keeps_rows) {
+            q8 = q.unpack();
+            s = scale.unpack();
+        }
+        at::NoGradGuard no_grad;
+        c10::cuda::CUDAGuard guard(grads[0].device());
+        const c10::Device device = grads[0].device();
+        void *stream = current_stream();
+        const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+        const Rows gy = operand_rows(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
+        const bool wants_x = keeps_weight && task_should_compute_output(0), wants_w = keeps_rows && task_should_compute_output(1);
+        const bool wants_b = task_should_compute_output(2);
+        const int64_t scratch = std::max(wants_x || wants_w ? th_linear_workspace_bytes(rows, di, dn) : 0, wants_b ? th_column_sum_workspace_bytes(rows, dn) : 0);
+        const Tensor workspace = scratch ? empty_like_shape({scratch}, at::kByte, device) : Tensor();
+        if (wants_x) {
+            const Rows wr = operand_rows(same(w, type, d_in * d_out), d_in);
+            out[0] = empty_like_shape(shape, type, device);
+            check(th_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(wr.keep), wr.stride, ptr(out[0]), d_in, ptr(workspace), scratch, rows, di, dn, code, stream),
+                  "th_linear_bwd_input");
+        }
+        if (wants_w) {
+            const int64_t pitch = pitch16(d_in);
+            q8 = restored(q8, at::kChar, rows * pitch);
+            s = restored(s, at::kFloat, rows);
+            const int64_t stride = (d_in + 7) / 8 * 8;
+            const Tensor x8 = empty_like_shape({rows, stride}, type, device);
+            check(th_dequantize_rows(ptr(q8), pitch, s.data_ptr<float>(), ptr(x8), stride, rows, di, code, stream), "th_dequantize_rows");
+            out[1] = empty_like_shape({d_out, d_in}, type, device);
+            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(x8), stride, ptr(out[1]), ptr(workspace), scratch, rows, di, dn, code, stream),
+                  "th_linear_bwd_weight");
+        }
+        if (wants_b) {
+            out[2] = empty_like_shape({d_out}, type, device);
+            check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), ptr(workspace), scratch, rows, dn, code, stream), "th_column_sum");
+        }
+        return out;
+    }
+};
+
+// checkpointed_linear(x, weight, bias)
+PyObject *py_checkpointed_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Tensor x, w, b;
+    if (n_args != 3 || !usual_mode() || !take(args[0], x) || !take(args[1], w) || !take(args[2], b)) TH_NOT_MINE;
+    if (!plain(x) || !plain(w) || w.dim() != 2 || w.numel() == 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) != w.size(1)) TH_NOT_MINE;
+    const at::ScalarType type = x.scalar_type();
+    const int64_t d_out = w.size(0), d_in = w.size(1);
+    if ((type != at::kHalf && type != at::kBFloat16) || w.scalar_type() != type || w.device() != x.device()) TH_NOT_MINE;
+    if (b.defined() && !parameter_like(b, x, {d_out})) TH_NOT_MINE;
+    Tensor y;
+    {
+        NoGil release;
+        const bool grad = torch::autograd::compute_requires_grad(x, w, b);
+        const bool keeps_rows = grad && w.requires_grad();
+        std::shared_ptr<CheckpointedLinearNode> node;
+        if (grad) node = make_node<CheckpointedLinearNode>(torch::autograd::collect_next_edges(x, w, b));
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            c10::cuda::CUDAGuard guard(x.device());
+            void *stream = current_stream();
+            const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+            const Rows xr = operand_rows(x, d_in), wr = operand_rows(w, d_in);
+            c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+            shape.back() = d_out;
+            y = empty_like_shape(shape, type, x.device());
+            const int64_t scratch = th_linear_workspace_bytes(xr.n, di, dn);
+            const Tensor workspace = scratch ? empty_like_shape({scratch}, at::kByte, x.device()) : Tensor();
+            check(th_linear_fwd(ptr(xr.keep), xr.stride, ptr(wr.keep), wr.stride, ptr(b), ptr(y), d_out, ptr(workspace), scratch, xr.n, di, dn, code, stream),
+                  "th_linear_fwd");
+            if (grad) {
+                node->rows = xr.n;
+                node->d_in = d_in;
+                node->d_out = d_out;
+                node->type = type;
+                node->shape.assign(x.sizes().begin(), x.sizes().end());
+                node->keeps_weight = x.requires_grad();
+                node->keeps_rows = keeps_rows;
+            }
+            if (keeps_rows) {
+                const int64_t pitch = pitch16(d_in);
+                const Tensor q8 = empty_like_shape({xr.n, pitch}, at::kChar, x.device()), s = empty_like_shape({xr.n}, at::kFloat, x.device());
+                check(th_quantize_rows(ptr(xr.keep), xr.stride, ptr(q8), pitch, s.data_ptr<float>(), xr.n, di, code, stream), "th_quantize_rows");
+                node->q = SavedVariable(q8, false);
+                node->scale = SavedVariable(s, false);
+            }
+        }
+        if (grad) {
+            if (node->keeps_weight) node->weight = SavedVariable(w, false);
+            torch::autograd::set_history(y, node);
+        }
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- module -------------------------------------------------------------------------------------------------
 
 // configure(level_geometry, host_primes): the package's Python helpers this module asks for geometry and primes
@@ -1273,7 +1646,7 @@ PyObject *py_defer(PyObject *, PyObject *flag) {
 #define TH_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
     TH_FAST(hash_encoding), TH_FAST(fully_fused_mlp), TH_FAST(reversible_mlp), TH_FAST(hash_encoded_mlp), TH_FAST(adam_steps),
-    TH_FAST(train_gradients), TH_FAST(configure),
+    TH_FAST(train_gradients), TH_FAST(configure), TH_FAST(rms_norm), TH_FAST(rms_norm_int8), TH_FAST(int8_linear), TH_FAST(checkpointed_linear),
     {"defer", py_defer, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

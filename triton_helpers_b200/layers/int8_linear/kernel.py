@@ -133,7 +133,11 @@ def int8_linear(
     Shapes:
         - x: :math:`(..., D_{in})`, output: :math:`(..., D_{out})`, bias: :math:`(D_{out},)`
     """
-    if isinstance(x, Int8Rows):
+    held = isinstance(x, Int8Rows)
+    out = _lib.native().int8_linear(None if held else x, *(x if held else (None, None)), *weight, bias, dtype)
+    if out is not NotImplemented:
+        return out
+    if held:
         if dtype is None:
             raise TypeError("8-bit rows do not say the type of the result: pass dtype")
         refuse_gradients("int8_linear", bias)

@@ -106,6 +106,9 @@ def rms_norm(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, eps: 
     Shapes:
         - x, residual, outputs: :math:`(..., D)`, weight: :math:`(D,)`
     """
+    out = _lib.native().rms_norm(x, weight, residual, eps)
+    if out is not NotImplemented:
+        return out
     return _rms_norm.apply(x, weight, residual, float(eps))
 
 
@@ -113,6 +116,9 @@ def rms_norm_int8(
     x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, eps: float = 1e-6
 ) -> Union[Int8Rows, Tuple[Int8Rows, Tensor]]:
     r"""``rms_norm`` with 8-bit rows as its output, for ``int8_linear``: ``rows``, or ``(rows, x + residual)``.  No gradient."""
+    out = _lib.native().rms_norm_int8(x, weight, residual, eps)
+    if out is not NotImplemented:
+        return Int8Rows(*out) if residual is None else (Int8Rows(out[0], out[1]), out[2])
     refuse_gradients("rms_norm_int8", x, weight, residual)
     with torch.no_grad():
         d = _validate(x, weight, residual)
