@@ -434,25 +434,21 @@ int th_column_sum(const void *g_dev, int64_t g_stride, void *out_dev, void *work
 
 /* y[r, n] = scale[r] * weight_scale[n] * sum_k q[r, k] weight[n, k] + bias[n]: 8-bit rows on both sides, exact
  * 32-bit integer sums (d_in up to 131071), y and bias in `dtype`; the bias may be null. */
-int64_t th_int8_linear_workspace_bytes(int64_t rows, int d_in, int d_out);
 int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev,
                    int64_t weight_stride, const float *weight_scale_dev, const void *bias_dev, void *y_dev,
-                   int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
-                   int d_out, int dtype, void *stream);
+                   int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, void *stream);
 
 /* The products of a linear layer in 16 bits with float32 sums: y = x w^T + b, grad_x = grad_y w and
  * grad_w = grad_y^T x (contiguous).  Operand rows start on 16 bytes (pointer and stride); outputs may lie anywhere.
- * One size of scratch covers the three.  Results repeat bit for bit. */
-int64_t th_linear_workspace_bytes(int64_t rows, int d_in, int d_out);
+ * Results repeat bit for bit. */
 int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *weight_dev, int64_t weight_stride,
-                  const void *bias_dev, void *y_dev, int64_t y_stride, void *workspace_dev,
-                  int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+                  const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out,
+                  int dtype, void *stream);
 int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *weight_dev,
-                        int64_t weight_stride, void *grad_x_dev, int64_t gx_stride, void *workspace_dev,
-                        int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+                        int64_t weight_stride, void *grad_x_dev, int64_t gx_stride, int64_t rows, int d_in,
+                        int d_out, int dtype, void *stream);
 int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
-                         void *grad_weight_dev, void *workspace_dev, int64_t workspace_bytes, int64_t rows,
-                         int d_in, int d_out, int dtype, void *stream);
+                         void *grad_weight_dev, int64_t rows, int d_in, int d_out, int dtype, void *stream);
 
 /* Device-side status word of these products (0 = fine, 1 = a bounded wait ran out and results are invalid).
  * Synchronises the device. */

@@ -165,10 +165,8 @@ def test_results_repeat_and_memory_behind_is_left():
     assert all(torch.equal(first, int8_linear(x, weight)) for _ in range(5))
     lib, rows = _lib.lib(), quantize_rows(x[:20])
     held = torch.full((22, 80), 7.0, device="cuda")  # rows and columns behind the result stay as they are
-    size = lib.th_int8_linear_workspace_bytes(20, 3000, 70)
-    scratch = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
     _lib.check(lib.th_int8_linear(rows.q.data_ptr(), rows.q.stride(0), rows.scale.data_ptr(), weight.q.data_ptr(), weight.q.stride(0), weight.scale.data_ptr(),
-                                  None, held.data_ptr(), 80, scratch.data_ptr(), size, 20, 3000, 70, 0, _lib.stream_ptr(x.device)), "th_int8_linear")  # fmt: skip
+                                  None, held.data_ptr(), 80, 20, 3000, 70, 0, _lib.stream_ptr(x.device)), "th_int8_linear")  # fmt: skip
     assert bool((held[20:] == 7).all()) and bool((held[:, 70:] == 7).all())
     assert_linear(held[:20, :70], rows, weight, None)
 

@@ -163,25 +163,13 @@ SIGNATURES = {
     "th_dequantize_rows": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
     "th_column_sum_workspace_bytes": (c_int64, [c_int64, c_int]),
     "th_column_sum": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
-    "th_int8_linear_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
     "th_int8_linear": (
         c_int,
-        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
-         c_int, c_void_p],
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p],
     ),
-    "th_linear_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
-    "th_linear_fwd": (
-        c_int,
-        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p],
-    ),
-    "th_linear_bwd_input": (
-        c_int,
-        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p],
-    ),
-    "th_linear_bwd_weight": (
-        c_int,
-        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p],
-    ),
+    "th_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
+    "th_linear_bwd_input": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
+    "th_linear_bwd_weight": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
     "th_linear_tc_status": (c_int, []),
 }  # fmt: skip
 

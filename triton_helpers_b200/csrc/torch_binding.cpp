@@ -26,7 +26,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
-#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <strings.h>
@@ -1478,17 +1477,16 @@ PyObject *py_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         shape.back() = d_out;
         y = empty_like_shape(shape, type, wq.device());
         const int di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
-        // one buffer: the rows in 8 bits, their scales, and the product's scratch
-        const int64_t pitch = pitch16(d_in), scratch = th_int8_linear_workspace_bytes(rows.n, di, dn);
-        const int64_t held = x.defined() ? rows.n * pitch : 0, scales = x.defined() ? pitch16(4 * rows.n) : 0;
-        const Tensor buffer = held + scratch ? empty_like_shape({held + scales + scratch}, at::kByte, wq.device()) : Tensor();
+        // one buffer: the rows in 8 bits and their scales
+        const int64_t pitch = pitch16(d_in), scales = pitch16(4 * rows.n);
+        const Tensor buffer = x.defined() ? empty_like_shape({rows.n * pitch + scales}, at::kByte, wq.device()) : Tensor();
         char *base = static_cast<char *>(ptr(buffer));
         const void *qp = x.defined() ? base : ptr(q);
-        float *sp = x.defined() ? reinterpret_cast<float *>(base + held) : static_cast<float *>(ptr(scale));
+        float *sp = x.defined() ? reinterpret_cast<float *>(base + rows.n * pitch) : static_cast<float *>(ptr(scale));
         if (x.defined())
             check(th_quantize_rows(ptr(x), rows.stride, base, pitch, sp, rows.n, di, x_code, current_stream()), "th_quantize_rows");
         check(th_int8_linear(qp, x.defined() ? pitch : rows.stride, sp, ptr(wq), w.stride, static_cast<const float *>(ptr(w_scale)), ptr(bias), ptr(y), d_out,
-                             scratch ? base + held + scales : nullptr, scratch, rows.n, di, dn, code, current_stream()),
+                             rows.n, di, dn, code, current_stream()),
               "th_int8_linear");
     }
     return THPVariable_Wrap(std::move(y));
@@ -1539,12 +1537,10 @@ struct CheckpointedLinearNode : public Node {
         const Rows gy = operand_rows(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
         const bool wants_x = keeps_weight && task_should_compute_output(0), wants_w = keeps_rows && task_should_compute_output(1);
         const bool wants_b = task_should_compute_output(2);
-        const int64_t scratch = std::max(wants_x || wants_w ? th_linear_workspace_bytes(rows, di, dn) : 0, wants_b ? th_column_sum_workspace_bytes(rows, dn) : 0);
-        const Tensor workspace = scratch ? empty_like_shape({scratch}, at::kByte, device) : Tensor();
         if (wants_x) {
             const Rows wr = operand_rows(same(w, type, d_in * d_out), d_in);
             out[0] = empty_like_shape(shape, type, device);
-            check(th_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(wr.keep), wr.stride, ptr(out[0]), d_in, ptr(workspace), scratch, rows, di, dn, code, stream),
+            check(th_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(wr.keep), wr.stride, ptr(out[0]), d_in, rows, di, dn, code, stream),
                   "th_linear_bwd_input");
         }
         if (wants_w) {
@@ -1555,11 +1551,13 @@ struct CheckpointedLinearNode : public Node {
             const Tensor x8 = empty_like_shape({rows, stride}, type, device);
             check(th_dequantize_rows(ptr(q8), pitch, s.data_ptr<float>(), ptr(x8), stride, rows, di, code, stream), "th_dequantize_rows");
             out[1] = empty_like_shape({d_out, d_in}, type, device);
-            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(x8), stride, ptr(out[1]), ptr(workspace), scratch, rows, di, dn, code, stream),
+            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(x8), stride, ptr(out[1]), rows, di, dn, code, stream),
                   "th_linear_bwd_weight");
         }
         if (wants_b) {
             out[2] = empty_like_shape({d_out}, type, device);
+            const int64_t scratch = th_column_sum_workspace_bytes(rows, dn);
+            const Tensor workspace = empty_like_shape({scratch}, at::kByte, device);
             check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), ptr(workspace), scratch, rows, dn, code, stream), "th_column_sum");
         }
         return out;
@@ -1592,9 +1590,7 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *args, Py_ssize_t n
             c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
             shape.back() = d_out;
             y = empty_like_shape(shape, type, x.device());
-            const int64_t scratch = th_linear_workspace_bytes(xr.n, di, dn);
-            const Tensor workspace = scratch ? empty_like_shape({scratch}, at::kByte, x.device()) : Tensor();
-            check(th_linear_fwd(ptr(xr.keep), xr.stride, ptr(wr.keep), wr.stride, ptr(b), ptr(y), d_out, ptr(workspace), scratch, xr.n, di, dn, code, stream),
+            check(th_linear_fwd(ptr(xr.keep), xr.stride, ptr(wr.keep), wr.stride, ptr(b), ptr(y), d_out, xr.n, di, dn, code, stream),
                   "th_linear_fwd");
             if (grad) {
                 node->rows = xr.n;

@@ -5,11 +5,17 @@
 // One persistent CTA per SM, or one pair of CTAs on one 256-row tile (cta_group::2).  Warp 0 brings operand boxes by TMA through a ring
 // of stages, warp 1 issues the MMAs, warps 4 to 7 empty one accumulator while the next tile fills the other.  Every operand
 // tile has rows of 128 bytes in the 128-byte swizzle: K-major as one box of 128 bytes x rows, MN-major as boxes of 64 columns x 64 K rows.
+//
+// What bounds a tile is its operands' way into the SM, 64 bytes a cycle: a K step of 128 bytes takes a 128 x 128 tile of one CTA 512
+// cycles (its MMAs 256), a 256 x 256 tile of a pair, which share the columns' operand, 512 as well (its MMAs 512).
+//
+// Few tiles: K is split over the CTAs of a cluster (up to eight), a tile a cluster.  Each leaves its sums in its shared memory and
+// finishes a part of the tile from everybody's, added in rank order, so that there is no scratch, no second launch, and results repeat.
 #pragma once
 
 #include "tc_tiles.cuh"
 
-#include <atomic>
+#include <algorithm>
 
 namespace th {
 namespace {
@@ -25,28 +31,29 @@ struct GemmArgs {
     int m, n, tiles_m, tiles_n, k_tiles, splits, tiles_per_split;
     uint32_t idesc;
     void *out;             // [m][out_stride], or [n][out_stride] where the product is transposed
-    long long out_stride, split_stride;
-    int out_dtype;         // kRaw32: the sums themselves, 32 bits each
+    long long out_stride;
+    int out_dtype;
     int out_tma;
     const float *lane_scale, *column_scale;  // along m and along n
     const void *bias;      // along n (along m where transposed)
     int bias_dtype;
 };
-constexpr int kRaw32 = 100;
 
-template <int EB, bool A_MN, bool B_MN, int BN, int CG>
+// CTAS: CTAs that share an SM
+template <int EB, bool A_MN, bool B_MN, int BN, int CG, int CTAS>
 struct GemmShape {
     static constexpr int kK = 128 / EB;  // K elements of a stage
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
-    static constexpr int kFixed = 4 * kStagingBoxes * kStagingBytes;
-    static constexpr int kSmem = 226 * 1024 - 2 * 2 * BN * 4;  // the scales and barriers are beside it
+    static constexpr int kFixed = CTAS == 1 ? 4 * kStagingBoxes * kStagingBytes : 0;  // transposed outputs have no staging
+    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * 2 * BN * 4;     // the scales and barriers are beside it
     static constexpr int kFit = (kSmem - kFixed - 1024) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kBytes = kStages * kStage + kFixed + 1024;
     static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr bool kSplits = kGemmRows * BN * 4 <= kStages * kStage;  // a tile's sums fit where the operands were
     static_assert(!(A_MN || B_MN) || EB == 2, "8-bit operands are K-major");
-    static_assert(kStages >= 3 && kTmemCols <= 512, "tile does not fit");
+    static_assert(kStages >= 3 && CTAS * kTmemCols <= 512, "tile does not fit");
 };
 
 // kind::i8 instruction descriptor: signed 8-bit operands, 32-bit integer sums
@@ -103,12 +110,12 @@ __device__ __forceinline__ void gemm_load(uint32_t dst, const CUtensorMap *map, 
 
 // The barrier at this offset in every CTA of the tile completes a phase once the MMAs issued so far have finished
 template <int CG>
-__device__ __forceinline__ void gemm_commit(uint32_t mbar) {
+__device__ __forceinline__ void gemm_commit(uint32_t mbar, uint32_t leader) {
     if constexpr (CG == 1)
         mma_commit(mbar);
     else
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mbar),
-                     "h"(static_cast<unsigned short>(3)) : "memory");
+                     "h"(static_cast<unsigned short>(3u << leader)) : "memory");
 }
 
 // Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.
@@ -161,42 +168,127 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int dtype) {
     return dtype == TH_F16 ? pack_pair<__half>(lo, hi) : pack_pair<__nv_bfloat16>(lo, hi);
 }
 
-// The 32 rows x 128 bytes that a warp has put into its staging box -> rows m0.., columns c0.. of the output
-__device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *c_map, unsigned char *out, uint32_t box, int m0, int c0, int out_bytes) {
+// The 32 rows x 128 bytes that a warp has put into its staging box -> rows m0.., columns c0.. of the output.  Where rows do not start on
+// 16 bytes a warp writes a row at a time, a word a lane, or two halves: eight rows are read ahead of their stores (3001 x 777 outputs of
+// 1000 bfloat16 products: STOREFIG).
+template <typename V, int PER>
+__device__ __forceinline__ void copy_rows(unsigned char *to, long long pitch, uint32_t box, int rows, int cols) {
     const int lane = threadIdx.x & 31;
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        V v[8][PER];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const int at = (lane + 32 * e) * static_cast<int>(sizeof(V));
+                const uint32_t from = box + (r0 + r) * 128 + ((((at >> 4) ^ r) << 4) | (at & 15));
+                if constexpr (sizeof(V) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r][e]) : "r"(from) : "memory");
+                else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v[r][e]) : "r"(from) : "memory");
+            }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                if (r0 + r < rows && lane + 32 * e < cols) reinterpret_cast<V *>(to + (r0 + r) * pitch)[lane + 32 * e] = v[r][e];
+    }
+}
+
+__device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *c_map, uint32_t box, int m0, int c0, int out_bytes) {
     if (g.out_tma) {
         fence_async_smem();
         __syncwarp();
-        if (lane == 0 && m0 < g.m && c0 < g.n) tma_store_2d(c_map, box, c0, m0);
+        if ((threadIdx.x & 31) == 0 && m0 < g.m && c0 < g.n) tma_store_2d(c_map, box, c0, m0);
         return;
     }
     __syncwarp();
     const int cols = min(128 / out_bytes, g.n - c0), rows = min(32, g.m - m0);
-    for (int r = 0; r < rows; ++r) {
-        unsigned char *to = out + (static_cast<long long>(m0 + r) * g.out_stride + c0) * out_bytes;
-        for (int c = lane; c < cols; c += 32) {
-            const int at = c * out_bytes;
-            const uint32_t from = box + r * 128 + ((((at >> 4) ^ (r & 7)) << 4) | (at & 15));
-            if (out_bytes == 4) {
-                uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-                reinterpret_cast<uint32_t *>(to)[c] = v;
-            } else {
-                unsigned short v;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-                reinterpret_cast<unsigned short *>(to)[c] = v;
-            }
-        }
-    }
+    const long long pitch = g.out_stride * out_bytes;
+    unsigned char *to = static_cast<unsigned char *>(g.out) + m0 * pitch + static_cast<long long>(c0) * out_bytes;
+    if (out_bytes == 4) copy_rows<uint32_t, 1>(to, pitch, box, rows, cols);
+    else if (pitch % 4 == 0 && cols % 2 == 0 && (reinterpret_cast<uintptr_t>(to) & 3) == 0) copy_rows<uint32_t, 1>(to, pitch, box, rows, cols / 2);
+    else copy_rows<unsigned short, 2>(to, pitch, box, rows, cols);
     __syncwarp();
 }
 
+// One result from its sum
+template <int EB>
+__device__ __forceinline__ float finished(uint32_t raw, float scale, float bias) {
+    if constexpr (EB == 1) return static_cast<float>(static_cast<int>(raw)) * scale + bias;
+    else return __uint_as_float(raw) + bias;
+}
+
+__device__ __forceinline__ void store_one(void *out, long long at, float v, int dtype) {
+    if (dtype == TH_F32) static_cast<float *>(out)[at] = v;
+    else if (dtype == TH_F16) static_cast<__half *>(out)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(v);
+}
+
+// Sums of a split tile in shared memory, in pieces of four along the output's rows: `line` is an output row of the tile, `piece` four of
+// its columns.  Writers have 32 lines (or, transposed, one line and 32 columns) a warp, readers one line: the swizzle serves both.
+template <int PIECES>
+__device__ __forceinline__ uint32_t exchange_at(uint32_t base, int line, int piece) {
+    return base + (line * PIECES + (piece ^ (line & (PIECES < 8 ? PIECES - 1 : 7)))) * 16;
+}
+
+__device__ __forceinline__ uint4 ld_cluster_16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// This CTA's part of a split tile.  A read of another CTA's shared memory takes some 600 cycles, so PIECES_AT_ONCE x RANKS (16) of them are
+// on their way together.
+template <int EB, int BN, int CG, bool SWAP, int PIECES_AT_ONCE, int RANKS>
+__device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &u, uint32_t rank, uint32_t smem, const float *scales, const float *biases) {
+    constexpr int kPieces = SWAP ? kGemmRows / 4 : BN / 4;
+    const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN, rows = max(0, min(kGemmRows, g.m - m0)), cols = min(BN, g.n - n0);
+    const int lines = SWAP ? cols : rows, along = SWAP ? rows : cols, total = lines * kPieces;
+    const int from = total * u.split / g.splits, to = total * (u.split + 1) / g.splits;
+    for (int first = from + static_cast<int>(threadIdx.x); first < to; first += PIECES_AT_ONCE * kGemmThreads) {
+        uint4 v[PIECES_AT_ONCE][RANKS];
+#pragma unroll
+        for (int p = 0; p < PIECES_AT_ONCE; ++p) {
+            const int i = first + p * kGemmThreads;
+            if (i < to) {
+                const uint32_t at = exchange_at<kPieces>(smem, i / kPieces, i % kPieces);
+#pragma unroll
+                for (int r = 0; r < RANKS; ++r)
+                    if (r < g.splits) v[p][r] = ld_cluster_16(in_cta(at, CG * r + rank));
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PIECES_AT_ONCE; ++p) {
+            const int i = first + p * kGemmThreads, line = i / kPieces, piece = i % kPieces;
+            if (i >= to || 4 * piece >= along) continue;
+            uint32_t sum[4] = {v[p][0].x, v[p][0].y, v[p][0].z, v[p][0].w};
+#pragma unroll
+            for (int r = 1; r < RANKS; ++r) {
+                if (r < g.splits) {
+                    const uint32_t part[4] = {v[p][r].x, v[p][r].y, v[p][r].z, v[p][r].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = EB == 1 ? sum[e] + part[e] : __float_as_uint(__uint_as_float(sum[e]) + __uint_as_float(part[e]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = 4 * piece + e;
+                if (c >= along) break;
+                const int mi = m0 + (SWAP ? c : line), ni = SWAP ? line : c;
+                const float scale = EB == 1 ? (g.lane_scale ? g.lane_scale[mi] : 1.f) * scales[ni] : 1.f;
+                const float bias = SWAP ? (g.bias ? bias_at(g.bias, g.bias_dtype, mi) : 0.f) : biases[ni];
+                store_one(g.out, SWAP ? static_cast<long long>(n0 + line) * g.out_stride + mi : static_cast<long long>(m0 + line) * g.out_stride + n0 + c,
+                          finished<EB>(sum[e], scale, bias), g.out_dtype);
+            }
+        }
+    }
+}
+
 // SWAP: the output is C transposed (A's rows are its columns): few tokens, with the weights on the accumulator's rows.
-template <int EB, bool A_MN, bool B_MN, int BN, int CG, bool SWAP>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+template <int EB, bool A_MN, bool B_MN, int BN, int CG, bool SWAP, int CTAS>
+__global__ void __launch_bounds__(kGemmThreads, CTAS)
 wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
                  const __grid_constant__ CUtensorMap c_map) {
-    using S = GemmShape<EB, A_MN, B_MN, BN, CG>;
+    using S = GemmShape<EB, A_MN, B_MN, BN, CG, CTAS>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
     __shared__ float scales[2][BN], biases[2][BN];
@@ -204,9 +296,14 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     __shared__ int abort_flag;
     const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    // within the tile: the pair's first CTA leads; the cluster holds one tile's CTAs for every part of K
+    const uint32_t place = CG == 2 ? cluster_rank() : 0, rank = place % CG, leader = place - rank;
     const int units = g.tiles_m * g.tiles_n * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&b_map)) : "memory");
+    }
     if (threadIdx.x == 0) {
         abort_flag = 0;
         const auto init = [](unsigned long long *bar, uint32_t count) {
@@ -249,7 +346,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                 ok = gemm_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
                 if (!ok) break;
                 if (elect_one()) {
-                    const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, 0) : mine;
+                    const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
                     if (rank == 0)
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
                     const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
@@ -292,45 +389,39 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         gemm_mma<EB, CG>(d, gemm_desc<A_MN>(a + k * a_step), gemm_desc<B_MN>(b + k * b_step), g.idesc, (kt > u.k0 || k > 0) ? 1u : 0u);
-                    gemm_commit<CG>(smem_addr(&empty[s]));
-                    if (kt == u.k1 - 1) gemm_commit<CG>(smem_addr(&acc_full[buf]));
+                    gemm_commit<CG>(smem_addr(&empty[s]), leader);
+                    if (kt == u.k1 - 1) gemm_commit<CG>(smem_addr(&acc_full[buf]), leader);
                 }
                 __syncwarp();
             }
         }
     } else if (warp >= 4) {
         // ---- sums -> output ----
-        const int quarter = warp & 3, out_bytes = g.out_dtype == TH_F32 || g.out_dtype == kRaw32 ? 4 : 2;
+        const int quarter = warp & 3, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
         const uint32_t staging = smem + S::kStages * S::kStage + quarter * kStagingBoxes * kStagingBytes;
+        constexpr int kStep = BN < 32 ? BN : 32;
         int done = 0, box = 0;
         for (int unit = first; unit < units; unit += step, ++done) {
             const GemmUnit u = gemm_unit(g, unit);
             const int buf = done & 1;
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter, n0 = u.tn * BN, m = m0 + lane;
-            const bool finish = g.out_dtype != kRaw32;
-            unsigned char *out = static_cast<unsigned char *>(g.out) + u.split * g.split_stride;
             float lane_scale = 1.f, lane_bias = 0.f;
-            if (finish) {
-                if (g.lane_scale) lane_scale = m < g.m ? g.lane_scale[m] : 0.f;
-                if (SWAP && g.bias) lane_bias = m < g.m ? bias_at(g.bias, g.bias_dtype, m) : 0.f;
-                // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
-                for (int c = threadIdx.x - 128; c < BN; c += 128) {
-                    const bool inside = n0 + c < g.n;
-                    scales[buf][c] = g.column_scale && inside ? g.column_scale[n0 + c] : 1.f;
-                    biases[buf][c] = !SWAP && g.bias && inside ? bias_at(g.bias, g.bias_dtype, n0 + c) : 0.f;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (g.lane_scale) lane_scale = m < g.m ? g.lane_scale[m] : 0.f;
+            if (SWAP && g.bias) lane_bias = m < g.m ? bias_at(g.bias, g.bias_dtype, m) : 0.f;
+            // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
+            for (int c = threadIdx.x - 128; c < BN; c += 128) {
+                const bool inside = n0 + c < g.n;
+                scales[buf][c] = g.column_scale && inside ? g.column_scale[n0 + c] : 1.f;
+                biases[buf][c] = !SWAP && g.bias && inside ? bias_at(g.bias, g.bias_dtype, n0 + c) : 0.f;
             }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
             if (!gemm_wait(smem_addr(&acc_full[buf]), (done >> 1) & 1, &abort_flag)) {
-                // the other warps' waits end too: they share the flag, and meet no barrier before they see it
-                if (finish) {
-                    for (unit += step; unit < units; unit += step) asm volatile("bar.sync 1, 128;" ::: "memory");
-                }
+                // the other warps' waits end too, but they may meet at the barriers of the units before
+                for (unit += step; unit < units; unit += step) asm volatile("bar.sync 1, 128;" ::: "memory");
                 break;
             }
             tc_fence_after();
             const uint32_t d = tmem + buf * BN + (static_cast<uint32_t>(32 * quarter) << 16);
-            constexpr int kStep = BN < 32 ? BN : 32;
 #pragma unroll 1
             for (int c0 = 0; c0 < BN; c0 += kStep) {
                 uint32_t raw[32];
@@ -343,31 +434,36 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                     __syncwarp();
                     if (lane == 0) {
                         if constexpr (CG == 2)
-                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), 0)) : "memory");
+                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), leader)) : "memory");
                         else
                             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
                     }
                 }
                 if (n0 + c0 >= g.n) continue;
-                if (finish) {
+                if constexpr (S::kSplits) {
+                    if (g.splits > 1) {  // the operands have been read: their shared memory takes the sums
+                        if constexpr (SWAP) {
 #pragma unroll
-                    for (int k = 0; k < kStep; ++k) {
-                        float v = EB == 1 ? static_cast<float>(static_cast<int>(raw[k])) : __uint_as_float(raw[k]);
-                        if (EB == 1) v = v * (lane_scale * scales[buf][c0 + k]);
-                        v += SWAP ? lane_bias : biases[buf][c0 + k];
-                        raw[k] = __float_as_uint(v);
+                            for (int k = 0; k < kStep; ++k)
+                                if (n0 + c0 + k < g.n)
+                                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(exchange_at<32>(smem, c0 + k, 8 * quarter + (lane >> 2)) + 4 * (lane & 3)), "r"(raw[k])
+                                                 : "memory");
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kStep / 4; ++j)
+                                st_shared_16(exchange_at<BN / 4>(smem, 32 * quarter + lane, c0 / 4 + j), make_uint4(raw[4 * j], raw[4 * j + 1], raw[4 * j + 2], raw[4 * j + 3]));
+                        }
+                        continue;
                     }
                 }
+#pragma unroll
+                for (int k = 0; k < kStep; ++k)
+                    raw[k] = __float_as_uint(finished<EB>(raw[k], lane_scale * scales[buf][c0 + k], SWAP ? lane_bias : biases[buf][c0 + k]));
                 if constexpr (SWAP) {
                     if (m < g.m) {
 #pragma unroll
-                        for (int k = 0; k < kStep; ++k) {
-                            if (n0 + c0 + k < g.n) {
-                                unsigned char *to = out + (static_cast<long long>(n0 + c0 + k) * g.out_stride + m) * out_bytes;
-                                if (out_bytes == 4) *reinterpret_cast<uint32_t *>(to) = raw[k];
-                                else *reinterpret_cast<unsigned short *>(to) = static_cast<unsigned short>(pack_out(__uint_as_float(raw[k]), 0.f, g.out_dtype));
-                            }
-                        }
+                        for (int k = 0; k < kStep; ++k)
+                            if (n0 + c0 + k < g.n) store_one(g.out, static_cast<long long>(n0 + c0 + k) * g.out_stride + m, __uint_as_float(raw[k]), g.out_dtype);
                     }
                 } else {
                     const uint32_t at = staging + (box % kStagingBoxes) * kStagingBytes + lane * 128;
@@ -381,7 +477,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
 #pragma unroll
                         for (int j = 0; j < kStep / 4; ++j)
                             st_shared_16(at + ((j ^ (lane & 7)) << 4), make_uint4(raw[4 * j], raw[4 * j + 1], raw[4 * j + 2], raw[4 * j + 3]));
-                        store_box(g, &c_map, out, at - lane * 128, m0, n0 + c0, 4);
+                        store_box(g, &c_map, at - lane * 128, m0, n0 + c0, 4);
                         ++box;
                     } else {
 #pragma unroll
@@ -393,7 +489,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                             st_shared_16(at + (((4 * half + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
                         }
                         if (half == 1 || n0 + c0 + 32 >= g.n) {
-                            store_box(g, &c_map, out, at - lane * 128, m0, n0 + (c0 & ~63), 2);
+                            store_box(g, &c_map, at - lane * 128, m0, n0 + (c0 & ~63), 2);
                             ++box;
                         }
                     }
@@ -403,6 +499,21 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
         if (!SWAP && g.out_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
 
+    if constexpr (S::kSplits) {
+        if (g.splits > 1) {
+            // ---- a split tile: this CTA's part of it, from everybody's sums ----
+            __syncwarp();
+            cluster_sync_all();
+            if (!abort_flag) {
+                const GemmUnit u = gemm_unit(g, first);
+                if (g.splits <= 2) finish_split<EB, BN, CG, SWAP, 8, 2>(g, u, rank, smem, scales[0], biases[0]);
+                else if (g.splits <= 4) finish_split<EB, BN, CG, SWAP, 4, 4>(g, u, rank, smem, scales[0], biases[0]);
+                else if constexpr (CG == 1) finish_split<EB, BN, CG, SWAP, 2, 8>(g, u, rank, smem, scales[0], biases[0]);
+            }
+            __syncwarp();
+            cluster_sync_all();  // everybody's sums have been read
+        }
+    }
     __syncthreads();
     if (abort_flag && threadIdx.x == 0) drain_copies(full, S::kStages);
     tc_fence_before();
@@ -437,13 +548,20 @@ struct Operand {
     int rows;          // extent along m or n
 };
 
-template <int EB, bool A_MN, bool B_MN, int BN, int CG, bool SWAP>
+template <int EB, bool A_MN, bool B_MN, int BN, int CG, bool SWAP, int CTAS>
 int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16, cudaStream_t stream) {
-    using S = GemmShape<EB, A_MN, B_MN, BN, CG>;
-    // first, because it makes the device's context current in this thread (an autograd thread may not have one yet), which the maps need
-    auto kernel = wide_gemm_kernel<EB, A_MN, B_MN, BN, CG, SWAP>;
-    if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "cudaFuncSetAttribute(wide_gemm_kernel)"))
-        return rc;
+    using S = GemmShape<EB, A_MN, B_MN, BN, CG, CTAS>;
+    auto kernel = wide_gemm_kernel<EB, A_MN, B_MN, BN, CG, SWAP, CTAS>;
+    // Once per thread and device, and ahead of the maps: it also makes the device's context current in this thread, which encoding
+    // a map needs and an autograd thread may not have yet.
+    static thread_local unsigned long long ready = 0;
+    int device = 0;
+    if (int rc = cuda_status(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+    if (device >= 64 || !(ready >> device & 1)) {
+        if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "cudaFuncSetAttribute(wide_gemm_kernel)"))
+            return rc;
+        if (device < 64) ready |= 1ull << device;
+    }
     CUtensorMap a_map, b_map, c_map;
     const auto operand = [&](CUtensorMap *map, const Operand &o, bool mn, int box_rows) {
         return mn ? matrix_map(map, o.base, o.rows, k, o.stride, EB, 64, 64) : matrix_map(map, o.base, k, o.rows, o.stride, EB, S::kK, box_rows);
@@ -458,23 +576,25 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     g.tiles_per_split = (g.k_tiles + g.splits - 1) / g.splits;
     g.splits = (g.k_tiles + g.tiles_per_split - 1) / g.tiles_per_split;
     g.idesc = EB == 1 ? instr_desc_i8(CG * kGemmRows, BN) : instr_desc(CG * kGemmRows, BN, bf16, A_MN, B_MN);
-    const int out_bytes = g.out_dtype == TH_F32 || g.out_dtype == kRaw32 ? 4 : 2;
+    const int out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
+    if (g.splits > (S::kSplits ? 8 / CG : 1)) return fail(TH_ERR_UNSUPPORTED, "matrix product: %d parts", g.splits);
     g.out_tma = !SWAP && g.splits == 1 && matrix_map(&c_map, g.out, g.n, g.m, g.out_stride, out_bytes, 128 / out_bytes, 32);
     if (!g.out_tma) c_map = a_map;  // not looked at
     const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "matrix product: too many tiles");
-    const int clusters = static_cast<int>(std::min<long long>(units, sm_count() / CG));
+    // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles
+    const long long clusters = g.splits > 1 ? units : std::min<long long>(units, CTAS * sm_count() / CG);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(clusters * CG);
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * CG));
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = S::kBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = CG;
+    attr.val.clusterDim.x = CG * g.splits;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = CG > 1 ? 1 : 0;
+    cfg.numAttrs = attr.val.clusterDim.x > 1 ? 1 : 0;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, g, a_map, b_map, c_map);
     note_launch();
     return cuda_status(err, "wide_gemm_kernel launch");

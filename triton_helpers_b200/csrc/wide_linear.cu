@@ -1,13 +1,11 @@
 // Linear layers of any width: 8-bit integers with a scale per token and per channel, and 16-bit products in the three forms that a
-// layer's forward and backward pass take.  The products are wide_gemm_kernel's; what is here chooses its tile and adds up split sums.
+// layer's forward and backward pass take.  The products are wide_gemm_kernel's; what is here chooses how they are cut.
 #include "wide_gemm.cuh"
-
-#include <algorithm>
 
 namespace th {
 namespace {
 
-// How a product is cut: tile width, CTAs per tile, transposed or not, and the parts that K is split into.
+// How a product is cut: tile width, CTAs per tile, transposed or not, and the parts that K is split into (within a cluster).
 struct ProductPlan {
     int bn, cg;
     bool swap;
@@ -16,79 +14,48 @@ struct ProductPlan {
 
 int divide_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Parts of K so that tiles x parts fill the GPU, each of at least `least` stages
-int split_count(long long tiles, int k_tiles, int least) {
-    const long long want = std::max(1ll, sm_count() / std::max(1ll, tiles));
-    const int parts = static_cast<int>(std::min<long long>(want, std::max(1, k_tiles / least)));
-    const int per = divide_up(k_tiles, parts);
-    return divide_up(k_tiles, per);
+// Clusters of `size` CTAs that run at one time, `per_sm` CTAs on an SM: what the runtime's occupancy query gives on a B200 (clusters stay
+// within a group of SMs, and groups differ), a little less where it is not even.
+int cluster_slots(int size, int per_sm) {
+    static const int one[8] = {148, 74, 44, 32, 25, 21, 14, 14}, two[8] = {296, 148, 90, 69, 54, 44, 36, 32};
+    return (per_sm == 1 ? one : two)[size - 1] * sm_count() / 148;
 }
 
+// The cheapest cut by an estimate in cycles: rounds of tiles x stages x cycles a stage (what its bytes take into the SM), what a pair
+// takes longer to start, and for split tiles the exchange of their sums.  All cuts measured on a B200, us (tile columns x CTAs x parts;
+// * is the one taken): 2048 x 2048 -> 2048 256x2x1* 17.9, 128x2x1 21, 128x1x1 26; 512 x 4096 -> 4096 128x2x1* 20.3, 256x2x2 21.9, 128x1x1
+// 25.5; gradient of 777 x 1000 weights from 3001 rows 128x2x2* 15.3, 128x1x2 16.5, 128x2x1 19.3, 256x2x1 24.6; of 512 x 512 weights from
+// 16384 rows 128x2x4* 22, 128x1x4 26, 256x2x1 79; 300 x 256 -> 512 128x1x1* 5.7, 128x2x1 6.8, 256x2x1 8.2.
 ProductPlan plan_product(int m, int n, int k, int elem_bytes) {
-    ProductPlan p{};
     const int k_tiles = divide_up(k, 128 / elem_bytes);
-    if (elem_bytes == 1 && m <= 128) {
-        p.swap = true;
-        p.cg = 1;
-        p.bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-        p.splits = split_count(divide_up(n, kGemmRows), k_tiles, 4);
-        return p;
+    ProductPlan best{};
+    double least = 0;
+    const auto consider = [&](int bn, int cg, bool swap, int per_sm, double stage, double exchange) {
+        const long long tiles = swap ? static_cast<long long>(divide_up(n, kGemmRows)) * divide_up(m, bn)
+                                     : static_cast<long long>(divide_up(m, cg * kGemmRows)) * divide_up(n, bn);
+        for (int s = 1; s * cg <= 8 && s <= k_tiles; ++s) {
+            const int per = divide_up(k_tiles, s);
+            if (divide_up(k_tiles, per) != s) continue;
+            const int slots = cluster_slots(s * cg, per_sm);
+            if (s > 1 && tiles > slots) break;
+            // CTAs that share an SM share its way in
+            const double rounds = per_sm == 1 ? divide_up(tiles, slots) : static_cast<double>(divide_up(tiles * s, sm_count()));
+            const double cost = rounds * per * stage + (cg == 2 ? 1800 : 0) + (s > 1 ? exchange : 0);
+            if (best.bn == 0 || cost < least) {
+                best = {bn, cg, swap, s};
+                least = cost;
+            }
+        }
+    };
+    if (elem_bytes == 1 && m <= 128) {  // tokens along the accumulator's columns: tiles no wider than they are
+        const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+        consider(bn, 1, true, 2, 2.0 * (kGemmRows + bn), 1500 + 8 * bn);
+        return best;
     }
-    const long long pairs = static_cast<long long>(divide_up(m, 256)) * divide_up(n, 256);
-    if (pairs >= 40) {
-        p.bn = 256;
-        p.cg = 2;
-        p.splits = 1;
-    } else {
-        p.bn = 128;
-        p.cg = 1;
-        p.splits = split_count(static_cast<long long>(divide_up(m, 128)) * divide_up(n, 128), k_tiles, 8);
-    }
-    return p;
-}
-
-int64_t product_workspace(int64_t m, int n, int k, int elem_bytes) {
-    if (m < 1 || n < 1 || k < 1 || m > 0x7fffffffll) return 0;
-    const ProductPlan p = plan_product(static_cast<int>(m), n, k, elem_bytes);
-    return p.splits > 1 ? static_cast<int64_t>(p.splits) * m * n * 4 : 0;
-}
-
-// ---- sums of a split product ------------------------------------------------------------------------------
-
-struct SplitArgs {
-    const uint32_t *partial;
-    int splits;
-    long long rows, split_elems;
-    int n;
-    const float *row_scale, *column_scale;
-    const void *bias;
-    int bias_dtype;
-    void *out;
-    long long out_stride;
-    int out_dtype;
-};
-
-// The parts are added in their order: integers exactly, float32 sums the same way at every call.
-template <bool INT>
-__global__ void __launch_bounds__(256) split_sum_kernel(const SplitArgs a) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
-    if (n >= a.n || row >= a.rows) return;
-    const uint32_t *p = a.partial + row * a.n + n;
-    float v;
-    if constexpr (INT) {
-        int sum = 0;
-        for (int s = 0; s < a.splits; ++s) sum += static_cast<int>(p[s * a.split_elems]);
-        v = static_cast<float>(sum) * (a.row_scale[row] * a.column_scale[n]);
-    } else {
-        v = 0.f;
-        for (int s = 0; s < a.splits; ++s) v += __uint_as_float(p[s * a.split_elems]);
-    }
-    if (a.bias) v += bias_at(a.bias, a.bias_dtype, n);
-    const long long at = row * a.out_stride + n;
-    if (a.out_dtype == TH_F32) static_cast<float *>(a.out)[at] = v;
-    else if (a.out_dtype == TH_F16) static_cast<__half *>(a.out)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
+    consider(256, 2, false, 1, 540, 9000);
+    consider(128, 2, false, 1, 410, 4500);
+    consider(128, 1, false, 1, 540, 4500);
+    return best;
 }
 
 // ---- one product ------------------------------------------------------------------------------------------
@@ -101,12 +68,10 @@ struct Product {
     void *out;
     long long out_stride;
     int out_dtype, bias_dtype;
-    void *workspace;
-    long long workspace_bytes;
 };
 
 template <int EB, bool A_MN, bool B_MN>
-int run_product(const char *what, const Product &p, bool bf16, cudaStream_t stream) {
+int run_product(const Product &p, bool bf16, cudaStream_t stream) {
     const ProductPlan plan = plan_product(p.a.rows, p.b.rows, p.k, EB);
     GemmArgs g{};
     g.splits = plan.splits;
@@ -117,48 +82,19 @@ int run_product(const char *what, const Product &p, bool bf16, cudaStream_t stre
     g.column_scale = plan.swap ? p.row_scale : p.column_scale;
     g.bias = p.bias;
     g.bias_dtype = p.bias_dtype;
-    if (plan.splits > 1) {
-        const long long elems = static_cast<long long>(p.a.rows) * p.b.rows;
-        if (!p.workspace || p.workspace_bytes < plan.splits * elems * 4 || !aligned_to(p.workspace, 16))
-            return fail(TH_ERR_WORKSPACE, "%s: scratch missing, too small or off 16 bytes", what);
-        g.out = p.workspace;
-        g.out_stride = p.b.rows;
-        g.split_stride = elems * 4;
-        g.out_dtype = kRaw32;
-    }
-    int rc = TH_ERR_UNSUPPORTED;
     if constexpr (EB == 1) {
         if (plan.swap) {
             switch (plan.bn) {
-                case 16: rc = launch_gemm<1, false, false, 16, 1, true>(g, p.b, p.a, p.k, false, stream); break;
-                case 32: rc = launch_gemm<1, false, false, 32, 1, true>(g, p.b, p.a, p.k, false, stream); break;
-                case 64: rc = launch_gemm<1, false, false, 64, 1, true>(g, p.b, p.a, p.k, false, stream); break;
-                default: rc = launch_gemm<1, false, false, 128, 1, true>(g, p.b, p.a, p.k, false, stream); break;
+                case 16: return launch_gemm<1, false, false, 16, 1, true, 2>(g, p.b, p.a, p.k, false, stream);
+                case 32: return launch_gemm<1, false, false, 32, 1, true, 2>(g, p.b, p.a, p.k, false, stream);
+                case 64: return launch_gemm<1, false, false, 64, 1, true, 2>(g, p.b, p.a, p.k, false, stream);
+                default: return launch_gemm<1, false, false, 128, 1, true, 2>(g, p.b, p.a, p.k, false, stream);
             }
         }
     }
-    if (!plan.swap) {
-        rc = plan.cg == 2 ? launch_gemm<EB, A_MN, B_MN, 256, 2, false>(g, p.a, p.b, p.k, bf16, stream)
-                          : launch_gemm<EB, A_MN, B_MN, 128, 1, false>(g, p.a, p.b, p.k, bf16, stream);
-    }
-    if (rc != TH_OK || plan.splits == 1) return rc;
-    SplitArgs s{};
-    s.partial = static_cast<const uint32_t *>(p.workspace);
-    s.splits = plan.splits;
-    s.rows = p.a.rows;
-    s.n = p.b.rows;
-    s.split_elems = s.rows * s.n;
-    s.row_scale = p.row_scale;
-    s.column_scale = p.column_scale;
-    s.bias = p.bias;
-    s.bias_dtype = p.bias_dtype;
-    s.out = p.out;
-    s.out_stride = p.out_stride;
-    s.out_dtype = p.out_dtype;
-    const unsigned gy = static_cast<unsigned>(std::min<long long>(s.rows, 32768));
-    const dim3 grid(divide_up(s.n, 256), gy, divide_up(s.rows, gy));
-    split_sum_kernel<EB == 1><<<grid, 256, 0, stream>>>(s);
-    return launch_status("split_sum_kernel");
+    if (plan.cg == 1) return launch_gemm<EB, A_MN, B_MN, 128, 1, false, 1>(g, p.a, p.b, p.k, bf16, stream);
+    return plan.bn == 256 ? launch_gemm<EB, A_MN, B_MN, 256, 2, false, 1>(g, p.a, p.b, p.k, bf16, stream)
+                          : launch_gemm<EB, A_MN, B_MN, 128, 2, false, 1>(g, p.a, p.b, p.k, bf16, stream);
 }
 
 int check_shape(const char *what, int64_t rows, int d_in, int d_out) {
@@ -183,11 +119,9 @@ extern "C" int th_linear_tc_status(void) {
     return status;
 }
 
-extern "C" int64_t th_int8_linear_workspace_bytes(int64_t rows, int d_in, int d_out) { return product_workspace(rows, d_out, d_in, 1); }
-
 extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride,
-                              const float *weight_scale_dev, const void *bias_dev, void *y_dev, int64_t y_stride, void *workspace_dev, int64_t workspace_bytes,
-                              int64_t rows, int d_in, int d_out, int dtype, void *stream) {
+                              const float *weight_scale_dev, const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out,
+                              int dtype, void *stream) {
     if (int rc = check_shape("th_int8_linear", rows, d_in, d_out)) return rc;
     // 128 x 128 x 131071 is the largest sum that 32 bits are sure to hold
     if (d_in > 131071) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: %d inputs, more than a 32-bit sum holds", d_in);
@@ -206,18 +140,11 @@ extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *
     p.out = y_dev;
     p.out_stride = y_stride;
     p.out_dtype = p.bias_dtype = dtype;
-    p.workspace = workspace_dev;
-    p.workspace_bytes = workspace_bytes;
-    return run_product<1, false, false>("th_int8_linear", p, false, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int64_t th_linear_workspace_bytes(int64_t rows, int d_in, int d_out) {
-    if (rows < 1 || rows > (1ll << 30)) return 0;
-    return std::max({product_workspace(rows, d_out, d_in, 2), product_workspace(rows, d_in, d_out, 2), product_workspace(d_out, d_in, static_cast<int>(rows), 2)});
+    return run_product<1, false, false>(p, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *weight_dev, int64_t weight_stride, const void *bias_dev, void *y_dev,
-                             int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream) {
+                             int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, void *stream) {
     if (int rc = check_shape("th_linear_fwd", rows, d_in, d_out)) return rc;
     if (int rc = check_16bit("th_linear_fwd", dtype)) return rc;
     if (rows == 0) return TH_OK;
@@ -231,14 +158,11 @@ extern "C" int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *we
     p.out = y_dev;
     p.out_stride = y_stride;
     p.out_dtype = p.bias_dtype = dtype;
-    p.workspace = workspace_dev;
-    p.workspace_bytes = workspace_bytes;
-    return run_product<2, false, false>("th_linear_fwd", p, dtype == TH_BF16, static_cast<cudaStream_t>(stream));
+    return run_product<2, false, false>(p, dtype == TH_BF16, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *weight_dev, int64_t weight_stride, void *grad_x_dev,
-                                   int64_t gx_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype,
-                                   void *stream) {
+                                   int64_t gx_stride, int64_t rows, int d_in, int d_out, int dtype, void *stream) {
     if (int rc = check_shape("th_linear_bwd_input", rows, d_in, d_out)) return rc;
     if (int rc = check_16bit("th_linear_bwd_input", dtype)) return rc;
     if (rows == 0) return TH_OK;
@@ -251,13 +175,11 @@ extern "C" int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, co
     p.out = grad_x_dev;
     p.out_stride = gx_stride;
     p.out_dtype = dtype;
-    p.workspace = workspace_dev;
-    p.workspace_bytes = workspace_bytes;
-    return run_product<2, false, true>("th_linear_bwd_input", p, dtype == TH_BF16, static_cast<cudaStream_t>(stream));
+    return run_product<2, false, true>(p, dtype == TH_BF16, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride, void *grad_weight_dev,
-                                    void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in, int d_out, int dtype, void *stream) {
+                                    int64_t rows, int d_in, int d_out, int dtype, void *stream) {
     if (int rc = check_shape("th_linear_bwd_weight", rows, d_in, d_out)) return rc;
     if (int rc = check_16bit("th_linear_bwd_weight", dtype)) return rc;
     if (!grad_weight_dev) return fail(TH_ERR_BAD_ARG, "th_linear_bwd_weight: null pointer");
@@ -271,7 +193,5 @@ extern "C" int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, c
     p.out = grad_weight_dev;
     p.out_stride = d_in;
     p.out_dtype = dtype;
-    p.workspace = workspace_dev;
-    p.workspace_bytes = workspace_bytes;
-    return run_product<2, true, true>("th_linear_bwd_weight", p, dtype == TH_BF16, at);
+    return run_product<2, true, true>(p, dtype == TH_BF16, at);
 }

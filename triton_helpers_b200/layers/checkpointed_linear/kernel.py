@@ -49,11 +49,6 @@ def _stride(t: Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
 
 
-def _scratch(lib, rows: int, d_in: int, d_out: int, device: torch.device) -> Tuple[Optional[Tensor], int]:
-    ws_bytes = lib.th_linear_workspace_bytes(rows, d_in, d_out)
-    return (torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None), ws_bytes
-
-
 class _checkpointed_linear(Function):
 
     @staticmethod
@@ -68,11 +63,10 @@ class _checkpointed_linear(Function):
         lib = _lib.lib()
         rows8 = None
         with torch.cuda.device(device):
-            workspace, ws_bytes = _scratch(lib, rows, d_in, d_out, device)
             _lib.check(
                 lib.th_linear_fwd(
-                    x2d.data_ptr(), _stride(x2d), w.data_ptr(), _stride(w), _lib.ptr(b), y.data_ptr(), d_out, _lib.ptr(workspace), ws_bytes,
-                    rows, d_in, d_out, code, _lib.stream_ptr(device),
+                    x2d.data_ptr(), _stride(x2d), w.data_ptr(), _stride(w), _lib.ptr(b), y.data_ptr(), d_out, rows, d_in,
+                    d_out, code, _lib.stream_ptr(device),
                 ),
                 "th_linear_fwd",
             )  # fmt: skip
@@ -101,15 +95,14 @@ class _checkpointed_linear(Function):
         dx = dw = db = None
         lib = _lib.lib()
         with torch.cuda.device(device):
-            workspace, ws_bytes = _scratch(lib, rows, d_in, d_out, device)
             stream = _lib.stream_ptr(device)
             if want_x:
                 w = _operand(weight, d_in)
                 dx = torch.empty(ctx.x_shape, dtype=dtype, device=device)
                 _lib.check(
                     lib.th_linear_bwd_input(
-                        gy2d.data_ptr(), _stride(gy2d), w.data_ptr(), _stride(w), dx.data_ptr(), d_in, _lib.ptr(workspace), ws_bytes, rows,
-                        d_in, d_out, code, stream,
+                        gy2d.data_ptr(), _stride(gy2d), w.data_ptr(), _stride(w), dx.data_ptr(), d_in, rows, d_in,
+                        d_out, code, stream,
                     ),
                     "th_linear_bwd_input",
                 )  # fmt: skip
@@ -125,8 +118,8 @@ class _checkpointed_linear(Function):
                 dw = torch.empty((d_out, d_in), dtype=dtype, device=device)
                 _lib.check(
                     lib.th_linear_bwd_weight(
-                        gy2d.data_ptr(), _stride(gy2d), x8.data_ptr(), _stride(x8), dw.data_ptr(), _lib.ptr(workspace), ws_bytes, rows, d_in,
-                        d_out, code, stream,
+                        gy2d.data_ptr(), _stride(gy2d), x8.data_ptr(), _stride(x8), dw.data_ptr(), rows, d_in, d_out, code,
+                        stream,
                     ),
                     "th_linear_bwd_weight",
                 )  # fmt: skip

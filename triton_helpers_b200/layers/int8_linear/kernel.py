@@ -165,15 +165,11 @@ def int8_linear(
         device = _lib.require_cuda(q, scale, w, w_scale, bias)
         bias = None if bias is None else bias.contiguous()
         y = torch.empty((*lead, d_out), dtype=dtype, device=device)
-        lib = _lib.lib()
         with torch.cuda.device(device):
-            ws_bytes = lib.th_int8_linear_workspace_bytes(q.shape[0], d_in, d_out)
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
             _lib.check(
-                lib.th_int8_linear(
+                _lib.lib().th_int8_linear(
                     q.data_ptr(), int8_stride(q), scale.data_ptr(), w.data_ptr(), int8_stride(w), w_scale.data_ptr(), _lib.ptr(bias),
-                    y.data_ptr(), d_out, _lib.ptr(workspace), ws_bytes, q.shape[0], d_in, d_out, _lib.DTYPE_CODE[dtype],
-                    _lib.stream_ptr(device),
+                    y.data_ptr(), d_out, q.shape[0], d_in, d_out, _lib.DTYPE_CODE[dtype], _lib.stream_ptr(device),
                 ),
                 "th_int8_linear",
             )  # fmt: skip
