@@ -450,7 +450,7 @@ int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *w
 int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
                          void *grad_weight_dev, int64_t rows, int d_in, int d_out, int dtype, void *stream);
 
-/* Device-side status word of these products (0 = fine, 1 = a bounded wait ran out and results are invalid).
+/* Device-side status word of these kernels (0 = fine, 1 = a bounded wait ran out and results are invalid).
  * Synchronises the device. */
 int th_linear_tc_status(void);
 

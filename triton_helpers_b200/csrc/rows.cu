@@ -28,8 +28,6 @@ template <>
 struct Raw<4> { using type = uint32_t; };
 template <>
 struct Raw<2> { using type = unsigned short; };
-template <>
-struct Raw<1> { using type = unsigned char; };
 
 template <typename T, int VB>
 struct Packet {
@@ -57,25 +55,69 @@ __device__ __forceinline__ void store_values(T *row, long long packet, const flo
     reinterpret_cast<typename Raw<VB>::type *>(row)[packet] = p.raw;
 }
 
-// The gain of a packet's columns: float32, or the rows' own type
-template <typename T, int N>
-__device__ __forceinline__ void load_gain(const void *gain, bool gain_f32, long long packet, float (&g)[N]) {
-    if (gain_f32) {
-        const float *p = static_cast<const float *>(gain) + packet * N;
-        if constexpr (N % 4 == 0) {
+// A row as 16-byte packets that start on 16 bytes, wherever the row itself starts: `shift` elements of the first packet lie ahead of it and
+// the last one may reach past it.  A packet holds one element of the row at least, so it lies in memory that is there; elements beside the
+// row are read as zeros and never written.  (5000 rows of 3001 bfloat16, an element at a time: SHIFTFIG.)
+template <typename T, bool SHIFT>
+struct Span {
+    static constexpr int N = 16 / static_cast<int>(sizeof(T));
+    int shift, d, packets;
+    __device__ Span(const void *row, int columns) {
+        d = columns;
+        shift = SHIFT ? static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)) : 0;
+        packets = SHIFT ? (shift + d + N - 1) / N : d / N;
+    }
+    __device__ __forceinline__ bool edge(int i) const { return SHIFT && (i == 0 || i == packets - 1); }
+    __device__ __forceinline__ bool inside(int i, int e) const { return static_cast<unsigned>(i * N + e - shift) < static_cast<unsigned>(d); }
+    __device__ __forceinline__ uint4 fetch(const T *row, int i) const { return reinterpret_cast<const uint4 *>(row - shift)[i]; }
+    __device__ __forceinline__ void widen(uint4 raw, int i, float (&f)[N]) const {
+        Packet<T, 16> p;
+        p.raw = raw;
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = to_float<T>(p.v[e]);
+        if (edge(i)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (!inside(i, e)) f[e] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void store(T *row, int i, const float (&f)[N]) const {
+        if (edge(i)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (inside(i, e)) row[i * N + e - shift] = from_float<T>(f[e]);
+        } else {
+            store_values<T, 16>(row - shift, i, f);
+        }
+    }
+    // The gain of a packet's columns: float32, or the rows' own type; it starts on 16 bytes itself
+    __device__ __forceinline__ void gains(const void *gain, bool gain_f32, int i, float (&g)[N]) const {
+        if constexpr (SHIFT) {
+            const int c = i * N - shift;
+            if (edge(i)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int at = min(max(c + e, 0), d - 1);
+                    g[e] = gain_f32 ? static_cast<const float *>(gain)[at] : to_float<T>(static_cast<const T *>(gain)[at]);
+                }
+            } else if (gain_f32) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[e] = __ldg(static_cast<const float *>(gain) + c + e);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[e] = to_float<T>(static_cast<const T *>(gain)[c + e]);
+            }
+        } else if (gain_f32) {
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(p + e));
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(gain) + i * N + e));
                 g[e] = v.x; g[e + 1] = v.y; g[e + 2] = v.z; g[e + 3] = v.w;
             }
         } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) g[e] = __ldg(p + e);
+            load_values<T, 16>(static_cast<const T *>(gain), i, g);
         }
-    } else {
-        load_values<T, N * static_cast<int>(sizeof(T))>(static_cast<const T *>(gain), packet, g);
     }
-}
+};
 
 // ---- sums and maxima over the threads that share a row ---------------------------------------------------
 
@@ -122,23 +164,31 @@ struct RowScale {
 // rint of a product of at most 127: adding 1.5 * 2^23 leaves the integer in the low byte
 __device__ __forceinline__ uint32_t quantum(float v, float inverse) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inverse), 12582912.f)); }
 
+// N (4 or 8) of them, the first in the lowest byte
 template <int N>
-__device__ __forceinline__ void store_quanta(signed char *row, long long packet, const float (&f)[N], const RowScale &s) {
-    uint32_t b[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) b[e] = s.finite ? quantum(f[e], s.inverse) : 0u;
-    if constexpr (N == 1) {
-        row[packet] = static_cast<signed char>(b[0]);
-    } else {
-        uint32_t w[N / 4];
+__device__ __forceinline__ unsigned long long quanta(const float (&f)[N], const RowScale &s) {
+    uint32_t w[2] = {0, 0};
+    if (s.finite) {
 #pragma unroll
         for (int e = 0; e < N; e += 4)
-            w[e / 4] = __byte_perm(__byte_perm(b[e], b[e + 1], 0x0040), __byte_perm(b[e + 2], b[e + 3], 0x0040), 0x5410);
-        if constexpr (N == 8)
-            reinterpret_cast<uint2 *>(row)[packet] = make_uint2(w[0], w[1]);
-        else
-            reinterpret_cast<uint32_t *>(row)[packet] = w[0];
+            w[e / 4] = __byte_perm(__byte_perm(quantum(f[e], s.inverse), quantum(f[e + 1], s.inverse), 0x0040),
+                                   __byte_perm(quantum(f[e + 2], s.inverse), quantum(f[e + 3], s.inverse), 0x0040), 0x5410);
     }
+    return w[0] | static_cast<unsigned long long>(w[1]) << 32;
+}
+
+template <int N>
+__device__ __forceinline__ void store_quanta(signed char *row, int i, unsigned long long b) {
+    if constexpr (N == 8) reinterpret_cast<unsigned long long *>(row)[i] = b;
+    else reinterpret_cast<uint32_t *>(row)[i] = static_cast<uint32_t>(b);
+}
+
+// Packets that lie `shift` columns before their place in the 8-bit row: a lane joins its last columns with its neighbour's first ones, so
+// a warp has one packet more than it stores.  Called by whole warps.
+template <int N>
+__device__ __forceinline__ void store_shifted_quanta(signed char *row, int i, int shift, int d, bool mine, unsigned long long b) {
+    const unsigned long long next = __shfl_down_sync(~0u, b, 1);
+    if (mine && i * N < d) store_quanta<N>(row, i, shift ? (b >> (8 * shift)) | (next << (8 * (N - shift))) : b);
 }
 
 // ---- forward: norm, norm with 8-bit rows, 8-bit rows alone ------------------------------------------------
@@ -151,28 +201,113 @@ struct RowFwdArgs {
     signed char *q;
     float *scale, *rstd;
     long long x_stride, residual_stride, q_stride, rows;
-    int d, packets, team, gain_f32;
+    int d, team, gain_f32;
     float eps;
 };
 
-// A team of 32 threads (several rows per CTA) or the whole CTA owns a row and keeps it in registers, P packets a thread; P = 0: rows
-// longer than that are read again for every step, by then from L2.  What is normalised is the sum as it is written, rounded, so that
-// the backward pass, which reads it, sees the same numbers.
-template <typename T, int VB, int P, int MODE, bool RES>
-__global__ void __launch_bounds__(kMaxTeam) row_fwd_kernel(const RowFwdArgs a) {
-    constexpr int N = VB / static_cast<int>(sizeof(T));
+// A team of 32 threads (several rows per CTA) or the whole CTA owns a row and keeps it in registers, P packets a thread.  What is
+// normalised is the sum as it is written, rounded, so that the backward pass, which reads it, sees the same numbers.
+template <typename T, int P, int MODE, bool RES, bool SHIFT, int THREADS>
+__global__ void __launch_bounds__(THREADS) row_fwd_kernel(const RowFwdArgs a) {
+    constexpr int N = 16 / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
     const int team = a.team, t = team == 32 ? threadIdx.x & 31 : threadIdx.x;
     const long long row = team == 32 ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;  // whole warps, and only where a warp is a team
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const Span<T, SHIFT> span(x, a.d);
+
+    // shifted 8-bit rows: a warp's last lane has the packet that the next warp's first one owns
+    constexpr bool kOverlap = SHIFT && MODE != kNorm;
+    constexpr int kOwn = kOverlap ? 31 : 32;
+    const int at = kOverlap ? (t >> 5) * kOwn + (t & 31) : t, step = team / 32 * kOwn;
+    const bool mine = !kOverlap || (t & 31) < kOwn;
+
+    uint4 raw[P], added[P];  // every load is on its way before the first is used
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int i = at + p * step;
+        raw[p] = added[p] = make_uint4(0, 0, 0, 0);
+        if (i < span.packets) {
+            raw[p] = span.fetch(x, i);
+            if constexpr (RES) added[p] = span.fetch(static_cast<const T *>(a.residual) + row * a.residual_stride, i);
+        }
+    }
+    float f[P][N];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int i = at + p * step;
+        span.widen(raw[p], i, f[p]);
+        if constexpr (RES) {
+            float r[N];
+            span.widen(added[p], i, r);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[p][e] = to_float<T>(from_float<T>(f[p][e] + r[e]));
+        }
+    }
+    if constexpr (MODE != kQuantize) {
+        float part = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < N; ++e) part = fmaf(f[p][e], f[p][e], part);
+        const float ss = team_sum(mine ? part : 0.f, team, red, turn);
+        const float rstd = rsqrtf(ss / static_cast<float>(a.d) + a.eps);
+        if (a.rstd && t == 0) a.rstd[row] = rstd;
+        if constexpr (RES) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (mine && at + p * step < span.packets) span.store(static_cast<T *>(a.sum) + row * a.d, at + p * step, f[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (at + p * step < span.packets) {
+                float g[N];
+                span.gains(a.gain, a.gain_f32 != 0, at + p * step, g);
+#pragma unroll
+                for (int e = 0; e < N; ++e) f[p][e] = f[p][e] * rstd * g[e];
+            }
+        }
+        if constexpr (MODE == kNorm) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (at + p * step < span.packets) span.store(static_cast<T *>(a.y) + row * a.d, at + p * step, f[p]);
+        }
+    }
+    if constexpr (MODE != kNorm) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < N; ++e) top = max(top, magnitude(f[p][e]));
+        const RowScale s(team_max(top, team, red, turn));
+        if (t == 0) a.scale[row] = s.scale;
+        signed char *q = a.q + row * a.q_stride;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int i = at + p * step;
+            const unsigned long long b = quanta<N>(f[p], s);
+            if constexpr (SHIFT) store_shifted_quanta<N>(q, i, span.shift, a.d, mine, b);
+            else if (i < span.packets) store_quanta<N>(q, i, b);
+        }
+    }
+}
+
+// Rows that are too long for registers, or whose tensors do not start alike: read again for every step, by then from L2.  VB = 16 bytes an
+// access where everything starts on them, else an element.
+template <typename T, int VB, int MODE, bool RES>
+__global__ void __launch_bounds__(kMaxTeam) row_fwd_stream_kernel(const RowFwdArgs a) {
+    constexpr int N = VB / static_cast<int>(sizeof(T));
+    __shared__ float red[2][32];
+    int turn = 0;
+    const int team = blockDim.x, packets = a.d / N;
+    const long long row = blockIdx.x;
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *res = RES ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
     T *sum = RES ? static_cast<T *>(a.sum) + row * a.d : nullptr;
-    T *y = MODE == kNorm ? static_cast<T *>(a.y) + row * a.d : nullptr;
-    signed char *q = MODE == kNorm ? nullptr : a.q + row * a.q_stride;
-
-    const auto fetch = [&](int i, float (&f)[N]) {
+    float f[N], rstd = 1.f;
+    const auto fetch = [&](int i) {
         load_values<T, VB>(x, i, f);
         if constexpr (RES) {
             float r[N];
@@ -181,157 +316,149 @@ __global__ void __launch_bounds__(kMaxTeam) row_fwd_kernel(const RowFwdArgs a) {
             for (int e = 0; e < N; ++e) f[e] = to_float<T>(from_float<T>(f[e] + r[e]));
         }
     };
-    const auto normed = [&](int i, const float (&f)[N], float rstd, float (&o)[N]) {
-        float g[N];
-        load_gain<T, N>(a.gain, a.gain_f32 != 0, i, g);
+    if constexpr (MODE != kQuantize) {
+        float ss = 0.f;
+        for (int i = threadIdx.x; i < packets; i += team) {
+            fetch(i);
+            if constexpr (RES) store_values<T, VB>(sum, i, f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = f[e] * rstd * g[e];
-    };
-
-    if constexpr (P > 0) {
-        float f[P][N];
+            for (int e = 0; e < N; ++e) ss = fmaf(f[e], f[e], ss);
+        }
+        ss = team_sum(ss, team, red, turn);
+        rstd = rsqrtf(ss / static_cast<float>(a.d) + a.eps);
+        if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+    }
+    const auto value = [&](int i) {
+        fetch(i);
+        if constexpr (MODE != kQuantize) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int i = t + p * team;
-            if (i < a.packets) {
-                fetch(i, f[p]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) f[p][e] = 0.f;
+            for (int e = 0; e < N; ++e) {
+                const long long c = static_cast<long long>(i) * N + e;
+                f[e] = f[e] * rstd * (a.gain_f32 ? __ldg(static_cast<const float *>(a.gain) + c) : to_float<T>(static_cast<const T *>(a.gain)[c]));
             }
         }
-        if constexpr (RES) {
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) store_values<T, VB>(sum, t + p * team, f[p]);
-        }
-        if constexpr (MODE != kQuantize) {
-            float ss = 0.f;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int e = 0; e < N; ++e) ss = fmaf(f[p][e], f[p][e], ss);
-            ss = team_sum(ss, team, red, turn);
-            const float rstd = rsqrtf(ss / static_cast<float>(a.d) + a.eps);
-            if (a.rstd && t == 0) a.rstd[row] = rstd;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) normed(t + p * team, f[p], rstd, f[p]);
-        }
-        if constexpr (MODE == kNorm) {
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) store_values<T, VB>(y, t + p * team, f[p]);
-        } else {
-            uint32_t top = 0;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int e = 0; e < N; ++e) top = max(top, magnitude(f[p][e]));
-            const RowScale s(team_max(top, team, red, turn));
-            if (t == 0) a.scale[row] = s.scale;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) store_quanta<N>(q, t + p * team, f[p], s);
+    };
+    if constexpr (MODE == kNorm) {
+        T *y = static_cast<T *>(a.y) + row * a.d;
+        for (int i = threadIdx.x; i < packets; i += team) {
+            value(i);
+            store_values<T, VB>(y, i, f);
         }
     } else {
-        float f[N], rstd = 1.f;
-        if constexpr (MODE != kQuantize) {
-            float ss = 0.f;
-            for (int i = t; i < a.packets; i += team) {
-                fetch(i, f);
-                if constexpr (RES) store_values<T, VB>(sum, i, f);
+        uint32_t top = 0;
+        for (int i = threadIdx.x; i < packets; i += team) {
+            value(i);
 #pragma unroll
-                for (int e = 0; e < N; ++e) ss = fmaf(f[e], f[e], ss);
-            }
-            ss = team_sum(ss, team, red, turn);
-            rstd = rsqrtf(ss / static_cast<float>(a.d) + a.eps);
-            if (a.rstd && t == 0) a.rstd[row] = rstd;
+            for (int e = 0; e < N; ++e) top = max(top, magnitude(f[e]));
         }
-        const auto again = [&](int i) {
-            fetch(i, f);
-            if constexpr (MODE != kQuantize) normed(i, f, rstd, f);
-        };
-        if constexpr (MODE == kNorm) {
-            for (int i = t; i < a.packets; i += team) {
-                again(i);
-                store_values<T, VB>(y, i, f);
-            }
-        } else {
-            uint32_t top = 0;
-            for (int i = t; i < a.packets; i += team) {
-                again(i);
-#pragma unroll
-                for (int e = 0; e < N; ++e) top = max(top, magnitude(f[e]));
-            }
-            const RowScale s(team_max(top, team, red, turn));
-            if (t == 0) a.scale[row] = s.scale;
-            for (int i = t; i < a.packets; i += team) {
-                again(i);
-                store_quanta<N>(q, i, f, s);
-            }
+        const RowScale s(team_max(top, team, red, turn));
+        if (threadIdx.x == 0) a.scale[row] = s.scale;
+        signed char *q = a.q + row * a.q_stride;
+        for (int i = threadIdx.x; i < packets; i += team) {
+            value(i);
+            if constexpr (N == 1) q[i] = s.finite ? static_cast<signed char>(quantum(f[0], s.inverse)) : 0;
+            else store_quanta<N>(q, i, quanta<N>(f, s));
         }
     }
 }
 
-// Threads that share a row and packets each of them holds: a warp up to four packets a lane, then as many threads as give each two,
-// up to the CTA's 1024.
+// Threads that share a row and packets each of them holds: a warp up to four packets a lane, then as many threads as give each
+// `wanted`, up to the CTA's 1024 (and `most` packets; 0: more than that).
 struct TeamPlan {
     int team, per_thread, block, rows_per_block;
 };
-TeamPlan team_plan(int packets, int most) {
+// `own`: packets of a warp's 32 that it does not share.
+TeamPlan team_plan(int packets, int wanted, int most, int own = 32) {
     TeamPlan p{};
-    if (packets <= 128) {
+    if (packets <= own * std::min(4, most)) {
         p.team = 32;
-        p.per_thread = (packets + 31) / 32;
         p.rows_per_block = 4;
         p.block = 128;
     } else {
-        p.team = 64;
-        while (p.team < kMaxTeam && p.team * 2 < packets) p.team *= 2;
-        p.per_thread = (packets + p.team - 1) / p.team;
+        p.team = std::min(kMaxTeam, std::max(64, ((packets + wanted - 1) / wanted + own - 1) / own * 32));
         p.rows_per_block = 1;
         p.block = p.team;
     }
+    const int step = p.team / 32 * own;
+    p.per_thread = (packets + step - 1) / step;
     int n = 1;
     while (n < p.per_thread) n *= 2;
     p.per_thread = n <= most ? n : 0;
     return p;
 }
 
-template <typename T, int VB, int MODE, bool RES>
-int launch_row_fwd(RowFwdArgs a, cudaStream_t stream) {
-    a.packets = a.d / (VB / static_cast<int>(sizeof(T)));
-    const TeamPlan plan = team_plan(a.packets, 8);
-    a.team = plan.team;
-    const long long blocks = (a.rows + plan.rows_per_block - 1) / plan.rows_per_block;
-    if (blocks > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
-    const dim3 grid(static_cast<unsigned>(blocks)), block(plan.block);
+// How the rows of several tensors lie
+enum { kPacked, kShifted, kAnyhow };
+struct Layout {
+    bool packed = true, alike = true;
+    uintptr_t start = ~uintptr_t(0), step = 0;
+    template <typename T>
+    void add(const void *p, long long stride, int d) {
+        if (!p) return;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p) & 15, by = static_cast<uintptr_t>(stride * static_cast<long long>(sizeof(T))) & 15;
+        packed = packed && at == 0 && by == 0 && d * static_cast<long long>(sizeof(T)) % 16 == 0;
+        if (start == ~uintptr_t(0)) {
+            start = at;
+            step = by;
+        }
+        alike = alike && at == start && by == step && at % sizeof(T) == 0;
+    }
+    int kind() const { return packed ? kPacked : alike ? kShifted : kAnyhow; }
+};
+// Packets of the longest span of d columns
+template <typename T>
+int span_packets(int d, int kind) {
+    constexpr int N = 16 / static_cast<int>(sizeof(T));
+    return kind == kPacked ? d / N : (d + 2 * N - 2) / N;
+}
+
+template <typename T, int MODE, bool RES, bool SHIFT, int THREADS>
+int launch_row_fwd(const RowFwdArgs &a, const TeamPlan &plan, unsigned blocks, cudaStream_t stream) {
+    const dim3 grid(blocks), block(plan.block);
     switch (plan.per_thread) {
-        case 1: row_fwd_kernel<T, VB, 1, MODE, RES><<<grid, block, 0, stream>>>(a); break;
-        case 2: row_fwd_kernel<T, VB, 2, MODE, RES><<<grid, block, 0, stream>>>(a); break;
-        case 4: row_fwd_kernel<T, VB, 4, MODE, RES><<<grid, block, 0, stream>>>(a); break;
-        case 8: row_fwd_kernel<T, VB, 8, MODE, RES><<<grid, block, 0, stream>>>(a); break;
-        default: row_fwd_kernel<T, VB, 0, MODE, RES><<<grid, block, 0, stream>>>(a); break;
+        case 1: row_fwd_kernel<T, 1, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
+        case 2: row_fwd_kernel<T, 2, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
+        case 4: row_fwd_kernel<T, 4, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
+        default: row_fwd_kernel<T, 8, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
     }
     return launch_status("row_fwd_kernel");
 }
 
-// 16-byte packets where every row of every tensor starts on 16 bytes and ends with a whole packet
-template <typename T>
-bool packed_rows(const void *p, long long stride, int d) {
-    return p == nullptr || (aligned_to(p, 16) && stride * static_cast<long long>(sizeof(T)) % 16 == 0 && d * static_cast<long long>(sizeof(T)) % 16 == 0);
+template <typename T, int MODE, bool RES>
+int plan_row_fwd(RowFwdArgs a, cudaStream_t stream) {
+    Layout rows;
+    rows.add<T>(a.x, a.x_stride, a.d);
+    rows.add<T>(a.residual, a.residual_stride, a.d);
+    rows.add<T>(a.sum, a.d, a.d);
+    rows.add<T>(a.y, a.d, a.d);
+    const bool gain = a.gain == nullptr || aligned_to(a.gain, 16);
+    const int kind = gain || rows.kind() == kShifted ? rows.kind() : kAnyhow;
+    const int packets = span_packets<T>(a.d, kind);
+    const TeamPlan plan = team_plan(packets, RES && packets <= 512 ? 2 : 4, 8, kind == kShifted && MODE != kNorm ? 31 : 32);
+    const long long blocks = (a.rows + plan.rows_per_block - 1) / plan.rows_per_block;
+    if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
+    const unsigned n = static_cast<unsigned>(blocks), all = static_cast<unsigned>(a.rows);
+    a.team = plan.team;
+    if (kind != kAnyhow && plan.per_thread) {
+        if (kind == kPacked)
+            return plan.block <= 256   ? launch_row_fwd<T, MODE, RES, false, 256>(a, plan, n, stream)
+                   : plan.block <= 512 ? launch_row_fwd<T, MODE, RES, false, 512>(a, plan, n, stream)
+                                       : launch_row_fwd<T, MODE, RES, false, kMaxTeam>(a, plan, n, stream);
+        return plan.block <= 256   ? launch_row_fwd<T, MODE, RES, true, 256>(a, plan, n, stream)
+               : plan.block <= 512 ? launch_row_fwd<T, MODE, RES, true, 512>(a, plan, n, stream)
+                                   : launch_row_fwd<T, MODE, RES, true, kMaxTeam>(a, plan, n, stream);
+    }
+    const int block = std::min(kMaxTeam, std::max(64, (a.d / 8 + 31) / 32 * 32));
+    if (kind == kPacked) row_fwd_stream_kernel<T, 16, MODE, RES><<<all, block, 0, stream>>>(a);
+    else row_fwd_stream_kernel<T, sizeof(T), MODE, RES><<<all, block, 0, stream>>>(a);
+    return launch_status("row_fwd_stream_kernel");
 }
 
 template <typename T, int MODE>
 int row_fwd(const RowFwdArgs &a, cudaStream_t stream) {
-    const bool packed = packed_rows<T>(a.x, a.x_stride, a.d) && packed_rows<T>(a.residual, a.residual_stride, a.d) && packed_rows<T>(a.sum, a.d, a.d) &&
-                        packed_rows<T>(a.y, a.d, a.d) && (a.gain == nullptr || aligned_to(a.gain, 16));
-    constexpr int E = sizeof(T);
-    if constexpr (MODE != kQuantize) {
-        if (a.residual) return packed ? launch_row_fwd<T, 16, MODE, true>(a, stream) : launch_row_fwd<T, E, MODE, true>(a, stream);
-    }
-    return packed ? launch_row_fwd<T, 16, MODE, false>(a, stream) : launch_row_fwd<T, E, MODE, false>(a, stream);
+    if constexpr (MODE != kQuantize)
+        if (a.residual) return plan_row_fwd<T, MODE, true>(a, stream);
+    return plan_row_fwd<T, MODE, false>(a, stream);
 }
 
 template <int MODE>
@@ -353,240 +480,471 @@ struct RowBwdArgs {
     void *dx;
     float *partial;
     long long s_stride, gy_stride, gs_stride, rows;
-    int d, packets, team, gain_f32;
+    int d, team, gain_f32;
 };
 
-template <typename T, int VB, int P, bool GS>
-__global__ void __launch_bounds__(kMaxTeam) norm_bwd_kernel(const RowBwdArgs a) {
+// Rows come through a ring of stages in shared memory, brought by bulk copies of one warp, so that what is in flight does not depend on
+// the registers that sums take (rows held in registers, 16384 x 4096 bfloat16: 111 us at best, by launch shape up to 260; RINGFIG).  Long
+// rows are shared by all consumer warps, short ones have a warp each.  A team's rows are a multiple of eight apart, so that each of
+// them starts alike and a thread's packets are the same columns in all.
+constexpr int kMaxRing = 8;
+constexpr unsigned long long kRingWaitNs = 1000000000ull;
+__device__ int g_rows_status = 0;  // 1 = a bounded wait ran out
+
+struct RingPlan {
+    int stages, rows;          // stages, rows of a stage
+    int slot;                  // bytes of one row's place, where rows lie apart
+    int tensor_bytes;          // of one tensor's part of a stage
+    int whole[3];              // s, gy, gs: a stage's rows are one piece of memory
+    long long blocks;          // stages in all
+};
+
+// After a wait that ran out everybody goes on with what is there, so that nobody is left at a barrier; the status says so.
+__device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
+    unsigned long long deadline = 0;
+    for (unsigned poll = 0;; ++poll) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return;
+        if ((poll & 63u) == 63u) {
+            if (*reinterpret_cast<volatile int *>(abort_flag)) return;
+            unsigned long long now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (deadline == 0) deadline = now + kRingWaitNs;
+            else if (now > deadline) break;
+        }
+    }
+    *reinterpret_cast<volatile int *>(abort_flag) = 1;
+    g_rows_status = 1;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// The sum over a team: a warp, or all consumers (who meet at barrier 1)
+template <int CONSUMERS>
+__device__ __forceinline__ float ring_sum(float v, bool wide, float (*red)[32], int &turn) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (!wide) return v;
+    float *slot = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+    v = (threadIdx.x & 31) < CONSUMERS / 32 ? slot[threadIdx.x & 31] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+}
+
+template <typename T, int P, bool GS, bool SHIFT, int CONSUMERS>
+__global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm_bwd_kernel(const RowBwdArgs a, const RingPlan ring) {
+    constexpr int N = 16 / static_cast<int>(sizeof(T)), kTensors = GS ? 3 : 2, kWarps = CONSUMERS / 32;
+    extern __shared__ __align__(16) unsigned char stages[];
+    __shared__ __align__(8) unsigned long long full[kMaxRing], empty[kMaxRing];
+    __shared__ float red[2][32];
+    __shared__ int abort_flag;
+    const auto shared = [](const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); };
+    const int stage_bytes = kTensors * ring.tensor_bytes;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < ring.stages; ++i) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared(&full[i])), "r"(1u) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared(&empty[i])), "r"(static_cast<uint32_t>(kWarps)) : "memory");
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const char *base[3] = {static_cast<const char *>(a.s), static_cast<const char *>(a.gy), static_cast<const char *>(a.gs)};
+    const long long pitch[3] = {a.s_stride * static_cast<long long>(sizeof(T)), a.gy_stride * static_cast<long long>(sizeof(T)),
+                                a.gs_stride * static_cast<long long>(sizeof(T))};
+    const long long row_bytes = a.d * static_cast<long long>(sizeof(T));
+    float acc[P][N];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[p][e] = 0.f;
+    const bool wide = a.team > 32;
+    const int t = wide ? threadIdx.x : lane;
+    int turn = 0, stage = 0;
+    uint32_t phase = 0;
+
+    if (warp == kWarps) {
+        // ---- rows -> shared memory: whole 16-byte granules that hold a byte of the rows ----
+        for (long long block = blockIdx.x; block < ring.blocks; block += gridDim.x) {
+            ring_wait(shared(&empty[stage]), phase ^ 1, &abort_flag);
+            const long long row0 = block * ring.rows;
+            const int rows = static_cast<int>(min(static_cast<long long>(ring.rows), a.rows - row0));
+            const uint32_t bar = shared(&full[stage]);
+            uint32_t mine = 0;
+            // a piece a lane: one per tensor, or one per row
+            const auto pieces = [&](bool send) {
+#pragma unroll
+                for (int k = 0; k < kTensors; ++k) {
+                    const uint32_t to = shared(stages) + stage * stage_bytes + k * ring.tensor_bytes;
+                    for (int r = lane; r < (ring.whole[k] ? 1 : rows); r += 32) {
+                        const uintptr_t at = reinterpret_cast<uintptr_t>(base[k] + (row0 + r) * pitch[k]);
+                        const uintptr_t end = at + (ring.whole[k] ? rows : 1) * row_bytes, from = at & ~uintptr_t(15);
+                        const uint32_t bytes = static_cast<uint32_t>((end - from + 15) & ~uintptr_t(15));
+                        if (send) bulk_load(to + r * ring.slot, reinterpret_cast<const void *>(from), bytes, bar);
+                        else mine += bytes;
+                    }
+                }
+            };
+            pieces(false);
+            const uint32_t total = __reduce_add_sync(~0u, mine);
+            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(total) : "memory");
+            __syncwarp();
+            pieces(true);
+            if (++stage == ring.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    } else {
+        const float inv_d = 1.f / static_cast<float>(a.d);
+        const int first = wide ? 0 : warp, apart = wide ? 1 : kWarps;  // a team's rows of a stage
+        const long long start = static_cast<long long>(blockIdx.x) * ring.rows;
+        // the same for all of the team's rows: where they start in their first packet, and where a stage's first row does
+        const Span<T, SHIFT> span(base[0] + (start + first) * pitch[0], a.d);
+        const int ahead = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(base[0] + start * pitch[0]) & 15) : 0, bytes = static_cast<int>(row_bytes);
+        const long long stride = static_cast<long long>(gridDim.x) * ring.rows;
+        // few columns a thread: their gains, and dy * rstd * gain between the two steps, stay in registers
+        constexpr bool kHold = P * N <= 16;
+        float gain[kHold ? P : 1][N];
+        if constexpr (kHold) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) gain[p][e] = 0.f;
+                if (t + p * a.team < span.packets) span.gains(a.gain, a.gain_f32 != 0, t + p * a.team, gain[p]);
+            }
+        }
+        float next_rstd = start + first < a.rows ? a.rstd[start + first] : 0.f;
+        for (long long row0 = start; row0 < a.rows; row0 += stride) {
+            ring_wait(shared(&full[stage]), phase, &abort_flag);
+            const unsigned char *in = stages + stage * stage_bytes;
+            const int rows = static_cast<int>(min(static_cast<long long>(ring.rows), a.rows - row0));
+            for (int r = first; r < rows; r += apart) {
+                const long long row = row0 + r;
+                const float rstd = next_rstd;
+                const long long following = r + apart < ring.rows ? row + apart : row0 + stride + first;
+                if (following < a.rows) next_rstd = a.rstd[following];
+                const uint4 *held[3];
+#pragma unroll
+                for (int k = 0; k < kTensors; ++k)
+                    held[k] = reinterpret_cast<const uint4 *>(in + k * ring.tensor_bytes + (ring.whole[k] ? (ahead + r * bytes) & ~15 : r * ring.slot));
+                float part = 0.f, w[kHold ? P : 1][N];
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const int i = t + p * a.team;
+                    if (i < span.packets) {
+                        float sv[N], (&g)[N] = gain[kHold ? p : 0], (&v)[N] = w[kHold ? p : 0];
+                        span.widen(held[0][i], i, sv);
+                        span.widen(held[1][i], i, v);
+                        if constexpr (!kHold) span.gains(a.gain, a.gain_f32 != 0, i, g);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            v[e] *= rstd;
+                            acc[p][e] = fmaf(v[e], sv[e], acc[p][e]);
+                            v[e] *= g[e];
+                            part = fmaf(v[e], sv[e], part);
+                        }
+                    }
+                }
+                // part: the sum of dy gain h;  ds = rstd (dy gain - h c) + gs = w - s rstd^2 c + gs
+                const float c = ring_sum<CONSUMERS>(part, wide, red, turn) * inv_d, k2 = -rstd * rstd * c;
+                T *dx = static_cast<T *>(a.dx) + row * a.d;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const int i = t + p * a.team;
+                    if (i < span.packets) {
+                        float sv[N], o[N], (&v)[N] = w[kHold ? p : 0];
+                        if constexpr (!kHold) {
+                            span.widen(held[1][i], i, v);
+                            span.gains(a.gain, a.gain_f32 != 0, i, sv);
+#pragma unroll
+                            for (int e = 0; e < N; ++e) v[e] = v[e] * rstd * sv[e];
+                        }
+                        span.widen(held[0][i], i, sv);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) o[e] = fmaf(sv[e], k2, v[e]);
+                        if constexpr (GS) {
+                            span.widen(held[2][i], i, sv);
+#pragma unroll
+                            for (int e = 0; e < N; ++e) o[e] += sv[e];
+                        }
+                        span.store(dx, i, o);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared(&empty[stage])) : "memory");
+            if (++stage == ring.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    }
+    __syncthreads();  // every stage has been read: their memory takes the sums
+    if (!a.partial) return;
+    float *out = a.partial + static_cast<long long>(blockIdx.x) * a.d;
+    const Span<T, SHIFT> span(base[0] + (static_cast<long long>(blockIdx.x) * ring.rows + (wide ? 0 : warp)) * pitch[0], a.d);
+    if (wide) {
+        if (warp == kWarps) return;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            if (t + p * a.team < span.packets)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (!SHIFT || span.inside(t + p * a.team, e)) out[(t + p * a.team) * N + e - span.shift] = acc[p][e];
+    } else {
+        float *columns = reinterpret_cast<float *>(stages);  // d floats: the CTA's warps one after the other
+        for (int k = 0; k < kWarps; ++k) {
+            if (k == warp) {
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    if (t + p * 32 < span.packets)
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+                            if (!SHIFT || span.inside(t + p * 32, e)) {
+                                float *at = columns + (t + p * 32) * N + e - span.shift;
+                                *at = k == 0 ? acc[p][e] : *at + acc[p][e];
+                            }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < a.d; i += blockDim.x) out[i] = columns[i];
+    }
+}
+
+// Rows that are too long for registers, or whose tensors do not start alike; the gain's gradient is a column sum of its own then.
+template <typename T, int VB, bool GS>
+__global__ void __launch_bounds__(kMaxTeam) norm_bwd_stream_kernel(const RowBwdArgs a) {
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
-    const int team = a.team, t = team == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int teams = team == 32 ? blockDim.x >> 5 : 1, mine = team == 32 ? threadIdx.x >> 5 : 0;
-    const float inv_d = 1.f / static_cast<float>(a.d);
-    constexpr int Q = P > 0 ? P : 1;
-    float acc[Q][N], gain[Q][N];
+    const int team = blockDim.x, packets = a.d / N;
+    const long long row = blockIdx.x;
+    const T *s = static_cast<const T *>(a.s) + row * a.s_stride, *gy = static_cast<const T *>(a.gy) + row * a.gy_stride;
+    const T *gs = GS ? static_cast<const T *>(a.gs) + row * a.gs_stride : nullptr;
+    T *dx = static_cast<T *>(a.dx) + row * a.d;
+    const float rstd = a.rstd[row];
+    float sv[N], w[N], rv[N], c = 0.f;
+    const auto fetch = [&](int i) {
+        load_values<T, VB>(s, i, sv);
+        load_values<T, VB>(gy, i, w);
 #pragma unroll
-    for (int p = 0; p < Q; ++p)
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[p][e] = gain[p][e] = 0.f;
-    if constexpr (P > 0) {
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-            if (t + p * team < a.packets) load_gain<T, N>(a.gain, a.gain_f32 != 0, t + p * team, gain[p]);
-    }
-    for (long long row = static_cast<long long>(blockIdx.x) * teams + mine; row < a.rows; row += static_cast<long long>(gridDim.x) * teams) {
-        const T *s = static_cast<const T *>(a.s) + row * a.s_stride, *gy = static_cast<const T *>(a.gy) + row * a.gy_stride;
-        const T *gs = GS ? static_cast<const T *>(a.gs) + row * a.gs_stride : nullptr;
-        T *dx = static_cast<T *>(a.dx) + row * a.d;
-        const float rstd = a.rstd[row];
-        float c = 0.f;
-        if constexpr (P > 0) {
-            Packet<T, VB> sp[P], yp[P], rp[P];
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int i = t + p * team;
-                if (i < a.packets) {
-                    sp[p].raw = reinterpret_cast<const typename Raw<VB>::type *>(s)[i];
-                    yp[p].raw = reinterpret_cast<const typename Raw<VB>::type *>(gy)[i];
-                    if constexpr (GS) rp[p].raw = reinterpret_cast<const typename Raw<VB>::type *>(gs)[i];
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float h = to_float<T>(sp[p].v[e]) * rstd, dy = to_float<T>(yp[p].v[e]);
-                        acc[p][e] = fmaf(dy, h, acc[p][e]);
-                        c = fmaf(dy * gain[p][e], h, c);
-                    }
-                }
-            c = team_sum(c, team, red, turn) * inv_d;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets) {
-                    float o[N];
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float h = to_float<T>(sp[p].v[e]) * rstd;
-                        o[e] = rstd * (to_float<T>(yp[p].v[e]) * gain[p][e] - h * c);
-                        if constexpr (GS) o[e] += to_float<T>(rp[p].v[e]);
-                    }
-                    store_values<T, VB>(dx, t + p * team, o);
-                }
-        } else {
-            float sv[N], yv[N], rv[N];
-            for (int i = t; i < a.packets; i += team) {
-                load_values<T, VB>(s, i, sv);
-                load_values<T, VB>(gy, i, yv);
-                load_gain<T, N>(a.gain, a.gain_f32 != 0, i, gain[0]);
-#pragma unroll
-                for (int e = 0; e < N; ++e) c = fmaf(yv[e] * gain[0][e], sv[e] * rstd, c);
-            }
-            c = team_sum(c, team, red, turn) * inv_d;
-            for (int i = t; i < a.packets; i += team) {
-                load_values<T, VB>(s, i, sv);
-                load_values<T, VB>(gy, i, yv);
-                load_gain<T, N>(a.gain, a.gain_f32 != 0, i, gain[0]);
-                if constexpr (GS) load_values<T, VB>(gs, i, rv);
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    yv[e] = rstd * (yv[e] * gain[0][e] - sv[e] * rstd * c);
-                    if constexpr (GS) yv[e] += rv[e];
-                }
-                store_values<T, VB>(dx, i, yv);
-            }
+        for (int e = 0; e < N; ++e) {
+            const long long col = static_cast<long long>(i) * N + e;
+            w[e] = w[e] * rstd * (a.gain_f32 ? __ldg(static_cast<const float *>(a.gain) + col) : to_float<T>(static_cast<const T *>(a.gain)[col]));
         }
+    };
+    for (int i = threadIdx.x; i < packets; i += team) {
+        fetch(i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) c = fmaf(w[e], sv[e], c);
     }
-    if constexpr (P > 0) {
-        if (!a.partial) return;
-        float *out = a.partial + static_cast<long long>(blockIdx.x) * a.d;
-        if (teams == 1) {
+    const float k = -rstd * rstd * (team_sum(c, team, red, turn) / static_cast<float>(a.d));
+    for (int i = threadIdx.x; i < packets; i += team) {
+        fetch(i);
+        if constexpr (GS) load_values<T, VB>(gs, i, rv);
 #pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (t + p * team < a.packets)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) out[(t + p * team) * N + e] = acc[p][e];
-        } else {
-            extern __shared__ float columns[];  // d floats: the CTA's teams one after the other
-            for (int k = 0; k < teams; ++k) {
-                if (k == mine) {
-#pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        if (t + p * team < a.packets)
-#pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                float *at = columns + (t + p * team) * N + e;
-                                *at = k == 0 ? acc[p][e] : *at + acc[p][e];
-                            }
-                }
-                __syncthreads();
-            }
-            for (int i = threadIdx.x; i < a.d; i += blockDim.x) out[i] = columns[i];
+        for (int e = 0; e < N; ++e) {
+            w[e] = fmaf(sv[e], k, w[e]);
+            if constexpr (GS) w[e] += rv[e];
         }
+        store_values<T, VB>(dx, i, w);
     }
 }
 
 // ---- column sums: partial rows per CTA, then their sum ------------------------------------------------------
 
-// partial[block y][column] = sum of g (times s * rstd where s is given) over the block's rows.  A lane has one column, so a warp reads
-// 32 neighbours; the rows of a block go round its eight warps.
-template <typename T>
+// partial[block y][column] = sum of g (times s * rstd where s is given) over the block's rows.  PER columns a lane, read as one word where the
+// rows allow it; the rows of a block go round its warps, four at a time on their way.
+template <typename T, int PER>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T *g, long long g_stride, const T *s, long long s_stride, const float *rstd, float *partial,
                                                          long long rows, int d, long long rows_per_block) {
-    __shared__ float part[8][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
+    __shared__ float part[8][32 * PER];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.x * 32 + lane) * PER;
     const long long first = blockIdx.y * rows_per_block, last = min(rows, first + rows_per_block);
-    float v = 0.f;
+    float v[PER] = {};
     if (col < d) {
+#pragma unroll 4
         for (long long r = first + warp; r < last; r += 8) {
-            const float dy = to_float<T>(g[r * g_stride + col]);
-            v += s ? dy * to_float<T>(s[r * s_stride + col]) * rstd[r] : dy;
+            float x[PER];
+            load_values<T, PER * static_cast<int>(sizeof(T))>(g + r * g_stride + col, 0, x);
+            if (s) {
+                float y[PER];
+                load_values<T, PER * static_cast<int>(sizeof(T))>(s + r * s_stride + col, 0, y);
+                const float k = rstd[r];
+#pragma unroll
+                for (int e = 0; e < PER; ++e) x[e] *= y[e] * k;
+            }
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[e] += x[e];
         }
     }
-    part[warp][lane] = v;
-    __syncthreads();
-    if (warp == 0 && col < d) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) v += part[k][lane];
-        partial[static_cast<long long>(blockIdx.y) * d + col] = v;
+    for (int e = 0; e < PER; ++e) part[warp][lane * PER + e] = v[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * PER; c += 256) {
+        if (blockIdx.x * 32 * PER + c >= d) break;
+        float sum = part[0][c];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) sum += part[k][c];
+        partial[static_cast<long long>(blockIdx.y) * d + blockIdx.x * 32 * PER + c] = sum;
     }
 }
 
 template <typename O>
-__global__ void __launch_bounds__(256) partial_sum_kernel(const float *partial, int count, int d, O *out) {
-    __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) partial_sum_kernel(const float *partial, int count, int d, O *out) {
+    __shared__ float part[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
     float v = 0.f;
-    if (col < d)
-        for (int k = warp; k < count; k += 8) v += partial[static_cast<long long>(k) * d + col];
+    if (col < d) {
+#pragma unroll 4
+        for (int k = warp; k < count; k += 32) v += partial[static_cast<long long>(k) * d + col];
+    }
     part[warp][lane] = v;
     __syncthreads();
-    if (warp == 0 && col < d) {
+    v = part[lane][warp];  // a warp a column
 #pragma unroll
-        for (int k = 1; k < 8; ++k) v += part[k][lane];
-        out[col] = from_float<O>(v);
-    }
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (lane == 0 && blockIdx.x * 32 + warp < d) out[blockIdx.x * 32 + warp] = from_float<O>(v);
 }
 
 int sum_partials(const float *partial, int count, int d, void *out, int out_dtype, cudaStream_t stream) {
     const dim3 grid((d + 31) / 32);
     if (out_dtype == TH_F32)
-        partial_sum_kernel<float><<<grid, 256, 0, stream>>>(partial, count, d, static_cast<float *>(out));
+        partial_sum_kernel<float><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<float *>(out));
     else if (out_dtype == TH_F16)
-        partial_sum_kernel<__half><<<grid, 256, 0, stream>>>(partial, count, d, static_cast<__half *>(out));
+        partial_sum_kernel<__half><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<__half *>(out));
     else
-        partial_sum_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(partial, count, d, static_cast<__nv_bfloat16 *>(out));
+        partial_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<__nv_bfloat16 *>(out));
     return launch_status("partial_sum_kernel");
 }
 
-// Partial rows a column sum is cut into: enough blocks for the GPU, at least 32 rows each
+// Partial rows a column sum is cut into: some sixteen blocks an SM, at least 64 rows each
 int column_parts(long long rows, int d) {
-    const long long columns = (d + 31) / 32;
-    const long long wanted = std::max(1ll, (8ll * sm_count() + columns - 1) / columns);
-    return static_cast<int>(std::max(1ll, std::min({wanted, (rows + 31) / 32, 1024ll})));
+    const long long columns = (d + 63) / 64;
+    const long long wanted = std::max(1ll, (16ll * sm_count() + columns - 1) / columns);
+    return static_cast<int>(std::max(1ll, std::min({wanted, (rows + 63) / 64, 512ll})));
 }
 
 template <typename T>
 int column_sums(const T *g, long long g_stride, const T *s, long long s_stride, const float *rstd, float *partial, int parts, long long rows, int d,
                 cudaStream_t stream) {
-    const dim3 grid((d + 31) / 32, parts);
-    column_sum_kernel<T><<<grid, 256, 0, stream>>>(g, g_stride, s, s_stride, rstd, partial, rows, d, (rows + parts - 1) / parts);
+    constexpr int kWide = 8 / static_cast<int>(sizeof(T));  // a word of 8 bytes
+    const auto whole = [&](const void *p, long long stride) { return aligned_to(p, 8) && stride % kWide == 0; };
+    const long long per = (rows + parts - 1) / parts;
+    if (d % kWide == 0 && whole(g, g_stride) && (!s || whole(s, s_stride))) {
+        column_sum_kernel<T, kWide><<<dim3((d + 32 * kWide - 1) / (32 * kWide), parts), 256, 0, stream>>>(g, g_stride, s, s_stride, rstd, partial, rows, d, per);
+    } else {
+        column_sum_kernel<T, 1><<<dim3((d + 31) / 32, parts), 256, 0, stream>>>(g, g_stride, s, s_stride, rstd, partial, rows, d, per);
+    }
     return launch_status("column_sum_kernel");
 }
 
 struct NormBwdPlan {
-    TeamPlan team;
-    int blocks, parts;  // partial rows: one per CTA, or (rows too long for registers) those of a column sum
+    int per_thread, team, consumers;  // packets of a thread (0: the stream kernel), threads of a row, consumer threads
+    int parts;                        // partial rows: one per CTA, or those of a column sum
+    RingPlan ring;
 };
 
-// `packed`: 16-byte packets.  Registers hold a thread's sums and gains: 32 columns at most.
-NormBwdPlan norm_bwd_plan(long long rows, int d, int dtype, bool packed) {
+// A thread sums 32 columns at most.  Up to four packets a lane a row is a warp's; longer ones are shared by 256 or 512 threads.  Two CTAs
+// share an SM where two stages of a CTA fit half of it.
+template <typename T>
+NormBwdPlan norm_bwd_plan(long long rows, int d, int kind, bool gs) {
+    constexpr int kMost = sizeof(T) == 4 ? 8 : 4;
     NormBwdPlan p{};
-    const int n = packed ? 16 / static_cast<int>(dtype_bytes(dtype)) : 1;
-    p.team = team_plan(d / n, packed ? (dtype == TH_F32 ? 8 : 4) : 8);
-    const int per_sm = std::max(1, 1024 / p.team.block);
-    p.blocks = static_cast<int>(std::min<long long>((rows + p.team.rows_per_block - 1) / p.team.rows_per_block, static_cast<long long>(sm_count()) * per_sm));
-    p.parts = p.team.per_thread ? p.blocks : column_parts(rows, d);
+    const int packets = span_packets<T>(d, kind);
+    p.parts = column_parts(rows, d);
+    if (kind == kAnyhow || packets > 512 * kMost) return p;
+    const bool wide = packets > 128;
+    p.consumers = packets > 512 ? 512 : 256;
+    p.team = wide ? p.consumers : 32;
+    RingPlan &r = p.ring;
+    r.slot = (packets + 1) * 16;
+    const int tensors = gs ? 3 : 2, budget = (p.consumers == 256 ? 110 : 222) * 1024;
+    // short rows: eight at a time, and more as long as a stage stays small
+    r.rows = wide ? 1 : 8;
+    while (!wide && r.rows < 64 && 2 * r.rows * r.slot * tensors <= 16 * 1024) r.rows *= 2;
+    r.tensor_bytes = r.rows * r.slot + 16;
+    r.stages = std::min(kMaxRing, budget / (tensors * r.tensor_bytes));
+    if (r.stages < 2) return p;
+    int n = 1;
+    while (n * p.team < packets) n *= 2;
+    p.per_thread = n;
+    r.blocks = (rows + r.rows - 1) / r.rows;
+    // one round of CTAs; where a row is a CTA's, a multiple of eight of them
+    const long long room = static_cast<long long>(sm_count()) * (p.consumers == 256 ? 2 : 1);
+    p.parts = static_cast<int>(wide ? std::min((r.blocks + 7) / 8 * 8, std::max(8ll, room / 8 * 8)) : std::min(r.blocks, room));
     return p;
 }
 
-template <typename T, int VB, bool GS>
+template <typename T, bool GS, bool SHIFT, int CONSUMERS>
 int launch_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
-    constexpr int N = VB / static_cast<int>(sizeof(T));
-    const dim3 grid(plan.blocks), block(plan.team.block);
-    const size_t smem = plan.team.team == 32 ? static_cast<size_t>(a.d) * 4 : 0;
-    switch (plan.team.per_thread) {
-        case 1: norm_bwd_kernel<T, VB, 1, GS><<<grid, block, smem, stream>>>(a); break;
-        case 2: norm_bwd_kernel<T, VB, 2, GS><<<grid, block, smem, stream>>>(a); break;
-        case 4: norm_bwd_kernel<T, VB, 4, GS><<<grid, block, smem, stream>>>(a); break;
-        case 8:
-            if constexpr (N < 8) norm_bwd_kernel<T, VB, 8, GS><<<grid, block, smem, stream>>>(a);
-            break;
-        default: norm_bwd_kernel<T, VB, 0, GS><<<grid, block, 0, stream>>>(a); break;
+    const size_t smem = static_cast<size_t>(plan.ring.stages) * (GS ? 3 : 2) * plan.ring.tensor_bytes;
+    const auto run = [&](auto kernel) -> int {
+        if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "cudaFuncSetAttribute(norm_bwd_kernel)"))
+            return rc;
+        kernel<<<plan.parts, CONSUMERS + 32, smem, stream>>>(a, plan.ring);
+        return launch_status("norm_bwd_kernel");
+    };
+    switch (plan.per_thread) {
+        case 1: return run(norm_bwd_kernel<T, 1, GS, SHIFT, CONSUMERS>);
+        case 2: return run(norm_bwd_kernel<T, 2, GS, SHIFT, CONSUMERS>);
+        case 4: return run(norm_bwd_kernel<T, 4, GS, SHIFT, CONSUMERS>);
+        default: break;
     }
-    return launch_status("norm_bwd_kernel");
+    if constexpr (sizeof(T) == 4) return run(norm_bwd_kernel<T, 8, GS, SHIFT, CONSUMERS>);
+    return fail(TH_ERR_UNSUPPORTED, "norm_bwd_kernel: %d packets a thread", plan.per_thread);
+}
+
+template <typename T, bool GS, bool SHIFT>
+int size_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
+    return plan.consumers == 256 ? launch_norm_bwd<T, GS, SHIFT, 256>(a, plan, stream) : launch_norm_bwd<T, GS, SHIFT, 512>(a, plan, stream);
 }
 
 template <typename T>
-int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, bool packed, const NormBwdPlan &plan, cudaStream_t stream) {
-    constexpr int E = sizeof(T);
-    a.packets = packed ? a.d / (16 / E) : a.d;
-    a.team = plan.team.team;
+int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, cudaStream_t stream) {
+    Layout rows;
+    rows.add<T>(a.s, a.s_stride, a.d);
+    rows.add<T>(a.gy, a.gy_stride, a.d);
+    rows.add<T>(a.gs, a.gs_stride, a.d);
+    rows.add<T>(a.dx, a.d, a.d);
+    const int kind = aligned_to(a.gain, 16) || rows.kind() == kShifted ? rows.kind() : kAnyhow;
+    NormBwdPlan plan = norm_bwd_plan<T>(a.rows, a.d, kind, a.gs != nullptr);
+    plan.ring.whole[0] = a.s_stride == a.d;
+    plan.ring.whole[1] = a.gy_stride == a.d;
+    plan.ring.whole[2] = a.gs_stride == a.d;
     float *partial = a.partial;
+    a.team = plan.team;
     if (!dgain) a.partial = nullptr;
     int rc;
-    if (a.gs)
-        rc = packed ? launch_norm_bwd<T, 16, true>(a, plan, stream) : launch_norm_bwd<T, E, true>(a, plan, stream);
-    else
-        rc = packed ? launch_norm_bwd<T, 16, false>(a, plan, stream) : launch_norm_bwd<T, E, false>(a, plan, stream);
-    if (rc != TH_OK || !dgain) return rc;
-    if (!plan.team.per_thread) {
-        rc = column_sums<T>(static_cast<const T *>(a.gy), a.gy_stride, static_cast<const T *>(a.s), a.s_stride, a.rstd, partial, plan.parts, a.rows, a.d, stream);
-        if (rc != TH_OK) return rc;
+    if (plan.per_thread) {
+        if (kind == kPacked) rc = a.gs ? size_norm_bwd<T, true, false>(a, plan, stream) : size_norm_bwd<T, false, false>(a, plan, stream);
+        else rc = a.gs ? size_norm_bwd<T, true, true>(a, plan, stream) : size_norm_bwd<T, false, true>(a, plan, stream);
+        return rc != TH_OK || !dgain ? rc : sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
     }
-    return sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
+    if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
+    const unsigned grid = static_cast<unsigned>(a.rows);
+    const int block = std::min(kMaxTeam, std::max(64, (a.d / 8 + 31) / 32 * 32));
+    if (kind == kPacked) {
+        if (a.gs) norm_bwd_stream_kernel<T, 16, true><<<grid, block, 0, stream>>>(a);
+        else norm_bwd_stream_kernel<T, 16, false><<<grid, block, 0, stream>>>(a);
+    } else {
+        if (a.gs) norm_bwd_stream_kernel<T, sizeof(T), true><<<grid, block, 0, stream>>>(a);
+        else norm_bwd_stream_kernel<T, sizeof(T), false><<<grid, block, 0, stream>>>(a);
+    }
+    rc = launch_status("norm_bwd_stream_kernel");
+    if (rc != TH_OK || !dgain) return rc;
+    rc = column_sums<T>(static_cast<const T *>(a.gy), a.gy_stride, static_cast<const T *>(a.s), a.s_stride, a.rstd, partial, plan.parts, a.rows, a.d, stream);
+    return rc != TH_OK ? rc : sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
 }
 
 // ---- 8-bit rows back to 16 or 32 bits --------------------------------------------------------------------------
@@ -627,6 +985,12 @@ int check_rows(const char *what, long long rows, int d, int dtype) {
 }
 
 }  // namespace
+
+int rows_status_word() {
+    int status = 0;
+    return cudaMemcpyFromSymbol(&status, g_rows_status, sizeof(int)) == cudaSuccess ? status : -1;
+}
+
 }  // namespace th
 
 using namespace th;
@@ -688,12 +1052,13 @@ extern "C" int th_dequantize_rows(const void *q_dev, int64_t q_stride, const flo
     return launch_status("dequantize_kernel");
 }
 
-// The scratch is the larger of what rows in 16-byte packets and rows read value by value take.
+// The most that any layout of the rows takes.
 extern "C" int64_t th_rms_norm_bwd_workspace_bytes(int64_t rows, int d, int dtype) {
     if (rows < 1 || d < 1 || !known_dtype(dtype)) return 0;
-    const int whole = 16 / static_cast<int>(dtype_bytes(dtype));
-    int parts = norm_bwd_plan(rows, d, dtype, false).parts;
-    if (d % whole == 0) parts = std::max(parts, norm_bwd_plan(rows, d, dtype, true).parts);
+    int parts = 0;
+    for (int kind : {kPacked, kShifted, kAnyhow})
+        for (bool gs : {false, true})
+            parts = std::max(parts, dtype == TH_F32 ? norm_bwd_plan<float>(rows, d, kind, gs).parts : norm_bwd_plan<__half>(rows, d, kind, gs).parts);
     return static_cast<int64_t>(parts) * d * 4;
 }
 
@@ -714,15 +1079,9 @@ extern "C" int th_rms_norm_bwd(const void *sum_dev, int64_t sum_stride, const vo
     a.s = sum_dev; a.gain = gain_dev; a.gy = grad_y_dev; a.gs = grad_sum_dev; a.rstd = rstd_dev; a.dx = grad_x_dev;
     a.partial = static_cast<float *>(workspace_dev);
     a.s_stride = sum_stride; a.gy_stride = gy_stride; a.gs_stride = gs_stride; a.rows = rows; a.d = d; a.gain_f32 = gain_dtype == TH_F32;
-    const auto run = [&](auto tag) {
-        using T = decltype(tag);
-        const bool packed = packed_rows<T>(a.s, a.s_stride, d) && packed_rows<T>(a.gy, a.gy_stride, d) && packed_rows<T>(a.gs, a.gs_stride, d) &&
-                            packed_rows<T>(a.dx, d, d) && aligned_to(a.gain, 16);
-        return norm_bwd<T>(a, grad_gain_dev, gain_dtype, packed, norm_bwd_plan(rows, d, dtype, packed), at);
-    };
-    if (dtype == TH_F32) return run(float{});
-    if (dtype == TH_F16) return run(__half{});
-    return run(__nv_bfloat16{});
+    if (dtype == TH_F32) return norm_bwd<float>(a, grad_gain_dev, gain_dtype, at);
+    if (dtype == TH_F16) return norm_bwd<__half>(a, grad_gain_dev, gain_dtype, at);
+    return norm_bwd<__nv_bfloat16>(a, grad_gain_dev, gain_dtype, at);
 }
 
 extern "C" int64_t th_column_sum_workspace_bytes(int64_t rows, int d) {

@@ -111,12 +111,17 @@ int check_16bit(const char *what, int dtype) {
 }  // namespace
 }  // namespace th
 
+namespace th {
+int rows_status_word();  // rows.cu
+}
+
 using namespace th;
 
 extern "C" int th_linear_tc_status(void) {
     int status = 0;
     if (cudaMemcpyFromSymbol(&status, g_tc_status, sizeof(int)) != cudaSuccess) return -1;
-    return status;
+    const int rows = rows_status_word();
+    return rows < 0 ? -1 : status | rows;
 }
 
 extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride,
