@@ -1,0 +1,36 @@
+// Launches that overlap their start with the end of the kernel before (programmatic dependent launch).  Each kernel of the wide layers lets
+// the next one start as soon as all of its own CTAs have (start_next), and touches no global memory before the kernels ahead of it
+// have finished (after_previous): what overlaps is the launch and the set-up of barriers, tensor memory and descriptors.  A neighbour that
+// knows nothing of this runs strictly before or after.
+#pragma once
+
+#include "common.cuh"
+
+namespace th {
+namespace {
+
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+int launch_chained(const char *what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, unsigned cluster, Args &&...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    note_launch();
+    return cuda_status(err, what);
+}
+
+}  // namespace
+}  // namespace th

@@ -5,9 +5,10 @@
 // 8-bit rows:  a = max(max_k |x_k|, 2^-100),  q_k = rint(x_k * (127 / a)),  scale = a / 127, all in float32, so that a row is the
 // same bits from any kernel (and from elementary operations elsewhere).  The floor keeps 127 / a finite: a row of zeros has zeros and
 // a scale of 2^-100 / 127.  A row that holds an infinity or a NaN gets zeros and a NaN as its scale: it reads back as NaN throughout.
-#include "common.cuh"
+#include "chained.cuh"
 
 #include <algorithm>
+#include <utility>
 
 namespace th {
 namespace {
@@ -212,6 +213,8 @@ __global__ void __launch_bounds__(THREADS) row_fwd_kernel(const RowFwdArgs a) {
     constexpr int N = 16 / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
+    start_next();
+    after_previous();
     const int team = a.team, t = team == 32 ? threadIdx.x & 31 : threadIdx.x;
     const long long row = team == 32 ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;  // whole warps, and only where a warp is a team
@@ -301,6 +304,8 @@ __global__ void __launch_bounds__(kMaxTeam) row_fwd_stream_kernel(const RowFwdAr
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
+    start_next();
+    after_previous();
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
@@ -414,14 +419,12 @@ int span_packets(int d, int kind) {
 
 template <typename T, int MODE, bool RES, bool SHIFT, int THREADS>
 int launch_row_fwd(const RowFwdArgs &a, const TeamPlan &plan, unsigned blocks, cudaStream_t stream) {
-    const dim3 grid(blocks), block(plan.block);
     switch (plan.per_thread) {
-        case 1: row_fwd_kernel<T, 1, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
-        case 2: row_fwd_kernel<T, 2, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
-        case 4: row_fwd_kernel<T, 4, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
-        default: row_fwd_kernel<T, 8, MODE, RES, SHIFT, THREADS><<<grid, block, 0, stream>>>(a); break;
+        case 1: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 1, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
+        case 2: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 2, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
+        case 4: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 4, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
+        default: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 8, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
     }
-    return launch_status("row_fwd_kernel");
 }
 
 template <typename T, int MODE, bool RES>
@@ -449,9 +452,8 @@ int plan_row_fwd(RowFwdArgs a, cudaStream_t stream) {
                                    : launch_row_fwd<T, MODE, RES, true, kMaxTeam>(a, plan, n, stream);
     }
     const int block = std::min(kMaxTeam, std::max(64, (a.d / 8 + 31) / 32 * 32));
-    if (kind == kPacked) row_fwd_stream_kernel<T, 16, MODE, RES><<<all, block, 0, stream>>>(a);
-    else row_fwd_stream_kernel<T, sizeof(T), MODE, RES><<<all, block, 0, stream>>>(a);
-    return launch_status("row_fwd_stream_kernel");
+    return launch_chained("row_fwd_stream_kernel", kind == kPacked ? row_fwd_stream_kernel<T, 16, MODE, RES> : row_fwd_stream_kernel<T, sizeof(T), MODE, RES>, all,
+                          block, 0, stream, 1, a);
 }
 
 template <typename T, int MODE>
@@ -547,6 +549,7 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
     __shared__ float red[2][32];
     __shared__ int abort_flag;
     const auto shared = [](const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); };
+    start_next();
     const int stage_bytes = kTensors * ring.tensor_bytes;
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -557,6 +560,7 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const char *base[3] = {static_cast<const char *>(a.s), static_cast<const char *>(a.gy), static_cast<const char *>(a.gs)};
     const long long pitch[3] = {a.s_stride * static_cast<long long>(sizeof(T)), a.gy_stride * static_cast<long long>(sizeof(T)),
@@ -727,6 +731,8 @@ __global__ void __launch_bounds__(kMaxTeam) norm_bwd_stream_kernel(const RowBwdA
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
+    start_next();
+    after_previous();
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
     const T *s = static_cast<const T *>(a.s) + row * a.s_stride, *gy = static_cast<const T *>(a.gy) + row * a.gy_stride;
@@ -769,6 +775,8 @@ template <typename T, int PER>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T *g, long long g_stride, const T *s, long long s_stride, const float *rstd, float *partial,
                                                          long long rows, int d, long long rows_per_block) {
     __shared__ float part[8][32 * PER];
+    start_next();
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.x * 32 + lane) * PER;
     const long long first = blockIdx.y * rows_per_block, last = min(rows, first + rows_per_block);
     float v[PER] = {};
@@ -803,6 +811,8 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T *g, long long g
 template <typename O>
 __global__ void __launch_bounds__(1024) partial_sum_kernel(const float *partial, int count, int d, O *out) {
     __shared__ float part[32][33];
+    start_next();
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (col < d) {
@@ -818,14 +828,10 @@ __global__ void __launch_bounds__(1024) partial_sum_kernel(const float *partial,
 }
 
 int sum_partials(const float *partial, int count, int d, void *out, int out_dtype, cudaStream_t stream) {
-    const dim3 grid((d + 31) / 32);
-    if (out_dtype == TH_F32)
-        partial_sum_kernel<float><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<float *>(out));
-    else if (out_dtype == TH_F16)
-        partial_sum_kernel<__half><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<__half *>(out));
-    else
-        partial_sum_kernel<__nv_bfloat16><<<grid, 1024, 0, stream>>>(partial, count, d, static_cast<__nv_bfloat16 *>(out));
-    return launch_status("partial_sum_kernel");
+    const unsigned grid = (d + 31) / 32;
+    if (out_dtype == TH_F32) return launch_chained("partial_sum_kernel", partial_sum_kernel<float>, grid, 1024, 0, stream, 1, partial, count, d, static_cast<float *>(out));
+    if (out_dtype == TH_F16) return launch_chained("partial_sum_kernel", partial_sum_kernel<__half>, grid, 1024, 0, stream, 1, partial, count, d, static_cast<__half *>(out));
+    return launch_chained("partial_sum_kernel", partial_sum_kernel<__nv_bfloat16>, grid, 1024, 0, stream, 1, partial, count, d, static_cast<__nv_bfloat16 *>(out));
 }
 
 // Partial rows a column sum is cut into: some sixteen blocks an SM, at least 64 rows each
@@ -841,12 +847,11 @@ int column_sums(const T *g, long long g_stride, const T *s, long long s_stride, 
     constexpr int kWide = 8 / static_cast<int>(sizeof(T));  // a word of 8 bytes
     const auto whole = [&](const void *p, long long stride) { return aligned_to(p, 8) && stride % kWide == 0; };
     const long long per = (rows + parts - 1) / parts;
-    if (d % kWide == 0 && whole(g, g_stride) && (!s || whole(s, s_stride))) {
-        column_sum_kernel<T, kWide><<<dim3((d + 32 * kWide - 1) / (32 * kWide), parts), 256, 0, stream>>>(g, g_stride, s, s_stride, rstd, partial, rows, d, per);
-    } else {
-        column_sum_kernel<T, 1><<<dim3((d + 31) / 32, parts), 256, 0, stream>>>(g, g_stride, s, s_stride, rstd, partial, rows, d, per);
-    }
-    return launch_status("column_sum_kernel");
+    if (d % kWide == 0 && whole(g, g_stride) && (!s || whole(s, s_stride)))
+        return launch_chained("column_sum_kernel", column_sum_kernel<T, kWide>, dim3((d + 32 * kWide - 1) / (32 * kWide), parts), 256, 0, stream, 1, g, g_stride, s,
+                              s_stride, rstd, partial, rows, d, per);
+    return launch_chained("column_sum_kernel", column_sum_kernel<T, 1>, dim3((d + 31) / 32, parts), 256, 0, stream, 1, g, g_stride, s, s_stride, rstd, partial, rows, d,
+                          per);
 }
 
 struct NormBwdPlan {
@@ -892,8 +897,7 @@ int launch_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t s
     const auto run = [&](auto kernel) -> int {
         if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "cudaFuncSetAttribute(norm_bwd_kernel)"))
             return rc;
-        kernel<<<plan.parts, CONSUMERS + 32, smem, stream>>>(a, plan.ring);
-        return launch_status("norm_bwd_kernel");
+        return launch_chained("norm_bwd_kernel", kernel, plan.parts, CONSUMERS + 32, smem, stream, 1, a, plan.ring);
     };
     switch (plan.per_thread) {
         case 1: return run(norm_bwd_kernel<T, 1, GS, SHIFT, CONSUMERS>);
@@ -934,14 +938,8 @@ int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, cudaStream_t stream) {
     if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
     const unsigned grid = static_cast<unsigned>(a.rows);
     const int block = std::min(kMaxTeam, std::max(64, (a.d / 8 + 31) / 32 * 32));
-    if (kind == kPacked) {
-        if (a.gs) norm_bwd_stream_kernel<T, 16, true><<<grid, block, 0, stream>>>(a);
-        else norm_bwd_stream_kernel<T, 16, false><<<grid, block, 0, stream>>>(a);
-    } else {
-        if (a.gs) norm_bwd_stream_kernel<T, sizeof(T), true><<<grid, block, 0, stream>>>(a);
-        else norm_bwd_stream_kernel<T, sizeof(T), false><<<grid, block, 0, stream>>>(a);
-    }
-    rc = launch_status("norm_bwd_stream_kernel");
+    if (kind == kPacked) rc = launch_chained("norm_bwd_stream_kernel", a.gs ? norm_bwd_stream_kernel<T, 16, true> : norm_bwd_stream_kernel<T, 16, false>, grid, block, 0, stream, 1, a);
+    else rc = launch_chained("norm_bwd_stream_kernel", a.gs ? norm_bwd_stream_kernel<T, sizeof(T), true> : norm_bwd_stream_kernel<T, sizeof(T), false>, grid, block, 0, stream, 1, a);
     if (rc != TH_OK || !dgain) return rc;
     rc = column_sums<T>(static_cast<const T *>(a.gy), a.gy_stride, static_cast<const T *>(a.s), a.s_stride, a.rstd, partial, plan.parts, a.rows, a.d, stream);
     return rc != TH_OK ? rc : sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
@@ -953,6 +951,8 @@ int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, cudaStream_t stream) {
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const signed char *q, long long q_stride, const float *scale, T *out, long long out_stride,
                                                          long long rows, int d, int chunks) {
+    start_next();
+    after_previous();
     const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     const long long row = id / chunks;
     if (row >= rows) return;
@@ -1043,13 +1043,10 @@ extern "C" int th_dequantize_rows(const void *q_dev, int64_t q_stride, const flo
     const dim3 grid(static_cast<unsigned>((rows * chunks + 255) / 256));
     cudaStream_t at = static_cast<cudaStream_t>(stream);
     const signed char *q = static_cast<const signed char *>(q_dev);
-    if (dtype == TH_F32)
-        dequantize_kernel<float><<<grid, 256, 0, at>>>(q, q_stride, scale_dev, static_cast<float *>(out_dev), out_stride, rows, d, chunks);
-    else if (dtype == TH_F16)
-        dequantize_kernel<__half><<<grid, 256, 0, at>>>(q, q_stride, scale_dev, static_cast<__half *>(out_dev), out_stride, rows, d, chunks);
-    else
-        dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, at>>>(q, q_stride, scale_dev, static_cast<__nv_bfloat16 *>(out_dev), out_stride, rows, d, chunks);
-    return launch_status("dequantize_kernel");
+    const auto run = [&](auto kernel, auto *out) { return launch_chained("dequantize_kernel", kernel, grid, 256, 0, at, 1, q, q_stride, scale_dev, out, out_stride, rows, d, chunks); };
+    if (dtype == TH_F32) return run(dequantize_kernel<float>, static_cast<float *>(out_dev));
+    if (dtype == TH_F16) return run(dequantize_kernel<__half>, static_cast<__half *>(out_dev));
+    return run(dequantize_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16 *>(out_dev));
 }
 
 // The most that any layout of the rows takes.

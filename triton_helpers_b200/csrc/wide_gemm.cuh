@@ -13,9 +13,11 @@
 // finishes a part of the tile from everybody's, added in rank order, so that there is no scratch, no second launch, and results repeat.
 #pragma once
 
+#include "chained.cuh"
 #include "tc_tiles.cuh"
 
 #include <algorithm>
+#include <utility>
 
 namespace th {
 namespace {
@@ -300,6 +302,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     const uint32_t place = CG == 2 ? cluster_rank() : 0, rank = place % CG, leader = place - rank;
     const int units = g.tiles_m * g.tiles_n * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
+    start_next();
     if (threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a_map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&b_map)) : "memory");
@@ -333,6 +336,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     if constexpr (CG == 2) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
+    after_previous();
 
     if (warp == 0) {
         // ---- operands ----
@@ -584,20 +588,7 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "matrix product: too many tiles");
     // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles
     const long long clusters = g.splits > 1 ? units : std::min<long long>(units, CTAS * sm_count() / CG);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * CG));
-    cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = S::kBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = CG * g.splits;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = attr.val.clusterDim.x > 1 ? 1 : 0;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, g, a_map, b_map, c_map);
-    note_launch();
-    return cuda_status(err, "wide_gemm_kernel launch");
+    return launch_chained("wide_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), kGemmThreads, S::kBytes, stream, CG * g.splits, g, a_map, b_map, c_map);
 }
 
 }  // namespace
