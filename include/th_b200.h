@@ -432,6 +432,13 @@ int64_t th_column_sum_workspace_bytes(int64_t rows, int d);
 int th_column_sum(const void *g_dev, int64_t g_stride, void *out_dev, void *workspace_dev,
                   int64_t workspace_bytes, int64_t rows, int d, int dtype, void *stream);
 
+/* th_dequantize_rows into x_dev and th_column_sum of g_dev (rows x d_out) into out_dev in one launch (float16 or
+ * bfloat16; the scratch is th_column_sum's): what the backward pass of a checkpointed linear layer needs ahead of
+ * the weight's gradient, and the bias's gradient. */
+int th_checkpoint_rows(const void *q_dev, int64_t q_stride, const float *scale_dev, void *x_dev, int64_t x_stride,
+                       int d_in, const void *g_dev, int64_t g_stride, void *out_dev, int d_out,
+                       void *workspace_dev, int64_t workspace_bytes, int64_t rows, int dtype, void *stream);
+
 /* y[r, n] = scale[r] * weight_scale[n] * sum_k q[r, k] weight[n, k] + bias[n]: 8-bit rows on both sides, exact
  * 32-bit integer sums (d_in up to 131071), y and bias in `dtype`; the bias may be null. */
 int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev,

@@ -24,8 +24,6 @@ struct Raw;
 template <>
 struct Raw<16> { using type = uint4; };
 template <>
-struct Raw<8> { using type = uint2; };
-template <>
 struct Raw<4> { using type = uint32_t; };
 template <>
 struct Raw<2> { using type = unsigned short; };
@@ -769,26 +767,31 @@ __global__ void __launch_bounds__(kMaxTeam) norm_bwd_stream_kernel(const RowBwdA
 
 // ---- column sums: partial rows per CTA, then their sum ------------------------------------------------------
 
-// partial[block y][column] = sum of g (times s * rstd where s is given) over the block's rows.  PER columns a lane, read as one word where the
-// rows allow it; the rows of a block go round its warps, four at a time on their way.
+struct ColumnArgs {
+    const void *g, *s;       // sums of g, or of g * s * rstd
+    const float *rstd;
+    void *out;               // [parts][d]: float32 partial rows, or the result itself where there is one part and `whole` is set
+    long long g_stride, s_stride, rows, per_part;
+    int d, whole;
+};
+
+// One block's columns over one part of the rows.  PER columns a lane: 16 bytes where the rows start on them (the last ones may reach past
+// the row, to values that no result is made of), else one; the rows go round the block's 32 warps, eight at a time on their way.
 template <typename T, int PER>
-__global__ void __launch_bounds__(256) column_sum_kernel(const T *g, long long g_stride, const T *s, long long s_stride, const float *rstd, float *partial,
-                                                         long long rows, int d, long long rows_per_block) {
-    __shared__ float part[8][32 * PER];
-    start_next();
-    after_previous();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (blockIdx.x * 32 + lane) * PER;
-    const long long first = blockIdx.y * rows_per_block, last = min(rows, first + rows_per_block);
+__device__ __forceinline__ void column_sums_of(const ColumnArgs &a, int block, int part_index, float *part) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (block * 32 + lane) * PER;
+    const long long first = part_index * a.per_part, last = min(a.rows, first + a.per_part);
+    const T *g = static_cast<const T *>(a.g), *s = static_cast<const T *>(a.s);
     float v[PER] = {};
-    if (col < d) {
-#pragma unroll 4
-        for (long long r = first + warp; r < last; r += 8) {
+    if (col < a.d) {
+#pragma unroll 8
+        for (long long r = first + warp; r < last; r += 32) {
             float x[PER];
-            load_values<T, PER * static_cast<int>(sizeof(T))>(g + r * g_stride + col, 0, x);
+            load_values<T, PER * static_cast<int>(sizeof(T))>(g + r * a.g_stride + col, 0, x);
             if (s) {
                 float y[PER];
-                load_values<T, PER * static_cast<int>(sizeof(T))>(s + r * s_stride + col, 0, y);
-                const float k = rstd[r];
+                load_values<T, PER * static_cast<int>(sizeof(T))>(s + r * a.s_stride + col, 0, y);
+                const float k = a.rstd[r];
 #pragma unroll
                 for (int e = 0; e < PER; ++e) x[e] *= y[e] * k;
             }
@@ -796,16 +799,32 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T *g, long long g
             for (int e = 0; e < PER; ++e) v[e] += x[e];
         }
     }
+    // the warps' sums: PER of them a thread, then the 32 / PER groups of every column
+    constexpr int kColumns = 32 * PER;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) part[warp][lane * PER + e] = v[e];
+    for (int e = 0; e < PER; ++e) part[warp * kColumns + lane * PER + e] = v[e];
     __syncthreads();
-    for (int c = threadIdx.x; c < 32 * PER; c += 256) {
-        if (blockIdx.x * 32 * PER + c >= d) break;
-        float sum = part[0][c];
+    const int c = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
+    float sum = 0.f;
 #pragma unroll
-        for (int k = 1; k < 8; ++k) sum += part[k][c];
-        partial[static_cast<long long>(blockIdx.y) * d + blockIdx.x * 32 * PER + c] = sum;
+    for (int k = 0; k < PER; ++k) sum += part[(group * PER + k) * kColumns + c];
+    __syncthreads();
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < kColumns && block * kColumns + c < a.d) {
+#pragma unroll
+        for (int k = 1; k < 32 / PER; ++k) sum += part[k * kColumns + c];
+        if (a.whole) static_cast<T *>(a.out)[block * kColumns + c] = from_float<T>(sum);
+        else static_cast<float *>(a.out)[static_cast<long long>(part_index) * a.d + block * kColumns + c] = sum;
     }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnArgs a) {
+    __shared__ float part[1024 * PER];
+    start_next();
+    after_previous();
+    column_sums_of<T, PER>(a, blockIdx.x, blockIdx.y, part);
 }
 
 template <typename O>
@@ -834,24 +853,30 @@ int sum_partials(const float *partial, int count, int d, void *out, int out_dtyp
     return launch_chained("partial_sum_kernel", partial_sum_kernel<__nv_bfloat16>, grid, 1024, 0, stream, 1, partial, count, d, static_cast<__nv_bfloat16 *>(out));
 }
 
-// Partial rows a column sum is cut into: some sixteen blocks an SM, at least 64 rows each
+// Partial rows a column sum is cut into: two blocks an SM, at least 128 rows each; up to 512 rows are summed at once.
 int column_parts(long long rows, int d) {
-    const long long columns = (d + 63) / 64;
-    const long long wanted = std::max(1ll, (16ll * sm_count() + columns - 1) / columns);
-    return static_cast<int>(std::max(1ll, std::min({wanted, (rows + 63) / 64, 512ll})));
+    if (rows <= 512) return 1;
+    const long long columns = (d + 255) / 256;
+    return static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / std::min<long long>(columns, 2ll * sm_count()), rows / 128, 256ll})));
 }
 
 template <typename T>
-int column_sums(const T *g, long long g_stride, const T *s, long long s_stride, const float *rstd, float *partial, int parts, long long rows, int d,
-                cudaStream_t stream) {
-    constexpr int kWide = 8 / static_cast<int>(sizeof(T));  // a word of 8 bytes
-    const auto whole = [&](const void *p, long long stride) { return aligned_to(p, 8) && stride % kWide == 0; };
-    const long long per = (rows + parts - 1) / parts;
-    if (d % kWide == 0 && whole(g, g_stride) && (!s || whole(s, s_stride)))
-        return launch_chained("column_sum_kernel", column_sum_kernel<T, kWide>, dim3((d + 32 * kWide - 1) / (32 * kWide), parts), 256, 0, stream, 1, g, g_stride, s,
-                              s_stride, rstd, partial, rows, d, per);
-    return launch_chained("column_sum_kernel", column_sum_kernel<T, 1>, dim3((d + 31) / 32, parts), 256, 0, stream, 1, g, g_stride, s, s_stride, rstd, partial, rows, d,
-                          per);
+int column_width(const ColumnArgs &a) {
+    constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+    const auto whole = [&](const void *p, long long stride) { return aligned_to(p, 16) && stride % kWide == 0; };
+    return whole(a.g, a.g_stride) && (!a.s || whole(a.s, a.s_stride)) ? kWide : 1;
+}
+
+// Column sums into `out` of the given type, by way of `partial` where there is more than one part
+template <typename T>
+int column_sums(ColumnArgs a, float *partial, void *out, int out_dtype, cudaStream_t stream) {
+    const int parts = column_parts(a.rows, a.d), width = column_width<T>(a);
+    a.per_part = (a.rows + parts - 1) / parts;
+    a.whole = parts == 1 && (out_dtype == TH_F32) == (sizeof(T) == 4);
+    a.out = a.whole ? out : partial;
+    const dim3 grid((a.d + 32 * width - 1) / (32 * width), parts);
+    const int rc = launch_chained("column_sum_kernel", width > 1 ? column_sum_kernel<T, 16 / sizeof(T)> : column_sum_kernel<T, 1>, grid, 1024, 0, stream, 1, a);
+    return rc != TH_OK || a.whole ? rc : sum_partials(partial, parts, a.d, out, out_dtype, stream);
 }
 
 struct NormBwdPlan {
@@ -941,26 +966,32 @@ int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, cudaStream_t stream) {
     if (kind == kPacked) rc = launch_chained("norm_bwd_stream_kernel", a.gs ? norm_bwd_stream_kernel<T, 16, true> : norm_bwd_stream_kernel<T, 16, false>, grid, block, 0, stream, 1, a);
     else rc = launch_chained("norm_bwd_stream_kernel", a.gs ? norm_bwd_stream_kernel<T, sizeof(T), true> : norm_bwd_stream_kernel<T, sizeof(T), false>, grid, block, 0, stream, 1, a);
     if (rc != TH_OK || !dgain) return rc;
-    rc = column_sums<T>(static_cast<const T *>(a.gy), a.gy_stride, static_cast<const T *>(a.s), a.s_stride, a.rstd, partial, plan.parts, a.rows, a.d, stream);
-    return rc != TH_OK ? rc : sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
+    ColumnArgs sums{};
+    sums.g = a.gy; sums.s = a.s; sums.rstd = a.rstd;
+    sums.g_stride = a.gy_stride; sums.s_stride = a.s_stride; sums.rows = a.rows; sums.d = a.d;
+    return column_sums<T>(sums, partial, dgain, gain_dtype, stream);
 }
 
 // ---- 8-bit rows back to 16 or 32 bits --------------------------------------------------------------------------
 
+struct DequantizeArgs {
+    const signed char *q;
+    const float *scale;
+    void *out;
+    long long q_stride, out_stride, rows;
+    int d, chunks;
+};
+
 // Sixteen columns a thread.  q * scale is rounded once, to T.
 template <typename T>
-__global__ void __launch_bounds__(256) dequantize_kernel(const signed char *q, long long q_stride, const float *scale, T *out, long long out_stride,
-                                                         long long rows, int d, int chunks) {
-    start_next();
-    after_previous();
-    const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    const long long row = id / chunks;
-    if (row >= rows) return;
-    const int c = static_cast<int>(id - row * chunks) * 16;
-    const float s = scale[row];
-    const signed char *src = q + row * q_stride + c;
-    T *dst = out + row * out_stride + c;
-    const bool whole = c + 16 <= d && ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
+__device__ __forceinline__ void dequantize(const DequantizeArgs &a, long long id) {
+    const long long row = id / a.chunks;
+    if (row >= a.rows) return;
+    const int c = static_cast<int>(id - row * a.chunks) * 16;
+    const float s = a.scale[row];
+    const signed char *src = a.q + row * a.q_stride + c;
+    T *dst = static_cast<T *>(a.out) + row * a.out_stride + c;
+    const bool whole = c + 16 <= a.d && ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
     if (whole) {
         const uint4 raw = *reinterpret_cast<const uint4 *>(src);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -971,8 +1002,39 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const signed char *q, l
             if (k % p.N == p.N - 1) reinterpret_cast<uint4 *>(dst)[k / p.N] = p.raw;
         }
     } else {
-        for (int k = 0; k < 16 && c + k < d; ++k) dst[k] = from_float<T>(static_cast<float>(src[k]) * s);
+        for (int k = 0; k < 16 && c + k < a.d; ++k) dst[k] = from_float<T>(static_cast<float>(src[k]) * s);
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a) {
+    start_next();
+    after_previous();
+    dequantize<T>(a, static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
+}
+
+// What the weight's gradient reads and the bias's gradient, in one launch: the first blocks sum columns (they take longer), the others turn
+// 8-bit rows into T.
+template <typename T, int PER>
+__global__ void __launch_bounds__(1024) checkpoint_rows_kernel(const DequantizeArgs rows, const ColumnArgs sums, int column_blocks, int sum_blocks) {
+    __shared__ float part[1024 * PER];
+    start_next();
+    after_previous();
+    if (blockIdx.x < sum_blocks) column_sums_of<T, PER>(sums, blockIdx.x % column_blocks, blockIdx.x / column_blocks, part);
+    else dequantize<T>(rows, static_cast<long long>(blockIdx.x - sum_blocks) * 1024 + threadIdx.x);
+}
+
+template <typename T>
+int checkpoint_rows(const DequantizeArgs &rows, ColumnArgs sums, float *partial, void *out, int dtype, cudaStream_t stream) {
+    const int parts = column_parts(sums.rows, sums.d), width = column_width<T>(sums), columns = (sums.d + 32 * width - 1) / (32 * width);
+    sums.per_part = (sums.rows + parts - 1) / parts;
+    sums.whole = parts == 1;
+    sums.out = sums.whole ? out : partial;
+    const long long blocks = static_cast<long long>(columns) * parts + (rows.rows * rows.chunks + 1023) / 1024;
+    if (blocks > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "th_checkpoint_rows: too many rows: %lld", rows.rows);
+    const int rc = launch_chained("checkpoint_rows_kernel", width > 1 ? checkpoint_rows_kernel<T, 16 / sizeof(T)> : checkpoint_rows_kernel<T, 1>,
+                                  static_cast<unsigned>(blocks), 1024, 0, stream, 1, rows, sums, columns, columns * parts);
+    return rc != TH_OK || sums.whole ? rc : sum_partials(partial, parts, sums.d, out, dtype, stream);
 }
 
 bool known_dtype(int dtype) { return dtype == TH_F32 || dtype == TH_F16 || dtype == TH_BF16; }
@@ -1042,11 +1104,9 @@ extern "C" int th_dequantize_rows(const void *q_dev, int64_t q_stride, const flo
     if (rows > (0x7fffffffll * 256) / chunks) return fail(TH_ERR_UNSUPPORTED, "th_dequantize_rows: too many rows: %lld", static_cast<long long>(rows));
     const dim3 grid(static_cast<unsigned>((rows * chunks + 255) / 256));
     cudaStream_t at = static_cast<cudaStream_t>(stream);
-    const signed char *q = static_cast<const signed char *>(q_dev);
-    const auto run = [&](auto kernel, auto *out) { return launch_chained("dequantize_kernel", kernel, grid, 256, 0, at, 1, q, q_stride, scale_dev, out, out_stride, rows, d, chunks); };
-    if (dtype == TH_F32) return run(dequantize_kernel<float>, static_cast<float *>(out_dev));
-    if (dtype == TH_F16) return run(dequantize_kernel<__half>, static_cast<__half *>(out_dev));
-    return run(dequantize_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16 *>(out_dev));
+    const DequantizeArgs a{static_cast<const signed char *>(q_dev), scale_dev, out_dev, q_stride, out_stride, rows, d, chunks};
+    return launch_chained("dequantize_kernel", dtype == TH_F32 ? dequantize_kernel<float> : dtype == TH_F16 ? dequantize_kernel<__half> : dequantize_kernel<__nv_bfloat16>,
+                          grid, 256, 0, at, 1, a);
 }
 
 // The most that any layout of the rows takes.
@@ -1094,14 +1154,28 @@ extern "C" int th_column_sum(const void *g_dev, int64_t g_stride, void *out_dev,
     if (!g_dev) return fail(TH_ERR_BAD_ARG, "th_column_sum: null pointer");
     if (!workspace_dev || workspace_bytes < th_column_sum_workspace_bytes(rows, d) || !aligned_to(workspace_dev, 4))
         return fail(TH_ERR_WORKSPACE, "th_column_sum: scratch missing or too small");
+    ColumnArgs sums{};
+    sums.g = g_dev; sums.g_stride = g_stride; sums.rows = rows; sums.d = d;
     float *partial = static_cast<float *>(workspace_dev);
-    const int parts = column_parts(rows, d);
-    int rc;
-    if (dtype == TH_F32)
-        rc = column_sums<float>(static_cast<const float *>(g_dev), g_stride, nullptr, 0, nullptr, partial, parts, rows, d, at);
-    else if (dtype == TH_F16)
-        rc = column_sums<__half>(static_cast<const __half *>(g_dev), g_stride, nullptr, 0, nullptr, partial, parts, rows, d, at);
-    else
-        rc = column_sums<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(g_dev), g_stride, nullptr, 0, nullptr, partial, parts, rows, d, at);
-    return rc != TH_OK ? rc : sum_partials(partial, parts, d, out_dev, dtype, at);
+    if (dtype == TH_F32) return column_sums<float>(sums, partial, out_dev, dtype, at);
+    if (dtype == TH_F16) return column_sums<__half>(sums, partial, out_dev, dtype, at);
+    return column_sums<__nv_bfloat16>(sums, partial, out_dev, dtype, at);
+}
+
+extern "C" int th_checkpoint_rows(const void *q_dev, int64_t q_stride, const float *scale_dev, void *x_dev, int64_t x_stride, int d_in, const void *g_dev,
+                                  int64_t g_stride, void *out_dev, int d_out, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int dtype, void *stream) {
+    if (int rc = check_rows("th_checkpoint_rows", rows, d_in, dtype)) return rc;
+    if (int rc = check_rows("th_checkpoint_rows", rows, d_out, dtype)) return rc;
+    if (dtype == TH_F32) return fail(TH_ERR_UNSUPPORTED, "th_checkpoint_rows: float16 or bfloat16");
+    if (rows == 0) return th_column_sum(g_dev, g_stride, out_dev, workspace_dev, workspace_bytes, rows, d_out, dtype, stream);
+    if (!q_dev || !scale_dev || !x_dev || !g_dev || !out_dev || q_stride < d_in || x_stride < d_in || g_stride < d_out)
+        return fail(TH_ERR_BAD_ARG, "th_checkpoint_rows: null pointer or short stride");
+    if (!workspace_dev || workspace_bytes < th_column_sum_workspace_bytes(rows, d_out) || !aligned_to(workspace_dev, 4))
+        return fail(TH_ERR_WORKSPACE, "th_checkpoint_rows: scratch missing or too small");
+    const DequantizeArgs a{static_cast<const signed char *>(q_dev), scale_dev, x_dev, q_stride, x_stride, rows, d_in, (d_in + 15) / 16};
+    ColumnArgs sums{};
+    sums.g = g_dev; sums.g_stride = g_stride; sums.rows = rows; sums.d = d_out;
+    float *partial = static_cast<float *>(workspace_dev);
+    cudaStream_t at = static_cast<cudaStream_t>(stream);
+    return dtype == TH_F16 ? checkpoint_rows<__half>(a, sums, partial, out_dev, dtype, at) : checkpoint_rows<__nv_bfloat16>(a, sums, partial, out_dev, dtype, at);
 }

@@ -1543,22 +1543,24 @@ struct CheckpointedLinearNode : public Node {
             check(th_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(wr.keep), wr.stride, ptr(out[0]), d_in, rows, di, dn, code, stream),
                   "th_linear_bwd_input");
         }
+        // one buffer: the rows back in 16 bits, and the scratch of the bias's sums
+        const int64_t stride = (d_in + 7) / 8 * 8, held = wants_w ? rows * stride * 2 : 0, scratch = wants_b ? th_column_sum_workspace_bytes(rows, dn) : 0;
+        const Tensor buffer = held + scratch ? empty_like_shape({pitch16(held) + scratch}, at::kByte, device) : Tensor();
+        char *x8 = static_cast<char *>(ptr(buffer)), *partial = x8 + pitch16(held);
+        if (wants_b) out[2] = empty_like_shape({d_out}, type, device);
         if (wants_w) {
             const int64_t pitch = pitch16(d_in);
             q8 = restored(q8, at::kChar, rows * pitch);
             s = restored(s, at::kFloat, rows);
-            const int64_t stride = (d_in + 7) / 8 * 8;
-            const Tensor x8 = empty_like_shape({rows, stride}, type, device);
-            check(th_dequantize_rows(ptr(q8), pitch, s.data_ptr<float>(), ptr(x8), stride, rows, di, code, stream), "th_dequantize_rows");
+            if (wants_b)
+                check(th_checkpoint_rows(ptr(q8), pitch, s.data_ptr<float>(), x8, stride, di, ptr(gy.keep), gy.stride, ptr(out[2]), dn, partial, scratch, rows, code, stream),
+                      "th_checkpoint_rows");
+            else
+                check(th_dequantize_rows(ptr(q8), pitch, s.data_ptr<float>(), x8, stride, rows, di, code, stream), "th_dequantize_rows");
             out[1] = empty_like_shape({d_out, d_in}, type, device);
-            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(x8), stride, ptr(out[1]), rows, di, dn, code, stream),
-                  "th_linear_bwd_weight");
-        }
-        if (wants_b) {
-            out[2] = empty_like_shape({d_out}, type, device);
-            const int64_t scratch = th_column_sum_workspace_bytes(rows, dn);
-            const Tensor workspace = empty_like_shape({scratch}, at::kByte, device);
-            check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), ptr(workspace), scratch, rows, dn, code, stream), "th_column_sum");
+            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, x8, stride, ptr(out[1]), rows, di, dn, code, stream), "th_linear_bwd_weight");
+        } else if (wants_b) {
+            check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), partial, scratch, rows, dn, code, stream), "th_column_sum");
         }
         return out;
     }

@@ -106,15 +106,28 @@ class _checkpointed_linear(Function):
                     ),
                     "th_linear_bwd_input",
                 )  # fmt: skip
+            if want_b:
+                db = torch.empty(d_out, dtype=dtype, device=device)
+                sum_bytes = lib.th_column_sum_workspace_bytes(rows, d_out)
+                partial = torch.empty(sum_bytes, dtype=torch.uint8, device=device)
             if want_w:
                 q, scale = int8_rows2d(Int8Rows(q, scale), "kept input")
                 x8 = _empty_operand(rows, d_in, gy2d)
-                _lib.check(
-                    lib.th_dequantize_rows(
-                        q.data_ptr(), int8_stride(q), scale.data_ptr(), x8.data_ptr(), _stride(x8), rows, d_in, code, stream
-                    ),
-                    "th_dequantize_rows",
-                )
+                if want_b:
+                    _lib.check(
+                        lib.th_checkpoint_rows(
+                            q.data_ptr(), int8_stride(q), scale.data_ptr(), x8.data_ptr(), _stride(x8), d_in, gy2d.data_ptr(), _stride(gy2d),
+                            db.data_ptr(), d_out, partial.data_ptr(), sum_bytes, rows, code, stream,
+                        ),
+                        "th_checkpoint_rows",
+                    )  # fmt: skip
+                else:
+                    _lib.check(
+                        lib.th_dequantize_rows(
+                            q.data_ptr(), int8_stride(q), scale.data_ptr(), x8.data_ptr(), _stride(x8), rows, d_in, code, stream
+                        ),
+                        "th_dequantize_rows",
+                    )
                 dw = torch.empty((d_out, d_in), dtype=dtype, device=device)
                 _lib.check(
                     lib.th_linear_bwd_weight(
@@ -123,10 +136,7 @@ class _checkpointed_linear(Function):
                     ),
                     "th_linear_bwd_weight",
                 )  # fmt: skip
-            if want_b:
-                db = torch.empty(d_out, dtype=dtype, device=device)
-                sum_bytes = lib.th_column_sum_workspace_bytes(rows, d_out)
-                partial = torch.empty(sum_bytes, dtype=torch.uint8, device=device)
+            elif want_b:
                 _lib.check(
                     lib.th_column_sum(
                         gy2d.data_ptr(), _stride(gy2d), db.data_ptr(), partial.data_ptr(), sum_bytes, rows, d_out, code, stream
