@@ -1,7 +1,7 @@
 /*
  * th_b200.h - C ABI of libth_b200.so: sm_100a CUDA kernels for the three fused
  * neural-field operators of triton_helpers (multiresolution hash encoding, fully
- * fused MLP, reversible fused MLP).
+ * fused MLP, reversible fused MLP), and for layers of wider networks.
  *
  * Conventions shared by every entry point
  *   - extern "C", plain pointers and sizes, no C++ or torch types.
@@ -444,6 +444,13 @@ int th_checkpoint_rows(const void *q_dev, int64_t q_stride, const float *scale_d
 int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev,
                    int64_t weight_stride, const float *weight_scale_dev, const void *bias_dev, void *y_dev,
                    int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+
+/* th_quantize_rows of x (rows x d_in, `x_dtype`) into scratch and th_int8_linear of the result. */
+int64_t th_quantized_linear_workspace_bytes(int64_t rows, int d_in);
+int th_quantized_linear(const void *x_dev, int64_t x_stride, int x_dtype, const void *weight_dev,
+                        int64_t weight_stride, const float *weight_scale_dev, const void *bias_dev, void *y_dev,
+                        int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
+                        int d_out, int dtype, void *stream);
 
 /* The products of a linear layer in 16 bits with float32 sums: y = x w^T + b, grad_x = grad_y w and
  * grad_w = grad_y^T x (contiguous).  Operand rows start on 16 bytes (pointer and stride); outputs may lie anywhere.

@@ -56,7 +56,8 @@ __device__ __forceinline__ void store_values(T *row, long long packet, const flo
 
 // A row as 16-byte packets that start on 16 bytes, wherever the row itself starts: `shift` elements of the first packet lie ahead of it and
 // the last one may reach past it.  A packet holds one element of the row at least, so it lies in memory that is there; elements beside the
-// row are read as zeros and never written.  (5000 rows of 3001 bfloat16, an element at a time: SHIFTFIG.)
+// row are read as zeros and never written.  (5000 rows of 3001 bfloat16, us: norm 27 an element at a
+// time, 18.6 so; to 8 bits 26 and 12.4.)
 template <typename T, bool SHIFT>
 struct Span {
     static constexpr int N = 16 / static_cast<int>(sizeof(T));
@@ -211,8 +212,8 @@ __global__ void __launch_bounds__(THREADS) row_fwd_kernel(const RowFwdArgs a) {
     constexpr int N = 16 / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
-    start_next();
     after_previous();
+    start_next();  // by now everything before is done: what follows depends on these rows alone (th_quantized_linear relies on it)
     const int team = a.team, t = team == 32 ? threadIdx.x & 31 : threadIdx.x;
     const long long row = team == 32 ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;  // whole warps, and only where a warp is a team
@@ -302,8 +303,8 @@ __global__ void __launch_bounds__(kMaxTeam) row_fwd_stream_kernel(const RowFwdAr
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
-    start_next();
     after_previous();
+    start_next();
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
@@ -484,7 +485,8 @@ struct RowBwdArgs {
 };
 
 // Rows come through a ring of stages in shared memory, brought by bulk copies of one warp, so that what is in flight does not depend on
-// the registers that sums take (rows held in registers, 16384 x 4096 bfloat16: 111 us at best, by launch shape up to 260; RINGFIG).  Long
+// the registers that sums take (16384 x 4096 bfloat16 with a residual: rows held in registers 111 us at best, by launch shape up to 260; a
+// ring 93, copied bytes' time 82; float32 16000 x 2048 80 of 80).  16-bit rows are bound by their instructions as well.  Long
 // rows are shared by all consumer warps, short ones have a warp each.  A team's rows are a multiple of eight apart, so that each of
 // them starts alike and a thread's packets are the same columns in all.
 constexpr int kMaxRing = 8;

