@@ -30,7 +30,7 @@ constexpr int kStagingBoxes = 2;              // per warp: one is filled while t
 constexpr unsigned long long kGemmWaitNs = 1000000000ull;
 
 struct GemmArgs {
-    int m, n, tiles_m, tiles_n, k_tiles, splits, tiles_per_split;
+    int m, n, tiles_m, tiles_n, group, k_tiles, splits, tiles_per_split;
     uint32_t idesc;
     void *out;             // [m][out_stride], or [n][out_stride] where the product is transposed
     long long out_stride;
@@ -146,13 +146,12 @@ struct GemmUnit {
     int tm, tn, split, k0, k1;
 };
 
-// Tiles go in groups of eight tile rows, down the group's columns, so that the tiles at work at one time share operands in L2.
+// Tiles go in groups of tile rows, down the group's columns: the rows' operand stays in L2 while the columns' passes by.
 __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs &g, int unit) {
-    constexpr int kGroup = 8;
     GemmUnit u;
     const int tile = unit / g.splits;
     u.split = unit - tile * g.splits;
-    const int per_group = kGroup * g.tiles_n, group = tile / per_group, first = group * kGroup, height = min(kGroup, g.tiles_m - first);
+    const int per_group = g.group * g.tiles_n, group = tile / per_group, first = group * g.group, height = min(g.group, g.tiles_m - first);
     const int r = tile - group * per_group;
     u.tm = first + r % height;
     u.tn = r / height;
@@ -592,6 +591,9 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     g.n = b.rows;
     g.tiles_m = (g.m + CG * kGemmRows - 1) / (CG * kGemmRows);
     g.tiles_n = (g.n + BN - 1) / BN;
+    // 32 MB of rows: half of what one die's L2 holds.  Sustained at the power limit, TFLOP/s by rows of a group (MB), 16384 x 4096 -> 16384 float16:
+    // 8 (16) 1294, 16 (32) 1342, 32 (64) 1196, a library's 1324; 8192 x 4096 -> 16384 8-bit: 8 (8) 2757, 16 (16) 2846, 32 (32) 2923.
+    g.group = static_cast<int>(std::max(4ll, std::min(32ll, (32ll << 20) / (static_cast<long long>(CG) * kGemmRows * k * EB))));
     g.k_tiles = (k + S::kK - 1) / S::kK;
     g.tiles_per_split = (g.k_tiles + g.splits - 1) / g.splits;
     g.splits = (g.k_tiles + g.tiles_per_split - 1) / g.tiles_per_split;
@@ -603,7 +605,7 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "matrix product: too many tiles");
     // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles
-    const long long clusters = g.splits > 1 ? units : std::min<long long>(units, CTAS * sm_count() / CG);
+    const long long clusters = g.splits > 1 ? units : std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
     return launch_chained("wide_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), kGemmThreads, S::kBytes, stream, CG * g.splits, g, a_map, b_map, c_map);
 }
 

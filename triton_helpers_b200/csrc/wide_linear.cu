@@ -18,7 +18,7 @@ int divide_up(long long a, long long b) { return static_cast<int>((a + b - 1) / 
 // within a group of SMs, and groups differ), a little less where it is not even.
 int cluster_slots(int size, int per_sm) {
     static const int one[8] = {148, 74, 44, 32, 25, 21, 14, 14}, two[8] = {296, 148, 90, 69, 54, 44, 36, 32};
-    return (per_sm == 1 ? one : two)[size - 1] * sm_count() / 148;
+    return std::max(1, (per_sm == 1 ? one : two)[size - 1] * sm_count() / 148);
 }
 
 // The cheapest cut by an estimate in cycles: rounds of tiles x stages x cycles a stage (what its bytes take into the SM), what a pair
