@@ -452,6 +452,12 @@ int th_quantized_linear(const void *x_dev, int64_t x_stride, int x_dtype, const 
                         int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
                         int d_out, int dtype, void *stream);
 
+/* dst = src for one or two matrices of 16-bit elements in one launch (host arrays of n entries): rows that do not start on 16
+ * bytes to rows that do, as the products below want their operands.  Destination rows hold d rounded up to eight
+ * elements, the last of them zeros. */
+int th_copy_rows(int n, const void *const *src_dev, const int64_t *src_stride, void *const *dst_dev,
+                 const int64_t *dst_stride, const int64_t *rows, const int *d, void *stream);
+
 /* The products of a linear layer in 16 bits with float32 sums: y = x w^T + b, grad_x = grad_y w and
  * grad_w = grad_y^T x (contiguous).  Operand rows start on 16 bytes (pointer and stride); outputs may lie anywhere.
  * Results repeat bit for bit. */

@@ -223,3 +223,29 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         g.sum().backward()  # not differentiable twice
     assert _lib.lib().th_linear_tc_status() == 0
+
+
+def test_memory_around_operands_is_left():
+    # padding beside the operands holds NaN: it meets neither a product nor a sum
+    wide, weights = normal(70, 48, dtype=torch.float16), normal(40, 40, seed=1, dtype=torch.float16)
+    wide[:, 33:], weights[:, 33:] = float("nan"), float("nan")
+    x, w, b = wide[:, :33], weights[:, :33], normal(40, seed=2, dtype=torch.float16)
+    leaf, wl, bl = wide.clone().requires_grad_(True), weights.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    gwide = normal(70, 48, seed=3, dtype=torch.float16)
+    gwide[:, 40:] = float("nan")
+    gy = gwide[:, :40]
+    y = checkpointed_linear(leaf[:, :33], wl[:, :33], bl)
+    dx, dw, db = torch.autograd.grad(y, [leaf, wl, bl], gy)
+    assert_pass(x, w, b, gy, y.detach(), [dx[:, :33], dw[:, :33], db])
+    assert bool((dx[:, 33:] == 0).all()) and bool((dw[:, 33:] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [511, 512, 513, 4099])
+def test_bias_gradient_of_few_and_many_rows(rows):
+    x, w, b = normal(rows, 16, dtype=torch.bfloat16), normal(300, 16, seed=1, dtype=torch.bfloat16), normal(300, seed=2, dtype=torch.bfloat16).requires_grad_(True)
+    gy = normal(rows, 300, seed=3, dtype=torch.bfloat16)
+    (alone,) = torch.autograd.grad(checkpointed_linear(x, w, b), [b], gy)
+    assert near(alone, gy.double().sum(0), gy.double().abs().sum(0), rows)
+    weight = w.clone().requires_grad_(True)
+    both = torch.autograd.grad(checkpointed_linear(x, weight, b), [b, weight], gy)
+    assert torch.equal(both[0], alone)

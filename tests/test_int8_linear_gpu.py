@@ -224,3 +224,31 @@ def test_refusals():
         int8_linear(normal(1, 131072), some_weight(1, 131072))
     with pytest.raises(TypeError):
         quantize_rows(x.double())
+
+
+def test_two_streams_at_once():
+    x, weight = [normal(n, 3000, seed=n) for n in (1, 90, 700)], some_weight(500, 3000)
+    want = [int8_linear(t, weight) for t in x]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in x], [[] for _ in x]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[k].append(int8_linear(x[k], weight))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(outs, want) for y in ys)
+
+
+def test_weights_quantised_right_before_their_use():
+    # the product may fetch weights while its input is quantised, but not before whatever wrote them has finished
+    x = normal(1, 8192, dtype=torch.float16)
+    weights = [normal(8192, 8192, seed=k, dtype=torch.float16) for k in range(2)]
+    want = [int8_linear(x, quantize_rows(w)) for w in weights]
+    torch.cuda.synchronize()
+    held = quantize_rows(weights[0])
+    for k in (1, 0, 1, 0, 1):
+        fresh = quantize_rows(weights[k])
+        held.q.copy_(fresh.q)
+        held.scale.copy_(fresh.scale)
+        assert torch.equal(int8_linear(x, held), want[k])
+        assert torch.equal(int8_linear(x, quantize_rows(weights[k])), want[k])

@@ -217,3 +217,38 @@ def test_refusals():
         rms_norm(x, gain.cpu())
     with pytest.raises(RuntimeError, match="no gradient"):
         rms_norm_int8(x, gain.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("d", [33, 64, 1028])
+def test_memory_around_rows_is_left(d):
+    # inputs inside larger tensors at odd places; what lies beside them is neither used nor written
+    for dtype in DTYPES:
+        wide = normal(9, d + 5, dtype=dtype)
+        wide[:, :3], wide[:, d + 3 :] = float("nan"), float("inf")
+        x = wide[:, 3 : d + 3]
+        gain = normal(d, seed=2, dtype=dtype)
+        before = wide.clone()
+        y, ref = rms_norm(x, gain), reference(x, gain, None, 1e-6)
+        assert near(y, ref["y"], ref["y"].abs())
+        assert torch.equal(rms_norm_int8(x, gain).q, rms_norm_int8(x.contiguous(), gain).q)
+        leaf, weight = wide.clone().requires_grad_(True), gain.clone().requires_grad_(True)
+        gy = normal(9, d, seed=3, dtype=dtype)
+        dwide, dw = torch.autograd.grad(rms_norm(leaf[:, 3 : d + 3], weight), [leaf, weight], gy)
+        ref = reference(x, gain, None, 1e-6, gy)
+        assert near(dwide[:, 3 : d + 3], ref["dx"], ref["dx_reach"]) and bool((dwide[:, :3] == 0).all()) and bool((dwide[:, d + 3 :] == 0).all())
+        assert near(dw, ref["dw"], ref["dw_reach"], 9 * 2.0**-24)
+        assert torch.equal(wide.nan_to_num(nan=7.0, posinf=8.0), before.nan_to_num(nan=7.0, posinf=8.0))
+
+
+@pytest.mark.parametrize("d", [48, 1000, 4097])
+def test_rows_at_every_start(d):
+    # rows that start at each of the places within 16 bytes, alike and not alike
+    for dtype in DTYPES:
+        base, other, gain = normal(7 * d + 16, dtype=dtype), normal(7 * d + 16, seed=1, dtype=dtype), normal(d, seed=2, dtype=dtype)
+        for at in range(0, 9, 1 if d == 48 else 3):
+            x, residual = base[at : at + 7 * d].view(7, d), other[at : at + 7 * d].view(7, d)
+            for r in (residual, other[: 7 * d].view(7, d)):
+                y, s = rms_norm(x, gain, r)
+                ref = reference(x, gain, r, 1e-6)
+                assert torch.equal(s, ref["s"]) and near(y, ref["y"], ref["y"].abs())
+                assert torch.equal(rms_norm_int8(x, gain, r)[0].q, rms_norm_int8(x.clone(), gain, r.clone())[0].q)

@@ -177,6 +177,7 @@ SIGNATURES = {
         [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
          c_void_p],
     ),
+    "th_copy_rows": (c_int, [c_int, _PTRP, _I64P, _PTRP, _I64P, _I64P, ctypes.POINTER(c_int), c_void_p]),
     "th_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
     "th_linear_bwd_input": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
     "th_linear_bwd_weight": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
@@ -195,7 +196,7 @@ class KernelTimer:
     LAUNCHING = ("th_field_fwd", "th_field_bwd", "th_hash_fwd", "th_hash_bwd", "th_hash_order", "th_hash_fwd_ordered", "th_hash_bwd_ordered", "th_mlp_fwd", "th_mlp_fwd_mse", "th_mlp_bwd", "th_rev_fwd", "th_rev_bwd",
                  "th_hash_fwd_cast", "th_hash_bwd_cast", "th_mlp_fwd_mse_ordered", "th_mse_grad", "th_adam_step", "th_adam_steps", "th_cast",
                  "th_scale_cast", "th_rms_norm_fwd", "th_rms_norm_int8", "th_rms_norm_bwd", "th_quantize_rows", "th_dequantize_rows",
-                 "th_column_sum", "th_checkpoint_rows", "th_int8_linear", "th_quantized_linear", "th_linear_fwd", "th_linear_bwd_input", "th_linear_bwd_weight")  # fmt: skip
+                 "th_column_sum", "th_checkpoint_rows", "th_copy_rows", "th_int8_linear", "th_quantized_linear", "th_linear_fwd", "th_linear_bwd_input", "th_linear_bwd_weight")  # fmt: skip
 
     def __init__(self):
         self.records = []

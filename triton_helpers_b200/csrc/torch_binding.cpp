@@ -1494,19 +1494,38 @@ PyObject *py_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// Rows of a 16-bit product's operand: they start on 16 bytes; a padded copy where they do not
-Rows operand_rows(const Tensor &t, int64_t width) {
-    Rows r;
-    if (rows_of(t, width, r)) {
-        if (r.n <= 1) r.stride = (width + 7) / 8 * 8;
-        if (r.stride % 8 == 0 && reinterpret_cast<uintptr_t>(ptr(t)) % 16 == 0) return r;
+// The operands of a 16-bit product: rows that start on 16 bytes, padded copies (of both in one launch) where they do not
+struct Operands {
+    Rows rows[2];
+    int n = 0;
+    const void *src[2];
+    void *dst[2];
+    int64_t src_stride[2], dst_stride[2], count[2];
+    int d[2], copies = 0;
+    Tensor keep[2];
+
+    const Rows &add(const Tensor &t, int64_t width) {
+        Rows &r = rows[n++];
+        const bool even = rows_of(t, width, r);
+        if (!even) rows_of(t.contiguous(), width, r);
+        const int64_t pitch = (width + 7) / 8 * 8;
+        if (r.n <= 1 && reinterpret_cast<uintptr_t>(ptr(r.keep)) % 16 == 0) r.stride = pitch;
+        if (r.stride % 8 == 0 && reinterpret_cast<uintptr_t>(ptr(r.keep)) % 16 == 0) return r;
+        keep[copies] = r.keep;
+        src[copies] = ptr(r.keep);
+        src_stride[copies] = r.stride;
+        r.keep = empty_like_shape({r.n, pitch}, t.scalar_type(), t.device());
+        r.stride = pitch;
+        dst[copies] = ptr(r.keep);
+        dst_stride[copies] = pitch;
+        count[copies] = r.n;
+        d[copies++] = static_cast<int>(width);
+        return r;
     }
-    r.n = t.numel() / width;
-    r.stride = (width + 7) / 8 * 8;
-    r.keep = empty_like_shape({r.n, r.stride}, t.scalar_type(), t.device());
-    r.keep.narrow(1, 0, width).copy_(t.reshape({r.n, width}));
-    return r;
-}
+    void settle(void *stream) {
+        if (copies) check(th_copy_rows(copies, src, src_stride, dst, dst_stride, count, d, stream), "th_copy_rows");
+    }
+};
 
 struct CheckpointedLinearNode : public Node {
     SavedVariable weight, q, scale;
@@ -1535,15 +1554,18 @@ struct CheckpointedLinearNode : public Node {
         const c10::Device device = grads[0].device();
         void *stream = current_stream();
         const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
-        const Rows gy = operand_rows(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
+        Operands operands;
+        const Rows &gy = operands.add(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
         const bool wants_x = keeps_weight && task_should_compute_output(0), wants_w = keeps_rows && task_should_compute_output(1);
         const bool wants_b = task_should_compute_output(2);
         if (wants_x) {
-            const Rows wr = operand_rows(same(w, type, d_in * d_out), d_in);
+            const Rows &wr = operands.add(same(w, type, d_in * d_out), d_in);
+            operands.settle(stream);
             out[0] = empty_like_shape(shape, type, device);
             check(th_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(wr.keep), wr.stride, ptr(out[0]), d_in, rows, di, dn, code, stream),
                   "th_linear_bwd_input");
         }
+        if (!wants_x) operands.settle(stream);
         // one buffer: the rows back in 16 bits, and the scratch of the bias's sums
         const int64_t stride = (d_in + 7) / 8 * 8, held = wants_w ? rows * stride * 2 : 0, scratch = wants_b ? th_column_sum_workspace_bytes(rows, dn) : 0;
         const Tensor buffer = held + scratch ? empty_like_shape({pitch16(held) + scratch}, at::kByte, device) : Tensor();
@@ -1589,7 +1611,9 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *args, Py_ssize_t n
             c10::cuda::CUDAGuard guard(x.device());
             void *stream = current_stream();
             const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
-            const Rows xr = operand_rows(x, d_in), wr = operand_rows(w, d_in);
+            Operands operands;
+            const Rows &xr = operands.add(x, d_in), &wr = operands.add(w, d_in);
+            operands.settle(stream);
             c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
             shape.back() = d_out;
             y = empty_like_shape(shape, type, x.device());

@@ -11,6 +11,7 @@ There is no such operator in triton_helpers, whose fused network ends at 64 colu
 Only the weight's gradient sees the 8-bit values: the output and the input's gradient are those of an ordinary layer, so the
 rounding does not add up from layer to layer.  A row's rounding is at most half a step, 1/254 of its largest magnitude.
 """
+from ctypes import c_int, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -36,8 +37,19 @@ def _validate(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[int, i
 def _operand(t: Tensor, width: int) -> Tensor:
     r"""``t`` as rows that start on 16 bytes, which is what the products read; a copy only where they do not."""
     t = t.reshape(-1, width)
-    if (width > 1 and t.stride(1) != 1) or t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < width)):
-        t = _empty_operand(t.shape[0], width, t).copy_(t)
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8):
+        out = _empty_operand(t.shape[0], width, t)
+        with torch.cuda.device(t.device):
+            _lib.check(
+                _lib.lib().th_copy_rows(
+                    1, (c_void_p * 1)(t.data_ptr()), _lib.i64_array([t.stride(0) if t.shape[0] > 1 else width]), (c_void_p * 1)(out.data_ptr()),
+                    _lib.i64_array([_stride(out)]), _lib.i64_array([t.shape[0]]), (c_int * 1)(width), _lib.stream_ptr(t.device),
+                ),
+                "th_copy_rows",
+            )  # fmt: skip
+        return out
     return t
 
 
