@@ -28,6 +28,7 @@ def test_rows_entry_points_refuse(library):
     assert library.th_rms_norm_fwd(AT, 8, None, 0, AT, 2, None, AT, None, 4, 8, 1e-6, 1, None) == -2 and said(library, b"gain")
     assert library.th_rms_norm_fwd(AT, 8, AT, 8, AT, 0, None, AT, None, 4, 8, 1e-6, 0, None) == -1 and said(library, b"null")  # residual without sum
     assert library.th_rms_norm_fwd(None, 8, None, 0, AT, 0, None, AT, None, 0, 8, 1e-6, 0, None) == 0  # no rows
+    assert library.th_rms_norm_fwd(AT + 2, 8, None, 0, AT, 0, None, AT, None, 4, 8, 1e-6, 0, None) == -3 and said(library, b"elements")
     assert library.th_rms_norm_int8(AT, 8, None, 0, AT, 0, None, AT, 8, AT, 4, 8, 1e-6, 0, None) == -3 and said(library, b"16 bytes")
     assert library.th_quantize_rows(AT, 8, AT + 8, 16, AT, 4, 8, 0, None) == -3
     assert library.th_quantize_rows(AT, 40, AT, 32, AT, 4, 40, 0, None) == -3  # rows longer than their stride

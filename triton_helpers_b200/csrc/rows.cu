@@ -8,6 +8,7 @@
 #include "chained.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 #include <utility>
 
 namespace th {
@@ -56,8 +57,7 @@ __device__ __forceinline__ void store_values(T *row, long long packet, const flo
 
 // A row as 16-byte packets that start on 16 bytes, wherever the row itself starts: `shift` elements of the first packet lie ahead of it and
 // the last one may reach past it.  A packet holds one element of the row at least, so it lies in memory that is there; elements beside the
-// row are read as zeros and never written.  (5000 rows of 3001 bfloat16, us: norm 27 an element at a
-// time, 18.6 so; to 8 bits 26 and 12.4.)
+// row are read as zeros and never written.  (5000 rows of 3001 bfloat16, us: norm 27 an element at a time, 18.6 so; to 8 bits 26 and 12.4.)
 template <typename T, bool SHIFT>
 struct Span {
     static constexpr int N = 16 / static_cast<int>(sizeof(T));
@@ -1100,6 +1100,12 @@ int check_rows(const char *what, long long rows, int d, int dtype) {
     return TH_OK;
 }
 
+int check_elements(const char *what, int dtype, std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (!aligned_to(p, dtype_bytes(dtype))) return fail(TH_ERR_ALIGNMENT, "%s: a pointer is off its elements' size", what);
+    return TH_OK;
+}
+
 }  // namespace
 
 int rows_status_word() {
@@ -1117,6 +1123,8 @@ extern "C" int th_rms_norm_fwd(const void *x_dev, int64_t x_stride, const void *
     if (gain_dtype != dtype && gain_dtype != TH_F32) return fail(TH_ERR_UNSUPPORTED, "th_rms_norm_fwd: the gain is float32 or of the rows' type");
     if (rows == 0) return TH_OK;
     if (!x_dev || !gain_dev || !y_dev || (residual_dev != nullptr) != (sum_dev != nullptr)) return fail(TH_ERR_BAD_ARG, "th_rms_norm_fwd: null pointer");
+    if (int rc = check_elements("th_rms_norm_fwd", dtype, {x_dev, residual_dev, sum_dev, y_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_fwd", gain_dtype, {gain_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.residual = residual_dev; a.gain = gain_dev; a.sum = sum_dev; a.y = y_dev; a.rstd = rstd_dev;
     a.x_stride = x_stride; a.residual_stride = residual_stride; a.rows = rows; a.d = d; a.gain_f32 = gain_dtype == TH_F32; a.eps = eps;
@@ -1131,6 +1139,8 @@ extern "C" int th_rms_norm_int8(const void *x_dev, int64_t x_stride, const void 
     if (!x_dev || !gain_dev || !q_dev || !scale_dev || (residual_dev != nullptr) != (sum_dev != nullptr))
         return fail(TH_ERR_BAD_ARG, "th_rms_norm_int8: null pointer");
     if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d) return fail(TH_ERR_ALIGNMENT, "th_rms_norm_int8: 8-bit rows start on 16 bytes");
+    if (int rc = check_elements("th_rms_norm_int8", dtype, {x_dev, residual_dev, sum_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_int8", gain_dtype, {gain_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.residual = residual_dev; a.gain = gain_dev; a.sum = sum_dev; a.q = static_cast<signed char *>(q_dev); a.scale = scale_dev;
     a.x_stride = x_stride; a.residual_stride = residual_stride; a.q_stride = q_stride; a.rows = rows; a.d = d; a.gain_f32 = gain_dtype == TH_F32; a.eps = eps;
@@ -1143,6 +1153,7 @@ extern "C" int th_quantize_rows(const void *x_dev, int64_t x_stride, void *q_dev
     if (rows == 0) return TH_OK;
     if (!x_dev || !q_dev || !scale_dev) return fail(TH_ERR_BAD_ARG, "th_quantize_rows: null pointer");
     if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d) return fail(TH_ERR_ALIGNMENT, "th_quantize_rows: 8-bit rows start on 16 bytes");
+    if (int rc = check_elements("th_quantize_rows", dtype, {x_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.q = static_cast<signed char *>(q_dev); a.scale = scale_dev;
     a.x_stride = x_stride; a.q_stride = q_stride; a.rows = rows; a.d = d;
@@ -1210,6 +1221,8 @@ extern "C" int th_rms_norm_bwd(const void *sum_dev, int64_t sum_stride, const vo
     if (!sum_dev || !gain_dev || !rstd_dev || !grad_y_dev || !grad_x_dev) return fail(TH_ERR_BAD_ARG, "th_rms_norm_bwd: null pointer");
     if (grad_gain_dev && (!workspace_dev || workspace_bytes < th_rms_norm_bwd_workspace_bytes(rows, d, dtype) || !aligned_to(workspace_dev, 16)))
         return fail(TH_ERR_WORKSPACE, "th_rms_norm_bwd: scratch missing, too small or off 16 bytes");
+    if (int rc = check_elements("th_rms_norm_bwd", dtype, {sum_dev, grad_y_dev, grad_sum_dev, grad_x_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_bwd", gain_dtype, {gain_dev, grad_gain_dev})) return rc;
     RowBwdArgs a{};
     a.s = sum_dev; a.gain = gain_dev; a.gy = grad_y_dev; a.gs = grad_sum_dev; a.rstd = rstd_dev; a.dx = grad_x_dev;
     a.partial = static_cast<float *>(workspace_dev);
