@@ -252,3 +252,10 @@ def test_weights_quantised_right_before_their_use():
         held.scale.copy_(fresh.scale)
         assert torch.equal(int8_linear(x, held), want[k])
         assert torch.equal(int8_linear(x, quantize_rows(weights[k])), want[k])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (9, 33), (4, 3001), (2, 70001)])
+def test_rows_back_at_odd_widths(shape, dtype):
+    rows = quantize_rows(normal(*shape))
+    assert torch.equal(dequantize_rows(rows, dtype), (rows.q.float() * rows.scale[:, None]).to(dtype))
