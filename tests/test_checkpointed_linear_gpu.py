@@ -249,3 +249,26 @@ def test_bias_gradient_of_few_and_many_rows(rows):
     weight = w.clone().requires_grad_(True)
     both = torch.autograd.grad(checkpointed_linear(x, weight, b), [b, weight], gy)
     assert torch.equal(both[0], alone)
+
+
+def test_offsets_past_32_bits():
+    x = normal(1, 64, dtype=torch.float16).expand(1_000_000, 64).contiguous()
+    x[-1] = normal(64, seed=5, dtype=torch.float16)
+    w = normal(2304, 64, seed=1, dtype=torch.float16).requires_grad_(True)
+    y = checkpointed_linear(x, w)  # 2.3e9 outputs
+    assert torch.equal(y[-1], checkpointed_linear(x[-1:], w)[0]) and torch.equal(y[-2], y[0])
+    gy = torch.zeros_like(y)
+    gy[-1] = 1
+    (dw,) = torch.autograd.grad(y, [w], gy)
+    want = dequantize_rows(quantize_rows(x[-1])).double().expand(2304, 64)
+    assert near(dw, want, want.abs(), 1, 1.01 * torch.finfo(torch.float16).eps / 2)
+
+
+@pytest.mark.parametrize("rows,d_in,d_out", [(930, 40, 14272), (130, 16, 16000), (3000, 70, 9000)])
+def test_tiles_that_lie_outside_in_part(rows, d_in, d_out):
+    # many short tiles a CTA, some of whose rows are all outside: what is stored ahead of them stays
+    x, w = normal(rows, d_in, dtype=torch.bfloat16), normal(d_out, d_in, seed=1, dtype=torch.bfloat16)
+    first = checkpointed_linear(x, w)
+    assert near(first, x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t(), d_in)
+    for _ in range(20):
+        assert torch.equal(checkpointed_linear(x, w), first)

@@ -259,3 +259,21 @@ def test_weights_quantised_right_before_their_use():
 def test_rows_back_at_odd_widths(shape, dtype):
     rows = quantize_rows(normal(*shape))
     assert torch.equal(dequantize_rows(rows, dtype), (rows.q.float() * rows.scale[:, None]).to(dtype))
+
+
+def test_offsets_past_32_bits():
+    x = normal(1, 64, dtype=torch.float16).expand(1_000_000, 64).contiguous()
+    x[-1] = normal(64, seed=5, dtype=torch.float16)
+    weight = some_weight(2304, 64)
+    y = int8_linear(x, weight)  # 2.3e9 outputs
+    assert torch.equal(y[-1], int8_linear(x[-1:], weight)[0]) and torch.equal(y[-2], y[0])
+
+
+@pytest.mark.parametrize("tokens,d_in,d_out", [(930, 40, 14272), (140, 16, 16000), (3000, 200, 9000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiles_that_lie_outside_in_part(tokens, d_in, d_out, dtype):
+    x, weight = normal(tokens, d_in, dtype=dtype), some_weight(d_out, d_in)
+    first = int8_linear(x, weight)
+    assert_linear(first, Int8Rows(*rows_by_definition(x)), weight, None)
+    for _ in range(20):
+        assert torch.equal(int8_linear(x, weight), first)

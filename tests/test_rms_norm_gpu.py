@@ -252,3 +252,16 @@ def test_rows_at_every_start(d):
                 ref = reference(x, gain, r, 1e-6)
                 assert torch.equal(s, ref["s"]) and near(y, ref["y"], ref["y"].abs())
                 assert torch.equal(rms_norm_int8(x, gain, r)[0].q, rms_norm_int8(x.clone(), gain, r.clone())[0].q)
+
+
+def test_offsets_past_32_bits():
+    rows, d = 70000, 32768  # 2.3e9 elements
+    x = torch.empty(rows, d, device="cuda", dtype=torch.bfloat16)
+    x.copy_(normal(1, d, dtype=torch.bfloat16))
+    x[-1] = normal(d, seed=5, dtype=torch.bfloat16)
+    gain = normal(d, seed=2, dtype=torch.bfloat16)
+    y = rms_norm(x, gain)
+    assert torch.equal(y[-1], rms_norm(x[-1], gain)) and torch.equal(y[-2], y[0])
+    del y
+    rows8 = rms_norm_int8(x, gain)
+    assert torch.equal(rows8.q[-1], rms_norm_int8(x[-1], gain).q) and torch.equal(rows8.q[-2], rows8.q[0])

@@ -199,7 +199,11 @@ __device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *
     if (g.out_tma) {
         fence_async_smem();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0 && m0 < g.m && c0 < g.n) tma_store_2d(c_map, box, c0, m0);
+        // a box outside the output is a group of its own all the same: the wait for a box's memory counts groups
+        if ((threadIdx.x & 31) == 0) {
+            if (m0 < g.m && c0 < g.n) tma_store_2d(c_map, box, c0, m0);
+            else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
         return;
     }
     __syncwarp();
