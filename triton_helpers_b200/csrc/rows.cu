@@ -1001,7 +1001,9 @@ struct DequantizeArgs {
     int d, chunks;
 };
 
-// Sixteen columns a thread.  q * scale is rounded once, to T.
+// Sixteen columns a thread.  q * scale is rounded once, to T: in 16 bits it is an operand of the weight's gradient.  Relative to that gradient's
+// norm the rounding is 1.6e-3 in bfloat16 and 2.0e-4 in float16, where the 8 bits themselves are 7e-3 to 2e-2.  Keeping what is rounded off would
+// take a second product of the weight's gradient's size, over the remainders: 193 us more of 690 at 8192 x 4096 -> 4096.
 template <typename T>
 __device__ __forceinline__ void dequantize(const DequantizeArgs &a, long long id) {
     const long long row = id / a.chunks;

@@ -9,7 +9,8 @@ There is no such operator in triton_helpers, whose fused network ends at 64 colu
     dx = dy w          dw = dy^T (q * scale)          db = sum over rows of dy
 
 Only the weight's gradient sees the 8-bit values: the output and the input's gradient are those of an ordinary layer, so the
-rounding does not add up from layer to layer.  A row's rounding is at most half a step, 1/254 of its largest magnitude.
+rounding does not add up from layer to layer.  A row's rounding is at most half a step, 1/254 of its largest magnitude; as an
+operand of the product ``q * scale`` is rounded once more, to the layer's 16-bit type.
 """
 from ctypes import c_int, c_void_p
 from typing import Optional, Tuple
