@@ -1432,12 +1432,14 @@ bool int8_rows(const Tensor &q, const Tensor &scale, Rows &r) {
     r.n = q.numel() / width;
     r.stride = pitch16(width);
     if (reinterpret_cast<uintptr_t>(ptr(q)) % 16 || (width > 1 && q.stride(-1) != 1)) return false;
-    if (r.n > 1) {  // evenly spaced rows
+    if (r.n > 1) {  // evenly spaced rows; expanded ones (a stride of zero) are Python's, which copies them
+        bool found = false;
         int64_t step = 0;
         for (int64_t k = q.dim() - 2; k >= 0; --k) {
             if (q.size(k) == 1) continue;
-            if (step == 0) r.stride = q.stride(k);
+            if (!found) r.stride = q.stride(k);
             else if (q.stride(k) != step) return false;
+            found = true;
             step = q.stride(k) * q.size(k);
         }
     }
