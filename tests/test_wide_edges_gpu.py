@@ -1,7 +1,10 @@
 r"""Layers for wide networks where a definition has to hold at its edges: roundings, layouts, scales, threads, modes."""
+import threading
+
 import pytest
 import torch
 
+from triton_helpers_b200 import _lib
 from triton_helpers_b200.layers.checkpointed_linear import checkpointed_linear
 from triton_helpers_b200.layers.int8_linear import Int8Rows, dequantize_rows, int8_linear, quantize_rows
 
@@ -41,3 +44,33 @@ def test_expanded_8_bit_weights():
     rows, one = quantize_rows(normal(5, 48)), quantize_rows(normal(1, 48, seed=1))
     weight = Int8Rows(one.q.expand(7, 48), one.scale.expand(7).contiguous())
     assert torch.equal(int8_linear(rows, weight, dtype=torch.float32), int8_linear(rows, one, dtype=torch.float32).expand(5, 7))
+
+
+def test_norm_backward_from_several_threads():
+    # two widths of one kernel with different amounts of shared memory, each from a host thread and a stream of its own
+    lib, failed = _lib.lib(), []
+    torch.cuda.synchronize()
+
+    def work(d, seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            s, gy, gs, gain = (normal(*shape, seed=seed + k, dtype=torch.float16) for k, shape in enumerate([(8, d), (8, d), (8, d), (d,)]))
+            rstd = torch.ones(8, device="cuda")
+            size = lib.th_rms_norm_bwd_workspace_bytes(8, d, 1)
+            dx, dw, scratch = torch.empty_like(s), torch.empty_like(gain), torch.empty(size, dtype=torch.uint8, device="cuda")
+            stream = _lib.stream_ptr(s.device)
+            for _ in range(3000):
+                rc = lib.th_rms_norm_bwd(
+                    s.data_ptr(), d, gain.data_ptr(), 1, rstd.data_ptr(), gy.data_ptr(), d, gs.data_ptr(), d, dx.data_ptr(), dw.data_ptr(),
+                    scratch.data_ptr(), size, 8, d, 1, stream,
+                )  # fmt: skip
+                if rc:
+                    failed.append((d, rc, lib.th_last_error_string()))
+                    return
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(d, 10 * k)) for k, d in enumerate([4096, 2320, 4096, 2320])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed

@@ -904,6 +904,9 @@ struct NormBwdPlan {
     RingPlan ring;
 };
 
+// Dynamic shared memory of a CTA's ring, at most
+constexpr int ring_budget(int consumers) { return (consumers == 256 ? 110 : 222) * 1024; }
+
 // A thread sums 32 columns at most.  Up to four packets a lane a row is a warp's; longer ones are shared by 256 or 512 threads.  Two CTAs
 // share an SM where two stages of a CTA fit half of it.
 template <typename T>
@@ -918,7 +921,7 @@ NormBwdPlan norm_bwd_plan(long long rows, int d, int kind, bool gs) {
     p.team = wide ? p.consumers : 32;
     RingPlan &r = p.ring;
     r.slot = (packets + 1) * 16;
-    const int tensors = gs ? 3 : 2, budget = (p.consumers == 256 ? 110 : 222) * 1024;
+    const int tensors = gs ? 3 : 2, budget = ring_budget(p.consumers);
     // short rows: eight at a time, and more as long as a stage stays small
     r.rows = wide ? 1 : 8;
     while (!wide && r.rows < 64 && 2 * r.rows * r.slot * tensors <= 16 * 1024) r.rows *= 2;
@@ -935,21 +938,33 @@ NormBwdPlan norm_bwd_plan(long long rows, int d, int kind, bool gs) {
     return p;
 }
 
+// The function's limit of shared memory is the most that any ring takes, set once per thread and device: it belongs to the device, where another
+// thread's launch of the same kernel may have another ring.
+template <typename T, int P, bool GS, bool SHIFT, int CONSUMERS>
+int launch_norm_bwd_of(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
+    auto kernel = norm_bwd_kernel<T, P, GS, SHIFT, CONSUMERS>;
+    static thread_local unsigned long long ready = 0;
+    int device = 0;
+    if (int rc = cuda_status(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+    if (device >= 64 || !(ready >> device & 1)) {
+        if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_budget(CONSUMERS)),
+                                 "cudaFuncSetAttribute(norm_bwd_kernel)"))
+            return rc;
+        if (device < 64) ready |= 1ull << device;
+    }
+    const size_t smem = static_cast<size_t>(plan.ring.stages) * (GS ? 3 : 2) * plan.ring.tensor_bytes;
+    return launch_chained("norm_bwd_kernel", kernel, plan.parts, CONSUMERS + 32, smem, stream, 1, a, plan.ring);
+}
+
 template <typename T, bool GS, bool SHIFT, int CONSUMERS>
 int launch_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
-    const size_t smem = static_cast<size_t>(plan.ring.stages) * (GS ? 3 : 2) * plan.ring.tensor_bytes;
-    const auto run = [&](auto kernel) -> int {
-        if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "cudaFuncSetAttribute(norm_bwd_kernel)"))
-            return rc;
-        return launch_chained("norm_bwd_kernel", kernel, plan.parts, CONSUMERS + 32, smem, stream, 1, a, plan.ring);
-    };
     switch (plan.per_thread) {
-        case 1: return run(norm_bwd_kernel<T, 1, GS, SHIFT, CONSUMERS>);
-        case 2: return run(norm_bwd_kernel<T, 2, GS, SHIFT, CONSUMERS>);
-        case 4: return run(norm_bwd_kernel<T, 4, GS, SHIFT, CONSUMERS>);
+        case 1: return launch_norm_bwd_of<T, 1, GS, SHIFT, CONSUMERS>(a, plan, stream);
+        case 2: return launch_norm_bwd_of<T, 2, GS, SHIFT, CONSUMERS>(a, plan, stream);
+        case 4: return launch_norm_bwd_of<T, 4, GS, SHIFT, CONSUMERS>(a, plan, stream);
         default: break;
     }
-    if constexpr (sizeof(T) == 4) return run(norm_bwd_kernel<T, 8, GS, SHIFT, CONSUMERS>);
+    if constexpr (sizeof(T) == 4) return launch_norm_bwd_of<T, 8, GS, SHIFT, CONSUMERS>(a, plan, stream);
     return fail(TH_ERR_UNSUPPORTED, "norm_bwd_kernel: %d packets a thread", plan.per_thread);
 }
 
