@@ -6,6 +6,7 @@
 // same bits from any kernel (and from elementary operations elsewhere).  The floor keeps 127 / a finite: a row of zeros has zeros and
 // a scale of 2^-100 / 127.  A row that holds an infinity or a NaN gets zeros and a NaN as its scale: it reads back as NaN throughout.
 #include "chained.cuh"
+#include "drain.cuh"
 
 #include <algorithm>
 #include <initializer_list>
@@ -518,16 +519,17 @@ struct RingPlan {
     long long blocks;          // stages in all
 };
 
-// After a wait that ran out everybody goes on with what is there, so that nobody is left at a barrier; the status says so.
-__device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
+// After a wait that ran out (false) nothing more is fetched, and the consumers go on with what is there, so that nobody is left at a barrier;
+// the status says so.
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
     unsigned long long deadline = 0;
     for (unsigned poll = 0;; ++poll) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
                      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return;
+        if (done) return true;
         if ((poll & 63u) == 63u) {
-            if (*reinterpret_cast<volatile int *>(abort_flag)) return;
+            if (*reinterpret_cast<volatile int *>(abort_flag)) return false;
             unsigned long long now;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
             if (deadline == 0) deadline = now + kRingWaitNs;
@@ -536,6 +538,7 @@ __device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, int *ab
     }
     *reinterpret_cast<volatile int *>(abort_flag) = 1;
     g_rows_status = 1;
+    return false;
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
@@ -596,7 +599,7 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
     if (warp == kWarps) {
         // ---- rows -> shared memory: whole 16-byte granules that hold a byte of the rows ----
         for (long long block = blockIdx.x; block < ring.blocks; block += gridDim.x) {
-            ring_wait(shared(&empty[stage]), phase ^ 1, &abort_flag);
+            if (!__all_sync(~0u, ring_wait(shared(&empty[stage]), phase ^ 1, &abort_flag))) break;
             const long long row0 = block * ring.rows;
             const int rows = static_cast<int>(min(static_cast<long long>(ring.rows), a.rows - row0));
             const uint32_t bar = shared(&full[stage]);
@@ -711,6 +714,11 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
         }
     }
     __syncthreads();  // every stage has been read: their memory takes the sums
+    if (abort_flag) {  // the same for all threads: nothing may land in this memory once another CTA has it
+        if (threadIdx.x == 0) drain_copies(full, ring.stages);
+        __syncthreads();
+        return;
+    }
     if (!a.partial) return;
     float *out = a.partial + static_cast<long long>(blockIdx.x) * a.d;
     const Span<T, SHIFT> span(base[0] + (static_cast<long long>(blockIdx.x) * ring.rows + (wide ? 0 : warp)) * pitch[0], a.d);
