@@ -121,25 +121,28 @@ __device__ __forceinline__ void gemm_commit(uint32_t mbar, uint32_t leader) {
                      "h"(static_cast<unsigned short>(3u << leader)) : "memory");
 }
 
-// Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.
+// Called by whole warps.  Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.  Lanes may
+// see the barrier and the flag in different orders, so they agree: what follows a wait is elected from, and left by, all of them.
 __device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
     unsigned long long deadline = 0;
+    uint32_t done;
     for (unsigned poll = 0;; ++poll) {
-        uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
                      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
+        if (done) break;
         if ((poll & 63u) == 63u) {
-            if (*reinterpret_cast<volatile int *>(abort_flag)) return false;
+            if (*reinterpret_cast<volatile int *>(abort_flag)) break;
             unsigned long long now;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
             if (deadline == 0) deadline = now + kGemmWaitNs;
-            else if (now > deadline) break;
+            else if (now > deadline) {
+                *reinterpret_cast<volatile int *>(abort_flag) = 1;
+                g_tc_status = 1;
+                break;
+            }
         }
     }
-    *reinterpret_cast<volatile int *>(abort_flag) = 1;
-    g_tc_status = 1;
-    return false;
+    return __all_sync(~0u, done != 0);
 }
 
 struct GemmUnit {
