@@ -74,3 +74,37 @@ def test_norm_backward_from_several_threads():
     for t in threads:
         t.join()
     assert not failed
+
+
+# few tokens, a tile per token group, split and whole products
+@pytest.mark.parametrize("tokens,d_in,d_out", [(1, 64, 40), (3, 4096, 200), (100, 512, 130), (300, 200, 77), (300, 4096, 64), (2100, 640, 1930)])
+@pytest.mark.parametrize("x_size,w_size", [(1e-30, 1e-6), (1e-20, 1e-17), (1e30, 1e-6), (1e18, 1e17), (1e-26, 1e30)])
+def test_scales_far_from_one(tokens, d_in, d_out, x_size, w_size):
+    # the scales' product, or a sum times one scale, is outside of what float32 holds well; the result is inside
+    rows = quantize_rows(normal(tokens, d_in) * x_size)
+    weight = quantize_rows(normal(d_out, d_in, seed=1) * w_size)
+    bias = normal(d_out, seed=2) * (x_size * w_size)
+    acc = rows.q.double() @ weight.q.double().t()
+    scaled = acc * rows.scale.double()[:, None] * weight.scale.double()
+    assert bool((scaled.abs() < 2.0**127).all())
+    for b in (None, bias):
+        y = int8_linear(rows, weight, b, dtype=torch.float32)
+        want = scaled if b is None else scaled + b.double()
+        # four roundings (conversion, product of the scales, product, bias), and half of float32's smallest step
+        assert bool(((y.double() - want).abs() <= 4.01 * 2.0**-24 * (scaled.abs() + (0 if b is None else b.double().abs())) + 2.0**-150).all())
+    if x_size * w_size > 2.0**-126:
+        y = int8_linear(rows, weight, dtype=torch.bfloat16)
+        assert bool(((y.double() - scaled).abs() <= (2.0**-8 + 4 * 2.0**-24) * scaled.abs() + 2.0**-134).all())
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_sums_of_nothing_under_the_largest_scales(tokens):
+    # x and w are orthogonal as integers: 0, and not 0 times an infinite product of the scales
+    x = torch.full((tokens, 64), torch.finfo(torch.float32).max, device="cuda")
+    w = torch.full((24, 64), 1e30, device="cuda")
+    w[:, ::2] *= -1
+    y = int8_linear(quantize_rows(x), quantize_rows(w), dtype=torch.float32)
+    assert bool((y == 0).all())
+    w[0] = 1e30  # one output is past float32
+    y = int8_linear(quantize_rows(x), quantize_rows(w), dtype=torch.float32)
+    assert bool((y[:, 0] == float("inf")).all()) and bool((y[:, 1:] == 0).all())

@@ -37,7 +37,7 @@ struct GemmArgs {
     int out_dtype;
     int out_tma;
     int early;             // A does not come from the kernel before: its first stages are fetched while that one runs
-    const float *lane_scale, *column_scale;  // along m and along n
+    const float *lane_scale, *column_scale;  // along m and along n (8 bits)
     const void *bias;      // along n (along m where transposed)
     int bias_dtype;
 };
@@ -49,7 +49,7 @@ struct GemmShape {
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
     static constexpr int kFixed = CTAS == 1 ? 4 * kStagingBoxes * kStagingBytes : 0;  // transposed outputs have no staging
-    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * 2 * BN * 4;     // the scales and barriers are beside it
+    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * 3 * BN * 4;     // the scales, biases and barriers are beside it
     static constexpr int kFit = (kSmem - kFixed - 1024) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kBytes = kStages * kStage + kFixed + 1024;
@@ -219,10 +219,18 @@ __device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *
     __syncwarp();
 }
 
+// A scale as two factors of about its square root: a power of two, and the rest.  A sum takes both scales' powers first, then the product of
+// the rests: neither the scales' product (2^-214 to 2^242 for 8-bit rows) nor a sum times one of them has to be a float32, only the result.  Where the
+// product is an ordinary float32 the results are the same bits as with it: sum x powers is exact, and rounding the product of the rests rounds it.
+__device__ __forceinline__ float2 split_scale(float scale) {
+    const uint32_t power = ((__float_as_uint(scale) >> 23 & 255u) + 127u) >> 1;  // the exponents' fields: half of the scale's, with the same bias
+    return make_float2(__uint_as_float(power << 23), scale * __uint_as_float((254u - power) << 23));
+}
+
 // One result from its sum
 template <int EB>
-__device__ __forceinline__ float finished(uint32_t raw, float scale, float bias) {
-    if constexpr (EB == 1) return static_cast<float>(static_cast<int>(raw)) * scale + bias;
+__device__ __forceinline__ float finished(uint32_t raw, float2 row, float2 column, float bias) {
+    if constexpr (EB == 1) return fmaf(static_cast<float>(static_cast<int>(raw)) * (row.x * column.x), row.y * column.y, bias);
     else return __uint_as_float(raw) + bias;
 }
 
@@ -248,7 +256,7 @@ __device__ __forceinline__ uint4 ld_cluster_16(uint32_t addr) {
 // This CTA's part of a split tile.  A read of another CTA's shared memory takes some 600 cycles, so PIECES_AT_ONCE x RANKS (16) of them are
 // on their way together.
 template <int EB, int BN, int CG, bool SWAP, int PIECES_AT_ONCE, int RANKS>
-__device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &u, uint32_t rank, uint32_t smem, const float *scales, const float *biases) {
+__device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &u, uint32_t rank, uint32_t smem, const float2 *scales, const float *biases) {
     constexpr int kPieces = SWAP ? kGemmRows / 4 : BN / 4;
     const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN, rows = max(0, min(kGemmRows, g.m - m0)), cols = min(BN, g.n - n0);
     const int lines = SWAP ? cols : rows, along = SWAP ? rows : cols, total = lines * kPieces;
@@ -283,10 +291,10 @@ __device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &
                 const int c = 4 * piece + e;
                 if (c >= along) break;
                 const int mi = m0 + (SWAP ? c : line), ni = SWAP ? line : c;
-                const float scale = EB == 1 ? (g.lane_scale ? g.lane_scale[mi] : 1.f) * scales[ni] : 1.f;
+                const float2 scale = EB == 1 ? split_scale(g.lane_scale[mi]) : make_float2(1.f, 1.f);
                 const float bias = SWAP ? (g.bias ? bias_at(g.bias, g.bias_dtype, mi) : 0.f) : biases[ni];
                 store_one(g.out, SWAP ? static_cast<long long>(n0 + line) * g.out_stride + mi : static_cast<long long>(m0 + line) * g.out_stride + n0 + c,
-                          finished<EB>(sum[e], scale, bias), g.out_dtype);
+                          finished<EB>(sum[e], scale, scales[ni], bias), g.out_dtype);
             }
         }
     }
@@ -300,7 +308,8 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     using S = GemmShape<EB, A_MN, B_MN, BN, CG, CTAS>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
-    __shared__ float scales[2][BN], biases[2][BN];
+    __shared__ float2 scales[2][BN];
+    __shared__ float biases[2][BN];
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
     const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -431,13 +440,14 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
             const GemmUnit u = gemm_unit(g, unit);
             const int buf = done & 1;
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter, n0 = u.tn * BN, m = m0 + lane;
-            float lane_scale = 1.f, lane_bias = 0.f;
-            if (g.lane_scale) lane_scale = m < g.m ? g.lane_scale[m] : 0.f;
+            float2 lane_scale = make_float2(1.f, 1.f);
+            float lane_bias = 0.f;
+            if (EB == 1 && m < g.m) lane_scale = split_scale(g.lane_scale[m]);
             if (SWAP && g.bias) lane_bias = m < g.m ? bias_at(g.bias, g.bias_dtype, m) : 0.f;
             // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
             for (int c = threadIdx.x - 128; c < BN; c += 128) {
                 const bool inside = n0 + c < g.n;
-                scales[buf][c] = g.column_scale && inside ? g.column_scale[n0 + c] : 1.f;
+                if (EB == 1) scales[buf][c] = split_scale(inside ? g.column_scale[n0 + c] : 0.f);
                 biases[buf][c] = !SWAP && g.bias && inside ? bias_at(g.bias, g.bias_dtype, n0 + c) : 0.f;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -484,7 +494,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                 }
 #pragma unroll
                 for (int k = 0; k < kStep; ++k)
-                    raw[k] = __float_as_uint(finished<EB>(raw[k], lane_scale * scales[buf][c0 + k], SWAP ? lane_bias : biases[buf][c0 + k]));
+                    raw[k] = __float_as_uint(finished<EB>(raw[k], lane_scale, scales[buf][c0 + k], SWAP ? lane_bias : biases[buf][c0 + k]));
                 if constexpr (SWAP) {
                     if (m < g.m) {
 #pragma unroll
