@@ -7,6 +7,7 @@ import torch
 from triton_helpers_b200 import _lib
 from triton_helpers_b200.layers.checkpointed_linear import checkpointed_linear
 from triton_helpers_b200.layers.int8_linear import Int8Rows, dequantize_rows, int8_linear, quantize_rows
+from triton_helpers_b200.layers.rms_norm import rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,46 @@ def test_sums_of_nothing_under_the_largest_scales(tokens):
     w[0] = 1e30  # one output is past float32
     y = int8_linear(quantize_rows(x), quantize_rows(w), dtype=torch.float32)
     assert bool((y[:, 0] == float("inf")).all()) and bool((y[:, 1:] == 0).all())
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request):
+    _lib.native().defer(request.param == "python")
+    yield request.param
+    _lib.native().defer(False)
+
+
+@pytest.mark.parametrize("leaf", [True, False])
+def test_a_second_derivative_is_refused_and_not_dropped(path, leaf):
+    def inputs(dtype):
+        x = normal(6, 32, dtype=dtype).requires_grad_(True)
+        return x, (lambda: x if leaf else x * 1), normal(32, seed=1, dtype=dtype).requires_grad_(True), normal(24, 32, seed=2, dtype=dtype).requires_grad_(True)
+
+    layers = {
+        "norm": (torch.float32, lambda h, gain, w: rms_norm(h, gain)),
+        "norm of a sum": (torch.float32, lambda h, gain, w: sum(rms_norm(h, gain, h))),
+        "linear": (torch.float16, lambda h, gain, w: checkpointed_linear(h, w)),
+    }
+    for dtype, layer in layers.values():
+        x, h, gain, w = inputs(dtype)
+        parameter = w if dtype == torch.float16 else gain
+        plain = torch.autograd.grad(layer(h(), gain, w).sum(), [x, parameter])
+        for k in range(2):
+            y = layer(h(), gain, w)
+            g = torch.autograd.grad(y.sum(), [x, parameter], create_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(g, plain))
+            loss = g[k].float().square().sum() + y.float().sum() + x.float().sum() + parameter.float().sum()
+            for call in (lambda: loss.backward(retain_graph=True), *(lambda t=t: torch.autograd.grad(loss, [t], retain_graph=True) for t in (x, parameter))):
+                with pytest.raises(RuntimeError, match="not differentiable twice"):
+                    call()
+        y = layer(h(), gain, w)  # an incoming gradient with a history of its own
+        scale = torch.ones((), device="cuda", dtype=y.dtype, requires_grad=True)
+        (g,) = torch.autograd.grad((y * scale).sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable twice"):
+            torch.autograd.grad(g.sum() + scale, [scale])
+    # the sum beside the norm is a sum: its derivatives of any order are
+    x = normal(6, 32).requires_grad_(True)
+    s = rms_norm(x, torch.ones(32, device="cuda"), x.detach())[1]
+    (g,) = torch.autograd.grad(s.square().sum(), [x], create_graph=True)
+    (second,) = torch.autograd.grad(g.sum(), [x])
+    assert torch.equal(second, torch.full_like(x, 2.0))

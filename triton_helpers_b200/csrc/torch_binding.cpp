@@ -22,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -1300,6 +1301,21 @@ bool norm_call(NormCall &c, PyObject *const *args, Py_ssize_t n_args) {
            rows_of(c.residual, c.d, c.rr);
 }
 
+// Gradients that are to be differentiated themselves (create_graph): as these kernels have no second derivative, their history is a node that
+// raises, on the way to everything that they depend on, so that no term of a loss goes missing.
+void refuse_second(const char *what, const Node &node, const variable_list &grads, variable_list &out) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges(node.next_edges());
+    for (const Tensor &g : grads)
+        if (g.defined()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    const std::shared_ptr<Node> error(new torch::autograd::Error(std::string(what) + " is not differentiable twice", std::move(edges)), torch::autograd::deleteNode);
+    for (Tensor &t : out) {
+        if (!t.defined()) continue;
+        t = t.detach();
+        torch::autograd::set_history(t, error);
+    }
+}
+
 struct RmsNormNode : public Node {
     SavedVariable s, gain, rstd;
     int64_t rows = 0, d = 0;
@@ -1321,6 +1337,11 @@ struct RmsNormNode : public Node {
             return out;
         }
         Tensor ss = s.unpack(shared_from_this()), g = gain.unpack(), r = rstd.unpack();
+        gradients(grads, added, ss, g, r, out);
+        refuse_second("rms_norm", *this, grads, out);
+        return out;
+    }
+    void gradients(const variable_list &grads, const Tensor &added, Tensor ss, Tensor g, Tensor r, variable_list &out) {
         at::NoGradGuard no_grad;
         ss = same(ss, type, rows * d);
         g = restored(g, gain_type, d);
@@ -1339,7 +1360,6 @@ struct RmsNormNode : public Node {
         if (task_should_compute_output(0)) out[0] = dx;
         if (task_should_compute_output(2)) out[2] = dx;
         out[1] = dg;
-        return out;
     }
 };
 
@@ -1551,6 +1571,11 @@ struct CheckpointedLinearNode : public Node {
             q8 = q.unpack();
             s = scale.unpack();
         }
+        gradients(grads, w, q8, s, out);
+        refuse_second("checkpointed_linear", *this, grads, out);
+        return out;
+    }
+    void gradients(const variable_list &grads, const Tensor &w, Tensor q8, Tensor s, variable_list &out) {
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(grads[0].device());
         const c10::Device device = grads[0].device();
@@ -1587,7 +1612,6 @@ struct CheckpointedLinearNode : public Node {
         } else if (wants_b) {
             check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), partial, scratch, rows, dn, code, stream), "th_column_sum");
         }
-        return out;
     }
 };
 

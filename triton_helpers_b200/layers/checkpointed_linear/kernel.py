@@ -18,10 +18,9 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ... import _lib
-from ..int8_linear.kernel import empty_int8_rows, int8_rows2d, int8_stride, Int8Rows
+from ..int8_linear.kernel import empty_int8_rows, first_order, int8_rows2d, int8_stride, Int8Rows
 
 
 def _validate(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[int, int]:
@@ -98,7 +97,7 @@ class _checkpointed_linear(Function):
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
-    @once_differentiable
+    @first_order("checkpointed_linear")
     def backward(ctx, gy: Tensor):
         weight, q, scale = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad

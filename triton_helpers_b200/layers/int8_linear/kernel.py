@@ -15,10 +15,12 @@ token and one per output channel a linear layer is an integer product and a fact
 
 The sums are exact in 32 bits (up to 131071 inputs) and rounded once, to the type of the result.
 """
-from typing import NamedTuple, Optional, Union
+from functools import wraps
+from typing import Callable, List, NamedTuple, Optional, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import Function
 
 from ... import _lib
 
@@ -41,6 +43,54 @@ def float_dtype(t: Tensor, what: str) -> torch.dtype:
 def refuse_gradients(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+class _Once(Function):
+    r"""A gradient as it is, with a history on the way to ``reach`` that raises."""
+
+    @staticmethod
+    def forward(ctx, what: str, grad: Tensor, *reach: Tensor) -> Tensor:
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} is not differentiable twice")
+
+
+def _leaves(ctx) -> List[Tensor]:
+    r"""The leaves that a node's inputs come from."""
+    nodes, seen, leaves = [ctx], set(), []
+    while nodes:
+        for node, _ in nodes.pop().next_functions:
+            if node is None or node in seen:
+                continue
+            seen.add(node)
+            if hasattr(node, "variable"):
+                leaves.append(node.variable)
+            else:
+                nodes.append(node)
+    return leaves
+
+
+def first_order(what: str) -> Callable:
+    r"""For a backward pass of kernels: gradients that are to be differentiated themselves (``create_graph``) raise where that happens,
+    whatever the loss is made of besides.  ``once_differentiable`` lets them pass as constants where the incoming gradient is one."""
+
+    def decorate(backward: Callable) -> Callable:
+        @wraps(backward)
+        def wrapper(ctx, *grads: Optional[Tensor]):
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            if not torch.is_grad_enabled():
+                return out
+            reach = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad] + _leaves(ctx)
+            passed = lambda t: t is None or any(t is g for g in grads)  # noqa: E731  an incoming gradient handed on keeps its own history
+            return tuple(t if passed(t) else _Once.apply(what, t.detach().requires_grad_(), *reach) for t in out)
+
+        return wrapper
+
+    return decorate
 
 
 def rows2d(t: Tensor, width: int) -> Tensor:

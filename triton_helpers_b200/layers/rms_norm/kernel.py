@@ -15,10 +15,9 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ... import _lib
-from ..int8_linear.kernel import Int8Rows, empty_int8_rows, float_dtype, refuse_gradients, row_stride, rows2d
+from ..int8_linear.kernel import Int8Rows, empty_int8_rows, first_order, float_dtype, refuse_gradients, row_stride, rows2d
 
 
 def _validate(x: Tensor, weight: Tensor, residual: Optional[Tensor]) -> int:
@@ -64,7 +63,7 @@ class _rms_norm(Function):
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
-    @once_differentiable
+    @first_order("rms_norm")
     def backward(ctx, gy: Optional[Tensor], gs: Optional[Tensor] = None):
         s, weight, rstd = ctx.saved_tensors
         want_x, want_w, want_r, _ = ctx.needs_input_grad
