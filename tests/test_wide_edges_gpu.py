@@ -7,7 +7,7 @@ import torch
 from triton_helpers_b200 import _lib
 from triton_helpers_b200.layers.checkpointed_linear import checkpointed_linear
 from triton_helpers_b200.layers.int8_linear import Int8Rows, dequantize_rows, int8_linear, quantize_rows
-from triton_helpers_b200.layers.rms_norm import rms_norm
+from triton_helpers_b200.layers.rms_norm import rms_norm, rms_norm_int8
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,31 @@ def test_a_second_derivative_is_refused_and_not_dropped(path, leaf):
     (g,) = torch.autograd.grad(s.square().sum(), [x], create_graph=True)
     (second,) = torch.autograd.grad(g.sum(), [x])
     assert torch.equal(second, torch.full_like(x, 2.0))
+
+
+def test_functions_without_a_gradient_refuse_one(path):
+    x, gain, w = normal(6, 32), normal(32, seed=1), quantize_rows(normal(24, 32, seed=2))
+    rows, bias = quantize_rows(x), normal(24, seed=3)
+    calls = {  # by the tensor that would need the gradient
+        "quantize_rows": (x, lambda t: quantize_rows(t)),
+        "dequantize_rows": (rows.scale, lambda t: dequantize_rows(Int8Rows(rows.q, t))),
+        "rms_norm_int8": (gain, lambda t: rms_norm_int8(x, t)),
+        "rms_norm_int8 ": (x, lambda t: rms_norm_int8(x, gain, t)),
+        "int8_linear": (x, lambda t: int8_linear(t, w)),
+        "int8_linear ": (bias, lambda t: int8_linear(x, w, t)),
+        "int8_linear  ": (w.scale, lambda t: int8_linear(x, Int8Rows(w.q, t))),
+        "int8_linear   ": (rows.scale, lambda t: int8_linear(Int8Rows(rows.q, t), w, dtype=torch.float32)),
+    }
+    for t, call in calls.values():
+        leaf = t.clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(leaf)
+        with torch.no_grad():
+            want, got = call(t), call(leaf)
+        assert all(torch.equal(a, b) for a, b in zip(*(v if isinstance(v, tuple) else (v,) for v in (want, got))) if torch.is_tensor(a))
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="no gradient"):
+                    call(dual)
+            call(t)  # without a tangent: as elsewhere

@@ -1490,7 +1490,7 @@ PyObject *py_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     if (code < 0 || (bias.defined() && (!plain(bias) || bias.dim() != 1 || bias.size(0) != d_out || !bias.is_contiguous() || bias.scalar_type() != type ||
                                         bias.device() != wq.device())))
         TH_NOT_MINE;
-    if (torch::autograd::compute_requires_grad(x, bias)) TH_NOT_MINE;
+    if (torch::autograd::compute_requires_grad(x, scale, w_scale, bias)) TH_NOT_MINE;
     Tensor y;
     {
         NoGil release;

@@ -20,7 +20,7 @@ from typing import Callable, List, NamedTuple, Optional, Union
 
 import torch
 from torch import Tensor
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from ... import _lib
 
@@ -41,8 +41,12 @@ def float_dtype(t: Tensor, what: str) -> torch.dtype:
 
 
 def refuse_gradients(what: str, *tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    # a tangent is carried without regard to no_grad
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise RuntimeError(f"{what} has no gradient: its inputs must not have tangents")
 
 
 class _Once(Function):
@@ -130,9 +134,15 @@ def int8_stride(q: Tensor) -> int:
     return q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
 
 
-@torch.no_grad()
 def quantize_rows(x: Tensor) -> Int8Rows:
-    r"""8-bit rows of ``x`` (..., K), float16, bfloat16 or float32; no gradient."""
+    r"""8-bit rows of ``x`` (..., K), float16, bfloat16 or float32.  No gradient: an ``x`` that requires one is refused outside of
+    ``torch.no_grad()``."""
+    refuse_gradients("quantize_rows", x)
+    with torch.no_grad():
+        return _quantize_rows(x)
+
+
+def _quantize_rows(x: Tensor) -> Int8Rows:
     assert x.dim() >= 1 and x.shape[-1] >= 1, "8-bit rows need at least one column"
     float_dtype(x, "x")
     device = _lib.require_cuda(x)
@@ -150,9 +160,15 @@ def quantize_rows(x: Tensor) -> Int8Rows:
     return out
 
 
-@torch.no_grad()
 def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> Tensor:
-    r"""``q * scale`` of 8-bit rows, rounded once to ``dtype`` (float16, bfloat16 or float32); contiguous."""
+    r"""``q * scale`` of 8-bit rows, rounded once to ``dtype`` (float16, bfloat16 or float32); contiguous.  No gradient: scales that
+    require one are refused outside of ``torch.no_grad()``."""
+    refuse_gradients("dequantize_rows", rows.scale)
+    with torch.no_grad():
+        return _dequantize_rows(rows, dtype)
+
+
+def _dequantize_rows(rows: Int8Rows, dtype: torch.dtype) -> Tensor:
     lead, width = rows.q.shape[:-1], rows.q.shape[-1]
     q, scale = int8_rows2d(rows, "dequantize_rows")
     device = _lib.require_cuda(q, scale)
@@ -190,10 +206,10 @@ def int8_linear(
     if held:
         if dtype is None:
             raise TypeError("8-bit rows do not say the type of the result: pass dtype")
-        refuse_gradients("int8_linear", bias)
+        refuse_gradients("int8_linear", x.scale, weight.scale, bias)
         rows = x
     else:
-        refuse_gradients("int8_linear", x, bias)
+        refuse_gradients("int8_linear", x, weight.scale, bias)
         dtype = float_dtype(x, "x") if dtype is None else dtype
         rows = None
     if dtype not in _lib.DTYPE_CODE:
