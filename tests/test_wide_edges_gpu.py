@@ -180,3 +180,23 @@ def test_functions_without_a_gradient_refuse_one(path):
                 with mode(), pytest.raises(RuntimeError, match="no gradient"):
                     call(dual)
             call(t)  # without a tangent: as elsewhere
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("given", [torch.float16, torch.bfloat16, torch.float32])
+def test_autocast_takes_the_type_that_it_is_given(given, dtype):
+    # 1e5 is past float16: it is finite in and out under bfloat16
+    size = 1e5 if dtype == torch.bfloat16 and given != torch.float16 else 1.0
+    x = (normal(30, 96) * size).to(given).requires_grad_(True)
+    w, b = normal(56, 96, seed=1, dtype=given).requires_grad_(True), normal(56, seed=2, dtype=given).requires_grad_(True)
+    gy = (normal(30, 56, seed=3) * size).to(dtype)
+    with torch.autocast("cuda", dtype):
+        y = checkpointed_linear(x, w, b)
+    grads = torch.autograd.grad(y, [x, w, b], gy)
+    cast = [t.detach().to(dtype).requires_grad_(True) for t in (x, w, b)]
+    want = checkpointed_linear(*cast)
+    assert y.dtype == dtype and bool(y.isfinite().all()) and torch.equal(y, want)
+    for got, leaf, exact in zip(grads, (x, w, b), torch.autograd.grad(want, cast, gy)):
+        assert got.dtype == leaf.dtype and torch.equal(got, exact.to(given))
+    with torch.autocast("cuda", dtype), torch.no_grad():
+        assert torch.equal(checkpointed_linear(x, w, b), y)

@@ -2,7 +2,7 @@ r"""Linear layer of any width that keeps its input in 8 bits for the backward pa
 
 There is no such operator in triton_helpers, whose fused network ends at 64 columns
 (``triton_helpers/layers/fully_fused_mlp/kernel.py:13-14``); this module follows its conventions: a
-``torch.autograd.Function`` plus a functional wrapper, ``(out, in)`` weights, autocast to float16.
+``torch.autograd.Function`` plus a functional wrapper, ``(out, in)`` weights.  Under autocast the layer runs in autocast's type.
 
     y = x w^T + b                     16-bit operands, float32 sums, rounded once
     kept: q, scale = 8-bit rows of x (``layers.int8_linear``): K + 4 bytes a row instead of 2 K
@@ -64,8 +64,13 @@ def _stride(t: Tensor) -> int:
 class _checkpointed_linear(Function):
 
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda", cast_inputs=torch.float16)
     def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
+        # the type to cast to is known at the call
+        cast = torch.amp.custom_fwd(_checkpointed_linear._forward, device_type="cuda", cast_inputs=torch.get_autocast_dtype("cuda"))
+        return cast(ctx, x, weight, bias)
+
+    @staticmethod
+    def _forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
         d_in, d_out = _validate(x, weight, bias)
         device = _lib.require_cuda(x, weight, bias)
         x2d, w = _operand(x, d_in), _operand(weight, d_in)
@@ -162,7 +167,7 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
     r"""Linear layer whose backward pass reads its input from 8-bit rows kept by the forward pass.
 
     Args:
-        x: float16 or bfloat16; under autocast any float type, cast to float16
+        x: float16 or bfloat16; under autocast any float type but float64, cast to autocast's (float16 or bfloat16)
         weight, bias: of x's type; the bias may be ``None``
 
     Shapes:
