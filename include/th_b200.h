@@ -393,9 +393,11 @@ int th_scale_cast(const float *src_dev, void *dst_dev, int64_t n_elems, float sc
  * columns: a root-mean-square norm, linear layers on 8-bit integers, and the products and 8-bit rows of
  * a linear layer that keeps its input in 8 bits for the backward pass.
  *
- * Matrices are rows of `d` elements with unit stride inside a row; strides count elements.
+ * Matrices are rows of `d` elements with unit stride inside a row; strides count elements.  A pointer off its
+ * elements' size is refused (TH_ERR_ALIGNMENT).
  * 8-bit rows:  a = max(max_k |x_k|, 2^-100);  q_k = rint(x_k * (127 / a));  scale = a / 127, in float32.
- * They start on 16 bytes (pointer and stride); bytes between d and the stride are never read.  A row
+ * They start on 16 bytes (pointer and stride); bytes between d and the stride are never read, and may be
+ * written where rows are made.  A row
  * that holds an infinity or a NaN gets zeros and the scale NaN.
  * ------------------------------------------------------------------------------------------ */
 

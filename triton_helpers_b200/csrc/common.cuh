@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/th_b200.h"
 
@@ -63,5 +64,12 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 inline size_t dtype_bytes(int code) { return code == TH_F32 ? 4 : 2; }
+
+// Pointers (null ones pass) to elements of one type
+inline int check_elements(const char *what, int dtype, std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (!aligned_to(p, dtype_bytes(dtype))) return fail(TH_ERR_ALIGNMENT, "%s: a pointer is off its elements' size", what);
+    return TH_OK;
+}
 
 }  // namespace th

@@ -9,7 +9,6 @@
 #include "drain.cuh"
 
 #include <algorithm>
-#include <initializer_list>
 #include <utility>
 
 namespace th {
@@ -1157,12 +1156,6 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyArgs a) {
     *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(a.dst[k]) + row * a.dst_stride[k] + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-int check_elements(const char *what, int dtype, std::initializer_list<const void *> pointers) {
-    for (const void *p : pointers)
-        if (!aligned_to(p, dtype_bytes(dtype))) return fail(TH_ERR_ALIGNMENT, "%s: a pointer is off its elements' size", what);
-    return TH_OK;
-}
-
 bool known_dtype(int dtype) { return dtype == TH_F32 || dtype == TH_F16 || dtype == TH_BF16; }
 
 int check_rows(const char *what, long long rows, int d, int dtype) {
@@ -1191,6 +1184,7 @@ extern "C" int th_rms_norm_fwd(const void *x_dev, int64_t x_stride, const void *
     if (!x_dev || !gain_dev || !y_dev || (residual_dev != nullptr) != (sum_dev != nullptr)) return fail(TH_ERR_BAD_ARG, "th_rms_norm_fwd: null pointer");
     if (int rc = check_elements("th_rms_norm_fwd", dtype, {x_dev, residual_dev, sum_dev, y_dev})) return rc;
     if (int rc = check_elements("th_rms_norm_fwd", gain_dtype, {gain_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_fwd", TH_F32, {rstd_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.residual = residual_dev; a.gain = gain_dev; a.sum = sum_dev; a.y = y_dev; a.rstd = rstd_dev;
     a.x_stride = x_stride; a.residual_stride = residual_stride; a.rows = rows; a.d = d; a.gain_f32 = gain_dtype == TH_F32; a.eps = eps;
@@ -1207,6 +1201,7 @@ extern "C" int th_rms_norm_int8(const void *x_dev, int64_t x_stride, const void 
     if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d) return fail(TH_ERR_ALIGNMENT, "th_rms_norm_int8: 8-bit rows start on 16 bytes");
     if (int rc = check_elements("th_rms_norm_int8", dtype, {x_dev, residual_dev, sum_dev})) return rc;
     if (int rc = check_elements("th_rms_norm_int8", gain_dtype, {gain_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_int8", TH_F32, {scale_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.residual = residual_dev; a.gain = gain_dev; a.sum = sum_dev; a.q = static_cast<signed char *>(q_dev); a.scale = scale_dev;
     a.x_stride = x_stride; a.residual_stride = residual_stride; a.q_stride = q_stride; a.rows = rows; a.d = d; a.gain_f32 = gain_dtype == TH_F32; a.eps = eps;
@@ -1220,6 +1215,7 @@ extern "C" int th_quantize_rows(const void *x_dev, int64_t x_stride, void *q_dev
     if (!x_dev || !q_dev || !scale_dev) return fail(TH_ERR_BAD_ARG, "th_quantize_rows: null pointer");
     if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d) return fail(TH_ERR_ALIGNMENT, "th_quantize_rows: 8-bit rows start on 16 bytes");
     if (int rc = check_elements("th_quantize_rows", dtype, {x_dev})) return rc;
+    if (int rc = check_elements("th_quantize_rows", TH_F32, {scale_dev})) return rc;
     RowFwdArgs a{};
     a.x = x_dev; a.q = static_cast<signed char *>(q_dev); a.scale = scale_dev;
     a.x_stride = x_stride; a.q_stride = q_stride; a.rows = rows; a.d = d;
@@ -1232,6 +1228,7 @@ extern "C" int th_dequantize_rows(const void *q_dev, int64_t q_stride, const flo
     if (rows == 0) return TH_OK;
     if (!q_dev || !scale_dev || !out_dev || q_stride < d || out_stride < d) return fail(TH_ERR_BAD_ARG, "th_dequantize_rows: null pointer or short stride");
     if (int rc = check_elements("th_dequantize_rows", dtype, {out_dev})) return rc;
+    if (int rc = check_elements("th_dequantize_rows", TH_F32, {scale_dev})) return rc;
     const DequantizeArgs a{static_cast<const signed char *>(q_dev), scale_dev, out_dev, q_stride, out_stride, rows, d, 0};
     cudaStream_t at = static_cast<cudaStream_t>(stream);
     if (dtype == TH_F32) return dequantize_rows<float>(a, at);
@@ -1288,6 +1285,7 @@ extern "C" int th_rms_norm_bwd(const void *sum_dev, int64_t sum_stride, const vo
         return fail(TH_ERR_WORKSPACE, "th_rms_norm_bwd: scratch missing, too small or off 16 bytes");
     if (int rc = check_elements("th_rms_norm_bwd", dtype, {sum_dev, grad_y_dev, grad_sum_dev, grad_x_dev})) return rc;
     if (int rc = check_elements("th_rms_norm_bwd", gain_dtype, {gain_dev, grad_gain_dev})) return rc;
+    if (int rc = check_elements("th_rms_norm_bwd", TH_F32, {rstd_dev})) return rc;
     RowBwdArgs a{};
     a.s = sum_dev; a.gain = gain_dev; a.gy = grad_y_dev; a.gs = grad_sum_dev; a.rstd = rstd_dev; a.dx = grad_x_dev;
     a.partial = static_cast<float *>(workspace_dev);
@@ -1310,6 +1308,7 @@ extern "C" int th_column_sum(const void *g_dev, int64_t g_stride, void *out_dev,
     if (!g_dev) return fail(TH_ERR_BAD_ARG, "th_column_sum: null pointer");
     if (!workspace_dev || workspace_bytes < th_column_sum_workspace_bytes(rows, d) || !aligned_to(workspace_dev, 4))
         return fail(TH_ERR_WORKSPACE, "th_column_sum: scratch missing or too small");
+    if (int rc = check_elements("th_column_sum", dtype, {g_dev, out_dev})) return rc;
     ColumnArgs sums{};
     sums.g = g_dev; sums.g_stride = g_stride; sums.rows = rows; sums.d = d;
     float *partial = static_cast<float *>(workspace_dev);
@@ -1328,6 +1327,8 @@ extern "C" int th_checkpoint_rows(const void *q_dev, int64_t q_stride, const flo
         return fail(TH_ERR_BAD_ARG, "th_checkpoint_rows: null pointer or short stride");
     if (!workspace_dev || workspace_bytes < th_column_sum_workspace_bytes(rows, d_out) || !aligned_to(workspace_dev, 4))
         return fail(TH_ERR_WORKSPACE, "th_checkpoint_rows: scratch missing or too small");
+    if (int rc = check_elements("th_checkpoint_rows", dtype, {x_dev, g_dev, out_dev})) return rc;
+    if (int rc = check_elements("th_checkpoint_rows", TH_F32, {scale_dev})) return rc;
     const DequantizeArgs a{static_cast<const signed char *>(q_dev), scale_dev, x_dev, q_stride, x_stride, rows, d_in, (d_in + 15) / 16};
     ColumnArgs sums{};
     sums.g = g_dev; sums.g_stride = g_stride; sums.rows = rows; sums.d = d_out;

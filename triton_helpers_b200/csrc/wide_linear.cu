@@ -112,13 +112,14 @@ int check_16bit(const char *what, int dtype) {
 
 bool known_dtype(int dtype) { return dtype == TH_F32 || dtype == TH_F16 || dtype == TH_BF16; }
 
-int check_int8(const void *weight, int64_t weight_stride, const float *weight_scale, const void *y, int64_t y_stride, int d_in, int d_out, int dtype) {
+int check_int8(const void *weight, int64_t weight_stride, const float *weight_scale, const void *bias, const void *y, int64_t y_stride, int d_in, int d_out, int dtype) {
     // 128 x 128 x 131071 is the largest sum that 32 bits are sure to hold
     if (d_in > 131071) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: %d inputs, more than a 32-bit sum holds", d_in);
     if (!known_dtype(dtype)) return fail(TH_ERR_UNSUPPORTED, "th_int8_linear: unknown dtype code %d", dtype);
     if (!weight || !weight_scale || !y || y_stride < d_out) return fail(TH_ERR_BAD_ARG, "th_int8_linear: null pointer or short stride");
     if (!aligned_to(weight, 16) || weight_stride % 16 || weight_stride < d_in) return fail(TH_ERR_ALIGNMENT, "th_int8_linear: 8-bit rows start on 16 bytes");
-    return TH_OK;
+    if (int rc = check_elements("th_int8_linear", TH_F32, {weight_scale})) return rc;
+    return check_elements("th_int8_linear", dtype, {bias, y});
 }
 
 }  // namespace
@@ -141,9 +142,10 @@ static int int8_linear(const void *q_dev, int64_t q_stride, const float *scale_d
                        const void *bias_dev, void *y_dev, int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, int weights_settled, void *stream) {
     if (int rc = check_shape("th_int8_linear", rows, d_in, d_out)) return rc;
     if (rows == 0 && d_in <= 131071 && known_dtype(dtype)) return TH_OK;
-    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
+    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
     if (!q_dev || !scale_dev) return fail(TH_ERR_BAD_ARG, "th_int8_linear: null pointer");
     if (!aligned_to(q_dev, 16) || q_stride % 16 || q_stride < d_in) return fail(TH_ERR_ALIGNMENT, "th_int8_linear: 8-bit rows start on 16 bytes");
+    if (int rc = check_elements("th_int8_linear", TH_F32, {scale_dev})) return rc;
     Product p{};
     p.a = {q_dev, q_stride, static_cast<int>(rows)};
     p.b = {weight_dev, weight_stride, d_out};
@@ -181,7 +183,7 @@ extern "C" int th_quantized_linear(const void *x_dev, int64_t x_stride, int x_dt
     // the product's refusals first: nothing is launched for a call that it does not take
     if (int rc = check_shape("th_quantized_linear", rows, d_in, d_out)) return rc;
     if (rows == 0) return int8_linear(q, pitch, scale, weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, 0, d_in, d_out, dtype, 0, stream);
-    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
+    if (int rc = check_int8(weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, d_in, d_out, dtype)) return rc;
     if (int rc = th_quantize_rows(x_dev, x_stride, q, pitch, scale, rows, d_in, x_dtype, stream)) return rc;
     return int8_linear(q, pitch, scale, weight_dev, weight_stride, weight_scale_dev, bias_dev, y_dev, y_stride, rows, d_in, d_out, dtype, 1, stream);
 }
@@ -193,6 +195,7 @@ extern "C" int th_linear_fwd(const void *x_dev, int64_t x_stride, const void *we
     if (rows == 0) return TH_OK;
     if (!x_dev || !weight_dev || !y_dev || x_stride < d_in || weight_stride < d_in || y_stride < d_out)
         return fail(TH_ERR_BAD_ARG, "th_linear_fwd: null pointer or short stride");
+    if (int rc = check_elements("th_linear_fwd", dtype, {bias_dev, y_dev})) return rc;
     Product p{};
     p.a = {x_dev, x_stride, static_cast<int>(rows)};
     p.b = {weight_dev, weight_stride, d_out};
@@ -211,6 +214,7 @@ extern "C" int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, co
     if (rows == 0) return TH_OK;
     if (!grad_y_dev || !weight_dev || !grad_x_dev || gy_stride < d_out || weight_stride < d_in || gx_stride < d_in)
         return fail(TH_ERR_BAD_ARG, "th_linear_bwd_input: null pointer or short stride");
+    if (int rc = check_elements("th_linear_bwd_input", dtype, {grad_x_dev})) return rc;
     Product p{};
     p.a = {grad_y_dev, gy_stride, static_cast<int>(rows)};
     p.b = {weight_dev, weight_stride, d_in};
@@ -229,6 +233,7 @@ extern "C" int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, c
     cudaStream_t at = static_cast<cudaStream_t>(stream);
     if (rows == 0) return cuda_status(cudaMemsetAsync(grad_weight_dev, 0, static_cast<size_t>(d_in) * d_out * 2, at), "th_linear_bwd_weight");
     if (!grad_y_dev || !x_dev || gy_stride < d_out || x_stride < d_in) return fail(TH_ERR_BAD_ARG, "th_linear_bwd_weight: null pointer or short stride");
+    if (int rc = check_elements("th_linear_bwd_weight", dtype, {grad_weight_dev})) return rc;
     Product p{};
     p.a = {grad_y_dev, gy_stride, d_out};
     p.b = {x_dev, x_stride, d_in};
