@@ -200,3 +200,37 @@ def test_autocast_takes_the_type_that_it_is_given(given, dtype):
         assert got.dtype == leaf.dtype and torch.equal(got, exact.to(given))
     with torch.autocast("cuda", dtype), torch.no_grad():
         assert torch.equal(checkpointed_linear(x, w, b), y)
+
+
+# both sides of every width at which another number of threads or of 16-byte packets a thread takes over
+PACKETS = [1, 2, 6, 7, 8, 9, 14, 16, 17, 30, 32, 33, 60, 64, 124, 128, 129, 256, 257, 496, 512, 513, 1000, 1024, 1025, 1984, 2048, 2049, 3968, 4096, 4097, 7936, 8192, 8193]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("packets", PACKETS)
+def test_widths_where_the_kernel_changes(packets, dtype):
+    per = 16 // dtype.itemsize
+    for d in {packets * per, max(1, packets * per - 3), packets * per + 1}:
+        x, r, gain = normal(2, d, dtype=dtype), normal(2, d, seed=1, dtype=dtype), (1 + 0.3 * normal(d, seed=2)).to(dtype)
+        gy, gs = normal(2, d, seed=3, dtype=dtype), normal(2, d, seed=4, dtype=dtype)
+        for residual in (None, r):
+            leaves = [t.clone().requires_grad_(True) for t in (x, gain)]
+            out = rms_norm(*leaves, residual, 1e-5)
+            y, s = out if residual is not None else (out, leaves[0])
+            grads = torch.autograd.grad(out, leaves, (gy, gs) if residual is not None else gy)
+            v, g, dy = s.detach().double(), gain.double(), gy.double()
+            rstd = (v.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+            h = v * rstd
+            c = (dy * g * h).mean(-1, keepdim=True)
+            dx = rstd * (dy * g - h * c) + (gs.double() if residual is not None else 0)
+            reach = rstd * ((dy * g).abs() + h.abs() * (dy * g * h).abs().mean(-1, keepdim=True)) + (gs.double().abs() if residual is not None else 0)
+            # a row's sum: up to 70 additions of a thread and 10 over the team, and some twenty roundings beside it; then the result's own half step
+            half, step = 1.01 * torch.finfo(dtype).eps / 2, 100 * 2.0**-24
+            for got, want, size in ((y, h * g, (h * g).abs()), (grads[0], dx, reach), (grads[1], (dy * h).sum(0), (dy * h).abs().sum(0))):
+                assert bool(((got.detach().double() - want).abs() <= step * size + half * want.abs() + 2.0**-25).all())
+            rows = rms_norm_int8(x, gain, residual, 1e-5)
+            rows = rows[0] if residual is not None else rows
+            top = (h * g).abs().amax(-1, keepdim=True)
+            assert bool(((rows.q.double() - h * g * 127 / top).abs() <= 0.5 + 127 * 3 * step).all())
+        rows, top = quantize_rows(x), x.float().abs().amax(-1, keepdim=True).clamp_min(2.0**-100)
+        assert torch.equal(rows.q, torch.round(x.float() * (torch.full_like(top, 127.0) / top)).to(torch.int8))

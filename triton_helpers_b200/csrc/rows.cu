@@ -433,14 +433,25 @@ int span_packets(int d, int kind) {
     return kind == kPacked ? d / N : (d + 2 * N - 2) / N;
 }
 
-template <typename T, int MODE, bool RES, bool SHIFT, int THREADS>
+// The kernels that team_plan asks for, over all widths: up to 256 threads have one to four packets each, up to 512 four (two where nine to sixteen
+// warps overlap and two are wanted), 1024 four or eight.
+template <typename T, int MODE, bool RES, bool SHIFT>
 int launch_row_fwd(const RowFwdArgs &a, const TeamPlan &plan, unsigned blocks, cudaStream_t stream) {
-    switch (plan.per_thread) {
-        case 1: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 1, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
-        case 2: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 2, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
-        case 4: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 4, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
-        default: return launch_chained("row_fwd_kernel", row_fwd_kernel<T, 8, MODE, RES, SHIFT, THREADS>, blocks, plan.block, 0, stream, 1, a);
+    const auto run = [&](auto kernel) { return launch_chained("row_fwd_kernel", kernel, blocks, plan.block, 0, stream, 1, a); };
+    const int threads = plan.block <= 256 ? 256 : plan.block <= 512 ? 512 : kMaxTeam;
+    switch (threads + plan.per_thread) {
+        case 256 + 1: return run(row_fwd_kernel<T, 1, MODE, RES, SHIFT, 256>);
+        case 256 + 2: return run(row_fwd_kernel<T, 2, MODE, RES, SHIFT, 256>);
+        case 256 + 4: return run(row_fwd_kernel<T, 4, MODE, RES, SHIFT, 256>);
+        case 512 + 2:
+            if constexpr (RES && SHIFT && MODE == kNormInt8) return run(row_fwd_kernel<T, 2, MODE, RES, SHIFT, 512>);
+            break;
+        case 512 + 4: return run(row_fwd_kernel<T, 4, MODE, RES, SHIFT, 512>);
+        case kMaxTeam + 4: return run(row_fwd_kernel<T, 4, MODE, RES, SHIFT, kMaxTeam>);
+        case kMaxTeam + 8: return run(row_fwd_kernel<T, 8, MODE, RES, SHIFT, kMaxTeam>);
+        default: break;
     }
+    return fail(TH_ERR_UNSUPPORTED, "row_fwd_kernel: %d packets for each of %d threads", plan.per_thread, plan.block);
 }
 
 template <typename T, int MODE, bool RES>
@@ -458,15 +469,8 @@ int plan_row_fwd(RowFwdArgs a, cudaStream_t stream) {
     if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
     const unsigned n = static_cast<unsigned>(blocks), all = static_cast<unsigned>(a.rows);
     a.team = plan.team;
-    if (kind != kAnyhow && plan.per_thread) {
-        if (kind == kPacked)
-            return plan.block <= 256   ? launch_row_fwd<T, MODE, RES, false, 256>(a, plan, n, stream)
-                   : plan.block <= 512 ? launch_row_fwd<T, MODE, RES, false, 512>(a, plan, n, stream)
-                                       : launch_row_fwd<T, MODE, RES, false, kMaxTeam>(a, plan, n, stream);
-        return plan.block <= 256   ? launch_row_fwd<T, MODE, RES, true, 256>(a, plan, n, stream)
-               : plan.block <= 512 ? launch_row_fwd<T, MODE, RES, true, 512>(a, plan, n, stream)
-                                   : launch_row_fwd<T, MODE, RES, true, kMaxTeam>(a, plan, n, stream);
-    }
+    if (kind != kAnyhow && plan.per_thread)
+        return kind == kPacked ? launch_row_fwd<T, MODE, RES, false>(a, plan, n, stream) : launch_row_fwd<T, MODE, RES, true>(a, plan, n, stream);
     const int block = std::min(kMaxTeam, std::max(64, (a.d / 8 + 31) / 32 * 32));
     return launch_chained("row_fwd_stream_kernel", kind == kPacked ? row_fwd_stream_kernel<T, 16, MODE, RES> : row_fwd_stream_kernel<T, sizeof(T), MODE, RES>, all,
                           block, 0, stream, 1, a);
@@ -963,21 +967,21 @@ int launch_norm_bwd_of(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_
     return launch_chained("norm_bwd_kernel", kernel, plan.parts, CONSUMERS + 32, smem, stream, 1, a, plan.ring);
 }
 
-template <typename T, bool GS, bool SHIFT, int CONSUMERS>
+// A row of one warp or of 256 threads has one to four packets a thread, one of 512 two to four, or eight of float32.
+template <typename T, bool GS, bool SHIFT>
 int launch_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
-    switch (plan.per_thread) {
-        case 1: return launch_norm_bwd_of<T, 1, GS, SHIFT, CONSUMERS>(a, plan, stream);
-        case 2: return launch_norm_bwd_of<T, 2, GS, SHIFT, CONSUMERS>(a, plan, stream);
-        case 4: return launch_norm_bwd_of<T, 4, GS, SHIFT, CONSUMERS>(a, plan, stream);
+    switch (plan.consumers + plan.per_thread) {
+        case 256 + 1: return launch_norm_bwd_of<T, 1, GS, SHIFT, 256>(a, plan, stream);
+        case 256 + 2: return launch_norm_bwd_of<T, 2, GS, SHIFT, 256>(a, plan, stream);
+        case 256 + 4: return launch_norm_bwd_of<T, 4, GS, SHIFT, 256>(a, plan, stream);
+        case 512 + 2: return launch_norm_bwd_of<T, 2, GS, SHIFT, 512>(a, plan, stream);
+        case 512 + 4: return launch_norm_bwd_of<T, 4, GS, SHIFT, 512>(a, plan, stream);
+        case 512 + 8:
+            if constexpr (sizeof(T) == 4) return launch_norm_bwd_of<T, 8, GS, SHIFT, 512>(a, plan, stream);
+            break;
         default: break;
     }
-    if constexpr (sizeof(T) == 4) return launch_norm_bwd_of<T, 8, GS, SHIFT, CONSUMERS>(a, plan, stream);
-    return fail(TH_ERR_UNSUPPORTED, "norm_bwd_kernel: %d packets a thread", plan.per_thread);
-}
-
-template <typename T, bool GS, bool SHIFT>
-int size_norm_bwd(const RowBwdArgs &a, const NormBwdPlan &plan, cudaStream_t stream) {
-    return plan.consumers == 256 ? launch_norm_bwd<T, GS, SHIFT, 256>(a, plan, stream) : launch_norm_bwd<T, GS, SHIFT, 512>(a, plan, stream);
+    return fail(TH_ERR_UNSUPPORTED, "norm_bwd_kernel: %d packets for each of %d threads", plan.per_thread, plan.consumers);
 }
 
 template <typename T>
@@ -997,8 +1001,8 @@ int norm_bwd(RowBwdArgs a, void *dgain, int gain_dtype, cudaStream_t stream) {
     if (!dgain) a.partial = nullptr;
     int rc;
     if (plan.per_thread) {
-        if (kind == kPacked) rc = a.gs ? size_norm_bwd<T, true, false>(a, plan, stream) : size_norm_bwd<T, false, false>(a, plan, stream);
-        else rc = a.gs ? size_norm_bwd<T, true, true>(a, plan, stream) : size_norm_bwd<T, false, true>(a, plan, stream);
+        if (kind == kPacked) rc = a.gs ? launch_norm_bwd<T, true, false>(a, plan, stream) : launch_norm_bwd<T, false, false>(a, plan, stream);
+        else rc = a.gs ? launch_norm_bwd<T, true, true>(a, plan, stream) : launch_norm_bwd<T, false, true>(a, plan, stream);
         return rc != TH_OK || !dgain ? rc : sum_partials(partial, plan.parts, a.d, dgain, gain_dtype, stream);
     }
     if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
