@@ -1,7 +1,10 @@
 // Launches that overlap their start with the end of the kernel before (programmatic dependent launch).  Each kernel of the wide layers lets
-// the next one start as soon as all of its own CTAs have (start_next), and touches no global memory before the kernels ahead of it
-// have finished (after_previous): what overlaps is the launch and the set-up of barriers, tensor memory and descriptors.  A neighbour that
-// knows nothing of this runs strictly before or after.
+// the next one start (start_next) and touches no global memory before the kernels ahead of it have finished (after_previous): what overlaps is
+// the launch and the set-up of barriers, tensor memory and descriptors.  A neighbour that knows nothing of this runs strictly before or after.
+//
+// One exception: a product that is told so (GemmArgs::early) fetches weights ahead of its wait.  It may only because the kernel ahead of it, which
+// makes 8-bit rows (row_fwd_kernel, row_fwd_stream_kernel), lets it start after its own wait and not before, so that whatever wrote the weights
+// has finished by then.  All other kernels let the next one start at once.
 #pragma once
 
 #include "common.cuh"

@@ -308,14 +308,15 @@ __global__ void __launch_bounds__(THREADS) row_fwd_kernel(const RowFwdArgs a) {
 }
 
 // Rows that are too long for registers, or whose tensors do not start alike: read again for every step, by then from L2.  VB = 16 bytes an
-// access where everything starts on them, else an element.
+// access where everything starts on them, else an element.  A view whose rows start elsewhere than the result's (column 3 of 16384 x 4104 on, 4096
+// wide, bfloat16) takes 121 us, packed rows 44.
 template <typename T, int VB, int MODE, bool RES>
 __global__ void __launch_bounds__(kMaxTeam) row_fwd_stream_kernel(const RowFwdArgs a) {
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
     after_previous();
-    start_next();
+    start_next();  // after the wait, as in row_fwd_kernel and for the same reason
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
@@ -464,6 +465,10 @@ int plan_row_fwd(RowFwdArgs a, cudaStream_t stream) {
     const bool gain = a.gain == nullptr || aligned_to(a.gain, 16);
     const int kind = gain || rows.kind() == kShifted ? rows.kind() : kAnyhow;
     const int packets = span_packets<T>(a.d, kind);
+    // Packets a thread, of 16 bytes each from every input: as many as keep some 64 bytes on their way.  2^26 bfloat16 values, us: without a residual
+    // 4096 columns 43.8 with four, 48.7 with two, 63 with one; with one 4096 columns 80.6 with four, 79.8 with two, 86 with one, and off 16 bytes 1537
+    // columns 122 and 112, 2500 columns 110 and 100.  Past 512 packets two would ask for CTAs of up to 1024 threads: 5120 to 8192 columns 80.5 with
+    // four, 79.7 with two, 12288 columns 82 and 117 (float32 the other way round there, 110 and 91; 4097 bfloat16 columns 122 and 106).
     const TeamPlan plan = team_plan(packets, RES && packets <= 512 ? 2 : 4, kind == kShifted && MODE != kNorm);
     const long long blocks = (a.rows + plan.rows_per_block - 1) / plan.rows_per_block;
     if (a.rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "too many rows: %lld", a.rows);
@@ -753,7 +758,8 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
     }
 }
 
-// Rows that are too long for registers, or whose tensors do not start alike; the gain's gradient is a column sum of its own then.
+// Rows that are too long for registers, or whose tensors do not start alike; the gain's gradient is a column sum of its own then.  (16384 rows of
+// 4096 bfloat16 that start at another column than the result's: 318 us, packed 84.)
 template <typename T, int VB, bool GS>
 __global__ void __launch_bounds__(kMaxTeam) norm_bwd_stream_kernel(const RowBwdArgs a) {
     constexpr int N = VB / static_cast<int>(sizeof(T));
@@ -918,8 +924,9 @@ struct NormBwdPlan {
 // Dynamic shared memory of a CTA's ring, at most
 constexpr int ring_budget(int consumers) { return (consumers == 256 ? 110 : 222) * 1024; }
 
-// A thread sums 32 columns at most.  Up to four packets a lane a row is a warp's; longer ones are shared by 256 or 512 threads.  Two CTAs
-// share an SM where two stages of a CTA fit half of it.
+// A thread sums 32 columns at most.  Up to four packets a lane a row is a warp's; longer ones are shared by 256 threads, with two CTAs an SM, as
+// long as a thread has no more than the two packets whose gains and products it can hold, then by 512 with one (2^26 bfloat16 values with the
+// sum's gradient, us: 4096 columns 95 with 256 threads, 136 with 512; 4097 columns 389 and 268, 6144 156 and 128, 8192 132 and 114).
 template <typename T>
 NormBwdPlan norm_bwd_plan(long long rows, int d, int kind, bool gs) {
     constexpr int kMost = sizeof(T) == 4 ? 8 : 4;

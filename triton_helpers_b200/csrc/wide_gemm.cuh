@@ -36,7 +36,7 @@ struct GemmArgs {
     long long out_stride;
     int out_dtype;
     int out_tma;
-    int early;             // A does not come from the kernel before: its first stages are fetched while that one runs
+    int early;             // A was complete before the kernel ahead let this one start (after its own wait): its first stages are fetched while that one runs
     const float *lane_scale, *column_scale;  // along m and along n (8 bits)
     const void *bias;      // along n (along m where transposed)
     int bias_dtype;
@@ -609,7 +609,7 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     g.tiles_m = (g.m + CG * kGemmRows - 1) / (CG * kGemmRows);
     g.tiles_n = (g.n + BN - 1) / BN;
     // 32 MB of rows: half of what one die's L2 holds.  Sustained at the power limit, TFLOP/s by rows of a group (MB), 16384 x 4096 -> 16384 float16:
-    // 8 (16) 1294, 16 (32) 1342, 32 (64) 1196, a library's 1324; 8192 x 4096 -> 16384 8-bit: 8 (8) 2757, 16 (16) 2846, 32 (32) 2923.
+    // 8 (16) 1327, 16 (32) 1345, 32 (64) 1196, a library's 1336; 8192 x 4096 -> 16384 8-bit: 8 (8) 2778, 16 (16) 2882, 32 (32) 2933.
     g.group = static_cast<int>(std::max(4ll, std::min(32ll, (32ll << 20) / (static_cast<long long>(CG) * kGemmRows * k * EB))));
     g.k_tiles = (k + S::kK - 1) / S::kK;
     g.tiles_per_split = (g.k_tiles + g.splits - 1) / g.splits;
