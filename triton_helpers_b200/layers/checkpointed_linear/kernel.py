@@ -13,7 +13,8 @@ rounding does not add up from layer to layer.  A row's rounding is at most half 
 operand of the product ``q * scale`` is rounded once more, to the layer's 16-bit type.
 """
 from ctypes import c_int, c_void_p
-from typing import Optional, Tuple
+from functools import lru_cache
+from typing import Callable, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -65,9 +66,7 @@ class _checkpointed_linear(Function):
 
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
-        # the type to cast to is known at the call
-        cast = torch.amp.custom_fwd(_checkpointed_linear._forward, device_type="cuda", cast_inputs=torch.get_autocast_dtype("cuda"))
-        return cast(ctx, x, weight, bias)
+        return _forward_in(torch.get_autocast_dtype("cuda"))(ctx, x, weight, bias)  # the type to cast to is known at the call
 
     @staticmethod
     def _forward(ctx, x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
@@ -161,6 +160,11 @@ class _checkpointed_linear(Function):
                     "th_column_sum",
                 )
         return dx, dw, db
+
+
+@lru_cache(maxsize=None)
+def _forward_in(dtype: torch.dtype) -> Callable:
+    return torch.amp.custom_fwd(_checkpointed_linear._forward, device_type="cuda", cast_inputs=dtype)
 
 
 def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:
