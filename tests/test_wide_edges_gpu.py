@@ -234,3 +234,41 @@ def test_widths_where_the_kernel_changes(packets, dtype):
             assert bool(((rows.q.double() - h * g * 127 / top).abs() <= 0.5 + 127 * 3 * step).all())
         rows, top = quantize_rows(x), x.float().abs().amax(-1, keepdim=True).clamp_min(2.0**-100)
         assert torch.equal(rows.q, torch.round(x.float() * (torch.full_like(top, 127.0) / top)).to(torch.int8))
+
+
+def test_threads_with_a_stream_each():
+    # pairs of CTAs, single ones and rows of several streams start beside one another, with deep queues: the bits of a pass alone
+    def passes(r, d, n, dtype):
+        x, res, g, w, b = normal(r, d, dtype=dtype), normal(r, d, seed=1, dtype=dtype), normal(d, seed=2, dtype=dtype), normal(n, d, seed=3, dtype=dtype) * 0.05, normal(n, seed=4, dtype=dtype)
+        gz, gs, w8 = normal(r, n, seed=5, dtype=dtype), normal(r, d, seed=6, dtype=dtype), quantize_rows(w)
+        leaves = [t.requires_grad_(True) for t in (x, res, g, w, b)]
+
+        def one():
+            y, s = rms_norm(x, g, res)
+            z = checkpointed_linear(y, w, b)
+            grads = torch.autograd.grad([z, s], leaves, [gz, gs])
+            with torch.no_grad():
+                rows, added = rms_norm_int8(x, g, res)
+                return [z.detach(), *grads, added, int8_linear(rows, w8, dtype=dtype), int8_linear(y.detach(), w8, b)]
+
+        return one
+
+    shapes = [(2100, 4100, 4096, torch.bfloat16), (2100, 4100, 77, torch.float16), (3, 100, 4096, torch.float16), (700, 100, 4096, torch.bfloat16)]
+    calls = [passes(*s) for s in shapes]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(60):
+                got[k] = calls[k]()
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for out, alone in zip(got, want) for a, b in zip(out, alone))
+    assert _lib.lib().th_linear_tc_status() == 0

@@ -338,6 +338,12 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if constexpr (CG == 2) {
+        // An allocation for a pair takes columns on both SMs: the other CTA must have started.  Without this, with other streams' CTAs starting at the same
+        // time, a pair in some 10^5 to 10^6 launches never got past it, and the GPU stood still.
+        __syncwarp();
+        cluster_sync_all();
+    }
     if (warp == 2) {
         if constexpr (CG == 1) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_holder)), "r"(S::kTmemCols) : "memory");
@@ -558,6 +564,10 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     if (warp == 2) {
         if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
+    }
+    if constexpr (CG == 2) {  // and neither CTA ends before both have given theirs back
+        __syncwarp();
+        cluster_sync_all();
     }
 }
 
