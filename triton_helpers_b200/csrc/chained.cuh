@@ -1,10 +1,12 @@
-// Launches that overlap their start with the end of the kernel before (programmatic dependent launch).  Each kernel of the wide layers lets
-// the next one start (start_next) and touches no global memory before the kernels ahead of it have finished (after_previous): what overlaps is
+// Launches that overlap their start with the end of the kernel before (programmatic dependent launch).  Each kernel of the wide layers waits for
+// the kernels ahead of it before it touches global memory, and lets the next one start after that wait (after_previous does both): what overlaps is
 // the launch and the set-up of barriers, tensor memory and descriptors.  A neighbour that knows nothing of this runs strictly before or after.
 //
-// One exception: a product that is told so (GemmArgs::early) fetches weights ahead of its wait.  It may only because the kernel ahead of it, which
-// makes 8-bit rows (row_fwd_kernel, row_fwd_stream_kernel), lets it start after its own wait and not before, so that whatever wrote the weights
-// has finished by then.  All other kernels let the next one start at once.
+// The order matters.  CTAs that have started early hold registers, shared memory and tensor memory while they wait, so they must only wait for a kernel
+// that needs no more of these: when its successor starts, all CTAs of a kernel have started, have their tensor memory and are past their own wait.
+//
+// One access comes ahead of the wait: a product that is told so (GemmArgs::early) fetches its first weights.  It may because whatever was launched
+// before the kernel ahead had finished when that one passed its wait.
 #pragma once
 
 #include "common.cuh"
@@ -12,8 +14,12 @@
 namespace th {
 namespace {
 
-__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// By all threads of the CTA
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __syncthreads();  // all of them are past it
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 template <typename... Params, typename... Args>
 int launch_chained(const char *what, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, unsigned cluster, Args &&...args) {

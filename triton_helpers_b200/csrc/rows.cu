@@ -220,7 +220,6 @@ __global__ void __launch_bounds__(THREADS) row_fwd_kernel(const RowFwdArgs a) {
     __shared__ float red[2][32];
     int turn = 0;
     after_previous();
-    start_next();  // by now everything before is done: what follows depends on these rows alone (th_quantized_linear relies on it)
     const int team = a.team;
     const bool part = team <= 32;  // of a warp
     const int t = part ? threadIdx.x & (team - 1) : threadIdx.x;
@@ -316,7 +315,6 @@ __global__ void __launch_bounds__(kMaxTeam) row_fwd_stream_kernel(const RowFwdAr
     __shared__ float red[2][32];
     int turn = 0;
     after_previous();
-    start_next();  // after the wait, as in row_fwd_kernel and for the same reason
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
@@ -577,7 +575,6 @@ __global__ void __launch_bounds__(CONSUMERS + 32, CONSUMERS == 256 ? 2 : 1) norm
     __shared__ float red[2][32];
     __shared__ int abort_flag;
     const auto shared = [](const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); };
-    start_next();
     const int stage_bytes = kTensors * ring.tensor_bytes;
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -765,7 +762,6 @@ __global__ void __launch_bounds__(kMaxTeam) norm_bwd_stream_kernel(const RowBwdA
     constexpr int N = VB / static_cast<int>(sizeof(T));
     __shared__ float red[2][32];
     int turn = 0;
-    start_next();
     after_previous();
     const int team = blockDim.x, packets = a.d / N;
     const long long row = blockIdx.x;
@@ -858,7 +854,6 @@ __device__ __forceinline__ void column_sums_of(const ColumnArgs &a, int block, i
 template <typename T, int PER>
 __global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnArgs a) {
     __shared__ float part[1024 * PER];
-    start_next();
     after_previous();
     column_sums_of<T, PER>(a, blockIdx.x, blockIdx.y, part);
 }
@@ -866,7 +861,6 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnArgs a) {
 template <typename O>
 __global__ void __launch_bounds__(1024) partial_sum_kernel(const float *partial, int count, int d, O *out) {
     __shared__ float part[32][33];
-    start_next();
     after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
     float v = 0.f;
@@ -1091,7 +1085,6 @@ __device__ __forceinline__ void dequantize_shifted(const DequantizeArgs &a, long
 
 template <typename T, bool SHIFT>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a) {
-    start_next();
     after_previous();
     const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     if constexpr (SHIFT) dequantize_shifted<T>(a, id);
@@ -1113,7 +1106,6 @@ int dequantize_rows(DequantizeArgs a, cudaStream_t stream) {
 template <typename T, int PER>
 __global__ void __launch_bounds__(1024) checkpoint_rows_kernel(const DequantizeArgs rows, const ColumnArgs sums, int column_blocks, int sum_blocks) {
     __shared__ float part[1024 * PER];
-    start_next();
     after_previous();
     if (blockIdx.x < sum_blocks) column_sums_of<T, PER>(sums, blockIdx.x % column_blocks, blockIdx.x / column_blocks, part);
     else dequantize<T>(rows, static_cast<long long>(blockIdx.x - sum_blocks) * 1024 + threadIdx.x);
@@ -1145,7 +1137,6 @@ struct CopyArgs {
 // Sixteen bytes of a destination a thread, from the four or five words that hold them; a word is read only where it holds a byte of the
 // row.  Zeros follow a row up to a whole chunk.
 __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyArgs a) {
-    start_next();
     after_previous();
     const int k = blockIdx.x >= a.first_block[1] ? 1 : 0;
     const int chunks = (a.d[k] + 7) / 8;

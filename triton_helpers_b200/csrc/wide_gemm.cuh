@@ -36,7 +36,7 @@ struct GemmArgs {
     long long out_stride;
     int out_dtype;
     int out_tma;
-    int early;             // A was complete before the kernel ahead let this one start (after its own wait): its first stages are fetched while that one runs
+    int early;             // A was complete before the kernel ahead passed its wait: its first stages are fetched while that one runs
     const float *lane_scale, *column_scale;  // along m and along n (8 bits)
     const void *bias;      // along n (along m where transposed)
     int bias_dtype;
@@ -318,7 +318,6 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     const uint32_t place = CG == 2 ? cluster_rank() : 0, rank = place % CG, leader = place - rank;
     const int units = g.tiles_m * g.tiles_n * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
-    start_next();
     if (threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a_map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&b_map)) : "memory");
@@ -358,27 +357,27 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
     if constexpr (CG == 2) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
-    if (!(SWAP && warp == 0)) after_previous();
+    int ahead = 0;  // stages whose A is on its way already
+    if constexpr (SWAP) {
+        if (warp == 0 && g.early && first < units) {
+            const GemmUnit u = gemm_unit(g, first);
+            ahead = min(S::kStages, u.k1 - u.k0);
+            if (elect_one()) {
+                for (int s = 0; s < ahead; ++s) {
+                    const uint32_t bar = smem_addr(&full[s]);
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(static_cast<uint32_t>(S::kStage)) : "memory");
+                    gemm_load<CG>(smem + s * S::kStage, &a_map, (u.k0 + s) * S::kK, u.tm * kGemmRows, bar);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    after_previous();
 
     if (warp == 0) {
         // ---- operands ----
-        int it = 0, ahead = 0;  // stages whose A is on its way already
+        int it = 0;
         bool ok = true;
-        if constexpr (SWAP) {
-            if (g.early && first < units) {
-                const GemmUnit u = gemm_unit(g, first);
-                ahead = min(S::kStages, u.k1 - u.k0);
-                if (elect_one()) {
-                    for (int s = 0; s < ahead; ++s) {
-                        const uint32_t bar = smem_addr(&full[s]);
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(static_cast<uint32_t>(S::kStage)) : "memory");
-                        gemm_load<CG>(smem + s * S::kStage, &a_map, (u.k0 + s) * S::kK, u.tm * kGemmRows, bar);
-                    }
-                }
-                __syncwarp();
-            }
-            after_previous();
-        }
         for (int unit = first; unit < units && ok; unit += step) {
             const GemmUnit u = gemm_unit(g, unit);
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
