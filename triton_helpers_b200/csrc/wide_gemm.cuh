@@ -121,9 +121,9 @@ __device__ __forceinline__ void gemm_commit(uint32_t mbar, uint32_t leader) {
                      "h"(static_cast<unsigned short>(3u << leader)) : "memory");
 }
 
-// Called by whole warps.  Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.  Lanes may
-// see the barrier and the flag in different orders, so they agree: what follows a wait is elected from, and left by, all of them.
-__device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
+// Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.  The answer is a lane's own: lanes may
+// see the barrier and the flag in different orders.
+__device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
     unsigned long long deadline = 0;
     uint32_t done;
     for (unsigned poll = 0;; ++poll) {
@@ -142,8 +142,11 @@ __device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *ab
             }
         }
     }
-    return __all_sync(~0u, done != 0);
+    return done != 0;
 }
+
+// A whole warp's: what follows a wait is left by all of its lanes or by none
+__device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *abort_flag) { return __all_sync(~0u, lane_wait(bar, parity, abort_flag)); }
 
 struct GemmUnit {
     int tm, tn, split, k0, k1;
@@ -383,9 +386,8 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
             for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
                 const int s = it % S::kStages;
-                ok = gemm_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
-                if (!ok) break;
-                if (elect_one()) {
+                const bool got = lane_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
+                if (elect_one() && got) {
                     const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
                     if (rank == 0 && it >= ahead)
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
@@ -404,7 +406,8 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                         gemm_load<CG>(b, &b_map, k, n0, bar);
                     }
                 }
-                __syncwarp();
+                ok = __all_sync(~0u, got);  // the lanes agree behind the issue (one token, 8192 -> 8192 in 8 bits: 14.2 us with the vote ahead of it, 14.0 so)
+                if (!ok) break;
             }
         }
     } else if (warp == 1 && rank == 0) {
@@ -421,10 +424,9 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
             const uint32_t d = tmem + buf * BN;
             for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
                 const int s = it % S::kStages;
-                ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
-                if (!ok) break;
+                const bool got = lane_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
                 tc_fence_after();
-                if (elect_one()) {
+                if (elect_one() && got) {
                     const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -432,7 +434,8 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
                     gemm_commit<CG>(smem_addr(&empty[s]), leader);
                     if (kt == u.k1 - 1) gemm_commit<CG>(smem_addr(&acc_full[buf]), leader);
                 }
-                __syncwarp();
+                ok = __all_sync(~0u, got);
+                if (!ok) break;
             }
         }
     } else if (warp >= 4) {
