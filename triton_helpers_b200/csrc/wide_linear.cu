@@ -171,7 +171,7 @@ extern "C" int64_t th_quantized_linear_workspace_bytes(int64_t rows, int d_in) {
 }
 
 // The quantising kernel lets the product start only once everything ahead of itself has finished, the weights included, so the product may
-// fetch its first weights while the rows are being quantised (one token, 8192 -> 8192: 18.5 -> 14.4 us).
+// fetch its first weights while the rows are being quantised (one token, 8192 -> 8192, weights from memory: 17.0 -> 16.7 us captured).
 extern "C" int th_quantized_linear(const void *x_dev, int64_t x_stride, int x_dtype, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
                                    const void *bias_dev, void *y_dev, int64_t y_stride, void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in,
                                    int d_out, int dtype, void *stream) {
