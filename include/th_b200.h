@@ -472,8 +472,90 @@ int th_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *w
 int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
                          void *grad_weight_dev, int64_t rows, int d_in, int d_out, int dtype, void *stream);
 
-/* Device-side status word of these kernels (0 = fine, 1 = a bounded wait ran out and results are invalid).
- * Synchronises the device. */
+/* ------------------------------------------------------------------------------------------
+ * Linear layers on 8-bit floating point.  NO COUNTERPART IN THE REFERENCE.
+ *
+ * 8-bit blocks: 128 neighbouring columns of one row, or of 128 rows of a weight (the last ones may be smaller):
+ *     a = max(max |x|, 2^-60);  q = e4m3(x * (448 / a)), to nearest even;  scale = a / 448, in float32.
+ * A block that holds an infinity or a NaN gets zeros and the scale NaN.  q starts on 16 bytes (pointer and stride);
+ * bytes between d and the stride are neither read nor written.  Scales lie anywhere: that of row (or of row / 128)
+ * r and column block b at scale_dev[r * scale_row + b * scale_block].
+ * ------------------------------------------------------------------------------------------ */
+
+/* Rows in blocks of 1 x 128: scale_dev[b * scale_block + r], scale_block >= rows. */
+int th_float8_rows(const void *x_dev, int64_t x_stride, void *q_dev, int64_t q_stride, float *scale_dev,
+                   int64_t scale_block, int64_t rows, int d, int dtype, void *stream);
+/* A weight in blocks of 128 x 128: scale_dev[(r / 128) * ceil(d / 128) + b]. */
+int th_float8_weight(const void *w_dev, int64_t w_stride, void *q_dev, int64_t q_stride, float *scale_dev, int64_t rows,
+                     int d, int dtype, void *stream);
+/* q * scale rounded to `dtype`; block_rows is 1 or 128. */
+int th_float8_values(const void *q_dev, int64_t q_stride, const float *scale_dev, int64_t scale_row,
+                     int64_t scale_block, int block_rows, void *out_dev, int64_t out_stride, int64_t rows, int d,
+                     int dtype, void *stream);
+
+/* y[r, n] = sum_b scale[r, b] weight_scale[n / 128, b] sum_{k in b} q[r, k] weight[n, k] + bias[n]: float32 sums, y and
+ * bias in `dtype`; the bias may be null.  Results repeat bit for bit. */
+int th_float8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, int64_t scale_row,
+                     int64_t scale_block, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
+                     int64_t weight_scale_row, int64_t weight_scale_block, const void *bias_dev, void *y_dev,
+                     int64_t y_stride, int64_t rows, int d_in, int d_out, int dtype, void *stream);
+
+/* th_float8_rows of x (rows x d_in, `x_dtype`) into scratch and th_float8_linear of the result. */
+int64_t th_float8_quantized_linear_workspace_bytes(int64_t rows, int d_in);
+int th_float8_quantized_linear(const void *x_dev, int64_t x_stride, int x_dtype, const void *weight_dev,
+                               int64_t weight_stride, const float *weight_scale_dev, int64_t weight_scale_row,
+                               int64_t weight_scale_block, const void *bias_dev, void *y_dev, int64_t y_stride,
+                               void *workspace_dev, int64_t workspace_bytes, int64_t rows, int d_in, int d_out,
+                               int dtype, void *stream);
+
+/* grad_x = grad_y weight for grad_y in blocks of 1 x 128 along d_out, weight (d_out x d_in) as above. */
+int th_float8_bwd_input(const void *grad_q_dev, int64_t grad_q_stride, const float *grad_scale_dev,
+                        int64_t grad_scale_row, int64_t grad_scale_block, const void *weight_dev,
+                        int64_t weight_stride, const float *weight_scale_dev, int64_t weight_scale_row,
+                        int64_t weight_scale_block, void *grad_x_dev, int64_t gx_stride, int64_t rows, int d_in,
+                        int d_out, int dtype, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Linear layers of several experts on rows sorted by expert.  NO COUNTERPART IN THE REFERENCE.
+ *
+ * Rows ends[e - 1] .. ends[e] - 1 belong to expert e (ends[-1] = 0); an end below the one before it counts as that one,
+ * an end above `rows` as `rows`.  Rows behind the last end get zeros.  The ends are read on the device.  16-bit operands
+ * (rows, weights and experts start on 16 bytes), float32 sums, results rounded once; they repeat bit for bit.
+ * ------------------------------------------------------------------------------------------ */
+int th_expert_linear_fwd(const void *x_dev, int64_t x_stride, const void *weight_dev, int64_t weight_stride,
+                         int64_t expert_stride, const int32_t *ends_dev, void *y_dev, int64_t y_stride, int64_t rows,
+                         int experts, int d_in, int d_out, int dtype, void *stream);
+int th_expert_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const void *weight_dev,
+                               int64_t weight_stride, int64_t expert_stride, const int32_t *ends_dev,
+                               void *grad_x_dev, int64_t gx_stride, int64_t rows, int experts, int d_in, int d_out,
+                               int dtype, void *stream);
+/* grad_weight is contiguous (experts, d_out, d_in); zeros for an expert without rows. */
+int th_expert_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
+                                const int32_t *ends_dev, void *grad_weight_dev, int64_t rows, int experts, int d_in,
+                                int d_out, int dtype, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The global norm of a list of gradients, and clipping by it.  NO COUNTERPART IN THE REFERENCE.  Lists are host arrays of
+ * n_tensors entries, each tensor contiguous; a float32 pair on the device holds
+ *     norm = sqrt(sum_k scale_k^2 sum_i g_k[i]^2)      factor = min(1, max_norm / (norm + 1e-6))
+ * ------------------------------------------------------------------------------------------ */
+int64_t th_grad_norm_workspace_bytes(int n_tensors, const int64_t *n_elems);
+/* grad_scale may be null (all one).  The sum takes any float32 elements, with partial sums in float64 in a fixed order. */
+int th_grad_norm(int n_tensors, const void *const *grad_dev, const int64_t *n_elems, const int *dtypes,
+                 const float *grad_scale, float max_norm, float *norm_factor_dev, void *workspace_dev,
+                 int64_t workspace_bytes, void *stream);
+/* Every tensor times the pair's factor; a factor of one leaves them untouched. */
+int th_scale_tensors(int n_tensors, void *const *tensor_dev, const int64_t *n_elems, const int *dtypes,
+                     const float *norm_factor_dev, void *stream);
+/* th_adam_steps for any number of tensors, with gradients times grad_scale_k times the pair's factor.  A norm that is not
+ * finite passes over every element: parameters and moments stay, and all are counted in skipped_dev. */
+int th_adam_clipped(int n_tensors, void *const *param_dev, void *const *grad_dev, float *const *exp_avg_dev,
+                    float *const *exp_avg_sq_dev, const int64_t *n_elems, const float *grad_scale, const int *zero_grad,
+                    const float *norm_factor_dev, float lr, float beta1, float beta2, float eps, int step, int dtype,
+                    int *skipped_dev, void *stream);
+
+/* Device-side status word of the kernels of wide layers, 8-bit layers and experts (0 = fine, 1 = a bounded wait ran
+ * out and results are invalid).  Synchronises the device. */
 int th_linear_tc_status(void);
 
 #ifdef __cplusplus

@@ -1,0 +1,295 @@
+// 8-bit floating-point blocks: rows in blocks of 1 x 128, weights in blocks of 128 x 128, and back.
+//
+//     a = max(max |x|, 2^-60) over the block      q = e4m3(x * (448 / a))      scale = a / 448
+//
+// Streaming kernels.  Sixteen lanes hold 128 columns of a row, eight each, so that a block's largest magnitude is one reduction within
+// half a warp.  Magnitudes are compared as integers: a NaN is above infinity, and infinity above every number.
+#include "chained.cuh"
+
+#include <algorithm>
+
+namespace th {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr int kQuantThreads = 256;
+constexpr float kLeast = 0x1p-60f, kTop = 448.f;
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Four values of e4m3, saturating (x * (448 / a) rounds to at most 448, so nothing does)
+__device__ __forceinline__ uint32_t four_e4m3(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+}
+
+__device__ __forceinline__ void four_floats(uint32_t q, float *v) {
+    uint32_t lo, hi;  // e4m3 -> f16 is exact
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(q)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(q >> 16)));
+    const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&lo)), b = __half22float2(*reinterpret_cast<__half2 *>(&hi));
+    v[0] = a.x;
+    v[1] = a.y;
+    v[2] = b.x;
+    v[3] = b.y;
+}
+
+// Eight elements of a row, zeros behind its end.  WIDE: they start on 16 bytes.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *from, int valid, float (&v)[8]) {
+    if (WIDE && valid >= 8) {
+        constexpr int N = 16 / static_cast<int>(sizeof(T));
+        struct __align__(16) Packet {
+            T v[N];
+        };
+#pragma unroll
+        for (int p = 0; p < 8 / N; ++p) {
+            const Packet in = reinterpret_cast<const Packet *>(from)[p];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[p * N + e] = to_float<T>(in.v[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < valid ? to_float<T>(from[e]) : 0.f;
+    }
+}
+
+// What a block's largest magnitude makes of it: the factor that its values take, and the scale; zeros and a NaN where it is not finite
+__device__ __forceinline__ float2 block_scale(uint32_t most) {
+    if (most >= 0x7f800000u) return make_float2(0.f, __uint_as_float(0x7fc00000u));
+    const float a = fmaxf(__uint_as_float(most), kLeast);
+    return make_float2(__fdiv_rn(kTop, a), __fdiv_rn(a, kTop));
+}
+
+__device__ __forceinline__ void store8(unsigned char *to, int valid, const float (&v)[8], float2 s) {
+    const bool finite = s.x != 0.f;
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float *x = v + 4 * h;
+        w[h] = finite ? four_e4m3(__fmul_rn(x[0], s.x), __fmul_rn(x[1], s.x), __fmul_rn(x[2], s.x), __fmul_rn(x[3], s.x)) : 0u;
+    }
+    if (valid >= 8) {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < valid) to[e] = static_cast<unsigned char>(w[e >> 2] >> (8 * (e & 3)));
+    }
+}
+
+struct QuantArgs {
+    const void *x;
+    long long x_stride;
+    unsigned char *q;
+    long long q_stride;
+    float *scale;
+    long long scale_block;
+    long long rows;
+    int d, blocks;
+};
+
+// A CTA takes 16 rows x kAhead column blocks: kAhead loads of each thread are on their way together, and the scales of neighbouring rows,
+// which lie side by side, leave together.
+constexpr int kAhead = 4;
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kQuantThreads) float8_rows_kernel(const QuantArgs a) {
+    after_previous();
+    const int part = threadIdx.x & 15;
+    const long long row = static_cast<long long>(blockIdx.y) * 16 + (threadIdx.x >> 4);
+    if (row >= a.rows) return;  // both halves of a warp work on their own
+    const unsigned mask = 0xffffu << (threadIdx.x & 16);
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    float v[kAhead][8];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int c = (blockIdx.x * kAhead + i) * kBlock + 8 * part;
+        load8<T, WIDE>(x + c, a.d - c, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int b = blockIdx.x * kAhead + i, c = b * kBlock + 8 * part;
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[i][e]));
+        most = __reduce_max_sync(mask, most);
+        if (b >= a.blocks) break;
+        const float2 s = block_scale(most);
+        if (part == 0) a.scale[b * a.scale_block + row] = s.y;
+        if (c < a.d) store8(a.q + row * a.q_stride + c, a.d - c, v[i], s);
+    }
+}
+
+// A CTA takes a block of 128 x 128: eight rows of each thread in registers
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kQuantThreads) float8_weight_kernel(const QuantArgs a) {
+    __shared__ uint32_t warps[kQuantThreads / 32];
+    after_previous();
+    const int c = blockIdx.x * kBlock + 8 * (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    const long long first = static_cast<long long>(blockIdx.y) * kBlock;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long row = first + r0 + 16 * i;
+        load8<T, WIDE>(static_cast<const T *>(a.x) + row * a.x_stride + c, row < a.rows ? a.d - c : 0, v[i]);
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[i][e]));
+    most = __reduce_max_sync(~0u, most);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kQuantThreads / 32; ++w) most = max(most, warps[w]);
+    const float2 s = block_scale(most);
+    if (threadIdx.x == 0) a.scale[static_cast<long long>(blockIdx.y) * a.blocks + blockIdx.x] = s.y;
+    if (c >= a.d) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long row = first + r0 + 16 * i;
+        if (row < a.rows) store8(a.q + row * a.q_stride + c, a.d - c, v[i], s);
+    }
+}
+
+struct ValueArgs {
+    const unsigned char *q;
+    long long q_stride;
+    const float *scale;
+    long long scale_row, scale_block;
+    int block_shift;  // 0 or 7: rows of a block
+    void *out;
+    long long out_stride;
+    long long rows;
+    int d;
+};
+
+// Sixteen columns a thread: one load of 16 bytes
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kQuantThreads) float8_values_kernel(const ValueArgs a) {
+    after_previous();
+    const int chunks = (a.d + 15) / 16;
+    const long long id = static_cast<long long>(blockIdx.x) * kQuantThreads + threadIdx.x, row = id / chunks;
+    if (row >= a.rows) return;
+    const int c = static_cast<int>(id - row * chunks) * 16, valid = a.d - c;
+    const float s = a.scale[(row >> a.block_shift) * a.scale_row + (c / kBlock) * a.scale_block];
+    const unsigned char *q = a.q + row * a.q_stride + c;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (valid >= 16) {
+        const uint4 in = *reinterpret_cast<const uint4 *>(q);
+        w[0] = in.x;
+        w[1] = in.y;
+        w[2] = in.z;
+        w[3] = in.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < valid) w[e >> 2] |= static_cast<uint32_t>(q[e]) << (8 * (e & 3));
+    }
+    T *out = static_cast<T *>(a.out) + row * a.out_stride + c;
+    constexpr int N = 16 / static_cast<int>(sizeof(T));
+    struct __align__(16) Packet {
+        T v[N];
+    };
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four_floats(w[k], v + 4 * k);
+    if (WIDE && valid >= 16) {
+#pragma unroll
+        for (int p = 0; p < 16 / N; ++p) {
+            Packet o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(v[p * N + e] * s);
+            reinterpret_cast<Packet *>(out)[p] = o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < valid) out[e] = from_float<T>(v[e] * s);
+    }
+}
+
+// least: the smallest stride of the floats' rows (rows that are read may overlap)
+int check_blocks(const char *what, const void *x, int64_t x_stride, int64_t least, const void *q, int64_t q_stride, const float *scale, int64_t rows, int d,
+                 int dtype) {
+    if (rows < 0 || d < 1) return fail(TH_ERR_BAD_ARG, "%s: %lld rows of %d", what, static_cast<long long>(rows), d);
+    if (rows > (1ll << 30) || d > (1 << 24)) return fail(TH_ERR_UNSUPPORTED, "%s: %lld rows of %d", what, static_cast<long long>(rows), d);
+    if (dtype != TH_F32 && dtype != TH_F16 && dtype != TH_BF16) return fail(TH_ERR_UNSUPPORTED, "%s: unknown dtype code %d", what, dtype);
+    if (rows == 0) return TH_OK;
+    if (!x || !q || !scale || x_stride < least) return fail(TH_ERR_BAD_ARG, "%s: null pointer or short stride", what);
+    if (!aligned_to(q, 16) || q_stride % 16 || q_stride < d) return fail(TH_ERR_ALIGNMENT, "%s: 8-bit rows start on 16 bytes", what);
+    if (int rc = check_elements(what, TH_F32, {scale})) return rc;
+    return check_elements(what, dtype, {x});
+}
+
+bool wide_rows(const void *x, int64_t stride, int dtype) { return aligned_to(x, 16) && stride * static_cast<int64_t>(dtype_bytes(dtype)) % 16 == 0; }
+
+// fn(T{}, std::integral_constant<bool, WIDE>{})
+template <typename Fn>
+int with_type(int dtype, bool wide, const Fn &fn) {
+    const auto at = [&](auto t) { return wide ? fn(t, std::true_type{}) : fn(t, std::false_type{}); };
+    return dtype == TH_F32 ? at(float{}) : dtype == TH_F16 ? at(__half{}) : at(__nv_bfloat16{});
+}
+
+}  // namespace
+}  // namespace th
+
+using namespace th;
+
+extern "C" int th_float8_rows(const void *x_dev, int64_t x_stride, void *q_dev, int64_t q_stride, float *scale_dev, int64_t scale_block, int64_t rows, int d,
+                              int dtype, void *stream) {
+    if (int rc = check_blocks("th_float8_rows", x_dev, x_stride, 0, q_dev, q_stride, scale_dev, rows, d, dtype)) return rc;
+    if (rows == 0) return TH_OK;
+    if (scale_block < rows) return fail(TH_ERR_BAD_ARG, "th_float8_rows: short stride of the scales");
+    QuantArgs a{x_dev, x_stride, static_cast<unsigned char *>(q_dev), q_stride, scale_dev, scale_block, rows, d, (d + kBlock - 1) / kBlock};
+    const unsigned columns = static_cast<unsigned>((a.blocks + kAhead - 1) / kAhead);
+    // a grid's second axis ends at 65535: rows beyond come in further launches
+    constexpr int64_t kMost = 65535ll * 16;
+    for (int64_t first = 0; first < rows; first += kMost) {
+        QuantArgs part = a;
+        part.x = static_cast<const char *>(x_dev) + first * x_stride * static_cast<int64_t>(dtype_bytes(dtype));
+        part.q += first * q_stride;
+        part.scale += first;
+        part.rows = std::min(kMost, rows - first);
+        const dim3 grid(columns, static_cast<unsigned>((part.rows + 15) / 16));
+        const int rc = with_type(dtype, wide_rows(x_dev, x_stride, dtype), [&](auto t, auto wide) {
+            return launch_chained("float8_rows_kernel launch", float8_rows_kernel<decltype(t), decltype(wide)::value>, grid, kQuantThreads, 0,
+                                  static_cast<cudaStream_t>(stream), 1, part);
+        });
+        if (rc) return rc;
+    }
+    return TH_OK;
+}
+
+extern "C" int th_float8_weight(const void *w_dev, int64_t w_stride, void *q_dev, int64_t q_stride, float *scale_dev, int64_t rows, int d, int dtype,
+                                void *stream) {
+    if (int rc = check_blocks("th_float8_weight", w_dev, w_stride, 0, q_dev, q_stride, scale_dev, rows, d, dtype)) return rc;
+    if (rows == 0) return TH_OK;
+    if (rows > 65535ll * kBlock) return fail(TH_ERR_UNSUPPORTED, "th_float8_weight: %lld rows", static_cast<long long>(rows));
+    const QuantArgs a{w_dev, w_stride, static_cast<unsigned char *>(q_dev), q_stride, scale_dev, 0, rows, d, (d + kBlock - 1) / kBlock};
+    const dim3 grid(static_cast<unsigned>(a.blocks), static_cast<unsigned>((rows + kBlock - 1) / kBlock));
+    return with_type(dtype, wide_rows(w_dev, w_stride, dtype), [&](auto t, auto wide) {
+        return launch_chained("float8_weight_kernel launch", float8_weight_kernel<decltype(t), decltype(wide)::value>, grid, kQuantThreads, 0,
+                              static_cast<cudaStream_t>(stream), 1, a);
+    });
+}
+
+extern "C" int th_float8_values(const void *q_dev, int64_t q_stride, const float *scale_dev, int64_t scale_row, int64_t scale_block, int block_rows,
+                                void *out_dev, int64_t out_stride, int64_t rows, int d, int dtype, void *stream) {
+    if (block_rows != 1 && block_rows != kBlock) return fail(TH_ERR_BAD_ARG, "th_float8_values: blocks of %d rows", block_rows);
+    if (int rc = check_blocks("th_float8_values", out_dev, out_stride, d, q_dev, q_stride, scale_dev, rows, d, dtype)) return rc;
+    if (rows == 0) return TH_OK;
+    if (scale_row < 0 || scale_block < 0) return fail(TH_ERR_BAD_ARG, "th_float8_values: negative stride of the scales");
+    const ValueArgs a{static_cast<const unsigned char *>(q_dev), q_stride, scale_dev, scale_row, scale_block, block_rows == 1 ? 0 : 7, out_dev, out_stride,
+                      rows, d};
+    const long long blocks = (rows * ((d + 15) / 16) + kQuantThreads - 1) / kQuantThreads;
+    if (blocks > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "th_float8_values: %lld rows of %d", static_cast<long long>(rows), d);
+    return with_type(dtype, wide_rows(out_dev, out_stride, dtype), [&](auto t, auto wide) {
+        return launch_chained("float8_values_kernel launch", float8_values_kernel<decltype(t), decltype(wide)::value>, static_cast<unsigned>(blocks), kQuantThreads,
+                              0, static_cast<cudaStream_t>(stream), 1, a);
+    });
+}

@@ -5,7 +5,7 @@
 // training step never leaves hand-written kernels between the forward and the next step.
 //
 // Both are pure streaming kernels: 128-bit loads and stores, grid-stride over 8-element packets.
-#include "common.cuh"
+#include "adam.cuh"
 
 namespace th {
 namespace {
@@ -68,42 +68,6 @@ mse_grad_kernel(const T *__restrict__ pred, const T *__restrict__ target, T *__r
         if (loss_sum) atomicAdd(loss_sum, total);
     }
 }
-
-struct AdamScalars {
-    float lr, beta1, beta2, eps;
-    float bias1, bias2_sqrt;  // 1 - beta1^t, sqrt(1 - beta2^t)
-    float grad_scale;         // multiplies the stored gradient (1 / loss scale / world size)
-    int zero_grad;            // write zeros back into the gradient buffer
-};
-
-// One element.  A gradient that is not finite (a 16-bit sum that overflowed, a NaN from upstream)
-// leaves the parameter and both moments as they were and is counted in `skipped`: one bad element
-// must not turn into inf / inf = NaN in the parameter and poison every later step.
-template <typename T>
-__device__ __forceinline__ T adam_one(T p, T g_in, float &m, float &v, const AdamScalars &a, int &skipped) {
-    const float g = to_float<T>(g_in) * a.grad_scale;
-    if (!isfinite(g)) {
-        ++skipped;
-        return p;
-    }
-    m = a.beta1 * m + (1.f - a.beta1) * g;
-    v = a.beta2 * v + (1.f - a.beta2) * g * g;
-    const float denom = sqrtf(v) / a.bias2_sqrt + a.eps;
-    return from_float<T>(to_float<T>(p) - (a.lr / a.bias1) * (m / denom));
-}
-
-// Elements of a parameter in one 16-byte packet, and the matching moments (float32: four, for twice the threads and half their
-// registers of eight: 3.3 M parameters 34.2 -> 26.4 us)
-template <typename T>
-constexpr int kPacket = 16 / sizeof(T);
-template <typename T>
-struct __align__(16) Packet16 {
-    T v[kPacket<T>];
-};
-template <int N>
-struct __align__(16) Moments {
-    float v[N];
-};
 
 // The same update for several tensors of one dtype in one launch: a small network's tensors are a few blocks each, and
 // a launch per tensor (seven for a table and a biased MLP: 43 us of kernels and 100 us of host time in a training step)

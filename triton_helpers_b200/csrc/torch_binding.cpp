@@ -1671,6 +1671,409 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *args, Py_ssize_t n
     END_HANDLE_TH_ERRORS
 }
 
+// ---- linear layers on 8-bit floating point -------------------------------------------------------------------
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// float8_linear(x, weight q, weight scale, bias, dtype): x a float tensor
+PyObject *py_float8_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Tensor x, wq, w_scale, bias;
+    if (n_args != 5 || !usual_mode() || !take(args[0], x) || !take(args[1], wq) || !take(args[2], w_scale) || !take(args[3], bias) ||
+        !(args[4] == Py_None || THPDtype_Check(args[4])))
+        TH_NOT_MINE;
+    if (!plain(x) || !plain(wq) || !plain(w_scale) || wq.dim() != 2 || wq.numel() == 0 || x.dim() < 1 || x.numel() == 0) TH_NOT_MINE;
+    const int64_t d_out = wq.size(0), d_in = wq.size(1);
+    int x_code = TH_F32;
+    Rows rows;
+    if (wq.scalar_type() != at::kFloat8_e4m3fn || w_scale.scalar_type() != at::kFloat || w_scale.dim() != 2 || w_scale.size(0) != blocks_of(d_out) ||
+        w_scale.size(1) != blocks_of(d_in) || w_scale.device() != wq.device() || x.device() != wq.device())
+        TH_NOT_MINE;
+    if ((d_in > 1 && wq.stride(1) != 1) || reinterpret_cast<uintptr_t>(ptr(wq)) % 16 || (d_out > 1 && (wq.stride(0) % 16 || wq.stride(0) < d_in))) TH_NOT_MINE;
+    if (x.size(-1) != d_in || !float_code(x, x_code) || !rows_of(x, d_in, rows)) TH_NOT_MINE;
+    const at::ScalarType type = args[4] == Py_None ? x.scalar_type() : reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+    const int code = dtype_code(type);
+    if (code < 0 || (bias.defined() && (!plain(bias) || bias.dim() != 1 || bias.size(0) != d_out || !bias.is_contiguous() || bias.scalar_type() != type ||
+                                        bias.device() != wq.device())))
+        TH_NOT_MINE;
+    if (torch::autograd::compute_requires_grad(x, w_scale, bias)) TH_NOT_MINE;
+    Tensor y;
+    {
+        NoGil release;
+        at::AutoDispatchBelowADInplaceOrView below;
+        c10::cuda::CUDAGuard guard(wq.device());
+        c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = d_out;
+        y = empty_like_shape(shape, type, wq.device());
+        const int di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+        const int64_t bytes = th_float8_quantized_linear_workspace_bytes(rows.n, di);
+        const Tensor buffer = empty_like_shape({bytes}, at::kByte, wq.device());
+        check(th_float8_quantized_linear(ptr(x), rows.stride, x_code, ptr(wq), d_out > 1 ? wq.stride(0) : pitch16(d_in), w_scale.data_ptr<float>(),
+                                         w_scale.stride(0), w_scale.stride(1), ptr(bias), ptr(y), d_out, ptr(buffer), bytes, rows.n, di, dn, code, current_stream()),
+              "th_float8_quantized_linear");
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// 8-bit blocks in one buffer: the values, 16 bytes between rows' starts or a multiple of that, then the scales
+struct HeldBlocks {
+    Tensor buffer;
+    int64_t pitch = 0, values = 0, scales = 0;
+
+    static HeldBlocks sized(int64_t rows, int64_t width, int64_t scales) {
+        HeldBlocks h;
+        h.pitch = pitch16(width);
+        h.values = rows * h.pitch;
+        h.scales = scales;
+        return h;
+    }
+    int64_t bytes() const { return values + 4 * scales; }
+    void make(c10::Device device) { buffer = empty_like_shape({bytes()}, at::kByte, device); }
+    char *q() const { return static_cast<char *>(ptr(buffer)); }
+    float *scale() const { return reinterpret_cast<float *>(q() + values); }
+};
+
+struct Float8LinearNode : public Node {
+    SavedVariable weight, input;
+    HeldBlocks w, x;  // their sizes
+    int64_t rows = 0, d_in = 0, d_out = 0;
+    c10::SmallVector<int64_t, 6> shape;
+    at::ScalarType type = at::kHalf;
+    bool keeps_weight = false, keeps_input = false;
+
+    std::string name() const override { return "Float8LinearBackward"; }
+    void release_variables() override {
+        weight.reset_data();
+        input.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        HeldBlocks held_w = w, held_x = x;
+        if (keeps_weight) held_w.buffer = weight.unpack();
+        if (keeps_input) held_x.buffer = input.unpack();
+        gradients(grads, held_w, held_x, out);
+        refuse_second("float8_training_linear", *this, grads, out);
+        return out;
+    }
+    void gradients(const variable_list &grads, HeldBlocks w, HeldBlocks x, variable_list &out) {
+        at::NoGradGuard no_grad;
+        const c10::Device device = grads[0].device();
+        c10::cuda::CUDAGuard guard(device);
+        void *stream = current_stream();
+        const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+        Operands operands;
+        const Rows &gy = operands.add(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
+        operands.settle(stream);
+        if (keeps_weight && task_should_compute_output(0)) {
+            w.buffer = restored(w.buffer, at::kByte, w.bytes());
+            HeldBlocks g = HeldBlocks::sized(rows, d_out, rows * blocks_of(d_out));
+            g.make(device);
+            check(th_float8_rows(ptr(gy.keep), gy.stride, g.q(), g.pitch, g.scale(), rows, rows, dn, code, stream), "th_float8_rows");
+            out[0] = empty_like_shape(shape, type, device);
+            check(th_float8_bwd_input(g.q(), g.pitch, g.scale(), 1, rows, w.q(), w.pitch, w.scale(), blocks_of(d_in), 1, ptr(out[0]), d_in, rows, di, dn, code, stream),
+                  "th_float8_bwd_input");
+        }
+        if (task_should_compute_output(2)) {
+            const int64_t bytes = th_column_sum_workspace_bytes(rows, dn);
+            const Tensor partial = empty_like_shape({bytes}, at::kByte, device);
+            out[2] = empty_like_shape({d_out}, type, device);
+            check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), ptr(partial), bytes, rows, dn, code, stream), "th_column_sum");
+        }
+        if (keeps_input && task_should_compute_output(1)) {
+            x.buffer = restored(x.buffer, at::kByte, x.bytes());
+            const int64_t stride = (d_in + 7) / 8 * 8;
+            const Tensor x16 = empty_like_shape({rows, stride}, type, device);
+            check(th_float8_values(x.q(), x.pitch, x.scale(), 1, rows, 1, ptr(x16), stride, rows, di, code, stream), "th_float8_values");
+            out[1] = empty_like_shape({d_out, d_in}, type, device);
+            check(th_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(x16), stride, ptr(out[1]), rows, di, dn, code, stream), "th_linear_bwd_weight");
+        }
+    }
+};
+
+// float8_training_linear(x, weight, bias)
+PyObject *py_float8_training_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Tensor x, w, b;
+    if (n_args != 3 || !usual_mode() || !take(args[0], x) || !take(args[1], w) || !take(args[2], b)) TH_NOT_MINE;
+    if (!plain(x) || !plain(w) || w.dim() != 2 || w.numel() == 0 || x.dim() < 1 || x.numel() == 0 || x.size(-1) != w.size(1)) TH_NOT_MINE;
+    const at::ScalarType type = x.scalar_type();
+    const int64_t d_out = w.size(0), d_in = w.size(1);
+    if ((type != at::kHalf && type != at::kBFloat16) || w.scalar_type() != type || w.device() != x.device()) TH_NOT_MINE;
+    if (b.defined() && !parameter_like(b, x, {d_out})) TH_NOT_MINE;
+    Rows xr, wr;
+    if (!rows_of(x, d_in, xr) || !rows_of(w, d_in, wr)) TH_NOT_MINE;
+    Tensor y;
+    {
+        NoGil release;
+        const bool grad = torch::autograd::compute_requires_grad(x, w, b);
+        std::shared_ptr<Float8LinearNode> node;
+        if (grad) node = make_node<Float8LinearNode>(torch::autograd::collect_next_edges(x, w, b));
+        HeldBlocks hx = HeldBlocks::sized(xr.n, d_in, xr.n * blocks_of(d_in)), hw = HeldBlocks::sized(d_out, d_in, blocks_of(d_out) * blocks_of(d_in));
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            c10::cuda::CUDAGuard guard(x.device());
+            void *stream = current_stream();
+            const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
+            hx.make(x.device());
+            hw.make(x.device());
+            check(th_float8_rows(ptr(xr.keep), xr.stride, hx.q(), hx.pitch, hx.scale(), xr.n, xr.n, di, code, stream), "th_float8_rows");
+            check(th_float8_weight(ptr(wr.keep), wr.stride, hw.q(), hw.pitch, hw.scale(), d_out, di, code, stream), "th_float8_weight");
+            c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+            shape.back() = d_out;
+            y = empty_like_shape(shape, type, x.device());
+            check(th_float8_linear(hx.q(), hx.pitch, hx.scale(), 1, xr.n, hw.q(), hw.pitch, hw.scale(), blocks_of(d_in), 1, ptr(b), ptr(y), d_out, xr.n, di, dn, code,
+                                   stream),
+                  "th_float8_linear");
+        }
+        if (grad) {
+            node->rows = xr.n;
+            node->d_in = d_in;
+            node->d_out = d_out;
+            node->type = type;
+            node->shape.assign(x.sizes().begin(), x.sizes().end());
+            node->keeps_weight = x.requires_grad();
+            node->keeps_input = w.requires_grad();
+            if (node->keeps_weight) node->weight = SavedVariable(hw.buffer, false);
+            if (node->keeps_input) node->input = SavedVariable(hx.buffer, false);
+            hw.buffer = hx.buffer = Tensor();
+            node->w = hw;
+            node->x = hx;
+            torch::autograd::set_history(y, node);
+        }
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- linear layers of several experts ------------------------------------------------------------------------
+
+// A weight (experts, out, in) whose rows and experts start on 16 bytes
+struct ExpertWeight {
+    Tensor keep;
+    int64_t row = 0, expert = 0;
+};
+
+bool expert_weight(const Tensor &w, ExpertWeight &out) {
+    const int64_t experts = w.size(0), d_out = w.size(1), d_in = w.size(2);
+    out.keep = w;
+    out.row = d_out > 1 ? w.stride(1) : (d_in + 7) / 8 * 8;
+    out.expert = experts > 1 ? w.stride(0) : (d_out * out.row + 7) / 8 * 8;
+    return (d_in == 1 || w.stride(2) == 1) && reinterpret_cast<uintptr_t>(ptr(w)) % 16 == 0 && out.row % 8 == 0 && out.expert % 8 == 0 && out.row >= d_in &&
+           out.expert >= d_out * out.row;
+}
+
+// A copy with padded rows where it is not such a weight already; `operands` makes the copy
+ExpertWeight aligned_experts(const Tensor &w, Operands &operands) {
+    ExpertWeight e;
+    if (expert_weight(w, e)) return e;
+    const int64_t d_out = w.size(1), d_in = w.size(2);
+    const Rows &r = operands.add(w.reshape({w.size(0) * d_out, d_in}), d_in);
+    e.keep = r.keep;
+    e.row = r.stride;
+    e.expert = d_out * r.stride;
+    return e;
+}
+
+struct ExpertLinearNode : public Node {
+    SavedVariable x, weight, ends;
+    int64_t rows = 0, experts = 0, d_in = 0, d_out = 0;
+    at::ScalarType type = at::kHalf;
+    bool keeps_weight = false, keeps_input = false;
+
+    std::string name() const override { return "ExpertLinearBackward"; }
+    void release_variables() override {
+        x.reset_data();
+        weight.reset_data();
+        ends.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        Tensor kept_x, kept_w, e = ends.unpack();
+        if (keeps_weight) kept_w = weight.unpack();
+        if (keeps_input) kept_x = x.unpack();
+        gradients(grads, kept_x, kept_w, e, out);
+        refuse_second("expert_linear", *this, grads, out);
+        return out;
+    }
+    void gradients(const variable_list &grads, const Tensor &kept_x, const Tensor &kept_w, Tensor e, variable_list &out) {
+        at::NoGradGuard no_grad;
+        const c10::Device device = grads[0].device();
+        c10::cuda::CUDAGuard guard(device);
+        void *stream = current_stream();
+        const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out), ne = static_cast<int>(experts);
+        e = restored(e, at::kInt, experts);
+        const int32_t *ends_dev = e.data_ptr<int32_t>();
+        const bool wants_x = keeps_weight && task_should_compute_output(0), wants_w = keeps_input && task_should_compute_output(1);
+        Operands first, second;  // two copies at most in a launch
+        const Rows &gy = first.add(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
+        ExpertWeight w;
+        if (wants_x) w = aligned_experts(same(kept_w, type, experts * d_in * d_out).view({experts, d_out, d_in}), first);
+        first.settle(stream);
+        if (wants_x) {
+            out[0] = empty_like_shape({rows, d_in}, type, device);
+            check(th_expert_linear_bwd_input(ptr(gy.keep), gy.stride, ptr(w.keep), w.row, w.expert, ends_dev, ptr(out[0]), d_in, rows, ne, di, dn, code, stream),
+                  "th_expert_linear_bwd_input");
+        }
+        if (wants_w) {
+            const Rows &xr = second.add(same(kept_x, type, rows * d_in), d_in);
+            second.settle(stream);
+            out[1] = empty_like_shape({experts, d_out, d_in}, type, device);
+            check(th_expert_linear_bwd_weight(ptr(gy.keep), gy.stride, ptr(xr.keep), xr.stride, ends_dev, ptr(out[1]), rows, ne, di, dn, code, stream),
+                  "th_expert_linear_bwd_weight");
+        }
+    }
+};
+
+// expert_linear(x, weight, ends)
+PyObject *py_expert_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    Tensor x, w, ends;
+    if (n_args != 3 || !usual_mode() || !take(args[0], x) || !take(args[1], w) || !take(args[2], ends)) TH_NOT_MINE;
+    if (!plain(x) || !plain(w) || !plain(ends) || w.dim() != 3 || w.numel() == 0 || x.dim() != 2 || x.numel() == 0 || x.size(1) != w.size(2)) TH_NOT_MINE;
+    const at::ScalarType type = x.scalar_type();
+    const int64_t experts = w.size(0), d_out = w.size(1), d_in = w.size(2), rows = x.size(0);
+    if ((type != at::kHalf && type != at::kBFloat16) || w.scalar_type() != type || w.device() != x.device() || experts > 1024) TH_NOT_MINE;
+    if (ends.scalar_type() != at::kInt || ends.dim() != 1 || ends.size(0) != experts || !ends.is_contiguous() || ends.device() != x.device()) TH_NOT_MINE;
+    Tensor y;
+    {
+        NoGil release;
+        const bool grad = torch::autograd::compute_requires_grad(x, w);
+        std::shared_ptr<ExpertLinearNode> node;
+        if (grad) node = make_node<ExpertLinearNode>(torch::autograd::collect_next_edges(x, w, ends));
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            c10::cuda::CUDAGuard guard(x.device());
+            void *stream = current_stream();
+            Operands operands;
+            const Rows &xr = operands.add(x, d_in);
+            const ExpertWeight e = aligned_experts(w, operands);
+            operands.settle(stream);
+            y = empty_like_shape({rows, d_out}, type, x.device());
+            check(th_expert_linear_fwd(ptr(xr.keep), xr.stride, ptr(e.keep), e.row, e.expert, ends.data_ptr<int32_t>(), ptr(y), d_out, rows, static_cast<int>(experts),
+                                       static_cast<int>(d_in), static_cast<int>(d_out), dtype_code(type), stream),
+                  "th_expert_linear_fwd");
+        }
+        if (grad) {
+            node->rows = rows;
+            node->experts = experts;
+            node->d_in = d_in;
+            node->d_out = d_out;
+            node->type = type;
+            node->keeps_weight = x.requires_grad();
+            node->keeps_input = w.requires_grad();
+            if (node->keeps_weight) node->weight = SavedVariable(w, false);
+            if (node->keeps_input) node->x = SavedVariable(x, false);
+            node->ends = SavedVariable(ends, false);
+            torch::autograd::set_history(y, node);
+        }
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- the global norm of gradients ----------------------------------------------------------------------------
+
+bool take_floats(PyObject *o, size_t n, std::vector<float> &out) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != static_cast<Py_ssize_t>(n)) return false;
+    out.resize(n);
+    for (size_t k = 0; k < n; ++k) {
+        double v;
+        if (!take(PyTuple_GET_ITEM(o, k), v)) return false;
+        out[k] = static_cast<float>(v);
+    }
+    return true;
+}
+
+// grad_norm(tensors, scales or None, max_norm) -> the float32 pair (norm, factor)
+PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    std::vector<Tensor> grads;
+    std::vector<float> scales;
+    double max_norm;
+    if (n_args != 3 || !usual_mode() || !take_list(args[0], grads) || !take(args[2], max_norm)) TH_NOT_MINE;
+    const size_t n = grads.size();
+    if (n == 0 || (args[1] != Py_None && !take_floats(args[1], n, scales))) TH_NOT_MINE;
+    std::vector<const void *> pointers(n);
+    std::vector<int64_t> sizes(n);
+    std::vector<int> codes(n);
+    for (size_t k = 0; k < n; ++k) {
+        const Tensor &t = grads[k];
+        if (!plain(t) || !t.is_contiguous() || t.device() != grads[0].device() || dtype_code(t.scalar_type()) < 0) TH_NOT_MINE;
+        pointers[k] = ptr(t);
+        sizes[k] = t.numel();
+        codes[k] = dtype_code(t.scalar_type());
+    }
+    Tensor pair;
+    {
+        NoGil release;
+        at::AutoDispatchBelowADInplaceOrView below;
+        c10::cuda::CUDAGuard guard(grads[0].device());
+        pair = empty_like_shape({2}, at::kFloat, grads[0].device());
+        const int64_t bytes = th_grad_norm_workspace_bytes(static_cast<int>(n), sizes.data());
+        const Tensor buffer = bytes ? empty_like_shape({bytes}, at::kByte, grads[0].device()) : Tensor();
+        check(th_grad_norm(static_cast<int>(n), pointers.data(), sizes.data(), codes.data(), scales.empty() ? nullptr : scales.data(), static_cast<float>(max_norm),
+                           pair.data_ptr<float>(), ptr(buffer), bytes, current_stream()),
+              "th_grad_norm");
+    }
+    return THPVariable_Wrap(std::move(pair));
+    END_HANDLE_TH_ERRORS
+}
+
+// adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grad, pair, lr, beta1, beta2, eps, step, skipped): the update of
+// tensors of one dtype on one device, gradients times their scale times the pair's factor
+PyObject *py_adam_clipped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    std::vector<Tensor> params, grads, m, v;
+    std::vector<float> scales;
+    double lr, beta1, beta2, eps;
+    int64_t step;
+    Tensor pair, skipped;
+    if (n_args != 13 || g_deferred.load(std::memory_order_relaxed) || !take_list(args[0], params) || !take_list(args[1], grads) || !take_list(args[2], m) ||
+        !take_list(args[3], v) || !take(args[6], pair) || !take(args[7], lr) || !take(args[8], beta1) || !take(args[9], beta2) || !take(args[10], eps) ||
+        !take(args[11], step) || !take(args[12], skipped))
+        TH_NOT_MINE;
+    const size_t n = params.size();
+    if (n == 0 || grads.size() != n || m.size() != n || v.size() != n || !take_floats(args[4], n, scales) || !PyTuple_Check(args[5]) ||
+        PyTuple_GET_SIZE(args[5]) != static_cast<Py_ssize_t>(n))
+        TH_NOT_MINE;
+    if (!plain(pair) || pair.scalar_type() != at::kFloat || pair.numel() != 2 || !pair.is_contiguous()) TH_NOT_MINE;
+    if (skipped.defined() && (!plain(skipped) || skipped.scalar_type() != at::kInt || skipped.device() != params[0].device())) TH_NOT_MINE;
+    std::vector<int> zero(n);
+    std::vector<void *> pp(n), gp(n);
+    std::vector<float *> mp(n), vp(n);
+    std::vector<int64_t> sizes(n);
+    for (size_t k = 0; k < n; ++k) {
+        zero[k] = PyObject_IsTrue(PyTuple_GET_ITEM(args[5], k)) == 1;
+        for (const Tensor *t : {&params[k], &grads[k], &m[k], &v[k]})
+            if (!plain(*t) || !t->is_contiguous() || t->device() != pair.device() || t->numel() != params[k].numel()) TH_NOT_MINE;
+        if (params[k].scalar_type() != params[0].scalar_type() || grads[k].scalar_type() != params[0].scalar_type() || m[k].scalar_type() != at::kFloat ||
+            v[k].scalar_type() != at::kFloat)
+            TH_NOT_MINE;
+        pp[k] = ptr(params[k]);
+        gp[k] = ptr(grads[k]);
+        mp[k] = m[k].data_ptr<float>();
+        vp[k] = v[k].data_ptr<float>();
+        sizes[k] = params[k].numel();
+    }
+    const int code = dtype_code(params[0].scalar_type());
+    if (code < 0) TH_NOT_MINE;
+    {
+        NoGil release;
+        c10::cuda::CUDAGuard guard(params[0].device());
+        check(th_adam_clipped(static_cast<int>(n), pp.data(), gp.data(), mp.data(), vp.data(), sizes.data(), scales.data(), zero.data(), pair.data_ptr<float>(),
+                              static_cast<float>(lr), static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(eps), static_cast<int>(step), code,
+                              skipped.defined() ? skipped.data_ptr<int>() : nullptr, current_stream()),
+              "th_adam_clipped");
+    }
+    // in-place updates that autograd has to know of
+    for (const Tensor &t : params) t.unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- module -------------------------------------------------------------------------------------------------
 
 // configure(level_geometry, host_primes): the package's Python helpers this module asks for geometry and primes
@@ -1696,6 +2099,7 @@ PyObject *py_defer(PyObject *, PyObject *flag) {
 PyMethodDef g_methods[] = {
     TH_FAST(hash_encoding), TH_FAST(fully_fused_mlp), TH_FAST(reversible_mlp), TH_FAST(hash_encoded_mlp), TH_FAST(adam_steps),
     TH_FAST(train_gradients), TH_FAST(configure), TH_FAST(rms_norm), TH_FAST(rms_norm_int8), TH_FAST(int8_linear), TH_FAST(checkpointed_linear),
+    TH_FAST(float8_linear), TH_FAST(float8_training_linear), TH_FAST(expert_linear), TH_FAST(grad_norm), TH_FAST(adam_clipped),
     {"defer", py_defer, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -9,8 +9,18 @@ replaces the separate zero-fill the hash-encoding backward needs before every st
 
 Elements whose gradient is not finite (an overflowed 16-bit sum, a NaN from upstream) are left
 untouched - parameter and moments - and counted; ``FusedAdam.skipped_elements()`` reads the count.
+
+Gradients may be clipped to a global norm on the way: all of them as one vector, its norm and the factor
+stay on the device, and the update multiplies by the factor as it reads::
+
+    norm = sqrt(sum_k scale_k^2 sum_i g_k[i]^2)        factor = min(1, max_norm / (norm + 1e-6))
+
+The sum is in float64, in a fixed order (results repeat bit for bit), and takes any float32 gradients: neither
+large nor small squares are lost. A norm that is not finite passes over the whole step: every element counts as skipped.
 """
-from typing import Dict, Iterable, Optional, Tuple
+import math
+from ctypes import c_float, c_int, c_void_p
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -59,6 +69,154 @@ def adam_updates(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, 
             adam_update(p, g, m, v, step, lr, betas, eps, scale, zero, skipped)
 
 
+# ---- the global norm ----------------------------------------------------------------------------------------
+
+
+def _flat(tensors: Sequence[Tensor], what: str) -> Tuple[List[Tensor], torch.device]:
+    r"""Checks a list of gradients and returns them contiguous (copied where they are not)."""
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise TypeError(f"{what}: gradients must be dense, got {t.layout}")
+        _lib.dtype_code(t)
+    device = _lib.require_cuda(*tensors)
+    return [t.detach().contiguous() for t in tensors], device
+
+
+def _lists(tensors: Sequence[Tensor]) -> tuple:
+    n = len(tensors)
+    return (
+        (c_void_p * n)(*(t.data_ptr() for t in tensors)),
+        _lib.i64_array([t.numel() for t in tensors]),
+        (c_int * n)(*(_lib.DTYPE_CODE[t.dtype] for t in tensors)),
+    )
+
+
+def _check_norm(max_norm: float) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    return max_norm
+
+
+def _norm_factor(tensors: Sequence[Tensor], scales: Optional[Sequence[float]], max_norm: float) -> Tensor:
+    r"""(norm, factor) of a list of gradients, a float32 pair on their device."""
+    tensors = list(tensors)
+    pair = _lib.native().grad_norm(tensors, None if scales is None else tuple(scales), max_norm)
+    if pair is not NotImplemented:
+        return pair
+    flat, device = _flat(tensors, "the global norm")
+    pointers, sizes, codes = _lists(flat)
+    lib = _lib.lib()
+    pair = torch.empty(2, dtype=torch.float32, device=device)
+    ws_bytes = lib.th_grad_norm_workspace_bytes(len(flat), sizes)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        _lib.check(
+            lib.th_grad_norm(
+                len(flat), pointers, sizes, codes, None if scales is None else (c_float * len(flat))(*scales), max_norm, pair.data_ptr(),
+                workspace.data_ptr(), ws_bytes, _lib.stream_ptr(device),
+            ),
+            "th_grad_norm",
+        )  # fmt: skip
+    return pair
+
+
+@torch.no_grad()
+def grad_norm(tensors: Sequence[Tensor], grad_scales: Optional[Sequence[float]] = None) -> Tensor:
+    r"""2-norm of all given tensors (float32, float16 or bfloat16, on one CUDA device) as one vector, each times its scale: a float32
+    scalar on their device, not synchronised. A tensor that is listed twice counts twice."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("the norm of no tensors has no device")
+    if grad_scales is not None and len(grad_scales) != len(tensors):
+        raise ValueError(f"{len(grad_scales)} scales for {len(tensors)} tensors")
+    return _norm_factor(tensors, grad_scales, math.inf)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float) -> Tensor:
+    r"""Scales the gradients of ``parameters`` in place so that their global 2-norm is at most ``max_norm``, and returns the norm that they
+    had (a float32 scalar on their device, not synchronised). As ``torch.nn.utils.clip_grad_norm_``: parameters without a gradient are passed
+    over, gradients whose norm is below ``max_norm`` stay as they are (and are not written), those of an infinite or NaN norm become zeros and
+    NaN. A parameter that is listed twice is taken once; gradients that share memory are not taken apart."""
+    max_norm = _check_norm(max_norm)
+    parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
+    if not grads:
+        return torch.tensor(0.0)
+    pair = _norm_factor(grads, None, max_norm)
+    flat, device = _flat(grads, "clip_grad_norm_")
+    pointers, sizes, codes = _lists(flat)
+    with torch.cuda.device(device):
+        _lib.check(
+            _lib.lib().th_scale_tensors(len(flat), pointers, sizes, codes, pair.data_ptr(), _lib.stream_ptr(device)), "th_scale_tensors"
+        )
+    for g, held in zip(grads, flat):
+        if held.data_ptr() != g.data_ptr():
+            g.copy_(held)  # a gradient that is not contiguous was scaled in a copy
+        else:
+            torch.autograd.graph.increment_version(g)
+    return pair[0]
+
+
+def _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, pair, step, lr, betas, eps, skipped) -> None:
+    r"""The update of parameters of one dtype and device, gradients times their scale times the pair's factor."""
+    done = _lib.native().adam_clipped(
+        params, grads, exp_avgs, exp_avg_sqs, tuple(grad_scales), tuple(zero_grads), pair, lr, betas[0], betas[1], eps, step, skipped
+    )
+    if done is not NotImplemented:
+        return
+    n = len(params)
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        if g.dtype != p.dtype or p.dtype != params[0].dtype or m.dtype != torch.float32 or v.dtype != torch.float32:
+            raise RuntimeError("a clipped update needs parameters and gradients of one dtype and float32 moments")
+        if not all(t.is_contiguous() and t.numel() == p.numel() for t in (p, g, m, v)):
+            raise RuntimeError("a clipped update needs contiguous parameters, gradients and moments of one size")
+    device = _lib.require_cuda(*params, *grads, *exp_avgs, *exp_avg_sqs, pair, skipped)
+    pointers = lambda tensors: (c_void_p * n)(*(t.data_ptr() for t in tensors))  # noqa: E731
+    with torch.cuda.device(device):
+        _lib.check(
+            _lib.lib().th_adam_clipped(
+                n, pointers(params), pointers(grads), pointers(exp_avgs), pointers(exp_avg_sqs), _lib.i64_array([p.numel() for p in params]),
+                (c_float * n)(*grad_scales), (c_int * n)(*map(int, zero_grads)), pair.data_ptr(), lr, betas[0], betas[1], eps, step,
+                _lib.dtype_code(params[0]), _lib.ptr(skipped), _lib.stream_ptr(device),
+            ),
+            "th_adam_clipped",
+        )  # fmt: skip
+    for p in params:
+        torch.autograd.graph.increment_version(p)
+
+
+@torch.no_grad()
+def clipped_adam_updates(
+    params: Sequence[Tensor],
+    grads: Sequence[Tensor],
+    exp_avgs: Sequence[Tensor],
+    exp_avg_sqs: Sequence[Tensor],
+    max_norm: float,
+    step: int,
+    lr: float,
+    betas: Tuple[float, float],
+    eps: float,
+    grad_scales: Optional[Sequence[float]] = None,
+    zero_grads: Optional[Sequence[bool]] = None,
+    skipped: Optional[Tensor] = None,
+) -> Tensor:
+    r"""Adam's update in place of parameters of one dtype and device, their gradients clipped to the global norm ``max_norm``; returns the
+    norm that they had, each times its scale (a float32 scalar on the device, not synchronised). Any number of contiguous tensors, with
+    gradients of the parameters' dtype and float32 moments; ``skipped`` as in ``adam_update``."""
+    max_norm = _check_norm(max_norm)
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    n = len(params)
+    grad_scales = [1.0] * n if grad_scales is None else list(grad_scales)
+    zero_grads = [False] * n if zero_grads is None else list(zero_grads)
+    if n == 0 or any(len(x) != n for x in (grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads)):
+        raise ValueError("a clipped update needs as many gradients, moments, scales and flags as parameters, and one at least")
+    pair = _norm_factor(grads, grad_scales, max_norm)
+    _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, pair, step, lr, betas, eps, skipped)
+    return pair[0]
+
+
 class FusedAdam(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable[Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8):
@@ -78,15 +236,22 @@ class FusedAdam(torch.optim.Optimizer):
         return sum(int(c.item()) for c in self._skipped.values())
 
     @torch.no_grad()
-    def step(self, grad_scale: float = 1.0, zero_grad: bool = False) -> None:
+    def step(self, grad_scale: float = 1.0, zero_grad: bool = False, max_norm: Optional[float] = None) -> Optional[Tensor]:
         r"""Update every parameter that has a gradient.
 
         ``grad_scale`` multiplies the stored gradients before use; ``zero_grad`` clears the
-        gradient buffers (kept allocated) as part of the update kernel.
+        gradient buffers (kept allocated) as part of the update kernel. ``max_norm`` clips the
+        scaled gradients of all groups to that global norm; the norm that they had is returned
+        (a float32 scalar on the device, not synchronised).
         """
-        for group in self.param_groups:
-            live = [p for p in group["params"] if p.grad is not None]
-            self.update(group, live, [p.grad for p in live], [grad_scale] * len(live), [zero_grad] * len(live))
+        groups = [(group, [p for p in group["params"] if p.grad is not None]) for group in self.param_groups]
+        pair = None
+        if max_norm is not None:
+            max_norm, grads = _check_norm(max_norm), [p.grad for _, live in groups for p in live]
+            pair = _norm_factor(grads, [grad_scale] * len(grads), max_norm) if grads else None
+        for group, live in groups:
+            self.update(group, live, [p.grad for p in live], [grad_scale] * len(live), [zero_grad] * len(live), pair)
+        return None if pair is None else pair[0]
 
     def watched(self) -> bool:
         r"""Whether something runs with, or counts, calls of ``step``: hooks of this optimizer or of every optimizer, a scheduler."""
@@ -94,8 +259,9 @@ class FusedAdam(torch.optim.Optimizer):
         return any(hooks) or "step" in self.__dict__
 
     @torch.no_grad()
-    def update(self, group, params, grads, grad_scales, zero_grads) -> None:
-        r"""``step`` on explicit gradients of some of ``group``'s parameters, each with its own scale and zero flag."""
+    def update(self, group, params, grads, grad_scales, zero_grads, pair: Optional[Tensor] = None) -> None:
+        r"""``step`` on explicit gradients of some of ``group``'s parameters, each with its own scale and zero flag; ``pair`` is the norm
+        and the factor that clips them."""
         batches: Dict[tuple, list] = {}  # tensors of one dtype, device and step go together
         for p, g, scale, zero in zip(params, grads, grad_scales, zero_grads):
             state = self.state[p]
@@ -107,4 +273,8 @@ class FusedAdam(torch.optim.Optimizer):
             batches.setdefault((p.dtype, p.device, state["step"]), []).append((p, g, state["exp_avg"], state["exp_avg_sq"], scale, zero))
         for (_, device, step), batch in batches.items():
             columns = [list(c) for c in zip(*batch)]
-            adam_updates(*columns, step, group["lr"], group["betas"], group["eps"], self._skip_counter(device))
+            hyper = (step, group["lr"], group["betas"], group["eps"], self._skip_counter(device))
+            if pair is None:
+                adam_updates(*columns, *hyper)
+            else:
+                _adam_clipped(*columns, pair, *hyper)

@@ -41,7 +41,7 @@ from .layers.hash_encoding import HashEncoding
 from .layers.hash_encoding.helpers import level_geometry
 from .layers.hash_encoding.kernel import _Launch
 from .layers.neural_field.kernel import FieldUnsupported, field_backward, field_forward
-from .optim import FusedAdam, adam_updates
+from .optim import FusedAdam, _check_norm, _norm_factor, adam_updates, clipped_adam_updates
 from .parallel import PendingReduce, allreduce_gradients, gradient_scales, level_passes
 
 
@@ -102,6 +102,9 @@ class NeuralFieldTrainer(nn.Module):
             with the first range.  Measured on 2 and 8 B200 with the cfg 3 step it gains nothing -
             the sum of 24 MB over NVLink takes about as long as the second pass over the points
             costs extra - so it is left to the caller to switch on (slower interconnects, larger tables).
+        max_grad_norm: clip the gradient of the mean loss over the global batch, table and MLP as one vector, to this
+            2-norm ahead of Adam; ``last_grad_norm`` is then the norm that the last step's gradient had (float32, on the
+            device). ``None`` (default): no clipping.
     """
 
     def __init__(
@@ -115,8 +118,11 @@ class NeuralFieldTrainer(nn.Module):
         group: Optional[dist.ProcessGroup] = None,
         backward_passes: Optional[int] = None,
         fused: Union[None, bool, str] = None,
+        max_grad_norm: Optional[float] = None,
     ):
         super().__init__()
+        self.max_grad_norm = None if max_grad_norm is None else _check_norm(max_grad_norm)
+        self.last_grad_norm: Optional[Tensor] = None
         self.fused = fused
         self._no_fused_forward = self._no_fused_backward = self._no_ordered = False
         self.encoding = encoding
@@ -174,7 +180,7 @@ class NeuralFieldTrainer(nn.Module):
         pred.backward(grad_out)
         allreduce_gradients([p.grad for p in self.parameters() if p.grad is not None], self.group)
         # d(mean over the global batch)/d pred = 2 (pred - target) / (N_global * C)
-        self.optimizer.step(grad_scale=2.0 / (pred.numel() * world * self.grad_out_scale))
+        self.last_grad_norm = self.optimizer.step(grad_scale=2.0 / (pred.numel() * world * self.grad_out_scale), max_norm=self.max_grad_norm)
         for p in self.parameters():
             p.grad = None
         return loss_sum / pred.numel()
@@ -215,14 +221,17 @@ class NeuralFieldTrainer(nn.Module):
             if self.optimizer.watched():  # by step hooks or a scheduler: the public step, on the parameters' grad
                 for p, g in zip(params, grads):
                     p.grad = g
-                self.optimizer.step(grad_scale=adam_scale, zero_grad=True)
+                self.last_grad_norm = self.optimizer.step(grad_scale=adam_scale, zero_grad=True, max_norm=self.max_grad_norm)
                 if enc.embeddings.grad is not st.table_grad:
                     st.table_grad.zero_()  # a hook put another gradient in its place
                 for p in params:
                     p.grad = None
             else:
-                zero = [True] + [False] * (len(params) - 1)
-                self.optimizer.update(self.optimizer.param_groups[0], params, grads, [adam_scale] * len(params), zero)
+                zero, scales, pair = [True] + [False] * (len(params) - 1), [adam_scale] * len(params), None
+                if self.max_grad_norm is not None:
+                    pair = _norm_factor(grads, scales, self.max_grad_norm)
+                    self.last_grad_norm = pair[0]
+                self.optimizer.update(self.optimizer.param_groups[0], params, grads, scales, zero, pair)
         except BaseException:
             self._state = None  # its table gradient may not be zero
             raise
@@ -345,10 +354,14 @@ class NeuralFieldTrainer(nn.Module):
         return st.loss_sum / (n * st.d_out)
 
     def _adam_direct(self, st: "_DirectState", table_scale: float, mlp_scale: float) -> None:
-        adam_updates(
-            (self.encoding.embeddings.data.view(-1), st.mlp_flat), (st.table_grad_flat, st.mlp_grad), (st.table_m, st.mlp_m), (st.table_v, st.mlp_v),
-            (table_scale, mlp_scale), (True, False), self._steps, self.lr, self.betas, self.eps, st.skipped,
-        )  # fmt: skip
+        tensors = (self.encoding.embeddings.data.view(-1), st.mlp_flat), (st.table_grad_flat, st.mlp_grad), (st.table_m, st.mlp_m), (st.table_v, st.mlp_v)
+        scales, zero = (table_scale, mlp_scale), (True, False)
+        if self.max_grad_norm is None:
+            adam_updates(*tensors, scales, zero, self._steps, self.lr, self.betas, self.eps, st.skipped)
+        else:
+            self.last_grad_norm = clipped_adam_updates(
+                *tensors, self.max_grad_norm, self._steps, self.lr, self.betas, self.eps, scales, zero, st.skipped
+            )
 
     def _step_native(self, coords: Tensor, targets: Tensor) -> Optional[Tensor]:
         r"""The direct step with its forward and backward in one native call; ``None`` where the Python sequence has to run
