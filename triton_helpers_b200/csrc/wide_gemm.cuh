@@ -629,7 +629,8 @@ int launch_gemm(GemmArgs g, const Operand &a, const Operand &b, int k, bool bf16
     g.idesc = EB == 1 ? instr_desc_i8(CG * kGemmRows, BN) : instr_desc(CG * kGemmRows, BN, bf16, A_MN, B_MN);
     const int out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
     if (g.splits > (S::kSplits ? 8 / CG : 1)) return fail(TH_ERR_UNSUPPORTED, "matrix product: %d parts", g.splits);
-    g.out_tma = !SWAP && g.splits == 1 && matrix_map(&c_map, g.out, g.n, g.m, g.out_stride, out_bytes, 128 / out_bytes, 32);
+    // a TMA store writes whole 16 bytes: rows that end inside of them are copied, so that what lies behind stays
+    g.out_tma = !SWAP && g.splits == 1 && static_cast<long long>(g.n) * out_bytes % 16 == 0 && matrix_map(&c_map, g.out, g.n, g.m, g.out_stride, out_bytes, 128 / out_bytes, 32);
     if (!g.out_tma) c_map = a_map;  // not looked at
     const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "matrix product: too many tiles");
