@@ -1,0 +1,467 @@
+// Products of 8-bit floating-point blocks on tcgen05 (kind::f8f6f4), with a scale for every 128 of K on both sides:
+//
+//     C[m, n] = sum_b a_scale[m, b] b_scale[n, b] P_b[m, n]        P_b[m, n] = sum_{k in block b} A[m, k] B[n, k]
+//
+// A stage of K is one block, 128 bytes.  The tensor cores leave P_b in one of a few accumulators in tensor memory; eight warps take it out while
+// they fill the next, and add it, times its scales, to sums that stay in their registers until the tile's K ends.  So what is summed in
+// the tensor cores is one block, and the sums over blocks are ordinary float32 ones.
+//
+// One persistent CTA per SM, or one pair of CTAs on one 256-row tile (cta_group::2): warp 0 brings operands by TMA through a ring of stages,
+// warp 1 issues the MMAs, warps 2 to 9 keep the sums.  Operand tiles have rows of 128 bytes in the 128-byte swizzle; a weight whose rows are
+// summed over (the input's gradient) is read MN-major as it lies, 128 rows x 128 columns a stage.
+//
+// Few tokens lie along the accumulator's columns, with 128 weight rows, one row of weight blocks, on its lanes; K is then split over the CTAs
+// of a cluster, as it is for few tiles (wide_gemm.cuh).
+#pragma once
+
+#include "wide_gemm.cuh"
+
+namespace th {
+namespace {
+
+constexpr int kF8Threads = 320;
+constexpr int kF8Warps = 8;        // that keep sums
+constexpr int kF8Block = 128;
+
+struct F8Scale {
+    const float *at;
+    long long row, block;  // strides: rows (or blocks of 128 rows) and blocks of K
+};
+
+struct F8Gemm {
+    GemmArgs g;
+    F8Scale tokens, weight;
+};
+
+template <int BN, int CG, bool SWAP, int CTAS>
+struct F8Shape {
+    static constexpr int kBRows = BN / CG;
+    static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
+    static constexpr int kStaging = SWAP ? 0 : kF8Warps * kStagingBoxes * kStagingBytes;
+    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4;  // the biases and barriers are beside it
+    static constexpr int kFit = (kSmem - kStaging - 1024) / kStage;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kBytes = kStages * kStage + kStaging + 1024;
+    static constexpr int kFitAccs = 512 / CTAS / BN, kAccs = kFitAccs > 4 ? 4 : kFitAccs;  // accumulators in tensor memory's 512 columns
+    static constexpr int kTmemCols = kAccs * BN < 32 ? 32 : kAccs * BN;
+    static constexpr int kColumns = BN / 2;  // of each of the two groups of four warps
+    static constexpr bool kSplits = kGemmRows * BN * 4 <= kStages * kStage;
+    static_assert(kStages >= 3 && kAccs >= 2 && CTAS * kTmemCols <= 512, "tile does not fit");
+};
+
+// kind::f8f6f4 instruction descriptor: e4m3 operands, float32 sums
+__host__ __device__ constexpr uint32_t instr_desc_e4m3(int m, int n, bool b_mn) {
+    return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+template <int CG>
+__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b),
+                     "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b),
+                     "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Two scales as one factor, or, where their product is far from one (or no float32 at all), as two factors that a sum takes one after
+// the other: results are then lost only where they are no float32 themselves.
+struct F8Factor {
+    float once, first, then;
+    bool far;
+};
+__device__ __forceinline__ F8Factor f8_factor(float a, float b) {
+    F8Factor f;
+    f.once = a * b;
+    const float2 x = split_scale(a), y = split_scale(b);
+    f.first = x.x * y.x;
+    f.then = x.y * y.y;
+    const float size = fabsf(f.once);
+    f.far = size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
+    return f;
+}
+
+// sums += raw * f over the 32 (or fewer) columns that a warp has read
+template <int N>
+__device__ __forceinline__ void add_scaled(float *sums, const uint32_t (&raw)[32], float f) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) sums[c] = fmaf(__uint_as_float(raw[c]), f, sums[c]);
+}
+
+template <int N>
+__device__ __forceinline__ void f8_read(uint32_t taddr, uint32_t (&raw)[32]) {
+    if constexpr (N == 32) tmem_ld32(taddr, raw);
+    else if constexpr (N == 16) tmem_ld16(taddr, raw);
+    else tmem_ld8_at(taddr, raw);
+}
+
+// SWAP: A is the weight, and the output is C transposed (A's rows are its columns).
+template <bool B_MN, int BN, int CG, bool SWAP, int CTAS>
+__global__ void __launch_bounds__(kF8Threads, CTAS)
+float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap c_map) {
+    using S = F8Shape<BN, CG, SWAP, CTAS>;
+    static_assert(!B_MN || S::kBRows == 128, "an MN-major box holds 128 columns");
+    const GemmArgs &g = f.g;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs];
+    __shared__ float biases[2][BN];
+    __shared__ uint32_t tmem_holder;
+    __shared__ int abort_flag;
+    const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // within the tile: the pair's first CTA leads; the cluster holds one tile's CTAs for every part of K
+    const uint32_t place = CG == 2 ? cluster_rank() : 0, rank = place % CG, leader = place - rank;
+    const int units = g.tiles_m * g.tiles_n * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
+
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&b_map)) : "memory");
+    }
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        const auto init = [](unsigned long long *bar, uint32_t count) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+        };
+        for (int s = 0; s < S::kStages; ++s) {
+            init(&full[s], 1);
+            init(&empty[s], 1);
+        }
+        for (int b = 0; b < S::kAccs; ++b) {
+            init(&acc_full[b], 1);
+            init(&acc_empty[b], kF8Warps * CG);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if constexpr (CG == 2) {  // an allocation for a pair takes columns on both SMs: the other CTA must have started
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (warp == 2) {
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_holder)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_holder)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
+    int ahead = 0;  // stages whose A is on its way already
+    if constexpr (SWAP) {
+        if (warp == 0 && g.early && first < units) {
+            const GemmUnit u = gemm_unit(g, first);
+            ahead = min(S::kStages, u.k1 - u.k0);
+            if (elect_one()) {
+                for (int s = 0; s < ahead; ++s) {
+                    const uint32_t bar = smem_addr(&full[s]);
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(static_cast<uint32_t>(S::kStage)) : "memory");
+                    gemm_load<CG>(smem + s * S::kStage, &a_map, (u.k0 + s) * kF8Block, u.tm * kGemmRows, bar);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    after_previous();
+
+    if (warp == 0) {
+        // ---- operands ----
+        int it = 0;
+        bool ok = true;
+        for (int unit = first; unit < units && ok; unit += step) {
+            const GemmUnit u = gemm_unit(g, unit);
+            const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
+            for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+                const int s = it % S::kStages;
+                const bool got = lane_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
+                if (elect_one() && got) {
+                    const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
+                    if (rank == 0 && it >= ahead)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
+                    const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
+                    const int k = kt * kF8Block;
+                    if (it >= ahead) gemm_load<CG>(a, &a_map, k, m0, bar);
+                    if constexpr (B_MN) gemm_load<CG>(b, &b_map, n0, k, bar);
+                    else gemm_load<CG>(b, &b_map, k, n0, bar);
+                }
+                ok = __all_sync(~0u, got);
+                if (!ok) break;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMAs ----
+        if (rank == 0) {
+            int it = 0;
+            bool ok = true;
+            constexpr uint32_t b_step = B_MN ? 32 * 128 : 32;
+            for (int unit = first; unit < units && ok; unit += step) {
+                const GemmUnit u = gemm_unit(g, unit);
+                for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+                    const int s = it % S::kStages, buf = it % S::kAccs;
+                    ok = gemm_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                    if (!ok) break;
+                    const bool got = lane_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
+                    tc_fence_after();
+                    if (elect_one() && got) {
+                        const uint32_t a = smem + s * S::kStage, b = a + S::kABytes, d = tmem + buf * BN;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) f8_mma<CG>(d, gemm_desc<false>(a + k * 32), gemm_desc<B_MN>(b + k * b_step), g.idesc, k > 0 ? 1u : 0u);
+                        gemm_commit<CG>(smem_addr(&empty[s]), leader);
+                        gemm_commit<CG>(smem_addr(&acc_full[buf]), leader);
+                    }
+                    ok = __all_sync(~0u, got);
+                    if (!ok) break;
+                }
+            }
+        }
+    } else {
+        // ---- sums, and the output ----
+        constexpr int kColumns = S::kColumns, kStep = kColumns < 32 ? kColumns : 32;
+        const int quarter = warp & 3, group = (warp - 2) >> 2, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
+        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 2) * kStagingBoxes * kStagingBytes;
+        int it = 0, done = 0, box = 0;
+        bool ok = true;
+        for (int unit = first; unit < units; unit += step, ++done) {
+            const GemmUnit u = gemm_unit(g, unit);
+            const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter, n0 = u.tn * BN + group * kColumns, m = m0 + lane;
+            // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
+            float *bias = biases[done & 1];
+            for (int c = threadIdx.x - 64; c < BN; c += 32 * kF8Warps) bias[c] = !SWAP && g.bias && u.tn * BN + c < g.n ? bias_at(g.bias, g.bias_dtype, u.tn * BN + c) : 0.f;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!ok) continue;  // a wait gave up: the barriers are met all the same
+            // Lanes are tokens (or, swapped, rows of one row of weight blocks), columns lie within one weight block (or are tokens: lane c, and
+            // lane c - 32, hold column c's scale)
+            const float *lane_scale = SWAP ? f.weight.at + static_cast<long long>(u.tm) * f.weight.row : f.tokens.at + static_cast<long long>(min(m, g.m - 1)) * f.tokens.row;
+            const long long lane_block = SWAP ? f.weight.block : f.tokens.block;
+            constexpr int kTokens = SWAP ? (kColumns + 31) / 32 : 1;
+            const float *column_scale[kTokens];
+#pragma unroll
+            for (int t = 0; t < kTokens; ++t)
+                column_scale[t] = SWAP ? f.tokens.at + static_cast<long long>(min(n0 + 32 * t + lane, g.n - 1)) * f.tokens.row
+                                       : f.weight.at + static_cast<long long>(min(n0, g.n - 1) / kF8Block) * (B_MN ? f.weight.block : f.weight.row);
+            const long long column_block = SWAP ? f.tokens.block : B_MN ? f.weight.row : f.weight.block;
+            float sums[kColumns];
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) sums[c] = 0.f;
+            // one block ahead of its use
+            float next_lane = lane_scale[u.k0 * lane_block], next_column[kTokens];
+#pragma unroll
+            for (int t = 0; t < kTokens; ++t) next_column[t] = column_scale[t][u.k0 * column_block];
+            for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+                const int buf = it % S::kAccs;
+                F8Factor factor[kTokens];
+                bool far = false;
+#pragma unroll
+                for (int t = 0; t < kTokens; ++t) {
+                    factor[t] = f8_factor(next_lane, next_column[t]);
+                    far |= factor[t].far;
+                }
+                far = __any_sync(~0u, far);
+                if (kt + 1 < u.k1) {
+                    next_lane = lane_scale[(kt + 1) * lane_block];
+#pragma unroll
+                    for (int t = 0; t < kTokens; ++t) next_column[t] = column_scale[t][(kt + 1) * column_block];
+                }
+                ok = gemm_wait(smem_addr(&acc_full[buf]), (it / S::kAccs) & 1, &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + buf * BN + group * kColumns + (static_cast<uint32_t>(32 * quarter) << 16);
+#pragma unroll
+                for (int c0 = 0; c0 < kColumns; c0 += kStep) {
+                    uint32_t raw[32];
+                    f8_read<kStep>(d + c0, raw);
+                    tmem_ld_wait();
+                    if (c0 + kStep >= kColumns) {
+                        // the accumulator is read: another block may fill it
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (CG == 2)
+                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), leader)) : "memory");
+                            else
+                                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
+                        }
+                    }
+                    if constexpr (SWAP) {
+                        const F8Factor &mine = factor[c0 / 32];
+                        if (far) {
+#pragma unroll
+                            for (int c = 0; c < kStep; ++c)
+                                sums[c0 + c] = fmaf(__uint_as_float(raw[c]) * __shfl_sync(~0u, mine.first, c), __shfl_sync(~0u, mine.then, c), sums[c0 + c]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < kStep; ++c) sums[c0 + c] = fmaf(__uint_as_float(raw[c]), __shfl_sync(~0u, mine.once, c), sums[c0 + c]);
+                        }
+                    } else {
+                        if (far) {
+#pragma unroll
+                            for (int c = 0; c < kStep; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * factor[0].first);
+                        }
+                        add_scaled<kStep>(sums + c0, raw, far ? factor[0].then : factor[0].once);
+                    }
+                }
+            }
+            if (!ok) continue;
+            if constexpr (S::kSplits) {
+                if (g.splits > 1) {  // the operands have been read: their shared memory takes the sums
+                    const int c_first = group * kColumns;
+                    if constexpr (SWAP) {
+#pragma unroll
+                        for (int c = 0; c < kColumns; ++c)
+                            if (n0 + c < g.n)
+                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(exchange_at<32>(smem, c_first + c, 8 * quarter + (lane >> 2)) + 4 * (lane & 3)), "f"(sums[c]) : "memory");
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kColumns / 4; ++j)
+                            st_shared_16(exchange_at<BN / 4>(smem, 32 * quarter + lane, c_first / 4 + j),
+                                         make_uint4(__float_as_uint(sums[4 * j]), __float_as_uint(sums[4 * j + 1]), __float_as_uint(sums[4 * j + 2]), __float_as_uint(sums[4 * j + 3])));
+                    }
+                    continue;
+                }
+            }
+            if constexpr (SWAP) {
+                const float add = g.bias && m < g.m ? bias_at(g.bias, g.bias_dtype, m) : 0.f;
+                if (m < g.m) {
+#pragma unroll
+                    for (int c = 0; c < kColumns; ++c)
+                        if (n0 + c < g.n) store_one(g.out, static_cast<long long>(n0 + c) * g.out_stride + m, sums[c] + add, g.out_dtype);
+                }
+            } else {
+#pragma unroll
+                for (int c0 = 0; c0 < kColumns; c0 += 32) {
+                    if (n0 + c0 >= g.n) break;
+                    const uint32_t at = staging + (box % kStagingBoxes) * kStagingBytes + lane * 128;
+                    const int half = out_bytes == 2 ? (c0 / 32) & 1 : 0;
+                    if (g.out_tma && half == 0) {
+                        // the box about to be written was handed to TMA kStagingBoxes stores ago
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingBoxes - 1) : "memory");
+                        __syncwarp();
+                    }
+                    float v[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) v[c] = sums[c0 + c] + bias[group * kColumns + c0 + c];
+                    if (out_bytes == 4) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            st_shared_16(at + ((j ^ (lane & 7)) << 4), make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                                                                                  __float_as_uint(v[4 * j + 3])));
+                        store_box(g, &c_map, at - lane * 128, m0, n0 + c0, 4);
+                        ++box;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = pack_out(v[8 * j + 2 * e], v[8 * j + 2 * e + 1], g.out_dtype);
+                            st_shared_16(at + (((4 * half + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                        }
+                        if (half == 1 || n0 + c0 + 32 >= g.n) {
+                            store_box(g, &c_map, at - lane * 128, m0, n0 + (c0 & ~63), 2);
+                            ++box;
+                        }
+                    }
+                }
+            }
+        }
+        if (!SWAP && g.out_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    }
+
+    if constexpr (S::kSplits) {
+        if (g.splits > 1) {
+            // ---- a split tile: this CTA's part of it, from everybody's sums ----
+            __syncwarp();
+            cluster_sync_all();
+            if (!abort_flag && warp >= 2) {
+                const GemmUnit u = gemm_unit(g, first);
+                const float2 *none = nullptr;
+                const int thread = threadIdx.x - 64;
+                if (g.splits <= 2) finish_split<2, BN, CG, SWAP, 8, 2>(g, u, rank, smem, none, biases[0], thread);
+                else if (g.splits <= 4) finish_split<2, BN, CG, SWAP, 4, 4>(g, u, rank, smem, none, biases[0], thread);
+                else if constexpr (CG == 1) finish_split<2, BN, CG, SWAP, 2, 8>(g, u, rank, smem, none, biases[0], thread);
+            }
+            __syncwarp();
+            cluster_sync_all();  // everybody's sums have been read
+        }
+    }
+    __syncthreads();
+    if (abort_flag && threadIdx.x == 0) drain_copies(full, S::kStages);
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();
+    if (warp == 2) {
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
+    }
+    if constexpr (CG == 2) {  // and neither CTA ends before both have given theirs back
+        __syncwarp();
+        cluster_sync_all();
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------
+
+struct F8Product {
+    Operand tokens, weight;  // 8-bit rows; the weight's extent is the output's columns
+    F8Scale token_scale, weight_scale;
+    int k;
+    const void *bias;
+    void *out;
+    long long out_stride;
+    int out_dtype;
+    int weights_settled;  // the weight was complete before the kernel ahead of this one began
+};
+
+template <bool B_MN, int BN, int CG, bool SWAP, int CTAS>
+int launch_float8(const F8Product &p, int splits, cudaStream_t stream) {
+    using S = F8Shape<BN, CG, SWAP, CTAS>;
+    auto kernel = float8_gemm_kernel<B_MN, BN, CG, SWAP, CTAS>;
+    // Once per thread and device, and ahead of the maps: it also makes the device's context current in this thread, which encoding
+    // a map needs and an autograd thread may not have yet.
+    static thread_local unsigned long long ready = 0;
+    int device = 0;
+    if (int rc = cuda_status(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+    if (device >= 64 || !(ready >> device & 1)) {
+        if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "cudaFuncSetAttribute(float8_gemm_kernel)"))
+            return rc;
+        if (device < 64) ready |= 1ull << device;
+    }
+    const Operand &a = SWAP ? p.weight : p.tokens, &b = SWAP ? p.tokens : p.weight;
+    CUtensorMap a_map, b_map, c_map;
+    if (!matrix_map(&a_map, a.base, p.k, a.rows, a.stride, 1, 128, kGemmRows) ||
+        !(B_MN ? matrix_map(&b_map, b.base, b.rows, p.k, b.stride, 1, 128, 128) : matrix_map(&b_map, b.base, p.k, b.rows, b.stride, 1, 128, S::kBRows)))
+        return fail(TH_ERR_ALIGNMENT, "8-bit product: operand rows must start on 16 bytes");
+    F8Gemm f{};
+    GemmArgs &g = f.g;
+    f.tokens = p.token_scale;
+    f.weight = p.weight_scale;
+    g.m = a.rows;
+    g.n = b.rows;
+    g.tiles_m = divide_up(g.m, CG * kGemmRows);
+    g.tiles_n = divide_up(g.n, BN);
+    g.group = static_cast<int>(std::max(4ll, std::min(32ll, (32ll << 20) / (static_cast<long long>(CG) * kGemmRows * p.k))));  // 32 MB of rows (wide_gemm.cuh)
+    g.k_tiles = divide_up(p.k, kF8Block);
+    g.tiles_per_split = divide_up(g.k_tiles, splits);
+    g.splits = divide_up(g.k_tiles, g.tiles_per_split);
+    g.idesc = instr_desc_e4m3(CG * kGemmRows, BN, B_MN);
+    g.out = p.out;
+    g.out_stride = p.out_stride;
+    g.out_dtype = g.bias_dtype = p.out_dtype;
+    g.bias = p.bias;
+    g.early = p.weights_settled;
+    const int out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
+    if (g.splits > (S::kSplits ? 8 / CG : 1)) return fail(TH_ERR_UNSUPPORTED, "8-bit product: %d parts", g.splits);
+    // a TMA store writes whole 16 bytes: rows that end inside of them are copied, so that what lies behind stays
+    g.out_tma = !SWAP && g.splits == 1 && static_cast<long long>(g.n) * out_bytes % 16 == 0 && matrix_map(&c_map, g.out, g.n, g.m, g.out_stride, out_bytes, 128 / out_bytes, 32);
+    if (!g.out_tma) c_map = a_map;  // not looked at
+    const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
+    if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "8-bit product: too many tiles");
+    // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles
+    const long long clusters = g.splits > 1 ? units : std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
+    return launch_chained("float8_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), kF8Threads, S::kBytes, stream, CG * g.splits, f, a_map, b_map, c_map);
+}
+
+}  // namespace
+}  // namespace th

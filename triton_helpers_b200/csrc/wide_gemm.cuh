@@ -256,15 +256,16 @@ __device__ __forceinline__ uint4 ld_cluster_16(uint32_t addr) {
     return v;
 }
 
-// This CTA's part of a split tile.  A read of another CTA's shared memory takes some 600 cycles, so PIECES_AT_ONCE x RANKS (16) of them are
+// This CTA's part of a split tile, by kGemmThreads threads.  A read of another CTA's shared memory takes some 600 cycles, so PIECES_AT_ONCE x RANKS (16) of them are
 // on their way together.
 template <int EB, int BN, int CG, bool SWAP, int PIECES_AT_ONCE, int RANKS>
-__device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &u, uint32_t rank, uint32_t smem, const float2 *scales, const float *biases) {
+__device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &u, uint32_t rank, uint32_t smem, const float2 *scales, const float *biases,
+                                             int thread) {
     constexpr int kPieces = SWAP ? kGemmRows / 4 : BN / 4;
     const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN, rows = max(0, min(kGemmRows, g.m - m0)), cols = min(BN, g.n - n0);
     const int lines = SWAP ? cols : rows, along = SWAP ? rows : cols, total = lines * kPieces;
     const int from = total * u.split / g.splits, to = total * (u.split + 1) / g.splits;
-    for (int first = from + static_cast<int>(threadIdx.x); first < to; first += PIECES_AT_ONCE * kGemmThreads) {
+    for (int first = from + thread; first < to; first += PIECES_AT_ONCE * kGemmThreads) {
         uint4 v[PIECES_AT_ONCE][RANKS];
 #pragma unroll
         for (int p = 0; p < PIECES_AT_ONCE; ++p) {
@@ -297,7 +298,7 @@ __device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &
                 const float2 scale = EB == 1 ? split_scale(g.lane_scale[mi]) : make_float2(1.f, 1.f);
                 const float bias = SWAP ? (g.bias ? bias_at(g.bias, g.bias_dtype, mi) : 0.f) : biases[ni];
                 store_one(g.out, SWAP ? static_cast<long long>(n0 + line) * g.out_stride + mi : static_cast<long long>(m0 + line) * g.out_stride + n0 + c,
-                          finished<EB>(sum[e], scale, scales[ni], bias), g.out_dtype);
+                          finished<EB>(sum[e], scale, EB == 1 ? scales[ni] : scale, bias), g.out_dtype);
             }
         }
     }
@@ -550,9 +551,9 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
             cluster_sync_all();
             if (!abort_flag) {
                 const GemmUnit u = gemm_unit(g, first);
-                if (g.splits <= 2) finish_split<EB, BN, CG, SWAP, 8, 2>(g, u, rank, smem, scales[0], biases[0]);
-                else if (g.splits <= 4) finish_split<EB, BN, CG, SWAP, 4, 4>(g, u, rank, smem, scales[0], biases[0]);
-                else if constexpr (CG == 1) finish_split<EB, BN, CG, SWAP, 2, 8>(g, u, rank, smem, scales[0], biases[0]);
+                if (g.splits <= 2) finish_split<EB, BN, CG, SWAP, 8, 2>(g, u, rank, smem, scales[0], biases[0], threadIdx.x);
+                else if (g.splits <= 4) finish_split<EB, BN, CG, SWAP, 4, 4>(g, u, rank, smem, scales[0], biases[0], threadIdx.x);
+                else if constexpr (CG == 1) finish_split<EB, BN, CG, SWAP, 2, 8>(g, u, rank, smem, scales[0], biases[0], threadIdx.x);
             }
             __syncwarp();
             cluster_sync_all();  // everybody's sums have been read
@@ -574,6 +575,15 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
+
+inline int divide_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+// Clusters of `size` CTAs that run at one time, `per_sm` CTAs on an SM: what the runtime's occupancy query gives on a B200 (clusters stay
+// within a group of SMs, and groups differ), a little less where it is not even.
+inline int cluster_slots(int size, int per_sm) {
+    static const int one[8] = {148, 74, 44, 32, 25, 21, 14, 14}, two[8] = {296, 148, 90, 69, 54, 44, 36, 32};
+    return std::max(1, (per_sm == 1 ? one : two)[size - 1] * sm_count() / 148);
+}
 
 // Rows of `inner` elements, `stride` elements apart; boxes of box_inner x box_outer in the 128-byte swizzle.
 bool matrix_map(CUtensorMap *map, const void *base, long long inner, long long outer, long long stride, int elem_bytes, int box_inner, int box_outer) {

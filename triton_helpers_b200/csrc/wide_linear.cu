@@ -12,15 +12,6 @@ struct ProductPlan {
     int splits;
 };
 
-int divide_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
-
-// Clusters of `size` CTAs that run at one time, `per_sm` CTAs on an SM: what the runtime's occupancy query gives on a B200 (clusters stay
-// within a group of SMs, and groups differ), a little less where it is not even.
-int cluster_slots(int size, int per_sm) {
-    static const int one[8] = {148, 74, 44, 32, 25, 21, 14, 14}, two[8] = {296, 148, 90, 69, 54, 44, 36, 32};
-    return std::max(1, (per_sm == 1 ? one : two)[size - 1] * sm_count() / 148);
-}
-
 // The cheapest cut by an estimate in cycles: rounds of tiles x stages x cycles a stage (what its bytes take into the SM), what a pair
 // takes longer to start, and for split tiles the exchange of their sums.  All cuts measured on a B200, us (tile columns x CTAs x parts;
 // * is the one taken): 2048 x 2048 -> 2048 256x2x1* 17.9, 128x2x1 21, 128x1x1 26; 512 x 4096 -> 4096 128x2x1* 20.3, 256x2x2 21.9, 128x1x1
@@ -127,6 +118,7 @@ int check_int8(const void *weight, int64_t weight_stride, const float *weight_sc
 
 namespace th {
 int rows_status_word();  // rows.cu
+int float8_status_word();  // float8_linear.cu
 }
 
 using namespace th;
@@ -134,8 +126,8 @@ using namespace th;
 extern "C" int th_linear_tc_status(void) {
     int status = 0;
     if (cudaMemcpyFromSymbol(&status, g_tc_status, sizeof(int)) != cudaSuccess) return -1;
-    const int rows = rows_status_word();
-    return rows < 0 ? -1 : status | rows;
+    const int rows = rows_status_word(), blocks = float8_status_word();
+    return rows < 0 || blocks < 0 ? -1 : status | rows | blocks;
 }
 
 static int int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
