@@ -7,7 +7,8 @@
 // the tensor cores is one block, and the sums over blocks are ordinary float32 ones.
 //
 // One persistent CTA per SM, or one pair of CTAs on one 256-row tile (cta_group::2): warp 0 brings operands by TMA through a ring of stages,
-// warp 1 issues the MMAs, warps 2 to 9 keep the sums.  Operand tiles have rows of 128 bytes in the 128-byte swizzle; a weight whose rows are
+// warp 1 issues the MMAs, warps 2 and 3 bring the scales, some blocks ahead, as products through a ring of their own, and warps 4 to 11 keep the
+// sums, with the registers that the others leave them.  Operand tiles have rows of 128 bytes in the 128-byte swizzle; a weight whose rows are
 // summed over (the input's gradient) is read MN-major as it lies, 128 rows x 128 columns a stage.
 //
 // Few tokens lie along the accumulator's columns, with 128 weight rows, one row of weight blocks, on its lanes; K is then split over the CTAs
@@ -19,9 +20,11 @@
 namespace th {
 namespace {
 
-constexpr int kF8Threads = 320;
+constexpr int kF8Threads = 384;
 constexpr int kF8Warps = 8;        // that keep sums
 constexpr int kF8Block = 128;
+constexpr int kF8Slots = 8;        // blocks whose scales are on their way or in use
+constexpr int kF8Batch = 4;        // blocks whose scales a warp asks for at a time
 
 struct F8Scale {
     const float *at;
@@ -33,12 +36,14 @@ struct F8Gemm {
     F8Scale tokens, weight;
 };
 
+// CTAS: CTAs that share an SM
 template <int BN, int CG, bool SWAP, int CTAS>
 struct F8Shape {
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
-    static constexpr int kStaging = SWAP ? 0 : kF8Warps * kStagingBoxes * kStagingBytes;
-    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4;  // the biases and barriers are beside it
+    static constexpr int kStaging = SWAP ? 0 : kF8Warps * kStagingBytes;
+    static constexpr int kFactors = SWAP ? BN : kGemmRows * (BN == 256 ? 2 : 1);  // of a block: a token's for every row of weight blocks
+    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4 - kF8Slots * kFactors * 4;  // biases, factors and barriers are beside it
     static constexpr int kFit = (kSmem - kStaging - 1024) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kBytes = kStages * kStage + kStaging + 1024;
@@ -46,6 +51,9 @@ struct F8Shape {
     static constexpr int kTmemCols = kAccs * BN < 32 ? 32 : kAccs * BN;
     static constexpr int kColumns = BN / 2;  // of each of the two groups of four warps
     static constexpr bool kSplits = kGemmRows * BN * 4 <= kStages * kStage;
+    // Registers a thread: at launch what the SM's 65536 allow; then the first four warps give theirs to those that keep sums
+    static constexpr int kLaunchRegs = CTAS == 1 ? 168 : 80, kFewRegs = CTAS == 1 ? 72 : 40, kSumRegs = CTAS == 1 ? 216 : 96;
+    static_assert(kFewRegs + 2 * kSumRegs <= 3 * kLaunchRegs, "more registers than the launch has");
     static_assert(kStages >= 3 && kAccs >= 2 && CTAS * kTmemCols <= 512, "tile does not fit");
 };
 
@@ -64,28 +72,29 @@ __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint3
                      "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Two scales as one factor, or, where their product is far from one (or no float32 at all), as two factors that a sum takes one after
-// the other: results are then lost only where they are no float32 themselves.
-struct F8Factor {
-    float once, first, then;
-    bool far;
-};
-__device__ __forceinline__ F8Factor f8_factor(float a, float b) {
-    F8Factor f;
-    f.once = a * b;
-    const float2 x = split_scale(a), y = split_scale(b);
-    f.first = x.x * y.x;
-    f.then = x.y * y.y;
-    const float size = fabsf(f.once);
-    f.far = size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
+// The scales' product is one factor where it is between 2^-100 and 2^100.  Where it is not (it may be no float32 at all) a sum takes two factors
+// one after the other, of about its square root each: results are then lost only where they are no float32 themselves.
+
+// Two neighbouring columns' float32 values as one operand of packed arithmetic
+__device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ float2 floats_of(unsigned long long v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
     return f;
 }
-
-// sums += raw * f over the 32 (or fewer) columns that a warp has read
-template <int N>
-__device__ __forceinline__ void add_scaled(float *sums, const uint32_t (&raw)[32], float f) {
-#pragma unroll
-    for (int c = 0; c < N; ++c) sums[c] = fmaf(__uint_as_float(raw[c]), f, sums[c]);
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 template <int N>
@@ -95,6 +104,48 @@ __device__ __forceinline__ void f8_read(uint32_t taddr, uint32_t (&raw)[32]) {
     else tmem_ld8_at(taddr, raw);
 }
 
+// Waits for the reads before, the registers of the last one among its operands: nothing that uses them moves ahead of it
+__device__ __forceinline__ void f8_read_wait(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+                   "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void f8_read_wait16(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+
+// Where a tile's scales lie: the rows of tokens, and the block (or blocks) of weight rows beside them
+template <bool B_MN, int BN, bool SWAP>
+struct F8Tile {
+    const float *tokens, *weight;
+    long long token_block, weight_block, token_row, weight_row;
+    int token0, tokens_end, weights_end;
+
+    __device__ __forceinline__ F8Tile(const F8Gemm &f, const GemmUnit &u, int m0) {
+        token0 = SWAP ? u.tn * BN : m0;
+        const int weight0 = SWAP ? u.tm : u.tn * BN / kF8Block;
+        tokens_end = SWAP ? f.g.n : f.g.m;
+        weights_end = (SWAP ? f.g.m : f.g.n) - 1;
+        token_row = f.tokens.row;
+        token_block = f.tokens.block;
+        // where K goes along a weight's rows its blocks are numbered the other way round
+        weight_row = B_MN ? f.weight.block : f.weight.row;
+        weight_block = B_MN ? f.weight.row : f.weight.block;
+        tokens = f.tokens.at + token0 * token_row;
+        weight = f.weight.at + weight0 * weight_row;
+        weights_end = weights_end / kF8Block - weight0;
+    }
+    __device__ __forceinline__ float token(int t, int kt) const { return tokens[min(t, tokens_end - 1 - token0) * token_row + kt * token_block]; }
+    __device__ __forceinline__ float of_weight(int group, int kt) const { return weight[min(group, weights_end) * weight_row + kt * weight_block]; }
+};
+
 // SWAP: A is the weight, and the output is C transposed (A's rows are its columns).
 template <bool B_MN, int BN, int CG, bool SWAP, int CTAS>
 __global__ void __launch_bounds__(kF8Threads, CTAS)
@@ -103,7 +154,10 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
     static_assert(!B_MN || S::kBRows == 128, "an MN-major box holds 128 columns");
     const GemmArgs &g = f.g;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs];
+    __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs], factor_full[kF8Slots],
+        factor_empty[kF8Slots];
+    __shared__ __align__(16) float factors[kF8Slots][S::kFactors];
+    __shared__ int far_factors[kF8Slots];
     __shared__ float biases[2][BN];
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
@@ -125,6 +179,10 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
         for (int s = 0; s < S::kStages; ++s) {
             init(&full[s], 1);
             init(&empty[s], 1);
+        }
+        for (int s = 0; s < kF8Slots; ++s) {
+            init(&factor_full[s], 1);
+            init(&factor_empty[s], kF8Warps);
         }
         for (int b = 0; b < S::kAccs; ++b) {
             init(&acc_full[b], 1);
@@ -167,6 +225,9 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
     }
     after_previous();
 
+    // Each side of the branch has its registers, so that a split tile is finished within it
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kFewRegs));
     if (warp == 0) {
         // ---- operands ----
         int it = 0;
@@ -218,91 +279,137 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
             }
         }
     } else {
+        // ---- scales: the even blocks' by one warp, the odd ones' by the other ----
+        constexpr int kRows = (SWAP ? BN : kGemmRows) / 32 > 0 ? (SWAP ? BN : kGemmRows) / 32 : 1, kGroups = SWAP ? 1 : BN == 256 ? 2 : 1;
+        int it0 = 0;
+        bool ok = true;
+        for (int unit = first; unit < units && ok; unit += step) {
+            const GemmUnit u = gemm_unit(g, unit);
+            const F8Tile<B_MN, BN, SWAP> tile(f, u, (u.tm * CG + static_cast<int>(rank)) * kGemmRows);
+            for (int kt = u.k0 + ((it0 ^ warp) & 1); kt < u.k1 && ok; kt += 2 * kF8Batch) {
+                float token[kF8Batch][kRows], weight[kF8Batch][kGroups];
+#pragma unroll
+                for (int b = 0; b < kF8Batch; ++b) {
+                    const int at = min(kt + 2 * b, u.k1 - 1);
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) token[b][r] = tile.token(32 * r + lane, at);
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q) weight[b][q] = tile.of_weight(q, at);
+                }
+#pragma unroll
+                for (int b = 0; b < kF8Batch; ++b) {
+                    if (kt + 2 * b >= u.k1) break;
+                    const int it = it0 + kt + 2 * b - u.k0, s = it % kF8Slots;
+                    bool far = false;
+                    ok = gemm_wait(smem_addr(&factor_empty[s]), ((it / kF8Slots) & 1) ^ 1, &abort_flag);
+                    if (!ok) break;
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                        for (int r = 0; r < kRows; ++r) {
+                            const float once = token[b][r] * weight[b][q], size = fabsf(once);
+                            far |= size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
+                            if (32 * r + lane < (SWAP ? BN : kGemmRows)) factors[s][q * kGemmRows + 32 * r + lane] = once;
+                        }
+                    far = __any_sync(~0u, far);
+                    if (lane == 0) {
+                        far_factors[s] = far;
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&factor_full[s])) : "memory");
+                    }
+                }
+            }
+            it0 += u.k1 - u.k0;
+        }
+    }
+    if constexpr (S::kSplits) {
+        if (g.splits > 1) {
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+    }
+    } else {
         // ---- sums, and the output ----
-        constexpr int kColumns = S::kColumns, kStep = kColumns < 32 ? kColumns : 32;
-        const int quarter = warp & 3, group = (warp - 2) >> 2, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
-        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 2) * kStagingBoxes * kStagingBytes;
-        int it = 0, done = 0, box = 0;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSumRegs));
+        constexpr int kColumns = S::kColumns, kStep = kColumns < 32 ? kColumns : 32, kChunks = kColumns / kStep;
+        const int quarter = warp & 3, group = (warp - 4) >> 2, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
+        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kStagingBytes;
+        int it = 0, done = 0;
         bool ok = true;
         for (int unit = first; unit < units; unit += step, ++done) {
             const GemmUnit u = gemm_unit(g, unit);
-            const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter, n0 = u.tn * BN + group * kColumns, m = m0 + lane;
+            const int tile_m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, m0 = tile_m0 + 32 * quarter, n0 = u.tn * BN + group * kColumns, m = m0 + lane;
             // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
             float *bias = biases[done & 1];
-            for (int c = threadIdx.x - 64; c < BN; c += 32 * kF8Warps) bias[c] = !SWAP && g.bias && u.tn * BN + c < g.n ? bias_at(g.bias, g.bias_dtype, u.tn * BN + c) : 0.f;
+            for (int c = threadIdx.x - 128; c < BN; c += 32 * kF8Warps) bias[c] = !SWAP && g.bias && u.tn * BN + c < g.n ? bias_at(g.bias, g.bias_dtype, u.tn * BN + c) : 0.f;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (!ok) continue;  // a wait gave up: the barriers are met all the same
-            // Lanes are tokens (or, swapped, rows of one row of weight blocks), columns lie within one weight block (or are tokens: lane c, and
-            // lane c - 32, hold column c's scale)
-            const float *lane_scale = SWAP ? f.weight.at + static_cast<long long>(u.tm) * f.weight.row : f.tokens.at + static_cast<long long>(min(m, g.m - 1)) * f.tokens.row;
-            const long long lane_block = SWAP ? f.weight.block : f.tokens.block;
-            constexpr int kTokens = SWAP ? (kColumns + 31) / 32 : 1;
-            const float *column_scale[kTokens];
+            unsigned long long sums[kColumns / 2];
 #pragma unroll
-            for (int t = 0; t < kTokens; ++t)
-                column_scale[t] = SWAP ? f.tokens.at + static_cast<long long>(min(n0 + 32 * t + lane, g.n - 1)) * f.tokens.row
-                                       : f.weight.at + static_cast<long long>(min(n0, g.n - 1) / kF8Block) * (B_MN ? f.weight.block : f.weight.row);
-            const long long column_block = SWAP ? f.tokens.block : B_MN ? f.weight.row : f.weight.block;
-            float sums[kColumns];
-#pragma unroll
-            for (int c = 0; c < kColumns; ++c) sums[c] = 0.f;
-            // one block ahead of its use
-            float next_lane = lane_scale[u.k0 * lane_block], next_column[kTokens];
-#pragma unroll
-            for (int t = 0; t < kTokens; ++t) next_column[t] = column_scale[t][u.k0 * column_block];
+            for (int c = 0; c < kColumns / 2; ++c) sums[c] = 0;
+#pragma unroll 1
             for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
-                const int buf = it % S::kAccs;
-                F8Factor factor[kTokens];
-                bool far = false;
-#pragma unroll
-                for (int t = 0; t < kTokens; ++t) {
-                    factor[t] = f8_factor(next_lane, next_column[t]);
-                    far |= factor[t].far;
-                }
-                far = __any_sync(~0u, far);
-                if (kt + 1 < u.k1) {
-                    next_lane = lane_scale[(kt + 1) * lane_block];
-#pragma unroll
-                    for (int t = 0; t < kTokens; ++t) next_column[t] = column_scale[t][(kt + 1) * column_block];
-                }
+                const int buf = it % S::kAccs, slot = it % kF8Slots;
+                ok = gemm_wait(smem_addr(&factor_full[slot]), (it / kF8Slots) & 1, &abort_flag);
+                if (!ok) break;
+                // a lane's (rows of weights share a column's, which is read where it is used)
+                const float factor = SWAP ? 0.f : factors[slot][(BN == 256 ? group * kGemmRows : 0) + 32 * quarter + lane];
+                const bool far = far_factors[slot] != 0;
                 ok = gemm_wait(smem_addr(&acc_full[buf]), (it / S::kAccs) & 1, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * BN + group * kColumns + (static_cast<uint32_t>(32 * quarter) << 16);
+                uint32_t raw[2][32] = {};
+                f8_read<kStep>(d, raw[0]);
+                const unsigned long long both = pair_of(__float_as_uint(factor), __float_as_uint(factor));
 #pragma unroll
-                for (int c0 = 0; c0 < kColumns; c0 += kStep) {
-                    uint32_t raw[32];
-                    f8_read<kStep>(d + c0, raw);
-                    tmem_ld_wait();
-                    if (c0 + kStep >= kColumns) {
+                for (int chunk = 0; chunk < kChunks; ++chunk) {
+                    if constexpr (kStep == 32) f8_read_wait(raw[chunk & 1]);
+                    else f8_read_wait16(raw[0]);
+                    if (chunk + 1 < kChunks) f8_read<kStep>(d + (chunk + 1) * kStep, raw[(chunk + 1) & 1]);  // on its way while this one is added
+                    else {
                         // the accumulator is read: another block may fill it
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
+                            // What is handed over lies in tensor memory, ordered by the fence above: a release to the cluster would also wait for
+                            // everything that is on its way from and to global memory
                             if constexpr (CG == 2)
-                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), leader)) : "memory");
+                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), leader)) : "memory");
                             else
                                 asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
                         }
                     }
-                    if constexpr (SWAP) {
-                        const F8Factor &mine = factor[c0 / 32];
-                        if (far) {
+                    uint32_t(&now)[32] = raw[chunk & 1];
+                    unsigned long long *to = sums + chunk * kStep / 2;
+                    if (far) {  // the scales' product is far from one, or no float32: two factors
+                        const F8Tile<B_MN, BN, SWAP> tile(f, u, tile_m0);
+                        const int mine = SWAP ? group * kColumns + chunk * 32 + lane : 32 * quarter + lane;
+                        const float2 x = split_scale(tile.token(mine, kt)), y = split_scale(tile.of_weight(SWAP || BN != 256 ? 0 : group, kt));
+                        const float once = x.x * y.x, then = x.y * y.y;
 #pragma unroll
-                            for (int c = 0; c < kStep; ++c)
-                                sums[c0 + c] = fmaf(__uint_as_float(raw[c]) * __shfl_sync(~0u, mine.first, c), __shfl_sync(~0u, mine.then, c), sums[c0 + c]);
-                        } else {
+                        for (int c = 0; c < kStep / 2; ++c) {
+                            const unsigned long long p = SWAP ? pair_of(__float_as_uint(__shfl_sync(~0u, once, 2 * c)), __float_as_uint(__shfl_sync(~0u, once, 2 * c + 1)))
+                                                              : pair_of(__float_as_uint(once), __float_as_uint(once));
+                            const unsigned long long q = SWAP ? pair_of(__float_as_uint(__shfl_sync(~0u, then, 2 * c)), __float_as_uint(__shfl_sync(~0u, then, 2 * c + 1)))
+                                                              : pair_of(__float_as_uint(then), __float_as_uint(then));
+                            to[c] = fma_pair(mul_pair(pair_of(now[2 * c], now[2 * c + 1]), p), q, to[c]);
+                        }
+                    } else if constexpr (SWAP) {
+                        const ulonglong2 *of_columns = reinterpret_cast<const ulonglong2 *>(&factors[slot][group * kColumns + chunk * kStep]);
 #pragma unroll
-                            for (int c = 0; c < kStep; ++c) sums[c0 + c] = fmaf(__uint_as_float(raw[c]), __shfl_sync(~0u, mine.once, c), sums[c0 + c]);
+                        for (int c = 0; c < kStep / 4; ++c) {
+                            const ulonglong2 four = of_columns[c];
+                            to[2 * c] = fma_pair(pair_of(now[4 * c], now[4 * c + 1]), four.x, to[2 * c]);
+                            to[2 * c + 1] = fma_pair(pair_of(now[4 * c + 2], now[4 * c + 3]), four.y, to[2 * c + 1]);
                         }
                     } else {
-                        if (far) {
 #pragma unroll
-                            for (int c = 0; c < kStep; ++c) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * factor[0].first);
-                        }
-                        add_scaled<kStep>(sums + c0, raw, far ? factor[0].then : factor[0].once);
+                        for (int c = 0; c < kStep / 2; ++c) to[c] = fma_pair(pair_of(now[2 * c], now[2 * c + 1]), both, to[c]);
                     }
                 }
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&factor_empty[slot])) : "memory");
             }
             if (!ok) continue;
             if constexpr (S::kSplits) {
@@ -312,12 +419,14 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
 #pragma unroll
                         for (int c = 0; c < kColumns; ++c)
                             if (n0 + c < g.n)
-                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(exchange_at<32>(smem, c_first + c, 8 * quarter + (lane >> 2)) + 4 * (lane & 3)), "f"(sums[c]) : "memory");
+                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(exchange_at<32>(smem, c_first + c, 8 * quarter + (lane >> 2)) + 4 * (lane & 3)),
+                                             "f"(c & 1 ? floats_of(sums[c / 2]).y : floats_of(sums[c / 2]).x) : "memory");
                     } else {
 #pragma unroll
                         for (int j = 0; j < kColumns / 4; ++j)
                             st_shared_16(exchange_at<BN / 4>(smem, 32 * quarter + lane, c_first / 4 + j),
-                                         make_uint4(__float_as_uint(sums[4 * j]), __float_as_uint(sums[4 * j + 1]), __float_as_uint(sums[4 * j + 2]), __float_as_uint(sums[4 * j + 3])));
+                                         make_uint4(__float_as_uint(floats_of(sums[2 * j]).x), __float_as_uint(floats_of(sums[2 * j]).y),
+                                                    __float_as_uint(floats_of(sums[2 * j + 1]).x), __float_as_uint(floats_of(sums[2 * j + 1]).y)));
                     }
                     continue;
                 }
@@ -327,29 +436,33 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                 if (m < g.m) {
 #pragma unroll
                     for (int c = 0; c < kColumns; ++c)
-                        if (n0 + c < g.n) store_one(g.out, static_cast<long long>(n0 + c) * g.out_stride + m, sums[c] + add, g.out_dtype);
+                        if (n0 + c < g.n) store_one(g.out, static_cast<long long>(n0 + c) * g.out_stride + m, (c & 1 ? floats_of(sums[c / 2]).y : floats_of(sums[c / 2]).x) + add,
+                                                   g.out_dtype);
                 }
             } else {
 #pragma unroll
                 for (int c0 = 0; c0 < kColumns; c0 += 32) {
                     if (n0 + c0 >= g.n) break;
-                    const uint32_t at = staging + (box % kStagingBoxes) * kStagingBytes + lane * 128;
+                    const uint32_t at = staging + lane * 128;
                     const int half = out_bytes == 2 ? (c0 / 32) & 1 : 0;
                     if (g.out_tma && half == 0) {
-                        // the box about to be written was handed to TMA kStagingBoxes stores ago
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingBoxes - 1) : "memory");
+                        // the box about to be written was handed to TMA a store ago
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
                     }
                     float v[32];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) v[c] = sums[c0 + c] + bias[group * kColumns + c0 + c];
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 two = floats_of(sums[(c0 + c) / 2]);
+                        v[c] = two.x + bias[group * kColumns + c0 + c];
+                        v[c + 1] = two.y + bias[group * kColumns + c0 + c + 1];
+                    }
                     if (out_bytes == 4) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             st_shared_16(at + ((j ^ (lane & 7)) << 4), make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
                                                                                   __float_as_uint(v[4 * j + 3])));
                         store_box(g, &c_map, at - lane * 128, m0, n0 + c0, 4);
-                        ++box;
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -358,32 +471,28 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                             for (int e = 0; e < 4; ++e) w[e] = pack_out(v[8 * j + 2 * e], v[8 * j + 2 * e + 1], g.out_dtype);
                             st_shared_16(at + (((4 * half + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
                         }
-                        if (half == 1 || n0 + c0 + 32 >= g.n) {
-                            store_box(g, &c_map, at - lane * 128, m0, n0 + (c0 & ~63), 2);
-                            ++box;
-                        }
+                        if (half == 1 || n0 + c0 + 32 >= g.n) store_box(g, &c_map, at - lane * 128, m0, n0 + (c0 & ~63), 2);
                     }
                 }
             }
         }
         if (!SWAP && g.out_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    }
-
-    if constexpr (S::kSplits) {
-        if (g.splits > 1) {
-            // ---- a split tile: this CTA's part of it, from everybody's sums ----
-            __syncwarp();
-            cluster_sync_all();
-            if (!abort_flag && warp >= 2) {
-                const GemmUnit u = gemm_unit(g, first);
-                const float2 *none = nullptr;
-                const int thread = threadIdx.x - 64;
-                if (g.splits <= 2) finish_split<2, BN, CG, SWAP, 8, 2>(g, u, rank, smem, none, biases[0], thread);
-                else if (g.splits <= 4) finish_split<2, BN, CG, SWAP, 4, 4>(g, u, rank, smem, none, biases[0], thread);
-                else if constexpr (CG == 1) finish_split<2, BN, CG, SWAP, 2, 8>(g, u, rank, smem, none, biases[0], thread);
+        if constexpr (S::kSplits) {
+            if (g.splits > 1) {
+                // ---- a split tile: this CTA's part of it, from everybody's sums ----
+                __syncwarp();
+                cluster_sync_all();
+                if (!abort_flag) {
+                    const GemmUnit u = gemm_unit(g, first);
+                    const float2 *none = nullptr;
+                    const int thread = threadIdx.x - 128;
+                    if (g.splits <= 2) finish_split<2, BN, CG, SWAP, 8, 2>(g, u, rank, smem, none, biases[0], thread);
+                    else if (g.splits <= 4) finish_split<2, BN, CG, SWAP, 4, 4>(g, u, rank, smem, none, biases[0], thread);
+                    else if constexpr (CG == 1) finish_split<2, BN, CG, SWAP, 2, 8>(g, u, rank, smem, none, biases[0], thread);
+                }
+                __syncwarp();
+                cluster_sync_all();  // everybody's sums have been read
             }
-            __syncwarp();
-            cluster_sync_all();  // everybody's sums have been read
         }
     }
     __syncthreads();
@@ -426,6 +535,9 @@ int launch_float8(const F8Product &p, int splits, cudaStream_t stream) {
     if (device >= 64 || !(ready >> device & 1)) {
         if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "cudaFuncSetAttribute(float8_gemm_kernel)"))
             return rc;
+        cudaFuncAttributes attributes;
+        if (int rc = cuda_status(cudaFuncGetAttributes(&attributes, kernel), "cudaFuncGetAttributes(float8_gemm_kernel)")) return rc;
+        if (attributes.numRegs < S::kLaunchRegs) return fail(TH_ERR_UNSUPPORTED, "8-bit product: built with %d registers a thread", attributes.numRegs);
         if (device < 64) ready |= 1ull << device;
     }
     const Operand &a = SWAP ? p.weight : p.tokens, &b = SWAP ? p.tokens : p.weight;
