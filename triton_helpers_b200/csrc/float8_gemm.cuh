@@ -20,10 +20,9 @@
 namespace th {
 namespace {
 
-constexpr int kF8Threads = 384;
-constexpr int kF8Warps = 8;        // that keep sums
 constexpr int kF8Block = 128;
-constexpr int kF8Slots = 8;        // blocks whose scales are on their way or in use
+constexpr int kF8Step = 16;        // columns of an accumulator that a warp reads at a time
+constexpr int kF8Piece = 32 * 32;  // bytes: 32 rows of 32 that a warp turns in shared memory where rows of the output do not start on 32 bytes
 constexpr int kF8Batch = 4;        // blocks whose scales a warp asks for at a time
 
 struct F8Scale {
@@ -41,19 +40,22 @@ template <int BN, int CG, bool SWAP, int CTAS>
 struct F8Shape {
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
-    static constexpr int kStaging = SWAP ? 0 : kF8Warps * kStagingBytes;
+    static constexpr int kGroups = CTAS == 1 ? 4 : 2;  // of four warps that keep sums
+    static constexpr int kWarps = 4 * kGroups, kThreads = 128 + 32 * kWarps;
+    static constexpr int kStaging = SWAP ? 0 : kWarps * kF8Piece;
     static constexpr int kFactors = SWAP ? BN : kGemmRows * (BN == 256 ? 2 : 1);  // of a block: a token's for every row of weight blocks
-    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4 - kF8Slots * kFactors * 4;  // biases, factors and barriers are beside it
+    static constexpr int kFitAccs = 512 / CTAS / BN, kAccs = kFitAccs > 4 ? 4 : kFitAccs;  // accumulators in tensor memory's 512 columns
+    static constexpr int kSlots = 3 * kAccs;  // blocks whose factors are held
+    static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4 - kSlots * 2 * kFactors * 4;  // biases, factors and barriers are beside it
     static constexpr int kFit = (kSmem - kStaging - 1024) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kBytes = kStages * kStage + kStaging + 1024;
-    static constexpr int kFitAccs = 512 / CTAS / BN, kAccs = kFitAccs > 4 ? 4 : kFitAccs;  // accumulators in tensor memory's 512 columns
     static constexpr int kTmemCols = kAccs * BN < 32 ? 32 : kAccs * BN;
-    static constexpr int kColumns = BN / 2;  // of each of the two groups of four warps
+    static constexpr int kColumns = BN / kGroups;  // of each group
     static constexpr bool kSplits = kGemmRows * BN * 4 <= kStages * kStage;
     // Registers a thread: at launch what the SM's 65536 allow; then the first four warps give theirs to those that keep sums
-    static constexpr int kLaunchRegs = CTAS == 1 ? 168 : 80, kFewRegs = CTAS == 1 ? 72 : 40, kSumRegs = CTAS == 1 ? 216 : 96;
-    static_assert(kFewRegs + 2 * kSumRegs <= 3 * kLaunchRegs, "more registers than the launch has");
+    static constexpr int kLaunchRegs = CTAS == 1 ? 96 : 80, kFewRegs = CTAS == 1 ? 64 : 40, kSumRegs = CTAS == 1 ? 104 : 96;
+    static_assert(kFewRegs + kGroups * kSumRegs <= (1 + kGroups) * kLaunchRegs, "more registers than the launch has");
     static_assert(kStages >= 3 && kAccs >= 2 && CTAS * kTmemCols <= 512, "tile does not fit");
 };
 
@@ -98,27 +100,69 @@ __device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, uns
 }
 
 template <int N>
-__device__ __forceinline__ void f8_read(uint32_t taddr, uint32_t (&raw)[32]) {
-    if constexpr (N == 32) tmem_ld32(taddr, raw);
-    else if constexpr (N == 16) tmem_ld16(taddr, raw);
-    else tmem_ld8_at(taddr, raw);
+__device__ __forceinline__ void f8_read(uint32_t taddr, uint32_t (&v)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                       "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                     : "r"(taddr)
+                     : "memory");
+    else
+        tmem_ld8_at(taddr, v);
 }
 
 // Waits for the reads before, the registers of the last one among its operands: nothing that uses them moves ahead of it
-__device__ __forceinline__ void f8_read_wait(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
-                   "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
+template <int N>
+__device__ __forceinline__ void f8_read_wait(uint32_t (&v)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                       "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                     :
+                     : "memory");
+    else
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+                     :
+                     : "memory");
 }
-__device__ __forceinline__ void f8_read_wait16(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-                 :
-                 : "memory");
+
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]) : "memory");
+}
+
+// 32 bytes of each of a warp's 32 rows -> rows m0.., columns c0.. of the output, through shared memory so that neighbouring lanes write
+// neighbouring elements
+__device__ __forceinline__ void copy_piece(const GemmArgs &g, uint32_t box, const uint32_t *v, int m0, int c0, int out_bytes) {
+    const int lane = threadIdx.x & 31, per_row = 32 / out_bytes, cols = min(per_row, g.n - c0), rows = min(32, g.m - m0);
+    __syncwarp();
+    const uint32_t at = box + lane * 32, turn = (lane >> 2) & 1;  // two lanes' halves change places, for the banks
+    st_shared_16(at + (turn << 4), make_uint4(v[0], v[1], v[2], v[3]));
+    st_shared_16(at + ((turn ^ 1) << 4), make_uint4(v[4], v[5], v[6], v[7]));
+    __syncwarp();
+    const int c = lane % per_row;
+    for (int r = lane / per_row; r < rows; r += 32 / per_row) {
+        const uint32_t from = box + r * 32 + ((c * out_bytes) ^ (((r >> 2) & 1) << 4));
+        const long long to = static_cast<long long>(m0 + r) * g.out_stride + c0 + c;
+        if (c < cols) {
+            if (out_bytes == 4) {
+                uint32_t x;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(from) : "memory");
+                static_cast<uint32_t *>(g.out)[to] = x;
+            } else {
+                unsigned short x;
+                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from) : "memory");
+                static_cast<unsigned short *>(g.out)[to] = x;
+            }
+        }
+    }
 }
 
 // Where a tile's scales lie: the rows of tokens, and the block (or blocks) of weight rows beside them
@@ -146,18 +190,23 @@ struct F8Tile {
     __device__ __forceinline__ float of_weight(int group, int kt) const { return weight[min(group, weights_end) * weight_row + kt * weight_block]; }
 };
 
+// An MN-major operand of 256 columns lies in two boxes of 128, whose distance is the descriptor's leading offset.
+template <bool MN>
+__device__ __forceinline__ uint64_t gemm_desc_b(uint32_t addr) {
+    return smem_desc(MN ? desc_low(addr) | ((128u * 128u >> 4) << 16) : desc_low(addr));
+}
+
 // SWAP: A is the weight, and the output is C transposed (A's rows are its columns).
 template <bool B_MN, int BN, int CG, bool SWAP, int CTAS>
-__global__ void __launch_bounds__(kF8Threads, CTAS)
-float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap c_map) {
+__global__ void __launch_bounds__(F8Shape<BN, CG, SWAP, CTAS>::kThreads, CTAS)
+float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map) {
     using S = F8Shape<BN, CG, SWAP, CTAS>;
-    static_assert(!B_MN || S::kBRows == 128, "an MN-major box holds 128 columns");
+    static_assert(!B_MN || S::kBRows % 128 == 0, "an MN-major box holds 128 columns");
     const GemmArgs &g = f.g;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs], factor_full[kF8Slots],
-        factor_empty[kF8Slots];
-    __shared__ __align__(16) float factors[kF8Slots][S::kFactors];
-    __shared__ int far_factors[kF8Slots];
+    __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs];
+    __shared__ __align__(16) float factors[S::kSlots][2][S::kFactors];
+    __shared__ int far_factors[S::kSlots];
     __shared__ float biases[2][BN];
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
@@ -180,13 +229,9 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
             init(&full[s], 1);
             init(&empty[s], 1);
         }
-        for (int s = 0; s < kF8Slots; ++s) {
-            init(&factor_full[s], 1);
-            init(&factor_empty[s], kF8Warps);
-        }
         for (int b = 0; b < S::kAccs; ++b) {
-            init(&acc_full[b], 1);
-            init(&acc_empty[b], kF8Warps * CG);
+            init(&acc_full[b], 2);  // the block's MMAs and its scales
+            init(&acc_empty[b], S::kWarps * CG);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -245,8 +290,10 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                     const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
                     const int k = kt * kF8Block;
                     if (it >= ahead) gemm_load<CG>(a, &a_map, k, m0, bar);
-                    if constexpr (B_MN) gemm_load<CG>(b, &b_map, n0, k, bar);
-                    else gemm_load<CG>(b, &b_map, k, n0, bar);
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < S::kBRows / 128; ++j) gemm_load<CG>(b + j * 128 * 128, &b_map, n0 + 128 * j, k, bar);
+                    } else gemm_load<CG>(b, &b_map, k, n0, bar);
                 }
                 ok = __all_sync(~0u, got);
                 if (!ok) break;
@@ -260,21 +307,20 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
             constexpr uint32_t b_step = B_MN ? 32 * 128 : 32;
             for (int unit = first; unit < units && ok; unit += step) {
                 const GemmUnit u = gemm_unit(g, unit);
-                for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+                for (int kt = u.k0; kt < u.k1 && ok; ++kt, ++it) {
                     const int s = it % S::kStages, buf = it % S::kAccs;
-                    ok = gemm_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                    ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
                     if (!ok) break;
-                    const bool got = lane_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
+                    const bool got = lane_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
                     tc_fence_after();
                     if (elect_one() && got) {
                         const uint32_t a = smem + s * S::kStage, b = a + S::kABytes, d = tmem + buf * BN;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) f8_mma<CG>(d, gemm_desc<false>(a + k * 32), gemm_desc<B_MN>(b + k * b_step), g.idesc, k > 0 ? 1u : 0u);
-                        gemm_commit<CG>(smem_addr(&empty[s]), leader);
+                        for (int k = 0; k < 4; ++k) f8_mma<CG>(d, gemm_desc<false>(a + k * 32), gemm_desc_b<B_MN>(b + k * b_step), g.idesc, k > 0 ? 1u : 0u);
                         gemm_commit<CG>(smem_addr(&acc_full[buf]), leader);
+                        gemm_commit<CG>(smem_addr(&empty[s]), leader);
                     }
                     ok = __all_sync(~0u, got);
-                    if (!ok) break;
                 }
             }
         }
@@ -299,22 +345,39 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
 #pragma unroll
                 for (int b = 0; b < kF8Batch; ++b) {
                     if (kt + 2 * b >= u.k1) break;
-                    const int it = it0 + kt + 2 * b - u.k0, s = it % kF8Slots;
+                    const int it = it0 + kt + 2 * b - u.k0, s = it % S::kSlots, buf = it % S::kAccs;
                     bool far = false;
-                    ok = gemm_wait(smem_addr(&factor_empty[s]), ((it / kF8Slots) & 1) ^ 1, &abort_flag);
+                    // The accumulator's block before is complete.  So block it - 2 kAccs has been read out by every warp, and the blocks before it have been
+                    // added: a slot that came round since is free.
+                    static_assert(S::kSlots > 2 * S::kAccs, "a slot may still be in use");
+                                        if (it >= S::kAccs) ok = gemm_wait(smem_addr(&acc_full[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
                     if (!ok) break;
 #pragma unroll
                     for (int q = 0; q < kGroups; ++q)
 #pragma unroll
                         for (int r = 0; r < kRows; ++r) {
-                            const float once = token[b][r] * weight[b][q], size = fabsf(once);
+                            const float size = fabsf(token[b][r] * weight[b][q]);
                             far |= size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
-                            if (32 * r + lane < (SWAP ? BN : kGemmRows)) factors[s][q * kGemmRows + 32 * r + lane] = once;
                         }
                     far = __any_sync(~0u, far);
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                        for (int r = 0; r < kRows; ++r) {
+                            const int at = q * kGemmRows + 32 * r + lane;
+                            if (32 * r + lane >= (SWAP ? BN : kGemmRows)) continue;
+                            if (far) {
+                                const float2 x = split_scale(token[b][r]), y = split_scale(weight[b][q]);
+                                factors[s][0][at] = x.x * y.x;
+                                factors[s][1][at] = x.y * y.y;
+                            } else {
+                                factors[s][0][at] = token[b][r] * weight[b][q];
+                            }
+                        }
+                    __syncwarp();
                     if (lane == 0) {
                         far_factors[s] = far;
-                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&factor_full[s])) : "memory");
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_full[buf])) : "memory");
                     }
                 }
             }
@@ -331,43 +394,42 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
     } else {
         // ---- sums, and the output ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSumRegs));
-        constexpr int kColumns = S::kColumns, kStep = kColumns < 32 ? kColumns : 32, kChunks = kColumns / kStep;
+        constexpr int kColumns = S::kColumns, kStep = kColumns < kF8Step ? kColumns : kF8Step, kChunks = kColumns / kStep;
         const int quarter = warp & 3, group = (warp - 4) >> 2, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
-        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kStagingBytes;
+        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kF8Piece;
         int it = 0, done = 0;
         bool ok = true;
+        const auto column = [&](int c) { return group * kColumns + c; };  // of the tile
         for (int unit = first; unit < units; unit += step, ++done) {
             const GemmUnit u = gemm_unit(g, unit);
-            const int tile_m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, m0 = tile_m0 + 32 * quarter, n0 = u.tn * BN + group * kColumns, m = m0 + lane;
+            const int tile_m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, m0 = tile_m0 + 32 * quarter, n0 = u.tn * BN, m = m0 + lane;
             // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
             float *bias = biases[done & 1];
-            for (int c = threadIdx.x - 128; c < BN; c += 32 * kF8Warps) bias[c] = !SWAP && g.bias && u.tn * BN + c < g.n ? bias_at(g.bias, g.bias_dtype, u.tn * BN + c) : 0.f;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int c = threadIdx.x - 128; c < BN; c += 32 * S::kWarps) bias[c] = !SWAP && g.bias && u.tn * BN + c < g.n ? bias_at(g.bias, g.bias_dtype, u.tn * BN + c) : 0.f;
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");
             if (!ok) continue;  // a wait gave up: the barriers are met all the same
             unsigned long long sums[kColumns / 2];
 #pragma unroll
             for (int c = 0; c < kColumns / 2; ++c) sums[c] = 0;
 #pragma unroll 1
             for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
-                const int buf = it % S::kAccs, slot = it % kF8Slots;
-                ok = gemm_wait(smem_addr(&factor_full[slot]), (it / kF8Slots) & 1, &abort_flag);
-                if (!ok) break;
-                // a lane's (rows of weights share a column's, which is read where it is used)
-                const float factor = SWAP ? 0.f : factors[slot][(BN == 256 ? group * kGemmRows : 0) + 32 * quarter + lane];
-                const bool far = far_factors[slot] != 0;
+                const int buf = it % S::kAccs, slot = it % S::kSlots;
                 ok = gemm_wait(smem_addr(&acc_full[buf]), (it / S::kAccs) & 1, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * BN + group * kColumns + (static_cast<uint32_t>(32 * quarter) << 16);
-                uint32_t raw[2][32] = {};
-                f8_read<kStep>(d, raw[0]);
-                const unsigned long long both = pair_of(__float_as_uint(factor), __float_as_uint(factor));
+                uint32_t raw[kStep];
+                f8_read<kStep>(d, raw);
+                // a lane's (swapped, it is a column's, and read where it is used)
+                constexpr bool kPairs = BN == 256;
+                const float *of_lane = &factors[slot][0][SWAP ? group * kColumns : (kPairs ? group / 2 * kGemmRows : 0) + 32 * quarter + lane];
+                unsigned long long both = 0;
+                if constexpr (!SWAP) both = pair_of(__float_as_uint(*of_lane), __float_as_uint(*of_lane));
+                const bool far = far_factors[slot] != 0;
 #pragma unroll
                 for (int chunk = 0; chunk < kChunks; ++chunk) {
-                    if constexpr (kStep == 32) f8_read_wait(raw[chunk & 1]);
-                    else f8_read_wait16(raw[0]);
-                    if (chunk + 1 < kChunks) f8_read<kStep>(d + (chunk + 1) * kStep, raw[(chunk + 1) & 1]);  // on its way while this one is added
-                    else {
+                    f8_read_wait<kStep>(raw);
+                    if (chunk + 1 == kChunks) {
                         // the accumulator is read: another block may fill it
                         tc_fence_before();
                         __syncwarp();
@@ -380,51 +442,47 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                                 asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
                         }
                     }
-                    uint32_t(&now)[32] = raw[chunk & 1];
                     unsigned long long *to = sums + chunk * kStep / 2;
-                    if (far) {  // the scales' product is far from one, or no float32: two factors
-                        const F8Tile<B_MN, BN, SWAP> tile(f, u, tile_m0);
-                        const int mine = SWAP ? group * kColumns + chunk * 32 + lane : 32 * quarter + lane;
-                        const float2 x = split_scale(tile.token(mine, kt)), y = split_scale(tile.of_weight(SWAP || BN != 256 ? 0 : group, kt));
-                        const float once = x.x * y.x, then = x.y * y.y;
-#pragma unroll
-                        for (int c = 0; c < kStep / 2; ++c) {
-                            const unsigned long long p = SWAP ? pair_of(__float_as_uint(__shfl_sync(~0u, once, 2 * c)), __float_as_uint(__shfl_sync(~0u, once, 2 * c + 1)))
-                                                              : pair_of(__float_as_uint(once), __float_as_uint(once));
-                            const unsigned long long q = SWAP ? pair_of(__float_as_uint(__shfl_sync(~0u, then, 2 * c)), __float_as_uint(__shfl_sync(~0u, then, 2 * c + 1)))
-                                                              : pair_of(__float_as_uint(then), __float_as_uint(then));
-                            to[c] = fma_pair(mul_pair(pair_of(now[2 * c], now[2 * c + 1]), p), q, to[c]);
-                        }
-                    } else if constexpr (SWAP) {
-                        const ulonglong2 *of_columns = reinterpret_cast<const ulonglong2 *>(&factors[slot][group * kColumns + chunk * kStep]);
+                    const float *then = of_lane + S::kFactors;
+                    if constexpr (SWAP) {
+                        const ulonglong2 *of_columns = reinterpret_cast<const ulonglong2 *>(of_lane + chunk * kStep);
 #pragma unroll
                         for (int c = 0; c < kStep / 4; ++c) {
                             const ulonglong2 four = of_columns[c];
-                            to[2 * c] = fma_pair(pair_of(now[4 * c], now[4 * c + 1]), four.x, to[2 * c]);
-                            to[2 * c + 1] = fma_pair(pair_of(now[4 * c + 2], now[4 * c + 3]), four.y, to[2 * c + 1]);
+                            unsigned long long x = pair_of(raw[4 * c], raw[4 * c + 1]), y = pair_of(raw[4 * c + 2], raw[4 * c + 3]);
+                            if (far) {
+                                const ulonglong2 more = reinterpret_cast<const ulonglong2 *>(then + chunk * kStep)[c];
+                                to[2 * c] = fma_pair(mul_pair(x, four.x), more.x, to[2 * c]);
+                                to[2 * c + 1] = fma_pair(mul_pair(y, four.y), more.y, to[2 * c + 1]);
+                            } else {
+                                to[2 * c] = fma_pair(x, four.x, to[2 * c]);
+                                to[2 * c + 1] = fma_pair(y, four.y, to[2 * c + 1]);
+                            }
                         }
+                    } else if (far) {
+                        const unsigned long long more = pair_of(__float_as_uint(*then), __float_as_uint(*then));
+#pragma unroll
+                        for (int c = 0; c < kStep / 2; ++c) to[c] = fma_pair(mul_pair(pair_of(raw[2 * c], raw[2 * c + 1]), both), more, to[c]);
                     } else {
 #pragma unroll
-                        for (int c = 0; c < kStep / 2; ++c) to[c] = fma_pair(pair_of(now[2 * c], now[2 * c + 1]), both, to[c]);
+                        for (int c = 0; c < kStep / 2; ++c) to[c] = fma_pair(pair_of(raw[2 * c], raw[2 * c + 1]), both, to[c]);
                     }
+                    if (chunk + 1 < kChunks) f8_read<kStep>(d + (chunk + 1) * kStep, raw);
                 }
-                __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&factor_empty[slot])) : "memory");
             }
             if (!ok) continue;
             if constexpr (S::kSplits) {
                 if (g.splits > 1) {  // the operands have been read: their shared memory takes the sums
-                    const int c_first = group * kColumns;
                     if constexpr (SWAP) {
 #pragma unroll
                         for (int c = 0; c < kColumns; ++c)
-                            if (n0 + c < g.n)
-                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(exchange_at<32>(smem, c_first + c, 8 * quarter + (lane >> 2)) + 4 * (lane & 3)),
+                            if (n0 + column(c) < g.n)
+                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(exchange_at<32>(smem, column(c), 8 * quarter + (lane >> 2)) + 4 * (lane & 3)),
                                              "f"(c & 1 ? floats_of(sums[c / 2]).y : floats_of(sums[c / 2]).x) : "memory");
                     } else {
 #pragma unroll
                         for (int j = 0; j < kColumns / 4; ++j)
-                            st_shared_16(exchange_at<BN / 4>(smem, 32 * quarter + lane, c_first / 4 + j),
+                            st_shared_16(exchange_at<BN / 4>(smem, 32 * quarter + lane, column(4 * j) / 4),
                                          make_uint4(__float_as_uint(floats_of(sums[2 * j]).x), __float_as_uint(floats_of(sums[2 * j]).y),
                                                     __float_as_uint(floats_of(sums[2 * j + 1]).x), __float_as_uint(floats_of(sums[2 * j + 1]).y)));
                     }
@@ -436,53 +494,50 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                 if (m < g.m) {
 #pragma unroll
                     for (int c = 0; c < kColumns; ++c)
-                        if (n0 + c < g.n) store_one(g.out, static_cast<long long>(n0 + c) * g.out_stride + m, (c & 1 ? floats_of(sums[c / 2]).y : floats_of(sums[c / 2]).x) + add,
-                                                   g.out_dtype);
+                        if (n0 + column(c) < g.n)
+                            store_one(g.out, static_cast<long long>(n0 + column(c)) * g.out_stride + m, (c & 1 ? floats_of(sums[c / 2]).y : floats_of(sums[c / 2]).x) + add,
+                                      g.out_dtype);
                 }
             } else {
+                unsigned char *row = static_cast<unsigned char *>(g.out) + static_cast<long long>(m) * g.out_stride * out_bytes;
 #pragma unroll
-                for (int c0 = 0; c0 < kColumns; c0 += 32) {
-                    if (n0 + c0 >= g.n) break;
-                    const uint32_t at = staging + lane * 128;
-                    const int half = out_bytes == 2 ? (c0 / 32) & 1 : 0;
-                    if (g.out_tma && half == 0) {
-                        // the box about to be written was handed to TMA a store ago
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        __syncwarp();
+                for (int c0 = 0; c0 < kColumns; c0 += 16) {
+                    const int at = column(c0);
+                    if (n0 + at >= g.n) break;
+                    if (g.bias) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) sums[c0 / 2 + c] = add_pair(sums[c0 / 2 + c], *reinterpret_cast<const unsigned long long *>(&bias[at + 2 * c]));
                     }
-                    float v[32];
+                    uint32_t v[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float2 two = floats_of(sums[(c0 + c) / 2]);
-                        v[c] = two.x + bias[group * kColumns + c0 + c];
-                        v[c + 1] = two.y + bias[group * kColumns + c0 + c + 1];
-                    }
-                    if (out_bytes == 4) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            st_shared_16(at + ((j ^ (lane & 7)) << 4), make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-                                                                                  __float_as_uint(v[4 * j + 3])));
-                        store_box(g, &c_map, at - lane * 128, m0, n0 + c0, 4);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = pack_out(v[8 * j + 2 * e], v[8 * j + 2 * e + 1], g.out_dtype);
-                            st_shared_16(at + (((4 * half + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                    for (int c = 0; c < 8; ++c) {
+                        const float2 two = floats_of(sums[c0 / 2 + c]);
+                        if (out_bytes == 4) {
+                            v[2 * c] = __float_as_uint(two.x);
+                            v[2 * c + 1] = __float_as_uint(two.y);
+                        } else {
+                            v[c] = pack_out(two.x, two.y, g.out_dtype);
                         }
-                        if (half == 1 || n0 + c0 + 32 >= g.n) store_box(g, &c_map, at - lane * 128, m0, n0 + (c0 & ~63), 2);
+                    }
+                    if (g.out_tma && n0 + at + 16 <= g.n) {  // rows start on 32 bytes: a lane writes its row
+                        if (m < g.m) {
+                            unsigned char *to = row + static_cast<long long>(n0 + at) * out_bytes;
+                            store_32(to, v);
+                            if (out_bytes == 4) store_32(to + 32, v + 8);
+                        }
+                    } else {
+                        copy_piece(g, staging, v, m0, n0 + at, out_bytes);
+                        if (out_bytes == 4 && n0 + at + 8 < g.n) copy_piece(g, staging, v + 8, m0, n0 + at + 8, 4);
                     }
                 }
             }
         }
-        if (!SWAP && g.out_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         if constexpr (S::kSplits) {
             if (g.splits > 1) {
                 // ---- a split tile: this CTA's part of it, from everybody's sums ----
                 __syncwarp();
                 cluster_sync_all();
-                if (!abort_flag) {
+                if (!abort_flag && threadIdx.x < 128 + kGemmThreads) {
                     const GemmUnit u = gemm_unit(g, first);
                     const float2 *none = nullptr;
                     const int thread = threadIdx.x - 128;
@@ -541,7 +596,7 @@ int launch_float8(const F8Product &p, int splits, cudaStream_t stream) {
         if (device < 64) ready |= 1ull << device;
     }
     const Operand &a = SWAP ? p.weight : p.tokens, &b = SWAP ? p.tokens : p.weight;
-    CUtensorMap a_map, b_map, c_map;
+    CUtensorMap a_map, b_map;
     if (!matrix_map(&a_map, a.base, p.k, a.rows, a.stride, 1, 128, kGemmRows) ||
         !(B_MN ? matrix_map(&b_map, b.base, b.rows, p.k, b.stride, 1, 128, 128) : matrix_map(&b_map, b.base, p.k, b.rows, b.stride, 1, 128, S::kBRows)))
         return fail(TH_ERR_ALIGNMENT, "8-bit product: operand rows must start on 16 bytes");
@@ -565,14 +620,12 @@ int launch_float8(const F8Product &p, int splits, cudaStream_t stream) {
     g.early = p.weights_settled;
     const int out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
     if (g.splits > (S::kSplits ? 8 / CG : 1)) return fail(TH_ERR_UNSUPPORTED, "8-bit product: %d parts", g.splits);
-    // a TMA store writes whole 16 bytes: rows that end inside of them are copied, so that what lies behind stays
-    g.out_tma = !SWAP && g.splits == 1 && static_cast<long long>(g.n) * out_bytes % 16 == 0 && matrix_map(&c_map, g.out, g.n, g.m, g.out_stride, out_bytes, 128 / out_bytes, 32);
-    if (!g.out_tma) c_map = a_map;  // not looked at
+    g.out_tma = aligned_to(g.out, 32) && g.out_stride * out_bytes % 32 == 0;  // here: rows start on 32 bytes
     const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "8-bit product: too many tiles");
     // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles
     const long long clusters = g.splits > 1 ? units : std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
-    return launch_chained("float8_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), kF8Threads, S::kBytes, stream, CG * g.splits, f, a_map, b_map, c_map);
+    return launch_chained("float8_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), S::kThreads, S::kBytes, stream, CG * g.splits, f, a_map, b_map);
 }
 
 }  // namespace

@@ -1,5 +1,6 @@
 // Linear layers on 8-bit floating-point blocks: the products are float8_gemm_kernel's; what is here chooses how they are cut.
 #include "float8_gemm.cuh"
+#include <cstdlib>
 
 namespace th {
 namespace {
@@ -38,6 +39,8 @@ F8Plan plan_float8(int m, int n, int k, bool b_mn) {
         consider(bn, 1, true, bn == 128 ? 1 : 2, 2.0 * (kGemmRows + bn), 1500 + 8 * bn);
         return best;
     }
+    static const int forced = getenv("TH_F8") ? atoi(getenv("TH_F8")) : 0;
+    if (forced) { consider(forced / 10, forced % 10, false, 1, 600, 9000); return best; }
     consider(256, 2, false, 1, 600, 9000);
     if (!b_mn) consider(128, 2, false, 1, 450, 4500);  // an MN-major weight comes 128 columns a CTA
     consider(128, 1, false, 1, 560, 4500);
@@ -58,6 +61,7 @@ int run_float8(const F8Product &p, cudaStream_t stream) {
         }
         if (plan.cg == 2 && plan.bn == 128) return launch_float8<false, 128, 2, false, 1>(p, plan.splits, stream);
     }
+    if (plan.cg == 1 && plan.bn == 256) return launch_float8<B_MN, 256, 1, false, 1>(p, plan.splits, stream);
     return plan.cg == 1 ? launch_float8<B_MN, 128, 1, false, 1>(p, plan.splits, stream) : launch_float8<B_MN, 256, 2, false, 1>(p, plan.splits, stream);
 }
 
