@@ -45,7 +45,7 @@ struct F8Shape {
     static constexpr int kStaging = SWAP ? 0 : kWarps * kF8Piece;
     static constexpr int kFactors = SWAP ? BN : kGemmRows * (BN == 256 ? 2 : 1);  // of a block: a token's for every row of weight blocks
     static constexpr int kFitAccs = 512 / CTAS / BN, kAccs = kFitAccs > 4 ? 4 : kFitAccs;  // accumulators in tensor memory's 512 columns
-    static constexpr int kSlots = 3 * kAccs;  // blocks whose factors are held
+    static constexpr int kSlots = 4 * kAccs;  // blocks whose factors are held
     static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - 2 * BN * 4 - kSlots * 2 * kFactors * 4;  // biases, factors and barriers are beside it
     static constexpr int kFit = (kSmem - kStaging - 1024) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
@@ -64,14 +64,39 @@ __host__ __device__ constexpr uint32_t instr_desc_e4m3(int m, int n, bool b_mn) 
     return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-template <int CG>
-__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A block's four MMAs, then the commits to its accumulator's and its stage's barriers, by the lane whose `issue` is not zero.  The instructions are
+// predicated and the warp stays together: behind a branch for one lane the four and their commits took longer (see the kernel).
+template <int CG, bool B_MN>
+__device__ __forceinline__ void f8_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t issue, uint32_t done_bar, uint32_t stage_bar, uint32_t leader) {
+    constexpr uint32_t kLeading = B_MN ? (128u * 128u >> 4) << 16 : 0u;  // an MN-major operand of 256 columns lies in two boxes of 128
+    constexpr uint32_t kStepB = B_MN ? 32 * 128 >> 4 : 2;
+    const uint32_t la = desc_low(a), lb = desc_low(b) | kLeading;
     if constexpr (CG == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b),
-                     "r"(idesc), "r"(accumulate) : "memory");
+        asm volatile(
+            "{\n\t.reg .pred p, t, f;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t"
+            "mov.b64 a0, {%1, %8};\n\tadd.s64 a1, a0, 2;\n\tadd.s64 a2, a0, 4;\n\tadd.s64 a3, a0, 6;\n\t"
+            "mov.b64 b0, {%2, %8};\n\tadd.s64 b1, b0, %7;\n\tadd.s64 b2, b1, %7;\n\tadd.s64 b3, b2, %7;\n\t"
+            "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a0, b0, %3, f;\n\t"
+            "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, t;\n\t"
+            "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, t;\n\t"
+            "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, t;\n\t"
+            "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"
+            "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}\n" ::"r"(d),
+            "r"(la), "r"(lb), "r"(idesc), "r"(issue), "r"(done_bar), "r"(stage_bar), "n"(kStepB), "r"(kDescHigh) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b),
-                     "r"(idesc), "r"(accumulate) : "memory");
+        asm volatile(
+            "{\n\t.reg .pred p, t, f;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t"
+            "mov.b64 a0, {%1, %8};\n\tadd.s64 a1, a0, 2;\n\tadd.s64 a2, a0, 4;\n\tadd.s64 a3, a0, 6;\n\t"
+            "mov.b64 b0, {%2, %8};\n\tadd.s64 b1, b0, %7;\n\tadd.s64 b2, b1, %7;\n\tadd.s64 b3, b2, %7;\n\t"
+            "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a0, b0, %3, f;\n\t"
+            "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a1, b1, %3, t;\n\t"
+            "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a2, b2, %3, t;\n\t"
+            "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a3, b3, %3, t;\n\t"
+            "@p tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %9;\n\t"
+            "@p tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], %9;\n\t}\n" ::"r"(d),
+            "r"(la), "r"(lb), "r"(idesc), "r"(issue), "r"(done_bar), "r"(stage_bar), "n"(kStepB), "r"(kDescHigh), "h"(static_cast<unsigned short>(3u << leader)) : "memory");
 }
 
 // The scales' product is one factor where it is between 2^-100 and 2^100.  Where it is not (it may be no float32 at all) a sum takes two factors
@@ -190,12 +215,6 @@ struct F8Tile {
     __device__ __forceinline__ float of_weight(int group, int kt) const { return weight[min(group, weights_end) * weight_row + kt * weight_block]; }
 };
 
-// An MN-major operand of 256 columns lies in two boxes of 128, whose distance is the descriptor's leading offset.
-template <bool MN>
-__device__ __forceinline__ uint64_t gemm_desc_b(uint32_t addr) {
-    return smem_desc(MN ? desc_low(addr) | ((128u * 128u >> 4) << 16) : desc_low(addr));
-}
-
 // SWAP: A is the weight, and the output is C transposed (A's rows are its columns).
 template <bool B_MN, int BN, int CG, bool SWAP, int CTAS>
 __global__ void __launch_bounds__(F8Shape<BN, CG, SWAP, CTAS>::kThreads, CTAS)
@@ -304,23 +323,19 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
         if (rank == 0) {
             int it = 0;
             bool ok = true;
-            constexpr uint32_t b_step = B_MN ? 32 * 128 : 32;
+            const uint32_t issue = elect_one() ? 1u : 0u;
+            __syncwarp();
             for (int unit = first; unit < units && ok; unit += step) {
                 const GemmUnit u = gemm_unit(g, unit);
                 for (int kt = u.k0; kt < u.k1 && ok; ++kt, ++it) {
                     const int s = it % S::kStages, buf = it % S::kAccs;
                     ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
                     if (!ok) break;
-                    const bool got = lane_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                    ok = gemm_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                    if (!ok) break;
                     tc_fence_after();
-                    if (elect_one() && got) {
-                        const uint32_t a = smem + s * S::kStage, b = a + S::kABytes, d = tmem + buf * BN;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) f8_mma<CG>(d, gemm_desc<false>(a + k * 32), gemm_desc_b<B_MN>(b + k * b_step), g.idesc, k > 0 ? 1u : 0u);
-                        gemm_commit<CG>(smem_addr(&acc_full[buf]), leader);
-                        gemm_commit<CG>(smem_addr(&empty[s]), leader);
-                    }
-                    ok = __all_sync(~0u, got);
+                    const uint32_t a = smem + s * S::kStage;
+                    f8_block<CG, B_MN>(tmem + buf * BN, a, a + S::kABytes, g.idesc, issue, smem_addr(&acc_full[buf]), smem_addr(&empty[s]), leader);
                 }
             }
         }
@@ -449,7 +464,7 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
 #pragma unroll
                         for (int c = 0; c < kStep / 4; ++c) {
                             const ulonglong2 four = of_columns[c];
-                            unsigned long long x = pair_of(raw[4 * c], raw[4 * c + 1]), y = pair_of(raw[4 * c + 2], raw[4 * c + 3]);
+                            const unsigned long long x = pair_of(raw[4 * c], raw[4 * c + 1]), y = pair_of(raw[4 * c + 2], raw[4 * c + 3]);
                             if (far) {
                                 const ulonglong2 more = reinterpret_cast<const ulonglong2 *>(then + chunk * kStep)[c];
                                 to[2 * c] = fma_pair(mul_pair(x, four.x), more.x, to[2 * c]);

@@ -1,6 +1,5 @@
 // Linear layers on 8-bit floating-point blocks: the products are float8_gemm_kernel's; what is here chooses how they are cut.
 #include "float8_gemm.cuh"
-#include <cstdlib>
 
 namespace th {
 namespace {
@@ -39,11 +38,9 @@ F8Plan plan_float8(int m, int n, int k, bool b_mn) {
         consider(bn, 1, true, bn == 128 ? 1 : 2, 2.0 * (kGemmRows + bn), 1500 + 8 * bn);
         return best;
     }
-    static const int forced = getenv("TH_F8") ? atoi(getenv("TH_F8")) : 0;
-    if (forced) { consider(forced / 10, forced % 10, false, 1, 600, 9000); return best; }
-    consider(256, 2, false, 1, 600, 9000);
-    if (!b_mn) consider(128, 2, false, 1, 450, 4500);  // an MN-major weight comes 128 columns a CTA
-    consider(128, 1, false, 1, 560, 4500);
+    consider(256, 2, false, 1, 1000, 9000);
+    if (!b_mn) consider(128, 2, false, 1, 800, 4500);  // an MN-major weight comes 128 columns a CTA
+    consider(128, 1, false, 1, 780, 4500);
     return best;
 }
 
@@ -61,7 +58,6 @@ int run_float8(const F8Product &p, cudaStream_t stream) {
         }
         if (plan.cg == 2 && plan.bn == 128) return launch_float8<false, 128, 2, false, 1>(p, plan.splits, stream);
     }
-    if (plan.cg == 1 && plan.bn == 256) return launch_float8<B_MN, 256, 1, false, 1>(p, plan.splits, stream);
     return plan.cg == 1 ? launch_float8<B_MN, 128, 1, false, 1>(p, plan.splits, stream) : launch_float8<B_MN, 256, 2, false, 1>(p, plan.splits, stream);
 }
 
