@@ -119,6 +119,7 @@ int check_int8(const void *weight, int64_t weight_stride, const float *weight_sc
 namespace th {
 int rows_status_word();  // rows.cu
 int float8_status_word();  // float8_linear.cu
+int expert_status_word();  // expert_linear.cu
 }
 
 using namespace th;
@@ -126,8 +127,8 @@ using namespace th;
 extern "C" int th_linear_tc_status(void) {
     int status = 0;
     if (cudaMemcpyFromSymbol(&status, g_tc_status, sizeof(int)) != cudaSuccess) return -1;
-    const int rows = rows_status_word(), blocks = float8_status_word();
-    return rows < 0 || blocks < 0 ? -1 : status | rows | blocks;
+    const int rows = rows_status_word(), blocks = float8_status_word(), experts = expert_status_word();
+    return rows < 0 || blocks < 0 || experts < 0 ? -1 : status | rows | blocks | experts;
 }
 
 static int int8_linear(const void *q_dev, int64_t q_stride, const float *scale_dev, const void *weight_dev, int64_t weight_stride, const float *weight_scale_dev,
