@@ -34,7 +34,9 @@ struct ExpertShape {
     static constexpr int kK = 64;
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
-    static constexpr int kFixed = SWAP ? 0 : 4 * kStagingBoxes * kStagingBytes;
+    static constexpr int kGroups = SWAP ? 1 : 2;  // of four warps that empty an accumulator, each its part of the columns
+    static constexpr int kThreads = 128 + 128 * kGroups, kColumns = BN / kGroups;
+    static constexpr int kFixed = SWAP ? 0 : 4 * kGroups * kPieceBytes;
     static constexpr int kTables = OVER_ROWS ? 4 * (kMostExperts + 1) : 8 * (kMostExperts + 1);
     static constexpr int kSmem = (CTAS == 1 ? 226 : 112) * 1024 - kTables;  // barriers are beside it
     static constexpr int kFit = (kSmem - kFixed - 1024) / kStage;
@@ -161,8 +163,8 @@ __device__ __forceinline__ ExpertTile expert_tile(const ExpertArgs &a, const int
 
 // SWAP: weights along the accumulator's lanes, rows along its columns; the output is C transposed
 template <bool A_MN, bool B_MN, int BN, int CG, bool SWAP, bool OVER_ROWS, int CTAS>
-__global__ void __launch_bounds__(kGemmThreads, CTAS)
-expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap c_map) {
+__global__ void __launch_bounds__(ExpertShape<A_MN, B_MN, BN, CG, SWAP, OVER_ROWS, CTAS>::kThreads, CTAS)
+expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map) {
     using S = ExpertShape<A_MN, B_MN, BN, CG, SWAP, OVER_ROWS, CTAS>;
     const GemmArgs &g = x.g;
     extern __shared__ unsigned char smem_raw[];
@@ -195,7 +197,7 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
         }
         for (int b = 0; b < 2; ++b) {
             init(&acc_full[b], 1);
-            init(&acc_empty[b], 4 * CG);
+            init(&acc_empty[b], 4 * S::kGroups * CG);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -324,27 +326,26 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                 if (!ok) break;
                 last_phase ^= 1u << s;
                 // boxes of 64 rows of 128 bytes; the swizzle stays within a row
-                constexpr int kBoxes = S::kStage / kBoxBytes;
-                const int chunks = (S::kK - rest) * 8;
-                for (int i = threadIdx.x - 64; i < kBoxes * chunks; i += 64) {
-                    const int box = i / chunks, c = i - box * chunks;
-                    st_shared_16(smem + s * S::kStage + box * kBoxBytes + rest * 128 + c * 16, make_uint4(0, 0, 0, 0));
-                }
-                asm volatile("fence.proxy.async;" ::: "memory");
+                const uint32_t at = smem + s * S::kStage + (threadIdx.x - 64) * 16;
+#pragma unroll
+                for (int box = 0; box < S::kStage / kBoxBytes; ++box)
+                    for (int r = rest - rest % 8; r < S::kK; r += 8)
+                        if (r + static_cast<int>(threadIdx.x - 64) / 8 >= rest) st_shared_16(at + box * kBoxBytes + r * 128, make_uint4(0, 0, 0, 0));
+                fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     const uint32_t bar = smem_addr(&last_ready[s]);
-                    if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, 0)) : "memory");
+                    if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, 0)) : "memory");
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
                 }
             }
         }
     } else {
         // ---- sums -> output ----
-        const int quarter = warp & 3;
-        const uint32_t staging = smem + S::kStages * S::kStage + quarter * kStagingBoxes * kStagingBytes;
-        constexpr int kStep = BN < 32 ? BN : 32;
-        int done = 0, box = 0;
+        const int quarter = warp & 3, group = (warp - 4) >> 2;
+        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kPieceBytes;
+        constexpr int kStep = S::kColumns < 32 ? S::kColumns : 32;
+        int done = 0;
         bool ok = true;
         for (int unit = start; unit < units && ok; unit += step) {
             const ExpertTile t = expert_tile<SWAP, OVER_ROWS>(x, firsts, tiles, unit);
@@ -359,13 +360,11 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
             // lanes and columns of this warp's part in the output, and where the output's rows end
             const int lane0 = SWAP ? t.tn * kGemmRows + 32 * quarter : (t.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter;
             const int row0 = OVER_ROWS ? t.expert * g.m + lane0 : t.first + lane0, rows_end = OVER_ROWS ? (t.expert + 1) * g.m : t.end;
-            const int column0 = SWAP ? t.first + t.tm * BN : t.tn * BN;
-            GemmArgs part = g;  // of the output's rows those up to the expert's end
-            part.m = rows_end;
-            part.out_tma = g.out_tma && row0 + 32 <= rows_end;
-            const uint32_t d = tmem + buf * BN + (static_cast<uint32_t>(32 * quarter) << 16);
+            const int column0 = SWAP ? t.first + t.tm * BN : t.tn * BN + group * S::kColumns;
+            unsigned short *row = static_cast<unsigned short *>(g.out) + static_cast<long long>(row0 + lane) * g.out_stride;
+            const uint32_t d = tmem + buf * BN + group * S::kColumns + (static_cast<uint32_t>(32 * quarter) << 16);
 #pragma unroll 1
-            for (int c0 = 0; c0 < BN; c0 += kStep) {
+            for (int c0 = 0; c0 < S::kColumns; c0 += kStep) {
                 uint32_t raw[32];
                 if (none) {
 #pragma unroll
@@ -374,13 +373,15 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                     if constexpr (kStep == 32) tmem_ld32(d + c0, raw);
                     else tmem_ld16(d + c0, raw);
                     tmem_ld_wait();
-                    if (c0 + kStep >= BN) {
+                    if (c0 + kStep >= S::kColumns) {
                         // the accumulator is read: the next tile but one may fill it
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
+                            // What is handed over lies in tensor memory, ordered by the fence above: a release to the cluster would also wait for the
+                            // results that are on their way to global memory
                             if constexpr (CG == 2)
-                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), 0)) : "memory");
+                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(smem_addr(&acc_empty[buf]), 0)) : "memory");
                             else
                                 asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
                         }
@@ -395,31 +396,23 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                                 store_one(g.out, static_cast<long long>(column0 + c0 + k) * g.out_stride + m, __uint_as_float(raw[k]), g.out_dtype);
                     }
                 } else {
-                    if (column0 + c0 >= g.n || row0 >= rows_end) continue;
-                    const uint32_t at = staging + (box % kStagingBoxes) * kStagingBytes + lane * 128;
-                    const int half = (c0 / 32) & 1;
-                    if (g.out_tma && half == 0) {
-                        // the box about to be written was handed to TMA kStagingBoxes stores ago
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingBoxes - 1) : "memory");
-                        __syncwarp();
-                    }
+                    const int at = column0 + c0;
+                    if (at >= g.n || row0 >= rows_end) continue;
+                    uint32_t v[16];
 #pragma unroll
-                    for (int j = 0; j < kStep / 8; ++j) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack_out(__uint_as_float(raw[8 * j + 2 * e]), __uint_as_float(raw[8 * j + 2 * e + 1]), g.out_dtype);
-                        st_shared_16(at + (((4 * half + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
-                    }
-                    if (half == 1 || column0 + c0 + 32 >= g.n) {
-                        store_box(part, &c_map, at - lane * 128, row0, column0 + (c0 & ~63), 2);
-                        // the wait for a box's memory counts groups: a copied one is an empty group
-                        if (g.out_tma && !part.out_tma && lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        ++box;
+                    for (int k = 0; k < 16; ++k) v[k] = pack_out(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]), g.out_dtype);
+                    if (g.out_tma && at + 32 <= g.n) {  // rows start on 32 bytes
+                        if (row0 + lane < rows_end) {
+                            store_32(reinterpret_cast<unsigned char *>(row + at), v);
+                            store_32(reinterpret_cast<unsigned char *>(row + at + 16), v + 8);
+                        }
+                    } else {
+                        copy_piece(g, staging, v, row0, rows_end, at, 2);
+                        if (at + 16 < g.n) copy_piece(g, staging, v + 8, row0, rows_end, at + 16, 2);
                     }
                 }
             }
         }
-        if (!SWAP && g.out_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         if constexpr (!OVER_ROWS) {
             // ---- rows behind the last expert: zeros, by all CTAs ----
             const int behind = firsts[x.experts], width = g.n;
@@ -428,7 +421,7 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
             const bool wide = g.out_tma || (stride % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0);
             const int per_row = wide ? width / 8 : width;
             const long long total = static_cast<long long>(x.rows - behind) * per_row;
-            for (long long i = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x - 128; i < total; i += static_cast<long long>(gridDim.x) * 128) {
+            for (long long i = static_cast<long long>(blockIdx.x) * (S::kThreads - 128) + threadIdx.x - 128; i < total; i += static_cast<long long>(gridDim.x) * (S::kThreads - 128)) {
                 const long long r = i / per_row;
                 const int c = static_cast<int>(i - r * per_row);
                 if (wide) *reinterpret_cast<uint4 *>(out + (behind + r) * stride + 8 * c) = make_uint4(0, 0, 0, 0);
@@ -488,7 +481,7 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
             return rc;
         if (device < 64) ready |= 1ull << device;
     }
-    CUtensorMap a_map, b_map, c_map;
+    CUtensorMap a_map, b_map;
     const auto operand = [](CUtensorMap *map, const ExpertOperand &o, bool mn, int box_rows) {
         return expert_map(map, o.base, o.inner, o.outer, o.stride, o.count, o.apart, mn ? 64 : box_rows);
     };
@@ -501,15 +494,13 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
     g.group = 16;  // 16 tile rows of 256 x 2048: 16 MB
     g.idesc = instr_desc(CG * kGemmRows, BN, bf16, A_MN, B_MN);
     const long long out_rows = OVER_ROWS ? static_cast<long long>(x.experts) * g.m : x.rows;
-    // a TMA store writes whole 16 bytes: rows that end inside of them are copied
-    g.out_tma = !SWAP && g.n % 8 == 0 && matrix_map(&c_map, g.out, g.n, out_rows, g.out_stride, 2, 64, 32);
-    if (!g.out_tma) c_map = a_map;  // not looked at
+    g.out_tma = aligned_to(g.out, 32) && g.out_stride % 16 == 0;  // here: rows start on 32 bytes
     // at most so many tiles: an expert's last one may be part of one
     const long long rows_of_tiles = OVER_ROWS ? static_cast<long long>(x.experts) * g.tiles_m : x.rows / x.tile_rows + std::min(x.experts, x.rows);
     const long long units = rows_of_tiles * g.tiles_n;
     if (units > 0x7fffffffll || out_rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "product of experts: too many tiles");
     const long long clusters = std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
-    return launch_chained("expert_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), kGemmThreads, S::kBytes, stream, CG, x, a_map, b_map, c_map);
+    return launch_chained("expert_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), S::kThreads, S::kBytes, stream, CG, x, a_map, b_map);
 }
 
 }  // namespace

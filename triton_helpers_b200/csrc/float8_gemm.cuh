@@ -22,7 +22,6 @@ namespace {
 
 constexpr int kF8Block = 128;
 constexpr int kF8Step = 16;        // columns of an accumulator that a warp reads at a time
-constexpr int kF8Piece = 32 * 32;  // bytes: 32 rows of 32 that a warp turns in shared memory where rows of the output do not start on 32 bytes
 constexpr int kF8Batch = 4;        // blocks whose scales a warp asks for at a time
 
 struct F8Scale {
@@ -42,7 +41,7 @@ struct F8Shape {
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
     static constexpr int kGroups = CTAS == 1 ? 4 : 2;  // of four warps that keep sums
     static constexpr int kWarps = 4 * kGroups, kThreads = 128 + 32 * kWarps;
-    static constexpr int kStaging = SWAP ? 0 : kWarps * kF8Piece;
+    static constexpr int kStaging = SWAP ? 0 : kWarps * kPieceBytes;
     static constexpr int kFactors = SWAP ? BN : kGemmRows * (BN == 256 ? 2 : 1);  // of a block: a token's for every row of weight blocks
     static constexpr int kFitAccs = 512 / CTAS / BN, kAccs = kFitAccs > 4 ? 4 : kFitAccs;  // accumulators in tensor memory's 512 columns
     static constexpr int kSlots = 4 * kAccs;  // blocks whose factors are held
@@ -156,38 +155,6 @@ __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, uns
     unsigned long long d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
-}
-
-__device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-                 "r"(v[7]) : "memory");
-}
-
-// 32 bytes of each of a warp's 32 rows -> rows m0.., columns c0.. of the output, through shared memory so that neighbouring lanes write
-// neighbouring elements
-__device__ __forceinline__ void copy_piece(const GemmArgs &g, uint32_t box, const uint32_t *v, int m0, int c0, int out_bytes) {
-    const int lane = threadIdx.x & 31, per_row = 32 / out_bytes, cols = min(per_row, g.n - c0), rows = min(32, g.m - m0);
-    __syncwarp();
-    const uint32_t at = box + lane * 32, turn = (lane >> 2) & 1;  // two lanes' halves change places, for the banks
-    st_shared_16(at + (turn << 4), make_uint4(v[0], v[1], v[2], v[3]));
-    st_shared_16(at + ((turn ^ 1) << 4), make_uint4(v[4], v[5], v[6], v[7]));
-    __syncwarp();
-    const int c = lane % per_row;
-    for (int r = lane / per_row; r < rows; r += 32 / per_row) {
-        const uint32_t from = box + r * 32 + ((c * out_bytes) ^ (((r >> 2) & 1) << 4));
-        const long long to = static_cast<long long>(m0 + r) * g.out_stride + c0 + c;
-        if (c < cols) {
-            if (out_bytes == 4) {
-                uint32_t x;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(from) : "memory");
-                static_cast<uint32_t *>(g.out)[to] = x;
-            } else {
-                unsigned short x;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from) : "memory");
-                static_cast<unsigned short *>(g.out)[to] = x;
-            }
-        }
-    }
 }
 
 // Where a tile's scales lie: the rows of tokens, and the block (or blocks) of weight rows beside them
@@ -411,7 +378,7 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSumRegs));
         constexpr int kColumns = S::kColumns, kStep = kColumns < kF8Step ? kColumns : kF8Step, kChunks = kColumns / kStep;
         const int quarter = warp & 3, group = (warp - 4) >> 2, out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
-        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kF8Piece;
+        const uint32_t staging = smem + S::kStages * S::kStage + (warp - 4) * kPieceBytes;
         int it = 0, done = 0;
         bool ok = true;
         const auto column = [&](int c) { return group * kColumns + c; };  // of the tile
@@ -541,8 +508,8 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                             if (out_bytes == 4) store_32(to + 32, v + 8);
                         }
                     } else {
-                        copy_piece(g, staging, v, m0, n0 + at, out_bytes);
-                        if (out_bytes == 4 && n0 + at + 8 < g.n) copy_piece(g, staging, v + 8, m0, n0 + at + 8, 4);
+                        copy_piece(g, staging, v, m0, g.m, n0 + at, out_bytes);
+                        if (out_bytes == 4 && n0 + at + 8 < g.n) copy_piece(g, staging, v + 8, m0, g.m, n0 + at + 8, 4);
                     }
                 }
             }

@@ -201,6 +201,41 @@ __device__ __forceinline__ void copy_rows(unsigned char *to, long long pitch, ui
     }
 }
 
+// Results straight from registers, a lane a row: 32 bytes at a time, which are whole sectors where rows start on them
+constexpr int kPieceBytes = 32 * 32;  // 32 rows of 32 bytes that a warp turns in shared memory where they do not
+
+__device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]) : "memory");
+}
+
+// 32 bytes of each of a warp's 32 rows -> rows m0.. below m_end, columns c0.. of the output, through shared memory so that neighbouring lanes write
+// neighbouring elements
+__device__ __forceinline__ void copy_piece(const GemmArgs &g, uint32_t box, const uint32_t *v, int m0, int m_end, int c0, int out_bytes) {
+    const int lane = threadIdx.x & 31, per_row = 32 / out_bytes, cols = min(per_row, g.n - c0), rows = min(32, m_end - m0);
+    __syncwarp();
+    const uint32_t at = box + lane * 32, turn = (lane >> 2) & 1;  // two lanes' halves change places, for the banks
+    st_shared_16(at + (turn << 4), make_uint4(v[0], v[1], v[2], v[3]));
+    st_shared_16(at + ((turn ^ 1) << 4), make_uint4(v[4], v[5], v[6], v[7]));
+    __syncwarp();
+    const int c = lane % per_row;
+    for (int r = lane / per_row; r < rows; r += 32 / per_row) {
+        const uint32_t from = box + r * 32 + ((c * out_bytes) ^ (((r >> 2) & 1) << 4));
+        const long long to = static_cast<long long>(m0 + r) * g.out_stride + c0 + c;
+        if (c < cols) {
+            if (out_bytes == 4) {
+                uint32_t x;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(from) : "memory");
+                static_cast<uint32_t *>(g.out)[to] = x;
+            } else {
+                unsigned short x;
+                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from) : "memory");
+                static_cast<unsigned short *>(g.out)[to] = x;
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *c_map, uint32_t box, int m0, int c0, int out_bytes) {
     if (g.out_tma) {
         fence_async_smem();
