@@ -36,40 +36,72 @@ __device__ __forceinline__ void four_floats(uint32_t q, float *v) {
     v[3] = b.y;
 }
 
-// Eight elements of a row, zeros behind its end.  WIDE: they start on 16 bytes.
+// Eight elements of a row as they lie in memory, zeros behind its end: 16-bit ones take half the registers that their values would.
+// WIDE: they start on 16 bytes.
+template <typename T>
+struct __align__(16) Eight {
+    T v[8];
+};
+
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T *from, int valid, float (&v)[8]) {
+__device__ __forceinline__ Eight<T> load8(const T *from, int valid) {
+    Eight<T> x;
     if (WIDE && valid >= 8) {
-        constexpr int N = 16 / static_cast<int>(sizeof(T));
-        struct __align__(16) Packet {
-            T v[N];
-        };
 #pragma unroll
-        for (int p = 0; p < 8 / N; ++p) {
-            const Packet in = reinterpret_cast<const Packet *>(from)[p];
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[p * N + e] = to_float<T>(in.v[e]);
-        }
+        for (unsigned p = 0; p < sizeof(x) / 16; ++p) reinterpret_cast<uint4 *>(&x)[p] = reinterpret_cast<const uint4 *>(from)[p];
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < valid ? to_float<T>(from[e]) : 0.f;
+        for (int e = 0; e < 8; ++e) x.v[e] = e < valid ? from[e] : from_float<T>(0.f);
+    }
+    return x;
+}
+
+// The largest magnitude of eight elements, as bits: float32's own, or two 16-bit ones that are compared side by side
+template <typename T>
+__device__ __forceinline__ uint32_t most_of(const Eight<T> &x) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(&x);
+        constexpr uint32_t kSigns = 0x7fff7fffu;
+        return __vmaxu2(__vmaxu2(w.x & kSigns, w.y & kSigns), __vmaxu2(w.z & kSigns, w.w & kSigns));
+    } else {
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude(x.v[e]));
+        return most;
     }
 }
-
-// What a block's largest magnitude makes of it: the factor that its values take, and the scale; zeros and a NaN where it is not finite
-__device__ __forceinline__ float2 block_scale(uint32_t most) {
-    if (most >= 0x7f800000u) return make_float2(0.f, __uint_as_float(0x7fc00000u));
-    const float a = fmaxf(__uint_as_float(most), kLeast);
-    return make_float2(__fdiv_rn(kTop, a), __fdiv_rn(a, kTop));
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 2) return __vmaxu2(a, b);
+    else return max(a, b);
+}
+// The same as the bits of a float32
+template <typename T>
+__device__ __forceinline__ uint32_t as_float_bits(uint32_t most) {
+    if constexpr (sizeof(T) == 4) return most;
+    const unsigned short one = static_cast<unsigned short>(max(most & 0xffffu, most >> 16));
+    return __float_as_uint(to_float<T>(*reinterpret_cast<const T *>(&one)));
 }
 
-__device__ __forceinline__ void store8(unsigned char *to, int valid, const float (&v)[8], float2 s) {
-    const bool finite = s.x != 0.f;
+// What a block's largest magnitude makes of it, in one division: for even lanes the factor that the block's values take (zero where it is not finite),
+// for odd ones its scale (then a NaN)
+__device__ __forceinline__ float block_part(uint32_t most) {
+    const bool odd = threadIdx.x & 1;
+    const float a = fmaxf(__uint_as_float(most), kLeast), part = __fdiv_rn(odd ? a : kTop, odd ? kTop : a);
+    return most < 0x7f800000u ? part : odd ? __uint_as_float(0x7fc00000u) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(unsigned char *to, int valid, const Eight<T> &from, float factor) {
+    const bool finite = factor != 0.f;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_float<T>(from.v[e]);
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const float *x = v + 4 * h;
-        w[h] = finite ? four_e4m3(__fmul_rn(x[0], s.x), __fmul_rn(x[1], s.x), __fmul_rn(x[2], s.x), __fmul_rn(x[3], s.x)) : 0u;
+        w[h] = finite ? four_e4m3(__fmul_rn(x[0], factor), __fmul_rn(x[1], factor), __fmul_rn(x[2], factor), __fmul_rn(x[3], factor)) : 0u;
     }
     if (valid >= 8) {
         *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
@@ -91,68 +123,94 @@ struct QuantArgs {
     int d, blocks;
 };
 
-// A CTA takes 16 rows x kAhead column blocks: kAhead loads of each thread are on their way together, and the scales of neighbouring rows,
-// which lie side by side, leave together.
+// A tile is 16 rows x kAhead column blocks: kAhead loads of each thread are on their way together, those of a CTA's next tile while it works on this one,
+// and the scales of neighbouring rows, which lie side by side, leave together.  8192 x 4096 bfloat16: with a tile a CTA 30 us.
 constexpr int kAhead = 4;
 
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kQuantThreads) float8_rows_kernel(const QuantArgs a) {
-    after_previous();
-    const int part = threadIdx.x & 15;
-    const long long row = static_cast<long long>(blockIdx.y) * 16 + (threadIdx.x >> 4);
-    if (row >= a.rows) return;  // both halves of a warp work on their own
-    const unsigned mask = 0xffffu << (threadIdx.x & 16);
+__device__ __forceinline__ void load_tile(const QuantArgs &a, int tile, int columns, Eight<T> (&v)[kAhead]) {
+    const int group = tile / columns, first = (tile - group * columns) * kAhead * kBlock + 8 * (threadIdx.x & 15);
+    const long long row = static_cast<long long>(group) * 16 + (threadIdx.x >> 4);
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    float v[kAhead][8];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = load8<T, WIDE>(x + first + i * kBlock, row < a.rows ? a.d - first - i * kBlock : 0);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_tile(const QuantArgs &a, int tile, int columns, const Eight<T> (&v)[kAhead]) {
+    const int group = tile / columns, first = (tile - group * columns) * kAhead, part = threadIdx.x & 15;
+    const long long row = static_cast<long long>(group) * 16 + (threadIdx.x >> 4);
+    const unsigned mask = 0xffffu << (threadIdx.x & 16);  // half a warp
+    // Four blocks' largest magnitudes at once: lanes hand each other the blocks that the other side goes on with, until four of them have one
+    // block to themselves; so the four blocks take one division, with five exchanges for 16 (8192 x 4096 bfloat16: 27.5 us block by block).
+    static_assert(kAhead == 4, "four blocks to sixteen lanes");
+    const bool high = part & 8, upper = part & 4;
+    uint32_t most[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) most[i] = most_of(v[i]);
+    const uint32_t first_two = larger<T>(high ? most[2] : most[0], __shfl_xor_sync(mask, high ? most[0] : most[2], 8));
+    const uint32_t last_two = larger<T>(high ? most[3] : most[1], __shfl_xor_sync(mask, high ? most[1] : most[3], 8));
+    uint32_t mine = larger<T>(upper ? last_two : first_two, __shfl_xor_sync(mask, upper ? first_two : last_two, 4));
+    mine = larger<T>(mine, __shfl_xor_sync(mask, mine, 2));
+    mine = larger<T>(mine, __shfl_xor_sync(mask, mine, 1));
+    const float part_of = block_part(as_float_bits<T>(mine));
+    const int b_mine = first + (part >> 2);
+    if ((part & 3) == 1 && b_mine < a.blocks && row < a.rows) a.scale[b_mine * a.scale_block + row] = part_of;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-        const int c = (blockIdx.x * kAhead + i) * kBlock + 8 * part;
-        load8<T, WIDE>(x + c, a.d - c, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        const int b = blockIdx.x * kAhead + i, c = b * kBlock + 8 * part;
-        uint32_t most = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[i][e]));
-        most = __reduce_max_sync(mask, most);
-        if (b >= a.blocks) break;
-        const float2 s = block_scale(most);
-        if (part == 0) a.scale[b * a.scale_block + row] = s.y;
-        if (c < a.d) store8(a.q + row * a.q_stride + c, a.d - c, v[i], s);
+        const float factor = __shfl_sync(mask, part_of, 4 * i, 16);
+        const int c = (first + i) * kBlock + 8 * part;
+        if (c < a.d && row < a.rows) store8(a.q + row * a.q_stride + c, a.d - c, v[i], factor);
     }
 }
 
-// A CTA takes a block of 128 x 128: eight rows of each thread in registers
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kQuantThreads) float8_weight_kernel(const QuantArgs a) {
-    __shared__ uint32_t warps[kQuantThreads / 32];
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) float8_rows_kernel(const QuantArgs a, int tiles, int columns) {
     after_previous();
+    int tile = blockIdx.x;
+    Eight<T> v[kAhead], next[kAhead];
+    load_tile<T, WIDE>(a, tile, columns, v);
+    while (true) {
+        const int then = tile + gridDim.x;
+        if (then < tiles) load_tile<T, WIDE>(a, then, columns, next);
+        finish_tile(a, tile, columns, v);
+        if (then >= tiles) break;
+        tile = then;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) v[i] = next[i];
+    }
+}
+
+// A CTA takes a block of 128 x 128: four rows of each thread in registers
+constexpr int kWeightThreads = 512;
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 2 ? 3 : 2) float8_weight_kernel(const QuantArgs a) {
+    __shared__ uint32_t warps[kWeightThreads / 32];
+    after_previous();
+    constexpr int kRows = kBlock * 16 / kWeightThreads;
     const int c = blockIdx.x * kBlock + 8 * (threadIdx.x & 15), r0 = threadIdx.x >> 4;
     const long long first = static_cast<long long>(blockIdx.y) * kBlock;
-    float v[8][8];
+    Eight<T> v[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long row = first + r0 + 16 * i;
-        load8<T, WIDE>(static_cast<const T *>(a.x) + row * a.x_stride + c, row < a.rows ? a.d - c : 0, v[i]);
+    for (int i = 0; i < kRows; ++i) {
+        const long long row = first + r0 + kWeightThreads / 16 * i;
+        v[i] = load8<T, WIDE>(static_cast<const T *>(a.x) + row * a.x_stride + c, row < a.rows ? a.d - c : 0);
     }
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[i][e]));
-    most = __reduce_max_sync(~0u, most);
+    for (int i = 0; i < kRows; ++i) most = larger<T>(most, most_of(v[i]));
+    most = __reduce_max_sync(~0u, as_float_bits<T>(most));
     if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = most;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kQuantThreads / 32; ++w) most = max(most, warps[w]);
-    const float2 s = block_scale(most);
-    if (threadIdx.x == 0) a.scale[static_cast<long long>(blockIdx.y) * a.blocks + blockIdx.x] = s.y;
+    most = __reduce_max_sync(~0u, warps[threadIdx.x & (kWeightThreads / 32 - 1)]);
+    const float part = block_part(most), factor = __shfl_sync(~0u, part, 0);
+    if (threadIdx.x == 1) a.scale[static_cast<long long>(blockIdx.y) * a.blocks + blockIdx.x] = part;
     if (c >= a.d) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long row = first + r0 + 16 * i;
-        if (row < a.rows) store8(a.q + row * a.q_stride + c, a.d - c, v[i], s);
+    for (int i = 0; i < kRows; ++i) {
+        const long long row = first + r0 + kWeightThreads / 16 * i;
+        if (row < a.rows) store8(a.q + row * a.q_stride + c, a.d - c, v[i], factor);
     }
 }
 
@@ -245,24 +303,15 @@ extern "C" int th_float8_rows(const void *x_dev, int64_t x_stride, void *q_dev, 
     if (int rc = check_blocks("th_float8_rows", x_dev, x_stride, 0, q_dev, q_stride, scale_dev, rows, d, dtype)) return rc;
     if (rows == 0) return TH_OK;
     if (scale_block < rows) return fail(TH_ERR_BAD_ARG, "th_float8_rows: short stride of the scales");
-    QuantArgs a{x_dev, x_stride, static_cast<unsigned char *>(q_dev), q_stride, scale_dev, scale_block, rows, d, (d + kBlock - 1) / kBlock};
-    const unsigned columns = static_cast<unsigned>((a.blocks + kAhead - 1) / kAhead);
-    // a grid's second axis ends at 65535: rows beyond come in further launches
-    constexpr int64_t kMost = 65535ll * 16;
-    for (int64_t first = 0; first < rows; first += kMost) {
-        QuantArgs part = a;
-        part.x = static_cast<const char *>(x_dev) + first * x_stride * static_cast<int64_t>(dtype_bytes(dtype));
-        part.q += first * q_stride;
-        part.scale += first;
-        part.rows = std::min(kMost, rows - first);
-        const dim3 grid(columns, static_cast<unsigned>((part.rows + 15) / 16));
-        const int rc = with_type(dtype, wide_rows(x_dev, x_stride, dtype), [&](auto t, auto wide) {
-            return launch_chained("float8_rows_kernel launch", float8_rows_kernel<decltype(t), decltype(wide)::value>, grid, kQuantThreads, 0,
-                                  static_cast<cudaStream_t>(stream), 1, part);
-        });
-        if (rc) return rc;
-    }
-    return TH_OK;
+    const QuantArgs a{x_dev, x_stride, static_cast<unsigned char *>(q_dev), q_stride, scale_dev, scale_block, rows, d, (d + kBlock - 1) / kBlock};
+    const int columns = (a.blocks + kAhead - 1) / kAhead;
+    const int64_t tiles = (rows + 15) / 16 * columns;
+    if (tiles > 0x7fffffff - 0x10000) return fail(TH_ERR_UNSUPPORTED, "th_float8_rows: %lld rows of %d", static_cast<long long>(rows), d);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, static_cast<int64_t>(sm_count()) * (dtype == TH_F32 ? 3 : 4)));
+    return with_type(dtype, wide_rows(x_dev, x_stride, dtype), [&](auto t, auto wide) {
+        return launch_chained("float8_rows_kernel launch", float8_rows_kernel<decltype(t), decltype(wide)::value>, grid, kQuantThreads, 0,
+                              static_cast<cudaStream_t>(stream), 1, a, static_cast<int>(tiles), columns);
+    });
 }
 
 extern "C" int th_float8_weight(const void *w_dev, int64_t w_stride, void *q_dev, int64_t q_stride, float *scale_dev, int64_t rows, int d, int dtype,
@@ -273,7 +322,7 @@ extern "C" int th_float8_weight(const void *w_dev, int64_t w_stride, void *q_dev
     const QuantArgs a{w_dev, w_stride, static_cast<unsigned char *>(q_dev), q_stride, scale_dev, 0, rows, d, (d + kBlock - 1) / kBlock};
     const dim3 grid(static_cast<unsigned>(a.blocks), static_cast<unsigned>((rows + kBlock - 1) / kBlock));
     return with_type(dtype, wide_rows(w_dev, w_stride, dtype), [&](auto t, auto wide) {
-        return launch_chained("float8_weight_kernel launch", float8_weight_kernel<decltype(t), decltype(wide)::value>, grid, kQuantThreads, 0,
+        return launch_chained("float8_weight_kernel launch", float8_weight_kernel<decltype(t), decltype(wide)::value>, grid, kWeightThreads, 0,
                               static_cast<cudaStream_t>(stream), 1, a);
     });
 }
