@@ -401,10 +401,10 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                     uint32_t v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = pack_out(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]), g.out_dtype);
-                    if (g.out_tma && at + 32 <= g.n) {  // rows start on 32 bytes
+                    if (g.out_tma && at + 32 <= g.n) {
                         if (row0 + lane < rows_end) {
-                            store_32(reinterpret_cast<unsigned char *>(row + at), v);
-                            store_32(reinterpret_cast<unsigned char *>(row + at + 16), v + 8);
+                            store_32(reinterpret_cast<unsigned char *>(row + at), v, g.out_tma);
+                            store_32(reinterpret_cast<unsigned char *>(row + at + 16), v + 8, g.out_tma);
                         }
                     } else {
                         copy_piece(g, staging, v, row0, rows_end, at, 2);
@@ -418,7 +418,7 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
             const int behind = firsts[x.experts], width = g.n;
             const long long stride = g.out_stride;
             unsigned short *out = static_cast<unsigned short *>(g.out);
-            const bool wide = g.out_tma || (stride % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0);
+            const bool wide = g.out_tma && width % 8 == 0;
             const int per_row = wide ? width / 8 : width;
             const long long total = static_cast<long long>(x.rows - behind) * per_row;
             for (long long i = static_cast<long long>(blockIdx.x) * (S::kThreads - 128) + threadIdx.x - 128; i < total; i += static_cast<long long>(gridDim.x) * (S::kThreads - 128)) {
@@ -494,7 +494,7 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
     g.group = 16;  // 16 tile rows of 256 x 2048: 16 MB
     g.idesc = instr_desc(CG * kGemmRows, BN, bf16, A_MN, B_MN);
     const long long out_rows = OVER_ROWS ? static_cast<long long>(x.experts) * g.m : x.rows;
-    g.out_tma = aligned_to(g.out, 32) && g.out_stride % 16 == 0;  // here: rows start on 32 bytes
+    g.out_tma = rows_start_on(g.out, g.out_stride, 2);
     // at most so many tiles: an expert's last one may be part of one
     const long long rows_of_tiles = OVER_ROWS ? static_cast<long long>(x.experts) * g.tiles_m : x.rows / x.tile_rows + std::min(x.experts, x.rows);
     const long long units = rows_of_tiles * g.tiles_n;

@@ -501,11 +501,11 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                             v[c] = pack_out(two.x, two.y, g.out_dtype);
                         }
                     }
-                    if (g.out_tma && n0 + at + 16 <= g.n) {  // rows start on 32 bytes: a lane writes its row
+                    if (g.out_tma && n0 + at + 16 <= g.n) {  // a lane writes its row
                         if (m < g.m) {
                             unsigned char *to = row + static_cast<long long>(n0 + at) * out_bytes;
-                            store_32(to, v);
-                            if (out_bytes == 4) store_32(to + 32, v + 8);
+                            store_32(to, v, g.out_tma);
+                            if (out_bytes == 4) store_32(to + 32, v + 8, g.out_tma);
                         }
                     } else {
                         copy_piece(g, staging, v, m0, g.m, n0 + at, out_bytes);
@@ -602,7 +602,7 @@ int launch_float8(const F8Product &p, int splits, cudaStream_t stream) {
     g.early = p.weights_settled;
     const int out_bytes = g.out_dtype == TH_F32 ? 4 : 2;
     if (g.splits > (S::kSplits ? 8 / CG : 1)) return fail(TH_ERR_UNSUPPORTED, "8-bit product: %d parts", g.splits);
-    g.out_tma = aligned_to(g.out, 32) && g.out_stride * out_bytes % 32 == 0;  // here: rows start on 32 bytes
+    g.out_tma = rows_start_on(g.out, g.out_stride, out_bytes);
     const long long units = static_cast<long long>(g.tiles_m) * g.tiles_n * g.splits;
     if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "8-bit product: too many tiles");
     // a split tile is one unit of every CTA of its cluster; otherwise CTAs go round the tiles

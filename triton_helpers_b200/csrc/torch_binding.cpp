@@ -1987,90 +1987,104 @@ bool take_floats(PyObject *o, size_t n, std::vector<float> &out) {
     return true;
 }
 
+// A list of contiguous tensors on one device as the entry points take it.  Only addresses are kept, and the interpreter's lock while they are used: a list
+// of some hundred tensors costs a microsecond for each ten.
+struct TensorList {
+    std::vector<void *> pointers;
+    std::vector<int64_t> sizes;
+    std::vector<int> codes;
+    c10::Device device{at::kCPU};
+
+    bool read(PyObject *o, std::vector<const Tensor *> *keep = nullptr) {
+        if (!PyTuple_Check(o) && !PyList_Check(o)) return false;
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+        if (n == 0) return false;
+        pointers.reserve(n);
+        sizes.reserve(n);
+        codes.reserve(n);
+        for (Py_ssize_t k = 0; k < n; ++k) {
+            PyObject *item = PySequence_Fast_GET_ITEM(o, k);
+            if (!THPVariable_CheckExact(item)) return false;
+            const Tensor &t = THPVariable_Unpack(item);
+            if (!plain(t) || !t.is_contiguous()) return false;
+            if (k == 0) device = t.device();
+            else if (t.device() != device) return false;
+            const int code = dtype_code(t.scalar_type());
+            if (code < 0) return false;
+            pointers.push_back(t.data_ptr());
+            sizes.push_back(t.numel());
+            codes.push_back(code);
+            if (keep) keep->push_back(&t);
+        }
+        return true;
+    }
+    int count() const { return static_cast<int>(pointers.size()); }
+};
+
+// The float32 pair (norm, factor) of a list of gradients
+Tensor norm_factor(const TensorList &grads, const std::vector<float> &scales, double max_norm) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor pair = empty_like_shape({2}, at::kFloat, grads.device);
+    const int64_t bytes = th_grad_norm_workspace_bytes(grads.count(), grads.sizes.data());
+    const Tensor buffer = bytes ? empty_like_shape({bytes}, at::kByte, grads.device) : Tensor();
+    check(th_grad_norm(grads.count(), grads.pointers.data(), grads.sizes.data(), grads.codes.data(), scales.empty() ? nullptr : scales.data(),
+                       static_cast<float>(max_norm), pair.data_ptr<float>(), ptr(buffer), bytes, current_stream()),
+          "th_grad_norm");
+    return pair;
+}
+
 // grad_norm(tensors, scales or None, max_norm) -> the float32 pair (norm, factor)
 PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
-    std::vector<Tensor> grads;
+    TensorList grads;
     std::vector<float> scales;
     double max_norm;
-    if (n_args != 3 || !usual_mode() || !take_list(args[0], grads) || !take(args[2], max_norm)) TH_NOT_MINE;
-    const size_t n = grads.size();
-    if (n == 0 || (args[1] != Py_None && !take_floats(args[1], n, scales))) TH_NOT_MINE;
-    std::vector<const void *> pointers(n);
-    std::vector<int64_t> sizes(n);
-    std::vector<int> codes(n);
-    for (size_t k = 0; k < n; ++k) {
-        const Tensor &t = grads[k];
-        if (!plain(t) || !t.is_contiguous() || t.device() != grads[0].device() || dtype_code(t.scalar_type()) < 0) TH_NOT_MINE;
-        pointers[k] = ptr(t);
-        sizes[k] = t.numel();
-        codes[k] = dtype_code(t.scalar_type());
-    }
-    Tensor pair;
-    {
-        NoGil release;
-        at::AutoDispatchBelowADInplaceOrView below;
-        c10::cuda::CUDAGuard guard(grads[0].device());
-        pair = empty_like_shape({2}, at::kFloat, grads[0].device());
-        const int64_t bytes = th_grad_norm_workspace_bytes(static_cast<int>(n), sizes.data());
-        const Tensor buffer = bytes ? empty_like_shape({bytes}, at::kByte, grads[0].device()) : Tensor();
-        check(th_grad_norm(static_cast<int>(n), pointers.data(), sizes.data(), codes.data(), scales.empty() ? nullptr : scales.data(), static_cast<float>(max_norm),
-                           pair.data_ptr<float>(), ptr(buffer), bytes, current_stream()),
-              "th_grad_norm");
-    }
-    return THPVariable_Wrap(std::move(pair));
+    if (n_args != 3 || !usual_mode() || !grads.read(args[0]) || !take(args[2], max_norm)) TH_NOT_MINE;
+    if (args[1] != Py_None && !take_floats(args[1], grads.pointers.size(), scales)) TH_NOT_MINE;
+    c10::cuda::CUDAGuard guard(grads.device);
+    return THPVariable_Wrap(norm_factor(grads, scales, max_norm));
     END_HANDLE_TH_ERRORS
 }
 
-// adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grad, pair, lr, beta1, beta2, eps, step, skipped): the update of
-// tensors of one dtype on one device, gradients times their scale times the pair's factor
+// adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales or None, zero_grad or None, pair or None, max_norm, lr, beta1, beta2, eps, step,
+// skipped): the update of tensors of one dtype on one device, gradients times their scale times the pair's factor; without a pair that of these
+// gradients and max_norm.  Returns the pair.
 PyObject *py_adam_clipped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
-    std::vector<Tensor> params, grads, m, v;
+    TensorList p, g, m, v;
+    std::vector<const Tensor *> params;
     std::vector<float> scales;
-    double lr, beta1, beta2, eps;
+    double max_norm, lr, beta1, beta2, eps;
     int64_t step;
     Tensor pair, skipped;
-    if (n_args != 13 || g_deferred.load(std::memory_order_relaxed) || !take_list(args[0], params) || !take_list(args[1], grads) || !take_list(args[2], m) ||
-        !take_list(args[3], v) || !take(args[6], pair) || !take(args[7], lr) || !take(args[8], beta1) || !take(args[9], beta2) || !take(args[10], eps) ||
-        !take(args[11], step) || !take(args[12], skipped))
+    if (n_args != 14 || !usual_mode() || !p.read(args[0], &params) || !g.read(args[1]) || !m.read(args[2]) || !v.read(args[3]) || !take(args[6], pair) ||
+        !take(args[7], max_norm) || !take(args[8], lr) || !take(args[9], beta1) || !take(args[10], beta2) || !take(args[11], eps) || !take(args[12], step) ||
+        !take(args[13], skipped))
         TH_NOT_MINE;
     const size_t n = params.size();
-    if (n == 0 || grads.size() != n || m.size() != n || v.size() != n || !take_floats(args[4], n, scales) || !PyTuple_Check(args[5]) ||
-        PyTuple_GET_SIZE(args[5]) != static_cast<Py_ssize_t>(n))
-        TH_NOT_MINE;
-    if (!plain(pair) || pair.scalar_type() != at::kFloat || pair.numel() != 2 || !pair.is_contiguous()) TH_NOT_MINE;
-    if (skipped.defined() && (!plain(skipped) || skipped.scalar_type() != at::kInt || skipped.device() != params[0].device())) TH_NOT_MINE;
-    std::vector<int> zero(n);
-    std::vector<void *> pp(n), gp(n);
-    std::vector<float *> mp(n), vp(n);
-    std::vector<int64_t> sizes(n);
-    for (size_t k = 0; k < n; ++k) {
-        zero[k] = PyObject_IsTrue(PyTuple_GET_ITEM(args[5], k)) == 1;
-        for (const Tensor *t : {&params[k], &grads[k], &m[k], &v[k]})
-            if (!plain(*t) || !t->is_contiguous() || t->device() != pair.device() || t->numel() != params[k].numel()) TH_NOT_MINE;
-        if (params[k].scalar_type() != params[0].scalar_type() || grads[k].scalar_type() != params[0].scalar_type() || m[k].scalar_type() != at::kFloat ||
-            v[k].scalar_type() != at::kFloat)
-            TH_NOT_MINE;
-        pp[k] = ptr(params[k]);
-        gp[k] = ptr(grads[k]);
-        mp[k] = m[k].data_ptr<float>();
-        vp[k] = v[k].data_ptr<float>();
-        sizes[k] = params[k].numel();
+    if (g.device != p.device || m.device != p.device || v.device != p.device || g.sizes != p.sizes || m.sizes != p.sizes || v.sizes != p.sizes) TH_NOT_MINE;
+    if (args[4] != Py_None && !take_floats(args[4], n, scales)) TH_NOT_MINE;
+    std::vector<int> zero(n, 0);
+    if (args[5] != Py_None) {
+        if (!PyTuple_Check(args[5]) || PyTuple_GET_SIZE(args[5]) != static_cast<Py_ssize_t>(n)) TH_NOT_MINE;
+        for (size_t k = 0; k < n; ++k) zero[k] = PyObject_IsTrue(PyTuple_GET_ITEM(args[5], k)) == 1;
     }
-    const int code = dtype_code(params[0].scalar_type());
-    if (code < 0) TH_NOT_MINE;
-    {
-        NoGil release;
-        c10::cuda::CUDAGuard guard(params[0].device());
-        check(th_adam_clipped(static_cast<int>(n), pp.data(), gp.data(), mp.data(), vp.data(), sizes.data(), scales.data(), zero.data(), pair.data_ptr<float>(),
-                              static_cast<float>(lr), static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(eps), static_cast<int>(step), code,
-                              skipped.defined() ? skipped.data_ptr<int>() : nullptr, current_stream()),
-              "th_adam_clipped");
-    }
+    if (pair.defined() && (!plain(pair) || pair.scalar_type() != at::kFloat || pair.numel() != 2 || !pair.is_contiguous() || pair.device() != p.device)) TH_NOT_MINE;
+    if (skipped.defined() && (!plain(skipped) || skipped.scalar_type() != at::kInt || skipped.device() != p.device)) TH_NOT_MINE;
+    const int code = p.codes[0];
+    for (size_t k = 0; k < n; ++k)
+        if (p.codes[k] != code || g.codes[k] != code || m.codes[k] != TH_F32 || v.codes[k] != TH_F32) TH_NOT_MINE;
+    c10::cuda::CUDAGuard guard(p.device);
+    if (!pair.defined()) pair = norm_factor(g, scales, max_norm);
+    if (scales.empty()) scales.assign(n, 1.f);
+    check(th_adam_clipped(static_cast<int>(n), p.pointers.data(), g.pointers.data(), reinterpret_cast<float *const *>(m.pointers.data()),
+                          reinterpret_cast<float *const *>(v.pointers.data()), p.sizes.data(), scales.data(), zero.data(), pair.data_ptr<float>(), static_cast<float>(lr),
+                          static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(eps), static_cast<int>(step), code,
+                          skipped.defined() ? skipped.data_ptr<int>() : nullptr, current_stream()),
+          "th_adam_clipped");
     // in-place updates that autograd has to know of
-    for (const Tensor &t : params) t.unsafeGetTensorImpl()->bump_version();
-    Py_RETURN_TRUE;
+    for (const Tensor *t : params) t->unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(pair);
     END_HANDLE_TH_ERRORS
 }
 

@@ -35,7 +35,7 @@ struct GemmArgs {
     void *out;             // [m][out_stride], or [n][out_stride] where the product is transposed
     long long out_stride;
     int out_dtype;
-    int out_tma;
+    int out_tma;           // results leave by TMA (kernels that write rows from registers: what rows start on)
     int early;             // A was complete before the kernel ahead passed its wait: its first stages are fetched while that one runs
     const float *lane_scale, *column_scale;  // along m and along n (8 bits)
     const void *bias;      // along n (along m where transposed)
@@ -204,9 +204,15 @@ __device__ __forceinline__ void copy_rows(unsigned char *to, long long pitch, ui
 // Results straight from registers, a lane a row: 32 bytes at a time, which are whole sectors where rows start on them
 constexpr int kPieceBytes = 32 * 32;  // 32 rows of 32 bytes that a warp turns in shared memory where they do not
 
-__device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-                 "r"(v[7]) : "memory");
+// aligned: 32 where rows start on 32 bytes, 16 where they start on 16
+__device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v, int aligned) {
+    if (aligned == 32) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                     "r"(v[7]) : "memory");
+    } else {
+        reinterpret_cast<uint4 *>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<uint4 *>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
 }
 
 // 32 bytes of each of a warp's 32 rows -> rows m0.. below m_end, columns c0.. of the output, through shared memory so that neighbouring lanes write
@@ -633,6 +639,13 @@ bool matrix_map(CUtensorMap *map, const void *base, long long inner, long long o
                                                        : CU_TENSOR_MAP_DATA_TYPE_UINT32;
     return encode(map, type, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What rows of results start on, as store_32 takes it; 0: they are copied through shared memory
+inline int rows_start_on(const void *out, long long stride, int elem_bytes) {
+    for (int bytes : {32, 16})
+        if (aligned_to(out, bytes) && stride * elem_bytes % bytes == 0) return bytes;
+    return 0;
 }
 
 struct Operand {

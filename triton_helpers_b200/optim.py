@@ -100,7 +100,6 @@ def _check_norm(max_norm: float) -> float:
 
 def _norm_factor(tensors: Sequence[Tensor], scales: Optional[Sequence[float]], max_norm: float) -> Tensor:
     r"""(norm, factor) of a list of gradients, a float32 pair on their device."""
-    tensors = list(tensors)
     pair = _lib.native().grad_norm(tensors, None if scales is None else tuple(scales), max_norm)
     if pair is not NotImplemented:
         return pair
@@ -159,13 +158,15 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     return pair[0]
 
 
-def _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, pair, step, lr, betas, eps, skipped) -> None:
-    r"""The update of parameters of one dtype and device, gradients times their scale times the pair's factor."""
+def _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, pair, max_norm, step, lr, betas, eps, skipped) -> Tensor:
+    r"""The update of parameters of one dtype and device, gradients times their scale times the pair's factor; without a pair that of these
+    gradients and ``max_norm``. Returns the pair."""
     done = _lib.native().adam_clipped(
-        params, grads, exp_avgs, exp_avg_sqs, tuple(grad_scales), tuple(zero_grads), pair, lr, betas[0], betas[1], eps, step, skipped
-    )
+        params, grads, exp_avgs, exp_avg_sqs, None if grad_scales is None else tuple(grad_scales), None if zero_grads is None else tuple(zero_grads), pair,
+        max_norm, lr, betas[0], betas[1], eps, step, skipped,
+    )  # fmt: skip
     if done is not NotImplemented:
-        return
+        return done
     n = len(params)
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
         if g.dtype != p.dtype or p.dtype != params[0].dtype or m.dtype != torch.float32 or v.dtype != torch.float32:
@@ -173,18 +174,21 @@ def _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads,
         if not all(t.is_contiguous() and t.numel() == p.numel() for t in (p, g, m, v)):
             raise RuntimeError("a clipped update needs contiguous parameters, gradients and moments of one size")
     device = _lib.require_cuda(*params, *grads, *exp_avgs, *exp_avg_sqs, pair, skipped)
+    if pair is None:
+        pair = _norm_factor(grads, grad_scales, max_norm)
     pointers = lambda tensors: (c_void_p * n)(*(t.data_ptr() for t in tensors))  # noqa: E731
     with torch.cuda.device(device):
         _lib.check(
             _lib.lib().th_adam_clipped(
                 n, pointers(params), pointers(grads), pointers(exp_avgs), pointers(exp_avg_sqs), _lib.i64_array([p.numel() for p in params]),
-                (c_float * n)(*grad_scales), (c_int * n)(*map(int, zero_grads)), pair.data_ptr(), lr, betas[0], betas[1], eps, step,
-                _lib.dtype_code(params[0]), _lib.ptr(skipped), _lib.stream_ptr(device),
+                (c_float * n)(*([1.0] * n if grad_scales is None else grad_scales)), (c_int * n)(*map(int, zero_grads or [0] * n)), pair.data_ptr(),
+                lr, betas[0], betas[1], eps, step, _lib.dtype_code(params[0]), _lib.ptr(skipped), _lib.stream_ptr(device),
             ),
             "th_adam_clipped",
         )  # fmt: skip
     for p in params:
         torch.autograd.graph.increment_version(p)
+    return pair
 
 
 @torch.no_grad()
@@ -205,16 +209,10 @@ def clipped_adam_updates(
     r"""Adam's update in place of parameters of one dtype and device, their gradients clipped to the global norm ``max_norm``; returns the
     norm that they had, each times its scale (a float32 scalar on the device, not synchronised). Any number of contiguous tensors, with
     gradients of the parameters' dtype and float32 moments; ``skipped`` as in ``adam_update``."""
-    max_norm = _check_norm(max_norm)
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
-    n = len(params)
-    grad_scales = [1.0] * n if grad_scales is None else list(grad_scales)
-    zero_grads = [False] * n if zero_grads is None else list(zero_grads)
-    if n == 0 or any(len(x) != n for x in (grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads)):
+    max_norm, n = _check_norm(max_norm), len(params)
+    if n == 0 or any(x is not None and len(x) != n for x in (grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads)):
         raise ValueError("a clipped update needs as many gradients, moments, scales and flags as parameters, and one at least")
-    pair = _norm_factor(grads, grad_scales, max_norm)
-    _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, pair, step, lr, betas, eps, skipped)
-    return pair[0]
+    return _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads, None, max_norm, step, lr, betas, eps, skipped)[0]
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -277,4 +275,4 @@ class FusedAdam(torch.optim.Optimizer):
             if pair is None:
                 adam_updates(*columns, *hyper)
             else:
-                _adam_clipped(*columns, pair, *hyper)
+                _adam_clipped(*columns, pair, 0.0, *hyper)
