@@ -21,7 +21,7 @@ namespace th {
 namespace {
 
 constexpr int kF8Block = 128;
-constexpr int kF8Step = 16;        // columns of an accumulator that a warp reads at a time
+constexpr int kF8Step = 64;        // columns of an accumulator that a warp reads at a time
 constexpr int kF8Batch = 4;        // blocks whose scales a warp asks for at a time
 
 struct F8Scale {
@@ -39,7 +39,7 @@ template <int BN, int CG, bool SWAP, int CTAS>
 struct F8Shape {
     static constexpr int kBRows = BN / CG;
     static constexpr int kABytes = kGemmRows * 128, kBBytes = kBRows * 128, kStage = kABytes + kBBytes;
-    static constexpr int kGroups = CTAS == 1 ? 4 : 2;  // of four warps that keep sums
+    static constexpr int kGroups = 2;  // of four warps that keep sums
     static constexpr int kWarps = 4 * kGroups, kThreads = 128 + 32 * kWarps;
     static constexpr int kStaging = SWAP ? 0 : kWarps * kPieceBytes;
     static constexpr int kFactors = SWAP ? BN : kGemmRows * (BN == 256 ? 2 : 1);  // of a block: a token's for every row of weight blocks
@@ -53,7 +53,7 @@ struct F8Shape {
     static constexpr int kColumns = BN / kGroups;  // of each group
     static constexpr bool kSplits = kGemmRows * BN * 4 <= kStages * kStage;
     // Registers a thread: at launch what the SM's 65536 allow; then the first four warps give theirs to those that keep sums
-    static constexpr int kLaunchRegs = CTAS == 1 ? 96 : 80, kFewRegs = CTAS == 1 ? 64 : 40, kSumRegs = CTAS == 1 ? 104 : 96;
+    static constexpr int kLaunchRegs = CTAS == 1 ? 168 : 80, kFewRegs = CTAS == 1 ? 56 : 40, kSumRegs = CTAS == 1 ? 224 : 96;
     static_assert(kFewRegs + kGroups * kSumRegs <= (1 + kGroups) * kLaunchRegs, "more registers than the launch has");
     static_assert(kStages >= 3 && kAccs >= 2 && CTAS * kTmemCols <= 512, "tile does not fit");
 };
@@ -101,10 +101,11 @@ __device__ __forceinline__ void f8_block(uint32_t d, uint32_t a, uint32_t b, uin
 // The scales' product is one factor where it is between 2^-100 and 2^100.  Where it is not (it may be no float32 at all) a sum takes two factors
 // one after the other, of about its square root each: results are then lost only where they are no float32 themselves.
 
-// Two neighbouring columns' float32 values as one operand of packed arithmetic
+// Two neighbouring columns' float32 values as one operand of packed arithmetic.  Volatile: what works on values read from tensor memory stays behind the
+// wait for them.
 __device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) {
     unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    asm volatile("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
     return v;
 }
 __device__ __forceinline__ float2 floats_of(unsigned long long v) {
@@ -114,41 +115,30 @@ __device__ __forceinline__ float2 floats_of(unsigned long long v) {
 }
 __device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
     unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
 __device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, unsigned long long b) {
     unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    asm volatile("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 
+// N neighbouring columns of this warp's lanes; they are there after tmem_ld_wait()
 template <int N>
 __device__ __forceinline__ void f8_read(uint32_t taddr, uint32_t (&v)[N]) {
-    if constexpr (N == 16)
+    if constexpr (N >= 32) {
+#pragma unroll
+        for (int c = 0; c < N; c += 32) tmem_ld32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+    } else if constexpr (N == 16) {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
                        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                      : "r"(taddr)
                      : "memory");
-    else
+    } else {
         tmem_ld8_at(taddr, v);
-}
-
-// Waits for the reads before, the registers of the last one among its operands: nothing that uses them moves ahead of it
-template <int N>
-__device__ __forceinline__ void f8_read_wait(uint32_t (&v)[N]) {
-    if constexpr (N == 16)
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                       "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-                     :
-                     : "memory");
-    else
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
-                     :
-                     : "memory");
+    }
 }
 
 __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
@@ -307,7 +297,7 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
             }
         }
     } else {
-        // ---- scales: the even blocks' by one warp, the odd ones' by the other ----
+        // ---- scales: the even blocks' by one warp, the odd ones' by the other (one warp for all of them: 545 -> 590 us at 8192 x 4096 -> 16384) ----
         constexpr int kRows = (SWAP ? BN : kGemmRows) / 32 > 0 ? (SWAP ? BN : kGemmRows) / 32 : 1, kGroups = SWAP ? 1 : BN == 256 ? 2 : 1;
         int it0 = 0;
         bool ok = true;
@@ -404,13 +394,13 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                 f8_read<kStep>(d, raw);
                 // a lane's (swapped, it is a column's, and read where it is used)
                 constexpr bool kPairs = BN == 256;
-                const float *of_lane = &factors[slot][0][SWAP ? group * kColumns : (kPairs ? group / 2 * kGemmRows : 0) + 32 * quarter + lane];
+                const float *of_lane = &factors[slot][0][SWAP ? group * kColumns : (kPairs ? group * kGemmRows : 0) + 32 * quarter + lane];
                 unsigned long long both = 0;
                 if constexpr (!SWAP) both = pair_of(__float_as_uint(*of_lane), __float_as_uint(*of_lane));
                 const bool far = far_factors[slot] != 0;
 #pragma unroll
                 for (int chunk = 0; chunk < kChunks; ++chunk) {
-                    f8_read_wait<kStep>(raw);
+                    tmem_ld_wait();
                     if (chunk + 1 == kChunks) {
                         // the accumulator is read: another block may fill it
                         tc_fence_before();
