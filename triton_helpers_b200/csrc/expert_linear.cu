@@ -7,14 +7,16 @@
 namespace th {
 namespace {
 
-// Columns of the accumulator for few rows an expert; 0 where rows fill tiles of their own
+// Columns of the accumulator for few rows an expert; 0 where rows fill tiles of their own.  64 experts, 2048 -> 1024 (268 MB of weights), us with 16, 32 and 64
+// columns and with 128-row tiles: 8 rows an expert 45.4, 46.0, 46.8, 50.3; 16 rows 48.0, 47.3, 48.0, 51.1; 32 rows 57.3, 49.8, 48.8, 51.6; 64 rows 80, 59.6, 52.8, 51.3.
 int few_rows(int rows, int experts) {
     const int average = divide_up(rows, experts);
     return average > 48 ? 0 : average <= 8 ? 16 : average <= 20 ? 32 : 64;
 }
 
 // Whether pairs of CTAs on 256 x 256 tiles are quicker than single ones on 128 x 128, by an estimate in cycles: rounds of tiles x (stages x cycles a
-// stage + what a tile takes besides).  Of an expert's tiles the last one is half empty on average.
+// stage + what a tile takes besides).  Pairs against single ones, us: 16384 rows of 32 experts 2048 -> 4096 249 / 304, its weights' gradient 266 / 356; 128 rows
+// for each of 64 experts 2048 -> 1024 63 / 67, 64 rows 59 / 51; 3001 rows of 7 experts 520 -> 336 10.2 / 8.8, the gradient 13.2 / 11.5.
 bool pairs_pay(double tiles_256, double tiles_128, double stages) {
     const double rounds_256 = std::ceil(tiles_256 / (sm_count() / 2)), rounds_128 = std::ceil(tiles_128 / sm_count());
     return rounds_256 * (stages * 520 + 1500) + 1800 < rounds_128 * (stages * 560 + 800);
@@ -29,8 +31,9 @@ int run_rows(ExpertArgs x, const ExpertOperand &rows, const ExpertOperand &weigh
         case 64: return launch_experts<B_MN, false, 64, 1, true, false, 2>(x, weight, rows, bf16, stream);
         default: break;
     }
-    const double half = 0.5 * x.experts;
-    if (pairs_pay((x.rows / 256.0 + half) * divide_up(x.g.n, 256), (x.rows / 128.0 + half) * divide_up(x.g.n, 128), divide_up(x.k, 64)))
+    // of an expert's tiles the last one is half empty on average; where its rows fit 128, a pair's tile would be so for sure
+    const double average = static_cast<double>(x.rows) / x.experts, half = 0.5 * x.experts;
+    if (average > 96 && pairs_pay((x.rows / 256.0 + half) * divide_up(x.g.n, 256), (x.rows / 128.0 + half) * divide_up(x.g.n, 128), divide_up(x.k, 64)))
         return launch_experts<false, B_MN, 256, 2, false, false, 1>(x, rows, weight, bf16, stream);
     return launch_experts<false, B_MN, 128, 1, false, false, 1>(x, rows, weight, bf16, stream);
 }

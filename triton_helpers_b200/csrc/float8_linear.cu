@@ -11,7 +11,10 @@ struct F8Plan {
 };
 
 // The cheapest cut by an estimate in cycles, as for the products without scales (wide_linear.cu): rounds of tiles x blocks of K x cycles a
-// block, what a pair takes longer to start, and for split tiles the exchange of their sums.
+// block, what a pair takes longer to start, and for split tiles the exchange of their sums.  Cuts measured on a B200, us (tile columns x CTAs x parts; * is
+// the one taken): 8192 x 4096 -> 4096 256x2x1* 142, 128x2x1 180, 128x1x1 181; 2048 x 2048 -> 2048 256x2x1* 17.2, 128x1x1 20.3, 128x2x1 20.9; 512 x 4096 -> 4096
+// 128x1x1* 18.4, 128x2x1 19.8, 256x2x2 22.2; 256 x 8192 -> 1024 128x1x5* 13.9, 128x1x4 14.5, 128x2x4 16.1, 256x2x1 36.9; 1023 x 2500 -> 1111 128x1x2* 14.7,
+// 128x2x1 15.5, 256x2x1 18.8; one token 4096 -> 4096 in 1, 2, 3, 4*, 8 parts 14.6, 11.9, 10.2, 9.7, 9.9; 100 tokens in 1, 2, 4*, 8 parts 29, 20.5, 16.6, 35.
 F8Plan plan_float8(int m, int n, int k, bool b_mn) {
     const int k_tiles = divide_up(k, kF8Block);
     F8Plan best{};
@@ -38,9 +41,9 @@ F8Plan plan_float8(int m, int n, int k, bool b_mn) {
         consider(bn, 1, true, bn == 128 ? 1 : 2, 2.0 * (kGemmRows + bn), 1500 + 8 * bn);
         return best;
     }
-    consider(256, 2, false, 1, 1000, 9000);
-    if (!b_mn) consider(128, 2, false, 1, 800, 4500);  // an MN-major weight comes 128 columns a CTA
-    consider(128, 1, false, 1, 780, 4500);
+    consider(256, 2, false, 1, 960, 9000);
+    if (!b_mn) consider(128, 2, false, 1, 720, 4500);  // an MN-major weight comes 128 columns a CTA
+    consider(128, 1, false, 1, 680, 4500);
     return best;
 }
 

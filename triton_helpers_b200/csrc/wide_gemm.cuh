@@ -216,30 +216,34 @@ __device__ __forceinline__ void store_32(unsigned char *to, const uint32_t *v, i
 }
 
 // 32 bytes of each of a warp's 32 rows -> rows m0.. below m_end, columns c0.. of the output, through shared memory so that neighbouring lanes write
-// neighbouring elements
+// neighbouring elements.  All are read ahead of their stores (3001 x 777 results of an 8-bit product: 20.4 us with each ahead of its own only).
+template <typename V>
+__device__ __forceinline__ void copy_piece_of(const GemmArgs &g, uint32_t box, int m0, int m_end, int c0) {
+    constexpr int kPerRow = 32 / static_cast<int>(sizeof(V)), kTurns = kPerRow;  // 32 / kPerRow rows a turn
+    const int lane = threadIdx.x & 31, c = lane % kPerRow, r0 = lane / kPerRow, rows = min(32, m_end - m0);
+    V x[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const int r = r0 + i * (32 / kPerRow);
+        const uint32_t from = box + r * 32 + ((c * static_cast<int>(sizeof(V))) ^ (((r >> 2) & 1) << 4));
+        if constexpr (sizeof(V) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[i]) : "r"(from) : "memory");
+        else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x[i]) : "r"(from) : "memory");
+    }
+    if (c0 + c >= g.n) return;
+    V *to = static_cast<V *>(g.out) + static_cast<long long>(m0 + r0) * g.out_stride + c0 + c;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+        if (r0 + i * (32 / kPerRow) < rows) to[i * (32 / kPerRow) * g.out_stride] = x[i];
+}
 __device__ __forceinline__ void copy_piece(const GemmArgs &g, uint32_t box, const uint32_t *v, int m0, int m_end, int c0, int out_bytes) {
-    const int lane = threadIdx.x & 31, per_row = 32 / out_bytes, cols = min(per_row, g.n - c0), rows = min(32, m_end - m0);
     __syncwarp();
-    const uint32_t at = box + lane * 32, turn = (lane >> 2) & 1;  // two lanes' halves change places, for the banks
+    const int lane = threadIdx.x & 31;
+    const uint32_t at = box + lane * 32, turn = (lane >> 2) & 1;  // two halves of a row change places every four rows, for the banks
     st_shared_16(at + (turn << 4), make_uint4(v[0], v[1], v[2], v[3]));
     st_shared_16(at + ((turn ^ 1) << 4), make_uint4(v[4], v[5], v[6], v[7]));
     __syncwarp();
-    const int c = lane % per_row;
-    for (int r = lane / per_row; r < rows; r += 32 / per_row) {
-        const uint32_t from = box + r * 32 + ((c * out_bytes) ^ (((r >> 2) & 1) << 4));
-        const long long to = static_cast<long long>(m0 + r) * g.out_stride + c0 + c;
-        if (c < cols) {
-            if (out_bytes == 4) {
-                uint32_t x;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(from) : "memory");
-                static_cast<uint32_t *>(g.out)[to] = x;
-            } else {
-                unsigned short x;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from) : "memory");
-                static_cast<unsigned short *>(g.out)[to] = x;
-            }
-        }
-    }
+    if (out_bytes == 4) copy_piece_of<uint32_t>(g, box, m0, m_end, c0);
+    else copy_piece_of<unsigned short>(g, box, m0, m_end, c0);
 }
 
 __device__ __forceinline__ void store_box(const GemmArgs &g, const CUtensorMap *c_map, uint32_t box, int m0, int c0, int out_bytes) {
