@@ -235,7 +235,8 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
             const ExpertTile t = expert_tile<SWAP, OVER_ROWS>(x, firsts, tiles, unit);
             // where this CTA's operand rows begin: lanes (A) and columns (B); rows of an expert count from its first
             const int lane0 = (t.tm * CG + static_cast<int>(rank)) * kGemmRows, column0 = t.tn * BN + static_cast<int>(rank) * S::kBRows;
-            const int a0 = SWAP ? t.tn * kGemmRows : OVER_ROWS ? lane0 : t.first + lane0, b0 = SWAP ? t.first + t.tm * BN : column0;
+            // a CTA of a pair that has none of the expert's rows reads outside of them all: zeros, which cost neither traffic nor much power
+            const int a0 = SWAP ? t.tn * kGemmRows : OVER_ROWS ? lane0 : t.first + lane0 < t.end ? t.first + lane0 : x.rows, b0 = SWAP ? t.first + t.tm * BN : column0;
             const int az = SWAP ? t.expert : 0, bz = SWAP || OVER_ROWS ? 0 : t.expert;
             const int stages = stages_of(t), rest = rest_of(t);
             for (int kt = 0; kt < stages; ++kt, ++it) {
