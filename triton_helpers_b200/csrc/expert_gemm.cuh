@@ -164,7 +164,8 @@ __device__ __forceinline__ ExpertTile expert_tile(const ExpertArgs &a, const int
 // SWAP: weights along the accumulator's lanes, rows along its columns; the output is C transposed
 template <bool A_MN, bool B_MN, int BN, int CG, bool SWAP, bool OVER_ROWS, int CTAS>
 __global__ void __launch_bounds__(ExpertShape<A_MN, B_MN, BN, CG, SWAP, OVER_ROWS, CTAS>::kThreads, CTAS)
-expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map) {
+expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
+                   const __grid_constant__ CUtensorMap few_map) {
     using S = ExpertShape<A_MN, B_MN, BN, CG, SWAP, OVER_ROWS, CTAS>;
     const GemmArgs &g = x.g;
     extern __shared__ unsigned char smem_raw[];
@@ -235,10 +236,11 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
             const ExpertTile t = expert_tile<SWAP, OVER_ROWS>(x, firsts, tiles, unit);
             // where this CTA's operand rows begin: lanes (A) and columns (B); rows of an expert count from its first
             const int lane0 = (t.tm * CG + static_cast<int>(rank)) * kGemmRows, column0 = t.tn * BN + static_cast<int>(rank) * S::kBRows;
-            // a CTA of a pair that has none of the expert's rows reads outside of them all: zeros, which cost neither traffic nor much power
-            const int a0 = SWAP ? t.tn * kGemmRows : OVER_ROWS ? lane0 : t.first + lane0 < t.end ? t.first + lane0 : x.rows, b0 = SWAP ? t.first + t.tm * BN : column0;
+            const int a0 = SWAP ? t.tn * kGemmRows : OVER_ROWS ? lane0 : t.first + lane0, b0 = SWAP ? t.first + t.tm * BN : column0;
             const int az = SWAP ? t.expert : 0, bz = SWAP || OVER_ROWS ? 0 : t.expert;
             const int stages = stages_of(t), rest = rest_of(t);
+            // An expert's last rows come 32 at a time, and those behind its end from outside of all rows: zeros, which cost no traffic and little power
+            const bool few = !SWAP && !OVER_ROWS && a0 + kGemmRows > t.end;
             for (int kt = 0; kt < stages; ++kt, ++it) {
                 const int s = it % S::kStages;
                 const bool got = lane_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
@@ -261,6 +263,9 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                     if constexpr (A_MN) {
                         expert_load<CG>(a, &a_map, a0, k, az, bar);
                         expert_load<CG>(a + kBoxBytes, &a_map, a0 + 64, k, az, bar);
+                    } else if (few) {
+#pragma unroll
+                        for (int r = 0; r < kGemmRows; r += 32) expert_load<CG>(a + r * 128, &few_map, k, a0 + r < t.end ? a0 + r : x.rows, az, bar);
                     } else {
                         expert_load<CG>(a, &a_map, k, a0, az, bar);
                     }
@@ -482,12 +487,14 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
             return rc;
         if (device < 64) ready |= 1ull << device;
     }
-    CUtensorMap a_map, b_map;
+    CUtensorMap a_map, b_map, few_map;
     const auto operand = [](CUtensorMap *map, const ExpertOperand &o, bool mn, int box_rows) {
         return expert_map(map, o.base, o.inner, o.outer, o.stride, o.count, o.apart, mn ? 64 : box_rows);
     };
     if (!operand(&a_map, a, A_MN, kGemmRows) || !operand(&b_map, b, B_MN, S::kBRows))
         return fail(TH_ERR_ALIGNMENT, "product of experts: operand rows must start on 16 bytes");
+    if (SWAP || OVER_ROWS) few_map = a_map;  // not looked at
+    else if (!operand(&few_map, a, false, 32)) return fail(TH_ERR_ALIGNMENT, "product of experts: operand rows must start on 16 bytes");
     GemmArgs &g = x.g;
     x.tile_rows = SWAP ? BN : CG * kGemmRows;
     g.tiles_m = OVER_ROWS ? divide_up(g.m, CG * kGemmRows) : 0;
@@ -501,7 +508,7 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
     const long long units = rows_of_tiles * g.tiles_n;
     if (units > 0x7fffffffll || out_rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "product of experts: too many tiles");
     const long long clusters = std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
-    return launch_chained("expert_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), S::kThreads, S::kBytes, stream, CG, x, a_map, b_map);
+    return launch_chained("expert_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), S::kThreads, S::kBytes, stream, CG, x, a_map, b_map, few_map);
 }
 
 }  // namespace
