@@ -107,6 +107,18 @@ def test_clip(dtype, max_norm):
         assert after <= max_norm * (1 + torch.finfo(dtype).eps) + tiny
 
 
+def test_python_and_native_paths_agree():
+    make = lambda: [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=t)) for n, t in ((1000, torch.float32), (33, torch.bfloat16), (4097, torch.float16))]  # noqa: E731
+    ours, theirs = make(), make()
+    for group in (ours, theirs):
+        for i, p in enumerate(group):
+            p.grad = normal(p.numel(), seed=i, dtype=p.dtype)
+    first = clip_grad_norm_(ours, 0.5)
+    with _lib.KernelTimer():  # leaves the call to Python
+        second = clip_grad_norm_(theirs, 0.5)
+    assert torch.equal(first, second) and all(torch.equal(p.grad, q.grad) for p, q in zip(ours, theirs))
+
+
 def test_clip_of_nothing_and_of_norms_that_are_not_finite():
     p = torch.zeros(5, device="cuda", requires_grad=True)
     assert float(clip_grad_norm_([p], 1.0)) == 0

@@ -90,6 +90,14 @@ def test_larger_sizes(counts, d, n, dtype):
     check(x, w, ends_of(counts), (0.1 * normal(rows, n, seed=2)).to(dtype))
 
 
+@pytest.mark.parametrize("experts,rows", [(1024, 3000), (1000, 300), (999, 60_000), (33, 1)])
+def test_many_experts(experts, rows):
+    g = torch.Generator().manual_seed(0)
+    counts = torch.bincount(torch.randint(0, experts, (rows,), generator=g) // 3 * 2 % experts, minlength=experts).tolist()
+    x, w = normal(rows, 64, dtype=torch.bfloat16), (normal(experts, 40, 64, seed=1) * 0.125).to(torch.bfloat16)
+    check(x, w, ends_of(counts), normal(rows, 40, seed=2, dtype=torch.bfloat16))
+
+
 @pytest.mark.parametrize("ends", [[5, 3, 9], [-4, 2, 100], [100, 100, 100], [0, 0, 0], [20, 0, 7], [-1, -2, -3]])
 def test_ends_out_of_order_or_range(ends):
     x, w = normal(20, 40, dtype=torch.float16), normal(3, 24, 40, seed=1, dtype=torch.float16)

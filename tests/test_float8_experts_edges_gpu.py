@@ -226,3 +226,19 @@ def test_offsets_beyond_32_bits():
     dx, dw = torch.autograd.grad(out, (few, big), torch.ones_like(out))
     total = few.detach().double().sum(0)
     assert float((dw[35, 8191].double() - total).abs().max()) <= 2.0**-7 * float(total.abs().max()) and not bool(dw[34].any()) and not bool(dw[0].any())
+
+
+def test_command_lines_run(tmp_path):
+    from triton_helpers_b200.benchmark import CLI
+    from triton_helpers_b200.layers.expert_linear.__main__ import Baseline, Experts
+    from triton_helpers_b200.layers.float8_linear.__main__ import Serving, Training
+
+    flags = ["benchmark", "-m", "fwd", "fwd-bwd", "-w", "2", "-r", "5", "-o", str(tmp_path)]
+    charts = CLI.entrypoint("Float8 Linear", [Training("training")], {"L": ((16, 300), "values"), "D": (256, "values"), "N": (128, "values")}, flags)
+    assert len(charts) == 2 and all(v > 0 for c in charts for row in c.rows for v in row)
+    charts = CLI.entrypoint("Float8 Linear", [Serving("serving")], {"L": ((16, 300), "values"), "D": (256, "values"), "N": (128, "values")},
+                            ["benchmark", "-m", "fwd", "-w", "2", "-r", "5"])  # fmt: skip
+    assert charts[0].rows[0][0] > 0
+    charts = CLI.entrypoint("Expert Linear", [Baseline("baseline"), Experts("experts")],
+                            {"L": ((64, 1000), "values"), "E": (4, "values"), "D": (256, "values"), "N": (128, "values")}, flags)  # fmt: skip
+    assert len(charts) == 2 and all(v > 0 for c in charts for row in c.rows for v in row)

@@ -2046,6 +2046,21 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// clip_grads(tensors, max_norm) -> the pair, the tensors scaled by its factor in place
+PyObject *py_clip_grads(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    TensorList grads;
+    std::vector<const Tensor *> tensors;
+    double max_norm;
+    if (n_args != 2 || !usual_mode() || !grads.read(args[0], &tensors) || !take(args[1], max_norm)) TH_NOT_MINE;
+    c10::cuda::CUDAGuard guard(grads.device);
+    const Tensor pair = norm_factor(grads, {}, max_norm);
+    check(th_scale_tensors(grads.count(), grads.pointers.data(), grads.sizes.data(), grads.codes.data(), pair.data_ptr<float>(), current_stream()), "th_scale_tensors");
+    for (const Tensor *t : tensors) t->unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(pair);
+    END_HANDLE_TH_ERRORS
+}
+
 // adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales or None, zero_grad or None, pair or None, max_norm, lr, beta1, beta2, eps, step,
 // skipped): the update of tensors of one dtype on one device, gradients times their scale times the pair's factor; without a pair that of these
 // gradients and max_norm.  Returns the pair.
@@ -2113,7 +2128,7 @@ PyObject *py_defer(PyObject *, PyObject *flag) {
 PyMethodDef g_methods[] = {
     TH_FAST(hash_encoding), TH_FAST(fully_fused_mlp), TH_FAST(reversible_mlp), TH_FAST(hash_encoded_mlp), TH_FAST(adam_steps),
     TH_FAST(train_gradients), TH_FAST(configure), TH_FAST(rms_norm), TH_FAST(rms_norm_int8), TH_FAST(int8_linear), TH_FAST(checkpointed_linear),
-    TH_FAST(float8_linear), TH_FAST(float8_training_linear), TH_FAST(expert_linear), TH_FAST(grad_norm), TH_FAST(adam_clipped),
+    TH_FAST(float8_linear), TH_FAST(float8_training_linear), TH_FAST(expert_linear), TH_FAST(grad_norm), TH_FAST(clip_grads), TH_FAST(adam_clipped),
     {"defer", py_defer, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -143,6 +143,9 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
     if not grads:
         return torch.tensor(0.0)
+    pair = _lib.native().clip_grads(grads, max_norm)
+    if pair is not NotImplemented:
+        return pair[0]
     pair = _norm_factor(grads, None, max_norm)
     flat, device = _flat(grads, "clip_grad_norm_")
     pointers, sizes, codes = _lists(flat)
