@@ -485,6 +485,11 @@ int th_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *
 /* Rows in blocks of 1 x 128: scale_dev[b * scale_block + r], scale_block >= rows. */
 int th_float8_rows(const void *x_dev, int64_t x_stride, void *q_dev, int64_t q_stride, float *scale_dev,
                    int64_t scale_block, int64_t rows, int d, int dtype, void *stream);
+/* The same of 16-bit rows, and a copy of them as the products in 16 bits want their operands (th_copy_rows): copy rows start on 16
+ * bytes and hold d rounded up to eight elements, the last of them zeros. */
+int th_float8_rows_copied(const void *x_dev, int64_t x_stride, void *q_dev, int64_t q_stride, float *scale_dev,
+                          int64_t scale_block, void *copy_dev, int64_t copy_stride, int64_t rows, int d, int dtype,
+                          void *stream);
 /* A weight in blocks of 128 x 128: scale_dev[(r / 128) * ceil(d / 128) + b]. */
 int th_float8_weight(const void *w_dev, int64_t w_stride, void *q_dev, int64_t q_stride, float *scale_dev, int64_t rows,
                      int d, int dtype, void *stream);

@@ -46,6 +46,8 @@ def test_block_entry_points_refuse(library):
     assert rows(AT, 8, AT, 16, AT, 3, 4, 8, 1, None) == -1 and said(library, b"scales")
     assert rows(AT, 8, AT, 1 << 25, AT, 4, 4, (1 << 24) + 1, 0, None) == -2
     assert rows(None, 8, None, 16, None, 0, 0, 8, 0, None) == 0
+    copied = lambda copy=AT, stride=8, dtype=1: library.th_float8_rows_copied(AT, 8, AT, 16, AT, 4, copy, stride, 4, 8, dtype, None)  # noqa: E731
+    assert copied(dtype=0) == -2 and copied(copy=None) == -1 and copied(stride=7) == -1 and copied(stride=12) == -3 and copied(copy=AT + 2) == -3
     weight = library.th_float8_weight
     assert weight(AT, 8, AT, 24, AT, 4, 8, 0, None) == -3
     assert weight(AT, 8, AT, 16, AT, 65535 * 128 + 1, 8, 0, None) == -2

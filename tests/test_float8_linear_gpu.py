@@ -1,4 +1,6 @@
 r"""8-bit floating-point blocks and the linear layers on them against a float64 statement of their definition."""
+from contextlib import nullcontext
+
 import pytest
 import torch
 
@@ -378,3 +380,22 @@ def test_second_derivatives_raise():
     (dx,) = torch.autograd.grad(float8_training_linear(x, w).float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="not differentiable twice"):
         dx.float().sum().backward()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("rows, n", [(33, 130), (1, 77), (40, 128), (150, 1)])
+def test_output_gradients_of_any_layout(rows, n, native):
+    # rows that start off 16 bytes, that are strided or shared: blocks and the 16-bit rows of the weight's product come out as those of a plain tensor
+    dtype = torch.bfloat16
+    x = normal(rows, 200, dtype=dtype, seed=3).requires_grad_()
+    w = normal(n, 200, dtype=dtype, seed=4).requires_grad_()
+    b = normal(n, dtype=dtype, seed=5).requires_grad_()
+    big = normal(2 * rows, n + 8, dtype=dtype, seed=6)
+    with nullcontext() if native else _lib.KernelTimer():
+        for gy in (big[:rows, 3 : 3 + n], big[::2, 8:], big[:rows, :n], big[1:2, :n].expand(rows, -1), big[:rows, 1 : 1 + n].contiguous()):
+            plain = torch.zeros(rows, -(-n // 8) * 8, dtype=dtype, device="cuda")
+            plain[:, :n] = gy
+            out = [torch.autograd.grad(float8_training_linear(x, w, b), (x, w, b), g) for g in (gy, plain[:, :n])]
+            assert all(torch.equal(got, want) for got, want in zip(*out))
+            (dw,) = torch.autograd.grad(float8_training_linear(x.detach(), w, None), w, gy)
+            assert torch.equal(dw, out[0][1])

@@ -183,6 +183,10 @@ SIGNATURES = {
     "th_linear_bwd_weight": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
     "th_linear_tc_status": (c_int, []),
     "th_float8_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "th_float8_rows_copied": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p],
+    ),
     "th_float8_weight": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "th_float8_values": (
         c_int,
@@ -242,7 +246,7 @@ class KernelTimer:
                  "th_hash_fwd_cast", "th_hash_bwd_cast", "th_mlp_fwd_mse_ordered", "th_mse_grad", "th_adam_step", "th_adam_steps", "th_cast",
                  "th_scale_cast", "th_rms_norm_fwd", "th_rms_norm_int8", "th_rms_norm_bwd", "th_quantize_rows", "th_dequantize_rows",
                  "th_column_sum", "th_checkpoint_rows", "th_copy_rows", "th_int8_linear", "th_quantized_linear", "th_linear_fwd", "th_linear_bwd_input", "th_linear_bwd_weight",
-                 "th_float8_rows", "th_float8_weight", "th_float8_values", "th_float8_linear", "th_float8_quantized_linear", "th_float8_bwd_input",
+                 "th_float8_rows", "th_float8_rows_copied", "th_float8_weight", "th_float8_values", "th_float8_linear", "th_float8_quantized_linear", "th_float8_bwd_input",
                  "th_expert_linear_fwd", "th_expert_linear_bwd_input", "th_expert_linear_bwd_weight", "th_grad_norm", "th_scale_tensors",
                  "th_adam_clipped")  # fmt: skip
 

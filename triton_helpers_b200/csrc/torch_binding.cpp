@@ -1763,14 +1763,29 @@ struct Float8LinearNode : public Node {
         c10::cuda::CUDAGuard guard(device);
         void *stream = current_stream();
         const int code = dtype_code(type), di = static_cast<int>(d_in), dn = static_cast<int>(d_out);
-        Operands operands;
-        const Rows &gy = operands.add(grads[0].scalar_type() == type ? grads[0] : grads[0].to(type), d_out);
-        operands.settle(stream);
-        if (keeps_weight && task_should_compute_output(0)) {
+        const bool wants_x = keeps_weight && task_should_compute_output(0), wants_w = keeps_input && task_should_compute_output(1);
+        const Tensor grad = grads[0].scalar_type() == type ? grads[0] : grads[0].to(type);
+        Rows gy = rows_or_copy(grad, d_out);
+        // the weight's product wants rows that start on 16 bytes: where they do not, the kernel that makes blocks of them copies them
+        const bool copied = wants_w && (gy.stride % 8 != 0 || reinterpret_cast<uintptr_t>(ptr(gy.keep)) % 16 != 0);
+        if (copied && !wants_x) {
+            Operands operands;
+            gy = operands.add(grad, d_out);
+            operands.settle(stream);
+        }
+        if (wants_x) {
             w.buffer = restored(w.buffer, at::kByte, w.bytes());
             HeldBlocks g = HeldBlocks::sized(rows, d_out, rows * blocks_of(d_out));
             g.make(device);
-            check(th_float8_rows(ptr(gy.keep), gy.stride, g.q(), g.pitch, g.scale(), rows, rows, dn, code, stream), "th_float8_rows");
+            if (copied) {
+                const int64_t pitch = (d_out + 7) / 8 * 8;
+                const Tensor rows16 = empty_like_shape({rows, pitch}, type, device);
+                check(th_float8_rows_copied(ptr(gy.keep), gy.stride, g.q(), g.pitch, g.scale(), rows, ptr(rows16), pitch, rows, dn, code, stream), "th_float8_rows_copied");
+                gy.keep = rows16;
+                gy.stride = pitch;
+            } else {
+                check(th_float8_rows(ptr(gy.keep), gy.stride, g.q(), g.pitch, g.scale(), rows, rows, dn, code, stream), "th_float8_rows");
+            }
             out[0] = empty_like_shape(shape, type, device);
             check(th_float8_bwd_input(g.q(), g.pitch, g.scale(), 1, rows, w.q(), w.pitch, w.scale(), blocks_of(d_in), 1, ptr(out[0]), d_in, rows, di, dn, code, stream),
                   "th_float8_bwd_input");
@@ -1781,7 +1796,7 @@ struct Float8LinearNode : public Node {
             out[2] = empty_like_shape({d_out}, type, device);
             check(th_column_sum(ptr(gy.keep), gy.stride, ptr(out[2]), ptr(partial), bytes, rows, dn, code, stream), "th_column_sum");
         }
-        if (keeps_input && task_should_compute_output(1)) {
+        if (wants_w) {
             x.buffer = restored(x.buffer, at::kByte, x.bytes());
             const int64_t stride = (d_in + 7) / 8 * 8;
             const Tensor x16 = empty_like_shape({rows, stride}, type, device);

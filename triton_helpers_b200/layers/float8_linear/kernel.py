@@ -313,7 +313,12 @@ class _float8_training_linear(Function):
         wq, w_scale, xq, x_scale = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad
         d_in, d_out, dtype, device = ctx.x_shape[-1], ctx.d_out, ctx.dtype, gy.device
-        gy2d = _operand(gy.to(dtype), d_out)
+        gy2d = rows2d(gy.to(dtype), d_out)
+        gy2d = gy2d if gy2d.shape[0] < 2 or gy2d.stride(0) >= d_out else gy2d.contiguous()
+        # the weight's product wants rows that start on 16 bytes: where they do not, the kernel that makes blocks of them copies them
+        copied = want_w and (gy2d.data_ptr() % 16 != 0 or row_stride(gy2d) % 8 != 0)
+        if copied and not want_x:
+            gy2d = _operand(gy2d, d_out)
         rows, code = gy2d.shape[0], _lib.DTYPE_CODE[dtype]
         dx = dw = db = None
         lib = _lib.lib()
@@ -321,7 +326,18 @@ class _float8_training_linear(Function):
             stream = _lib.stream_ptr(device)
             if want_x:
                 g8 = _empty_rows((rows,), d_out, device)
-                _make_rows(gy2d, g8)
+                if copied:
+                    rows16 = _empty_operand(rows, d_out, gy2d)
+                    _lib.check(
+                        lib.th_float8_rows_copied(
+                            gy2d.data_ptr(), row_stride(gy2d), g8.q.data_ptr(), _pitch(d_out), g8.scale.data_ptr(), rows, rows16.data_ptr(),
+                            _stride(rows16), rows, d_out, code, stream,
+                        ),
+                        "th_float8_rows_copied",
+                    )  # fmt: skip
+                    gy2d = rows16
+                else:
+                    _make_rows(gy2d, g8)
                 w = _weight2d(Float8Blocks(wq, w_scale), "kept weight")
                 dx = torch.empty(ctx.x_shape, dtype=dtype, device=device)
                 _lib.check(
