@@ -102,7 +102,13 @@ __device__ __forceinline__ void f8_block(uint32_t d, uint32_t a, uint32_t b, uin
 }
 
 // The scales' product is one factor where it is between 2^-100 and 2^100.  Where it is not (it may be no float32 at all) a sum takes two factors
-// one after the other, of about its square root each: results are then lost only where they are no float32 themselves.
+// one after the other, of about its square root each: results are then lost only where they are no float32 themselves.  The second one, of the rests that
+// split_scale leaves, is beyond float32 itself where both scales are near its end (2^126 and up).  Every sum but zero is then infinite (sums of products are 2^-18 at
+// least, the first factor 2^126): the largest float32 in its place says so too, and leaves a sum of zero at zero.
+__device__ __forceinline__ float rests_of(float a, float b) {
+    const float product = a * b;
+    return isinf(product) && isfinite(a) && isfinite(b) ? copysignf(0x1.fffffep127f, product) : product;
+}
 
 // Two neighbouring columns' float32 values as one operand of packed arithmetic.  Volatile: what works on values read from tensor memory stays behind the
 // wait for them.
@@ -344,7 +350,7 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
                             if (far) {
                                 const float2 x = split_scale(token[b][r]), y = split_scale(weight[b][q]);
                                 factors[s][0][at] = x.x * y.x;
-                                factors[s][1][at] = x.y * y.y;
+                                factors[s][1][at] = rests_of(x.y, y.y);
                             } else {
                                 factors[s][0][at] = token[b][r] * weight[b][q];
                             }
