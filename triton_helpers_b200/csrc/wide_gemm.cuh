@@ -275,10 +275,17 @@ __device__ __forceinline__ float2 split_scale(float scale) {
     return make_float2(__uint_as_float(power << 23), scale * __uint_as_float((254u - power) << 23));
 }
 
-// One result from its sum
+// One side's factors with four moved from the rest to the power, so that the product of two finite scales' rests (below 2^130 otherwise) is always a float32: an
+// infinite one would make a NaN of a sum of zero.
+__device__ __forceinline__ float2 split_scale_low(float scale) {
+    const float2 f = split_scale(scale);
+    return make_float2(4.f * f.x, 0.25f * f.y);
+}
+
+// One result from its sum.  The powers come one after the other: their product may be beyond float32.
 template <int EB>
 __device__ __forceinline__ float finished(uint32_t raw, float2 row, float2 column, float bias) {
-    if constexpr (EB == 1) return fmaf(static_cast<float>(static_cast<int>(raw)) * (row.x * column.x), row.y * column.y, bias);
+    if constexpr (EB == 1) return fmaf(static_cast<float>(static_cast<int>(raw)) * row.x * column.x, row.y * column.y, bias);
     else return __uint_as_float(raw) + bias;
 }
 
@@ -340,7 +347,7 @@ __device__ __forceinline__ void finish_split(const GemmArgs &g, const GemmUnit &
                 const int c = 4 * piece + e;
                 if (c >= along) break;
                 const int mi = m0 + (SWAP ? c : line), ni = SWAP ? line : c;
-                const float2 scale = EB == 1 ? split_scale(g.lane_scale[mi]) : make_float2(1.f, 1.f);
+                const float2 scale = EB == 1 ? split_scale_low(g.lane_scale[mi]) : make_float2(1.f, 1.f);
                 const float bias = SWAP ? (g.bias ? bias_at(g.bias, g.bias_dtype, mi) : 0.f) : biases[ni];
                 store_one(g.out, SWAP ? static_cast<long long>(n0 + line) * g.out_stride + mi : static_cast<long long>(m0 + line) * g.out_stride + n0 + c,
                           finished<EB>(sum[e], scale, EB == 1 ? scales[ni] : scale, bias), g.out_dtype);
@@ -496,7 +503,7 @@ wide_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap a_map, co
             const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows + 32 * quarter, n0 = u.tn * BN, m = m0 + lane;
             float2 lane_scale = make_float2(1.f, 1.f);
             float lane_bias = 0.f;
-            if (EB == 1 && m < g.m) lane_scale = split_scale(g.lane_scale[m]);
+            if (EB == 1 && m < g.m) lane_scale = split_scale_low(g.lane_scale[m]);
             if (SWAP && g.bias) lane_bias = m < g.m ? bias_at(g.bias, g.bias_dtype, m) : 0.f;
             // double buffered: a warp that fills the next tile's values has met, at the barrier before, those that read the last but one's
             for (int c = threadIdx.x - 128; c < BN; c += 128) {
