@@ -192,7 +192,7 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
     __shared__ __align__(8) unsigned long long full[S::kStages], empty[S::kStages], acc_full[S::kAccs], acc_empty[S::kAccs];
     __shared__ __align__(16) float factors[S::kSlots][2][S::kFactors];
     __shared__ int far_factors[S::kSlots];
-    __shared__ float biases[2][BN];
+    __shared__ __align__(16) float biases[2][BN];  // read two at a time
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
     const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
