@@ -307,7 +307,7 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                     ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
                     if constexpr (OVER_ROWS) {
                         if (ok && rest && kt == stages - 1) {
-                            ok = gemm_wait(smem_addr(&last_ready[s]), (last_phase >> s) & 1, &abort_flag);
+                            ok = gemm_wait<CG == 2>(smem_addr(&last_ready[s]), (last_phase >> s) & 1, &abort_flag);
                             last_phase ^= 1u << s;
                         }
                     }
@@ -346,7 +346,8 @@ expert_gemm_kernel(const ExpertArgs x, const __grid_constant__ CUtensorMap a_map
                 __syncwarp();
                 if (lane == 0) {
                     const uint32_t bar = smem_addr(&last_ready[s]);
-                    if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, 0)) : "memory");
+                    // the leader's MMAs read this CTA's boxes and the zeros in them: a release to the cluster, once an expert's tile
+                    if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar, 0)) : "memory");
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
                 }
             }

@@ -122,13 +122,18 @@ __device__ __forceinline__ void gemm_commit(uint32_t mbar, uint32_t leader) {
 }
 
 // Bounded: a wait of a second raises the status word and the CTA's abort flag, which ends the other waits.  The answer is a lane's own: lanes may
-// see the barrier and the flag in different orders.
+// see the barrier and the flag in different orders.  CLUSTER: what the other CTA's threads wrote ahead of their arrivals (released to the cluster) is seen behind it.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
     unsigned long long deadline = 0;
     uint32_t done;
     for (unsigned poll = 0;; ++poll) {
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if constexpr (CLUSTER)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                         : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                         : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) break;
         if ((poll & 63u) == 63u) {
             if (*reinterpret_cast<volatile int *>(abort_flag)) break;
@@ -146,7 +151,10 @@ __device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, int *ab
 }
 
 // A whole warp's: what follows a wait is left by all of its lanes or by none
-__device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *abort_flag) { return __all_sync(~0u, lane_wait(bar, parity, abort_flag)); }
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, int *abort_flag) {
+    return __all_sync(~0u, lane_wait<CLUSTER>(bar, parity, abort_flag));
+}
 
 struct GemmUnit {
     int tm, tn, split, k0, k1;
