@@ -370,7 +370,7 @@ int th_mse_grad(const void *pred_dev, const void *target_dev, void *grad_dev, fl
  * buffer is cleared in the same pass (the table gradient must start at zero every step,
  * triton_helpers/layers/hash_encoding/kernel.py:636).  An element whose scaled gradient is not
  * finite keeps its parameter and moments and adds one to *skipped_dev (a device int the caller
- * zeroes and reads; may be null). */
+ * zeroes and reads, which stays at 2^31 - 1; may be null). */
 int th_adam_step(void *param_dev, void *grad_dev, float *exp_avg_dev, float *exp_avg_sq_dev, int64_t n_elems,
                  float lr, float beta1, float beta2, float eps, int step, float grad_scale, int zero_grad,
                  int dtype, int *skipped_dev, void *stream);

@@ -29,6 +29,19 @@ __device__ __forceinline__ T adam_one(T p, T g_in, float &m, float &v, const Ada
     return from_float<T>(to_float<T>(p) - (a.lr / a.bias1) * (m / denom));
 }
 
+// Adds n to the count of elements passed over, which stays at 2^31 - 1 (a step of 100 M parameters whose norm is not finite counts them all).  A thread adds only
+// after it has seen less, 4096 at a time: with the 148 x 2048 threads that run at once the unsigned word stays below 2^31 + 1.3e9, and whoever
+// takes it past the most brings it back.
+__device__ __forceinline__ void count_skipped(int *total, int n) {
+    constexpr unsigned kMost = 0x7fffffffu;
+    unsigned *at = reinterpret_cast<unsigned *>(total);
+    while (n > 0 && *reinterpret_cast<volatile unsigned *>(at) < kMost) {
+        const unsigned piece = static_cast<unsigned>(min(n, 4096));
+        if (atomicAdd(at, piece) + piece > kMost) atomicMin(at, kMost);
+        n -= static_cast<int>(piece);
+    }
+}
+
 // Elements of a parameter in one 16-byte packet, and the matching moments (float32: four, for twice the threads and half their
 // registers of eight: 3.3 M parameters 34.2 -> 26.4 us)
 template <typename T>

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kClipThreads) adam_clipped_kernel(const __grid
         param[i] = adam_one<T>(param[i], grad[i], exp_avg[i], exp_avg_sq[i], a, skipped);
         if (zero) grad[i] = from_float<T>(0.f);
     }
-    if (skipped_total && skipped) atomicAdd(skipped_total, skipped);
+    if (skipped_total && skipped) count_skipped(skipped_total, skipped);
 }
 
 long long total_elements(int n_tensors, const int64_t *n_elems) {

@@ -124,7 +124,7 @@ adam_many_kernel(const __grid_constant__ AdamTensors t, AdamScalars a, int *__re
         a.zero_grad = t.zero_grad[k];
         skipped += adam_walk<T>(static_cast<T *>(t.param[k]), static_cast<T *>(t.grad[k]), t.exp_avg[k], t.exp_avg_sq[k], t.n[k], a);
     }
-    if (skipped_total && skipped) atomicAdd(skipped_total, skipped);
+    if (skipped_total && skipped) count_skipped(skipped_total, skipped);
 }
 
 struct CastTensors {

@@ -8,7 +8,8 @@ second moment underflows (``g*g < 6e-8`` for ``|g| < 2.4e-4``) and the update di
 replaces the separate zero-fill the hash-encoding backward needs before every step.
 
 Elements whose gradient is not finite (an overflowed 16-bit sum, a NaN from upstream) are left
-untouched - parameter and moments - and counted; ``FusedAdam.skipped_elements()`` reads the count.
+untouched - parameter and moments - and counted; ``FusedAdam.skipped_elements()`` reads the count
+(on each device at most 2^31 - 1, where it stays).
 
 Gradients may be clipped to a global norm on the way: all of them as one vector, its norm and the factor
 stay on the device, and the update multiplies by the factor as it reads::
@@ -46,7 +47,7 @@ def adam_update(
     r"""One ``th_adam_step`` launch: ``param`` (float32 / float16 / bfloat16, contiguous) is updated in
     place from ``grad`` (same dtype and element count) times ``grad_scale``; ``exp_avg`` / ``exp_avg_sq``
     are float32.  ``skipped`` is an int32 device counter of elements passed over because their gradient
-    was not finite."""
+    was not finite; it stays at 2^31 - 1."""
     if grad.dtype != param.dtype or not param.is_contiguous() or not grad.is_contiguous():
         raise RuntimeError("adam_update needs contiguous parameters and same-dtype contiguous gradients")
     device = _lib.require_cuda(param, grad, exp_avg, exp_avg_sq, skipped)
