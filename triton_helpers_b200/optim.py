@@ -252,7 +252,8 @@ class FusedAdam(torch.optim.Optimizer):
             max_norm, grads = _check_norm(max_norm), [p.grad for _, live in groups for p in live]
             pair = _norm_factor(grads, [grad_scale] * len(grads), max_norm) if grads else None
         for group, live in groups:
-            self.update(group, live, [p.grad for p in live], [grad_scale] * len(live), [zero_grad] * len(live), pair)
+            # an `update` that knows nothing of clipping is not told of it
+            self.update(group, live, [p.grad for p in live], [grad_scale] * len(live), [zero_grad] * len(live), *(() if pair is None else (pair,)))
         return None if pair is None else pair[0]
 
     def watched(self) -> bool:

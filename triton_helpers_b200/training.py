@@ -180,10 +180,17 @@ class NeuralFieldTrainer(nn.Module):
         pred.backward(grad_out)
         allreduce_gradients([p.grad for p in self.parameters() if p.grad is not None], self.group)
         # d(mean over the global batch)/d pred = 2 (pred - target) / (N_global * C)
-        self.last_grad_norm = self.optimizer.step(grad_scale=2.0 / (pred.numel() * world * self.grad_out_scale), max_norm=self.max_grad_norm)
+        self._optimizer_step(grad_scale=2.0 / (pred.numel() * world * self.grad_out_scale))
         for p in self.parameters():
             p.grad = None
         return loss_sum / pred.numel()
+
+    def _optimizer_step(self, **kwargs) -> None:
+        r"""The public ``step``, which a caller may have replaced: it is told of clipping only where that was asked for."""
+        if self.max_grad_norm is None:
+            self.optimizer.step(**kwargs)
+        else:
+            self.last_grad_norm = self.optimizer.step(**kwargs, max_norm=self.max_grad_norm)
 
     def _step_float32(self, coords: Tensor, targets: Tensor) -> Optional[Tensor]:
         r"""The same step without an autograd graph: forward and backward in one native call on kept buffers, then the
@@ -221,7 +228,7 @@ class NeuralFieldTrainer(nn.Module):
             if self.optimizer.watched():  # by step hooks or a scheduler: the public step, on the parameters' grad
                 for p, g in zip(params, grads):
                     p.grad = g
-                self.last_grad_norm = self.optimizer.step(grad_scale=adam_scale, zero_grad=True, max_norm=self.max_grad_norm)
+                self._optimizer_step(grad_scale=adam_scale, zero_grad=True)
                 if enc.embeddings.grad is not st.table_grad:
                     st.table_grad.zero_()  # a hook put another gradient in its place
                 for p in params:
@@ -231,7 +238,7 @@ class NeuralFieldTrainer(nn.Module):
                 if self.max_grad_norm is not None:
                     pair = _norm_factor(grads, scales, self.max_grad_norm)
                     self.last_grad_norm = pair[0]
-                self.optimizer.update(self.optimizer.param_groups[0], params, grads, scales, zero, pair)
+                self.optimizer.update(self.optimizer.param_groups[0], params, grads, scales, zero, *(() if pair is None else (pair,)))
         except BaseException:
             self._state = None  # its table gradient may not be zero
             raise
