@@ -549,11 +549,12 @@ int64_t th_grad_norm_workspace_bytes(int n_tensors, const int64_t *n_elems);
 int th_grad_norm(int n_tensors, const void *const *grad_dev, const int64_t *n_elems, const int *dtypes,
                  const float *grad_scale, float max_norm, float *norm_factor_dev, void *workspace_dev,
                  int64_t workspace_bytes, void *stream);
-/* Every tensor times the pair's factor; a factor of one leaves them untouched. */
+/* Every tensor times the pair's factor; a factor of one leaves them untouched.  No two of them overlap. */
 int th_scale_tensors(int n_tensors, void *const *tensor_dev, const int64_t *n_elems, const int *dtypes,
                      const float *norm_factor_dev, void *stream);
 /* th_adam_steps for any number of tensors, with gradients times grad_scale_k times the pair's factor.  A norm that is not
- * finite passes over every element: parameters and moments stay, and all are counted in skipped_dev. */
+ * finite passes over every element: parameters and moments stay, and all are counted in skipped_dev.  No two tensors
+ * overlap. */
 int th_adam_clipped(int n_tensors, void *const *param_dev, void *const *grad_dev, float *const *exp_avg_dev,
                     float *const *exp_avg_sq_dev, const int64_t *n_elems, const float *grad_scale, const int *zero_grad,
                     const float *norm_factor_dev, float lr, float beta1, float beta2, float eps, int step, int dtype,

@@ -138,7 +138,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     r"""Scales the gradients of ``parameters`` in place so that their global 2-norm is at most ``max_norm``, and returns the norm that they
     had (a float32 scalar on their device, not synchronised). As ``torch.nn.utils.clip_grad_norm_``: parameters without a gradient are passed
     over, gradients whose norm is below ``max_norm`` stay as they are (and are not written), those of an infinite or NaN norm become zeros and
-    NaN. A parameter that is listed twice is taken once; gradients that share memory are not taken apart."""
+    NaN. A parameter that is listed twice is taken once. A gradient that several parameters hold counts for each of them in the norm and is scaled
+    once; gradients that overlap otherwise must not be given."""
     max_norm = _check_norm(max_norm)
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     grads = list({id(p): p.grad for p in parameters if p.grad is not None}.values())
@@ -148,6 +149,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     if pair is not NotImplemented:
         return pair[0]
     pair = _norm_factor(grads, None, max_norm)
+    grads = list({(g.data_ptr(), g.shape, g.stride(), g.dtype): g for g in grads}.values())  # a gradient that several parameters hold is scaled once
     flat, device = _flat(grads, "clip_grad_norm_")
     pointers, sizes, codes = _lists(flat)
     with torch.cuda.device(device):
@@ -177,6 +179,8 @@ def _adam_clipped(params, grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads,
             raise RuntimeError("a clipped update needs parameters and gradients of one dtype and float32 moments")
         if not all(t.is_contiguous() and t.numel() == p.numel() for t in (p, g, m, v)):
             raise RuntimeError("a clipped update needs contiguous parameters, gradients and moments of one size")
+    if len({p.data_ptr() for p in params if p.numel()}) != sum(p.numel() > 0 for p in params):
+        raise ValueError("a clipped update takes a parameter once")
     device = _lib.require_cuda(*params, *grads, *exp_avgs, *exp_avg_sqs, pair, skipped)
     if pair is None:
         pair = _norm_factor(grads, grad_scales, max_norm)
@@ -212,7 +216,7 @@ def clipped_adam_updates(
 ) -> Tensor:
     r"""Adam's update in place of parameters of one dtype and device, their gradients clipped to the global norm ``max_norm``; returns the
     norm that they had, each times its scale (a float32 scalar on the device, not synchronised). Any number of contiguous tensors, with
-    gradients of the parameters' dtype and float32 moments; ``skipped`` as in ``adam_update``."""
+    gradients of the parameters' dtype and float32 moments, each parameter once; ``skipped`` as in ``adam_update``."""
     max_norm, n = _check_norm(max_norm), len(params)
     if n == 0 or any(x is not None and len(x) != n for x in (grads, exp_avgs, exp_avg_sqs, grad_scales, zero_grads)):
         raise ValueError("a clipped update needs as many gradients, moments, scales and flags as parameters, and one at least")
