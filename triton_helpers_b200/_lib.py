@@ -368,6 +368,12 @@ def i64_array(values: Sequence[int]):
     return (c_int64 * len(values))(*values)
 
 
+def refuse_trace(what: str) -> None:
+    r"""A trace records torch's operators: of a function that launches kernels by itself it would keep the empty result."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced by torch.jit")
+
+
 def require_cuda(*tensors: Optional[Tensor]) -> torch.device:
     r"""All given tensors must live on one CUDA device (hash_encoding/kernel.py:560-564 of the reference)."""
     devices = {t.device for t in tensors if t is not None}

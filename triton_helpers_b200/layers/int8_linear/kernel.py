@@ -41,6 +41,7 @@ def float_dtype(t: Tensor, what: str) -> torch.dtype:
 
 
 def refuse_gradients(what: str, *tensors: Optional[Tensor]) -> None:
+    _lib.refuse_trace(what)
     given = [t for t in tensors if t is not None]
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")

@@ -104,6 +104,7 @@ def _norm_factor(tensors: Sequence[Tensor], scales: Optional[Sequence[float]], m
     pair = _lib.native().grad_norm(tensors, None if scales is None else tuple(scales), max_norm)
     if pair is not NotImplemented:
         return pair
+    _lib.refuse_trace("the global norm")
     flat, device = _flat(tensors, "the global norm")
     pointers, sizes, codes = _lists(flat)
     lib = _lib.lib()
