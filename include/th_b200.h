@@ -534,7 +534,7 @@ int th_expert_linear_bwd_input(const void *grad_y_dev, int64_t gy_stride, const 
                                int64_t weight_stride, int64_t expert_stride, const int32_t *ends_dev,
                                void *grad_x_dev, int64_t gx_stride, int64_t rows, int experts, int d_in, int d_out,
                                int dtype, void *stream);
-/* grad_weight is contiguous (experts, d_out, d_in); zeros for an expert without rows. */
+/* grad_weight is contiguous (experts, d_out, d_in); zeros for an expert without rows.  experts * d_out: at most 2^31 - 257. */
 int th_expert_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride,
                                 const int32_t *ends_dev, void *grad_weight_dev, int64_t rows, int experts, int d_in,
                                 int d_out, int dtype, void *stream);

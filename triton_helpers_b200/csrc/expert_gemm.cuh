@@ -507,12 +507,11 @@ int launch_experts(ExpertArgs x, const ExpertOperand &a, const ExpertOperand &b,
     g.tiles_n = SWAP ? divide_up(g.n, kGemmRows) : divide_up(g.n, BN);
     g.group = 16;  // 16 tile rows of 256 x 2048: 16 MB
     g.idesc = instr_desc(CG * kGemmRows, BN, bf16, A_MN, B_MN);
-    const long long out_rows = OVER_ROWS ? static_cast<long long>(x.experts) * g.m : x.rows;
     g.out_tma = rows_start_on(g.out, g.out_stride, 2);
     // at most so many tiles: an expert's last one may be part of one
     const long long rows_of_tiles = OVER_ROWS ? static_cast<long long>(x.experts) * g.tiles_m : x.rows / x.tile_rows + std::min(x.experts, x.rows);
     const long long units = rows_of_tiles * g.tiles_n;
-    if (units > 0x7fffffffll || out_rows > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "product of experts: too many tiles");
+    if (units > 0x7fffffffll) return fail(TH_ERR_UNSUPPORTED, "product of experts: too many tiles");
     const long long clusters = std::min<long long>(units, std::max(1, CTAS * sm_count() / CG));
     return launch_chained("expert_gemm_kernel launch", kernel, static_cast<unsigned>(clusters * CG), S::kThreads, S::kBytes, stream, CG, x, a_map, b_map, few_map);
 }

@@ -123,6 +123,8 @@ extern "C" int th_expert_linear_bwd_input(const void *grad_y_dev, int64_t gy_str
 extern "C" int th_expert_linear_bwd_weight(const void *grad_y_dev, int64_t gy_stride, const void *x_dev, int64_t x_stride, const int32_t *ends_dev,
                                            void *grad_weight_dev, int64_t rows, int experts, int d_in, int d_out, int dtype, void *stream) {
     if (int rc = check_experts("th_expert_linear_bwd_weight", rows, experts, d_in, d_out, dtype, ends_dev)) return rc;
+    // rows of all experts' gradients are counted in 32 bits, those behind the end of the last tile (256 rows at most) with them
+    if (static_cast<int64_t>(experts) * d_out > 0x7fffffffll - 256) return fail(TH_ERR_UNSUPPORTED, "th_expert_linear_bwd_weight: %d experts, %d -> %d", experts, d_in, d_out);
     if (!grad_weight_dev) return fail(TH_ERR_BAD_ARG, "th_expert_linear_bwd_weight: null pointer");
     if (int rc = check_elements("th_expert_linear_bwd_weight", dtype, {grad_weight_dev})) return rc;
     cudaStream_t at = static_cast<cudaStream_t>(stream);
