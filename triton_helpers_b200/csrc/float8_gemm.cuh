@@ -258,120 +258,120 @@ float8_gemm_kernel(const F8Gemm f, const __grid_constant__ CUtensorMap a_map, co
     // Each side of the branch has its registers, so that a split tile is finished within it
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kFewRegs));
-    if (warp == 0) {
-        // ---- operands ----
-        int it = 0;
-        bool ok = true;
-        for (int unit = first; unit < units && ok; unit += step) {
-            const GemmUnit u = gemm_unit(g, unit);
-            const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
-            for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
-                const int s = it % S::kStages;
-                const bool got = lane_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
-                if (elect_one() && got) {
-                    const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
-                    if (rank == 0 && it >= ahead)
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
-                    const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
-                    const int k = kt * kF8Block;
-                    if (it >= ahead) gemm_load<CG>(a, &a_map, k, m0, bar);
-                    if constexpr (B_MN) {
-#pragma unroll
-                        for (int j = 0; j < S::kBRows / 128; ++j) gemm_load<CG>(b + j * 128 * 128, &b_map, n0 + 128 * j, k, bar);
-                    } else gemm_load<CG>(b, &b_map, k, n0, bar);
-                }
-                ok = __all_sync(~0u, got);
-                if (!ok) break;
-            }
-        }
-    } else if (warp == 1) {
-        // ---- MMAs ----
-        if (rank == 0) {
+        if (warp == 0) {
+            // ---- operands ----
             int it = 0;
             bool ok = true;
-            const uint32_t issue = elect_one() ? 1u : 0u;
-            __syncwarp();
             for (int unit = first; unit < units && ok; unit += step) {
                 const GemmUnit u = gemm_unit(g, unit);
-                for (int kt = u.k0; kt < u.k1 && ok; ++kt, ++it) {
-                    const int s = it % S::kStages, buf = it % S::kAccs;
-                    ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
+                const int m0 = (u.tm * CG + static_cast<int>(rank)) * kGemmRows, n0 = u.tn * BN + static_cast<int>(rank) * S::kBRows;
+                for (int kt = u.k0; kt < u.k1; ++kt, ++it) {
+                    const int s = it % S::kStages;
+                    const bool got = lane_wait(smem_addr(&empty[s]), ((it / S::kStages) & 1) ^ 1, &abort_flag);
+                    if (elect_one() && got) {
+                        const uint32_t mine = smem_addr(&full[s]), bar = CG == 2 ? in_cta(mine, leader) : mine;
+                        if (rank == 0 && it >= ahead)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mine), "r"(static_cast<uint32_t>(CG * S::kStage)) : "memory");
+                        const uint32_t a = smem + s * S::kStage, b = a + S::kABytes;
+                        const int k = kt * kF8Block;
+                        if (it >= ahead) gemm_load<CG>(a, &a_map, k, m0, bar);
+                        if constexpr (B_MN) {
+#pragma unroll
+                            for (int j = 0; j < S::kBRows / 128; ++j) gemm_load<CG>(b + j * 128 * 128, &b_map, n0 + 128 * j, k, bar);
+                        } else gemm_load<CG>(b, &b_map, k, n0, bar);
+                    }
+                    ok = __all_sync(~0u, got);
                     if (!ok) break;
-                    ok = gemm_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a = smem + s * S::kStage;
-                    f8_block<CG, B_MN>(tmem + buf * BN, a, a + S::kABytes, g.idesc, issue, smem_addr(&acc_full[buf]), smem_addr(&empty[s]), leader);
                 }
             }
-        }
-    } else {
-        // ---- scales: the even blocks' by one warp, the odd ones' by the other (one warp for all of them: 545 -> 590 us at 8192 x 4096 -> 16384) ----
-        constexpr int kRows = (SWAP ? BN : kGemmRows) / 32 > 0 ? (SWAP ? BN : kGemmRows) / 32 : 1, kGroups = SWAP ? 1 : BN == 256 ? 2 : 1;
-        int it0 = 0;
-        bool ok = true;
-        for (int unit = first; unit < units && ok; unit += step) {
-            const GemmUnit u = gemm_unit(g, unit);
-            const F8Tile<B_MN, BN, SWAP> tile(f, u, (u.tm * CG + static_cast<int>(rank)) * kGemmRows);
-            for (int kt = u.k0 + ((it0 ^ warp) & 1); kt < u.k1 && ok; kt += 2 * kF8Batch) {
-                float token[kF8Batch][kRows], weight[kF8Batch][kGroups];
-#pragma unroll
-                for (int b = 0; b < kF8Batch; ++b) {
-                    const int at = min(kt + 2 * b, u.k1 - 1);
-#pragma unroll
-                    for (int r = 0; r < kRows; ++r) token[b][r] = tile.token(32 * r + lane, at);
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q) weight[b][q] = tile.of_weight(q, at);
-                }
-#pragma unroll
-                for (int b = 0; b < kF8Batch; ++b) {
-                    if (kt + 2 * b >= u.k1) break;
-                    const int it = it0 + kt + 2 * b - u.k0, s = it % S::kSlots, buf = it % S::kAccs;
-                    bool far = false;
-                    // The accumulator's block before is complete.  So block it - 2 kAccs has been read out by every warp, and the blocks before it have been
-                    // added: a slot that came round since is free.
-                    static_assert(S::kSlots > 2 * S::kAccs, "a slot may still be in use");
-                                        if (it >= S::kAccs) ok = gemm_wait(smem_addr(&acc_full[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
-                    if (!ok) break;
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q)
-#pragma unroll
-                        for (int r = 0; r < kRows; ++r) {
-                            const float size = fabsf(token[b][r] * weight[b][q]);
-                            far |= size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
-                        }
-                    far = __any_sync(~0u, far);
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q)
-#pragma unroll
-                        for (int r = 0; r < kRows; ++r) {
-                            const int at = q * kGemmRows + 32 * r + lane;
-                            if (32 * r + lane >= (SWAP ? BN : kGemmRows)) continue;
-                            if (far) {
-                                const float2 x = split_scale(token[b][r]), y = split_scale(weight[b][q]);
-                                factors[s][0][at] = x.x * y.x;
-                                factors[s][1][at] = rests_of(x.y, y.y);
-                            } else {
-                                factors[s][0][at] = token[b][r] * weight[b][q];
-                            }
-                        }
-                    __syncwarp();
-                    if (lane == 0) {
-                        far_factors[s] = far;
-                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_full[buf])) : "memory");
+        } else if (warp == 1) {
+            // ---- MMAs ----
+            if (rank == 0) {
+                int it = 0;
+                bool ok = true;
+                const uint32_t issue = elect_one() ? 1u : 0u;
+                __syncwarp();
+                for (int unit = first; unit < units && ok; unit += step) {
+                    const GemmUnit u = gemm_unit(g, unit);
+                    for (int kt = u.k0; kt < u.k1 && ok; ++kt, ++it) {
+                        const int s = it % S::kStages, buf = it % S::kAccs;
+                        ok = gemm_wait(smem_addr(&full[s]), (it / S::kStages) & 1, &abort_flag);
+                        if (!ok) break;
+                        ok = gemm_wait(smem_addr(&acc_empty[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t a = smem + s * S::kStage;
+                        f8_block<CG, B_MN>(tmem + buf * BN, a, a + S::kABytes, g.idesc, issue, smem_addr(&acc_full[buf]), smem_addr(&empty[s]), leader);
                     }
                 }
             }
-            it0 += u.k1 - u.k0;
+        } else {
+            // ---- scales: the even blocks' by one warp, the odd ones' by the other (one warp for all of them: 545 -> 590 us at 8192 x 4096 -> 16384) ----
+            constexpr int kRows = (SWAP ? BN : kGemmRows) / 32 > 0 ? (SWAP ? BN : kGemmRows) / 32 : 1, kGroups = SWAP ? 1 : BN == 256 ? 2 : 1;
+            int it0 = 0;
+            bool ok = true;
+            for (int unit = first; unit < units && ok; unit += step) {
+                const GemmUnit u = gemm_unit(g, unit);
+                const F8Tile<B_MN, BN, SWAP> tile(f, u, (u.tm * CG + static_cast<int>(rank)) * kGemmRows);
+                for (int kt = u.k0 + ((it0 ^ warp) & 1); kt < u.k1 && ok; kt += 2 * kF8Batch) {
+                    float token[kF8Batch][kRows], weight[kF8Batch][kGroups];
+#pragma unroll
+                    for (int b = 0; b < kF8Batch; ++b) {
+                        const int at = min(kt + 2 * b, u.k1 - 1);
+#pragma unroll
+                        for (int r = 0; r < kRows; ++r) token[b][r] = tile.token(32 * r + lane, at);
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q) weight[b][q] = tile.of_weight(q, at);
+                    }
+#pragma unroll
+                    for (int b = 0; b < kF8Batch; ++b) {
+                        if (kt + 2 * b >= u.k1) break;
+                        const int it = it0 + kt + 2 * b - u.k0, s = it % S::kSlots, buf = it % S::kAccs;
+                        bool far = false;
+                        // The accumulator's block before is complete.  So block it - 2 kAccs has been read out by every warp, and the blocks before it have been
+                        // added: a slot that came round since is free.
+                        static_assert(S::kSlots > 2 * S::kAccs, "a slot may still be in use");
+                        if (it >= S::kAccs) ok = gemm_wait(smem_addr(&acc_full[buf]), ((it / S::kAccs) & 1) ^ 1, &abort_flag);
+                        if (!ok) break;
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                            for (int r = 0; r < kRows; ++r) {
+                                const float size = fabsf(token[b][r] * weight[b][q]);
+                                far |= size < 0x1p-100f || size > 0x1p100f;  // a NaN is not
+                            }
+                        far = __any_sync(~0u, far);
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                            for (int r = 0; r < kRows; ++r) {
+                                const int at = q * kGemmRows + 32 * r + lane;
+                                if (32 * r + lane >= (SWAP ? BN : kGemmRows)) continue;
+                                if (far) {
+                                    const float2 x = split_scale(token[b][r]), y = split_scale(weight[b][q]);
+                                    factors[s][0][at] = x.x * y.x;
+                                    factors[s][1][at] = rests_of(x.y, y.y);
+                                } else {
+                                    factors[s][0][at] = token[b][r] * weight[b][q];
+                                }
+                            }
+                        __syncwarp();
+                        if (lane == 0) {
+                            far_factors[s] = far;
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_full[buf])) : "memory");
+                        }
+                    }
+                }
+                it0 += u.k1 - u.k0;
+            }
         }
-    }
-    if constexpr (S::kSplits) {
-        if (g.splits > 1) {
-            __syncwarp();
-            cluster_sync_all();
-            cluster_sync_all();
+        if constexpr (S::kSplits) {
+            if (g.splits > 1) {
+                __syncwarp();
+                cluster_sync_all();
+                cluster_sync_all();
+            }
         }
-    }
     } else {
         // ---- sums, and the output ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSumRegs));

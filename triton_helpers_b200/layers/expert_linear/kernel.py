@@ -127,7 +127,8 @@ def expert_linear(x: Tensor, weight: Tensor, ends: Tensor) -> Tensor:
         x: float16 or bfloat16 rows sorted by expert; under autocast any float type but float64, cast to autocast's (float16 or bfloat16)
         weight: one matrix for each expert, of x's type
         ends: int32 or int64 on the device: the first row behind each expert's, the cumulative sum of the experts' numbers of rows
-            (``torch.cumsum(counts, 0)``). int32 is what the kernels read; int64 is converted.
+            (``torch.cumsum(counts, 0, dtype=torch.int32)``). int32 is what the kernels read; int64, which ``cumsum`` gives by itself, is
+            converted by two more kernels, and such calls take the longer way through Python.
 
     Shapes:
         - x: :math:`(R, D_{in})`, output: :math:`(R, D_{out})`

@@ -16,8 +16,9 @@ stay on the device, and the update multiplies by the factor as it reads::
 
     norm = sqrt(sum_k scale_k^2 sum_i g_k[i]^2)        factor = min(1, max_norm / (norm + 1e-6))
 
-The sum is in float64, in a fixed order (results repeat bit for bit), and takes any float32 gradients: neither
-large nor small squares are lost. A norm that is not finite passes over the whole step: every element counts as skipped.
+Squares are added in float32 over 16 bytes of gradients and in float64 from there, in a fixed order (results repeat bit
+for bit); 16 bytes whose largest element is outside of 2^-50 .. 2^50 are added in float64 throughout, so that neither large nor small
+squares are lost. A norm that is not finite passes over the whole step: every element counts as skipped.
 """
 import math
 from ctypes import c_float, c_int, c_void_p
